@@ -2,7 +2,8 @@
  * namitorch_amd.h — C ABI of the MI355X (gfx950) optimizer-step library.
  *
  * This is the drop-in boundary for NamiTorch's optimizer-step hot path:
- * AdamW.step(), GradScaler unscale_/finite-check/update and clip_grad_norm_.
+ * AdamW.step(), GradScaler unscale_/finite-check/update and clip_grad_norm_,
+ * and for the operators of the residual path (layer norm, dropout).
  * Every entry point takes plain pointers, sizes and a hipStream_t passed as
  * `void*`; no framework types cross the boundary.  Callers (the Python host
  * layer in namitorch_amd/, through ctypes) own every tensor buffer: memory
@@ -529,6 +530,71 @@ int32_t nt_tensor_scalar(const void *in, int32_t in_dtype, void *out,
  */
 int32_t nt_any_negative(const void *array, int32_t dtype, uint64_t count,
                         int32_t *flag, void *stream);
+
+/* ---- residual-path operators --------------------------------------------- */
+
+/*
+ * Layer norm of `rows` rows of `width` elements (1..2**30), with its backward
+ * pass (reference: layer_norm forward/input_backward/affine_backward,
+ * backends/cuda/normalization.py:56-157, there for float32 and widths up to
+ * 8192):
+ *
+ *   mean = sum x / width, rstd = 1 / sqrt(sum (x - mean)^2 / width + eps)
+ *   y = (x - mean) rstd weight + bias
+ *
+ * Arrays are contiguous; `dtype` (float32, float16, bfloat16) is that of the
+ * activations and their gradients, `weight_dtype` that or float32, for
+ * weight, bias and their gradients; NULL weight is ones, NULL bias zeros.
+ * mean and rstd (float32, one per row) are written when not NULL (both or
+ * neither) and are what the backward entry reads.  A NULL dweight or dbias
+ * is not computed.  Sums are float32 in a fixed order; values are rounded
+ * once, when stored.  A row holding an infinity or NaN gives NaN outputs.
+ * Outputs overlap neither inputs nor one another.  Work is queued on
+ * `stream` of `device`; the backward entries take their workspace from the
+ * library's pool in that stream's order and refuse (NT_ERR_RUNTIME) a stream
+ * in capture when they need it.  With no rows the forward entries do
+ * nothing, the backward entries write zero dweight and dbias.
+ */
+int32_t nt_layer_norm(int32_t device, const void *x, int32_t dtype, const void *weight,
+                      const void *bias, int32_t weight_dtype, float eps, void *y,
+                      float *mean, float *rstd, uint64_t rows, uint64_t width, void *stream);
+int32_t nt_layer_norm_backward(int32_t device, const void *dy, const void *x, int32_t dtype,
+                               const float *mean, const float *rstd, const void *weight,
+                               int32_t weight_dtype, void *dx, void *dweight, void *dbias,
+                               uint64_t rows, uint64_t width, void *stream);
+
+/*
+ * Dropout with a mask that is never stored.  Element i of the flat array is
+ * dropped (set to zero, whatever it holds) when its 16-bit number is below
+ * `threshold` (0..65536; p = threshold / 65536), and otherwise multiplied by
+ * 65536 / (65536 - threshold) in float32 and rounded once.  The number of
+ * element i is half i % 2 (low half first) of word i % 8 / 2 of
+ * Philox4x32-10 with counter (i / 8, offset) and key `seed` (64 bits each,
+ * low word first).  The backward pass is the same call on the gradient.
+ * `y` may be `x`; otherwise they do not overlap.
+ */
+int32_t nt_dropout(int32_t device, const void *x, int32_t dtype, void *y, uint64_t count,
+                   uint32_t threshold, uint64_t seed, uint64_t offset, void *stream);
+
+/*
+ * The edge between two sublayers in one pass: total = dropout(x) + residual
+ * (threshold 0: x + residual), y = layer norm of total before its rounding;
+ * total and y are rounded once each.  Backward: dresidual = the norm's
+ * gradient at total, plus dtotal (the gradient total receives elsewhere;
+ * NULL: none), and dx = dropout's gradient of it.  Arguments as above.
+ */
+int32_t nt_dropout_add_layer_norm(int32_t device, const void *x, const void *residual, int32_t dtype,
+                                  const void *weight, const void *bias, int32_t weight_dtype,
+                                  float eps, uint32_t threshold, uint64_t seed, uint64_t offset,
+                                  void *total, void *y, float *mean, float *rstd, uint64_t rows,
+                                  uint64_t width, void *stream);
+int32_t nt_dropout_add_layer_norm_backward(int32_t device, const void *dy, const void *dtotal,
+                                           const void *total, int32_t dtype, const float *mean,
+                                           const float *rstd, const void *weight,
+                                           int32_t weight_dtype, uint32_t threshold, uint64_t seed,
+                                           uint64_t offset, void *dx, void *dresidual,
+                                           void *dweight, void *dbias, uint64_t rows,
+                                           uint64_t width, void *stream);
 
 /* ---- measurement ------------------------------------------------------- */
 

@@ -41,6 +41,7 @@ NT_OP_DIV = 1
 c_void_p = ctypes.c_void_p
 c_int32 = ctypes.c_int32
 c_int64 = ctypes.c_int64
+c_uint32 = ctypes.c_uint32
 c_uint64 = ctypes.c_uint64
 c_float = ctypes.c_float
 c_double = ctypes.c_double
@@ -164,6 +165,17 @@ SIGNATURES = {
     "nt_any_negative": (c_int32, [c_void_p, c_int32, c_uint64, c_void_p, c_void_p]),
     "nt_amp_flat_stats_noalloc": (c_int32, [c_int32, c_void_p, c_int32, c_uint64, c_float, c_int32, c_void_p, c_void_p,
                                             c_double, c_double, c_int32, c_double, c_double, c_int32, c_void_p]),
+    "nt_layer_norm": (c_int32, [c_int32, c_void_p, c_int32, c_void_p, c_void_p, c_int32, c_float, c_void_p, c_void_p,
+                                c_void_p, c_uint64, c_uint64, c_void_p]),
+    "nt_layer_norm_backward": (c_int32, [c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_int32,
+                                         c_void_p, c_void_p, c_void_p, c_uint64, c_uint64, c_void_p]),
+    "nt_dropout": (c_int32, [c_int32, c_void_p, c_int32, c_void_p, c_uint64, c_uint32, c_uint64, c_uint64, c_void_p]),
+    "nt_dropout_add_layer_norm": (c_int32, [c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_int32, c_float,
+                                            c_uint32, c_uint64, c_uint64, c_void_p, c_void_p, c_void_p, c_void_p,
+                                            c_uint64, c_uint64, c_void_p]),
+    "nt_dropout_add_layer_norm_backward": (c_int32, [c_int32, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p,
+                                                     c_void_p, c_int32, c_uint32, c_uint64, c_uint64, c_void_p,
+                                                     c_void_p, c_void_p, c_void_p, c_uint64, c_uint64, c_void_p]),
     "nt_stream_probe": (c_int32, [ctypes.POINTER(c_void_p), c_int32, c_int32, ctypes.POINTER(c_void_p), c_int32, c_int32,
                                   c_uint64, c_void_p]),
     "nt_malloc": (c_int32, [c_int32, c_uint64, c_void_p, ctypes.POINTER(c_void_p)]),
