@@ -534,7 +534,7 @@ int32_t nt_any_negative(const void *array, int32_t dtype, uint64_t count,
 /* ---- residual-path operators --------------------------------------------- */
 
 /*
- * Layer norm of `rows` rows of `width` elements (1..2**30), with its backward
+ * Layer norm of `rows` rows of `width` elements (1..2**24), with its backward
  * pass (reference: layer_norm forward/input_backward/affine_backward,
  * backends/cuda/normalization.py:56-157, there for float32 and widths up to
  * 8192):

@@ -16,6 +16,7 @@
 #include <hip/hip_runtime.h>
 
 #include <initializer_list>
+#include <type_traits>
 
 #include "nt_internal.hpp"
 #include "nt_philox.hpp"
@@ -78,6 +79,417 @@ __device__ __forceinline__ float block_sum_f32(float v, float *shared) {
     float total = 0.0f;
     for (uint32_t k = 0; k < blockDim.x / 64u; ++k) total += shared[k];
     return total;
+}
+
+// ---- eight consecutive elements ------------------------------------------------------------------
+// What a lane holds of a row at a time: one 16-byte access of a 16-bit type,
+// two of float32, and one call of the mask's generator.  Where rows do not
+// start on 16 bytes the same accesses run unaligned (gfx950 takes any
+// alignment), and the lane at a row's ragged end goes element by element.
+constexpr int kGroup = 8;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef __attribute__((address_space(1))) u32x4 gu32x4;
+typedef __attribute__((address_space(1))) u32x4_any gu32x4_any;
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+template <class T> struct Raw8 {
+    static constexpr int kWords = sizeof(typename T::raw) / 2;      // 16-byte words
+    u32x4 w[kWords];
+};
+
+template <class T, bool EVEN>
+__device__ __forceinline__ void load8(Raw8<T> &out, const void *base, uint64_t i) {
+    const auto *p = reinterpret_cast<const typename T::raw *>(base) + i;
+#pragma unroll
+    for (int k = 0; k < Raw8<T>::kWords; ++k) {
+        if constexpr (EVEN) out.w[k] = gload<true, u32x4, gu32x4>(p + k * 4);
+        else out.w[k] = gload<true, u32x4, gu32x4_any>(p + k * 4);
+    }
+}
+
+template <class T, bool EVEN>
+__device__ __forceinline__ void store8(void *base, uint64_t i, const Raw8<T> &in) {
+    auto *p = reinterpret_cast<typename T::raw *>(base) + i;
+#pragma unroll
+    for (int k = 0; k < Raw8<T>::kWords; ++k) {
+        if constexpr (EVEN) gstore<true, u32x4, gu32x4>(p + k * 4, in.w[k]);
+        else gstore<true, u32x4, gu32x4_any>(p + k * 4, in.w[k]);
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void widen8(float (&out)[8], const Raw8<T> &in) {
+    if constexpr (T::code == NT_F32) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) out[k] = bits_f32(in.w[k >> 2][k & 3]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint32_t w = in.w[0][k >> 1];
+            if constexpr (T::code == NT_BF16) out[k] = bits_f32(k & 1 ? w & 0xffff0000u : w << 16);
+            else out[k] = f16_to_f32((uint16_t)(k & 1 ? w >> 16 : w & 0xffffu));
+        }
+    }
+}
+
+// One rounding to nearest even each (v_cvt_pk_bf16_f32, v_cvt_pk_f16_f32).
+template <class T>
+__device__ __forceinline__ void narrow8(Raw8<T> &out, const float (&in)[8]) {
+    if constexpr (T::code == NT_F32) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) out.w[k >> 2][k & 3] = f32_bits(in[k]);
+    } else {
+        f32x8 v;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = in[k];
+        if constexpr (T::code == NT_BF16) out.w[0] = __builtin_bit_cast(u32x4, __builtin_convertvector(v, bf16x8));
+        else out.w[0] = __builtin_bit_cast(u32x4, __builtin_convertvector(v, f16x8));
+    }
+}
+
+// The `left` (< 8) elements of a row's ragged end; the others read as zero.
+template <class T>
+__device__ __forceinline__ void load_end(Raw8<T> &out, const void *base, uint64_t i, uint32_t left) {
+    const auto *p = reinterpret_cast<const typename T::raw *>(base) + i;
+#pragma unroll
+    for (int k = 0; k < Raw8<T>::kWords; ++k) out.w[k] = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (uint32_t k = 0; k < 8; ++k) {
+        if (k >= left) continue;
+        if constexpr (T::code == NT_F32) out.w[k >> 2][k & 3] = f32_bits(p[k]);
+        else out.w[0][k >> 1] |= (uint32_t)p[k] << (16 * (k & 1));
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void store_end(void *base, uint64_t i, const Raw8<T> &in, uint32_t left) {
+    auto *p = reinterpret_cast<typename T::raw *>(base) + i;
+#pragma unroll
+    for (uint32_t k = 0; k < 8; ++k) {
+        if (k >= left) continue;
+        if constexpr (T::code == NT_F32) p[k] = bits_f32(in.w[k >> 2][k & 3]);
+        else p[k] = (uint16_t)(in.w[0][k >> 1] >> (16 * (k & 1)));
+    }
+}
+
+// Elements [c, c + 8) of the row that starts at `base + row`, c < width.
+template <class T, bool EVEN>
+__device__ __forceinline__ void load_part(Raw8<T> &out, const void *base, uint64_t row, uint32_t c, uint32_t width) {
+    if (EVEN || c + kGroup <= width) load8<T, EVEN>(out, base, row + c);
+    else load_end<T>(out, base, row + c, width - c);
+}
+template <class T, bool EVEN>
+__device__ __forceinline__ void store_part(void *base, uint64_t row, uint32_t c, uint32_t width, const Raw8<T> &in) {
+    if (EVEN || c + kGroup <= width) store8<T, EVEN>(base, row + c, in);
+    else store_end<T>(base, row + c, in, width - c);
+}
+
+// Elements [c, c + 8) of weight or bias; `absent` where there is none.
+__device__ __forceinline__ void load_params(float (&out)[8], const void *base, int32_t dtype, uint32_t c,
+                                            uint32_t width, float absent) {
+    if (base == nullptr || c + kGroup > width) {
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) out[k] = c + k < width ? load_param(base, dtype, c + k, absent) : 0.0f;
+    } else if (dtype == NT_F32) {
+        Raw8<TF32> raw;
+        load8<TF32, false>(raw, base, c);
+        widen8<TF32>(out, raw);
+    } else if (dtype == NT_F16) {
+        Raw8<TF16> raw;
+        load8<TF16, false>(raw, base, c);
+        widen8<TF16>(out, raw);
+    } else {
+        Raw8<TBF16> raw;
+        load8<TBF16, false>(raw, base, c);
+        widen8<TBF16>(out, raw);
+    }
+}
+
+// Numbers of the eight elements from flat index i on: one call where i is a
+// multiple of eight, else the two groups they straddle, shifted together.
+template <bool EVEN>
+__device__ __forceinline__ PhiloxWords numbers8(uint64_t i, const Mask &m) {
+    PhiloxWords words = philox(i >> 3, m.offset, m.seed);
+    if constexpr (!EVEN) {
+        const PhiloxWords next = philox((i >> 3) + 1, m.offset, m.seed);
+        const uint32_t shift = (uint32_t)i & 7u;
+        const bool by4 = shift & 4u, by2 = shift & 2u, by1 = shift & 1u;
+        const uint32_t a = by4 ? words.w[2] : words.w[0], b = by4 ? words.w[3] : words.w[1];
+        const uint32_t c = by4 ? next.w[0] : words.w[2], d = by4 ? next.w[1] : words.w[3];
+        const uint32_t e = by4 ? next.w[2] : next.w[0], f = by4 ? next.w[3] : next.w[1];
+        const uint32_t p = by2 ? b : a, q = by2 ? c : b, r = by2 ? d : c, s = by2 ? e : d, t = by2 ? f : e;
+        words.w[0] = by1 ? __builtin_amdgcn_alignbit(q, p, 16) : p;
+        words.w[1] = by1 ? __builtin_amdgcn_alignbit(r, q, 16) : q;
+        words.w[2] = by1 ? __builtin_amdgcn_alignbit(s, r, 16) : r;
+        words.w[3] = by1 ? __builtin_amdgcn_alignbit(t, s, 16) : s;
+    }
+    return words;
+}
+
+__device__ __forceinline__ void drop8(float (&v)[8], const PhiloxWords &words, const Mask &m) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = philox_half(words, k) >= m.threshold ? v[k] * m.factor : 0.0f;
+}
+
+// ---- rows that fit in registers ----------------------------------------------------------------------
+// `lanes` (a power of two) lanes hold a row in `parts` groups of eight each,
+// group k of lane l at column 8 (k lanes + l).  Rows of at most 64 lanes share
+// waves and workgroups and need no barrier; wider ones have a workgroup of
+// their own.  The row is read once, all sums come from registers, and the
+// next row is on its way while this one is summed.
+constexpr int kRowThreads = 256;        // lanes of a workgroup of rows that are at most as wide
+constexpr int kWideThreads = 1024;      // at most, for wider rows
+
+// Sum over the `lanes` lanes of a row, the same on each.  Rows of several
+// waves go through `shared`, of which consecutive sums use the two halves in
+// turn: a wave that writes a half again has passed the barrier of the sum in
+// between, which no wave reaches before it has read that half.
+template <int MAX_WAVES>
+struct RowSum {
+    float (*shared)[MAX_WAVES];
+    uint32_t lanes;
+    uint32_t half = 0;
+    __device__ __forceinline__ float operator()(float v) {
+#pragma unroll
+        for (uint32_t off = 1; off < 64u; off <<= 1)
+            if (off < lanes) v += __shfl_xor(v, (int)off, 64);
+        if (lanes <= 64u) return v;
+        float *slot = shared[half];
+        half ^= 1u;
+        if ((threadIdx.x & 63u) == 0u) slot[threadIdx.x >> 6] = v;
+        __syncthreads();
+        float total = 0.0f;
+        for (uint32_t k = 0; k < lanes / 64u; ++k) total += slot[k];
+        return total;
+    }
+};
+
+template <class T, int EDGE, int PARTS, bool EVEN, int THREADS>
+__global__ __launch_bounds__(THREADS) void norm_kernel(NormForward a, uint32_t lanes) {
+    __shared__ float shared[2][THREADS / 64];
+    RowSum<THREADS / 64> row_sum{shared, lanes};
+    const uint32_t lane = threadIdx.x & (lanes - 1u), in_block = threadIdx.x / lanes, per_block = blockDim.x / lanes;
+    const float width = (float)a.width;
+    uint32_t column[PARTS];
+    float weight[PARTS][8], bias[PARTS][8];
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+        column[p] = ((uint32_t)p * lanes + lane) * kGroup;
+        load_params(weight[p], a.weight, a.weight_dtype, column[p], a.width, 1.0f);
+        load_params(bias[p], a.bias, a.weight_dtype, column[p], a.width, 0.0f);
+    }
+    const uint64_t stride = (uint64_t)gridDim.x * per_block;
+    uint64_t row = (uint64_t)blockIdx.x * per_block + in_block;
+    Raw8<T> x[PARTS], r[PARTS];
+    const auto fetch = [&](uint64_t which) {
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            if (which >= a.rows || column[p] >= a.width) continue;
+            load_part<T, EVEN>(x[p], a.x, which * a.width, column[p], a.width);
+            if constexpr (EDGE != kNone) load_part<T, EVEN>(r[p], a.residual, which * a.width, column[p], a.width);
+        }
+    };
+    fetch(row);
+    for (; row < a.rows; row += stride) {
+        const uint64_t base = row * a.width;
+        float t[PARTS][8];
+        float sum = 0.0f;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            const bool mine = column[p] < a.width;
+            if (mine) {
+                widen8<T>(t[p], x[p]);
+                if constexpr (EDGE == kDropAdd) drop8(t[p], numbers8<EVEN>(base + column[p], a.mask), a.mask);
+                if constexpr (EDGE != kNone) {
+                    float add[8];
+                    widen8<T>(add, r[p]);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) t[p][k] += add[k];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const bool in_row = EVEN ? mine : column[p] + (uint32_t)k < a.width;
+                t[p][k] = in_row ? t[p][k] : 0.0f;
+                sum += t[p][k];
+            }
+        }
+        fetch(row + stride);
+        const float mean = row_sum(sum) / width;
+        float squares = 0.0f;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const bool in_row = EVEN ? column[p] < a.width : column[p] + (uint32_t)k < a.width;
+                const float d = t[p][k] - mean;
+                squares = in_row ? __builtin_fmaf(d, d, squares) : squares;
+            }
+        const float rstd = 1.0f / __builtin_sqrtf(row_sum(squares) / width + a.eps);
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            if (column[p] >= a.width) continue;
+            Raw8<T> out;
+            if constexpr (EDGE != kNone) {
+                narrow8<T>(out, t[p]);
+                store_part<T, EVEN>(a.total, base, column[p], a.width, out);
+            }
+            float y[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] = __builtin_fmaf((t[p][k] - mean) * rstd, weight[p][k], bias[p][k]);
+            narrow8<T>(out, y);
+            store_part<T, EVEN>(a.y, base, column[p], a.width, out);
+        }
+        if (a.mean != nullptr && lane == 0) {
+            a.mean[row] = mean;
+            a.rstd[row] = rstd;
+        }
+    }
+}
+
+// The backward pass of the same tiling.  dw and db of a lane's columns stay
+// in registers over all rows of the workgroup; rows that share a workgroup
+// are joined at the end, and each workgroup writes one row of partial sums.
+template <class T, int EDGE, int PARTS, bool EVEN, int THREADS>
+__global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormBackward a, uint32_t lanes) {
+    __shared__ float shared[2][2 * (THREADS / 64)];
+    __shared__ float join[THREADS > kRowThreads ? 1 : PARTS * 16 * 64];
+    RowSum<2 * (THREADS / 64)> row_sum{shared, lanes};
+    const uint32_t lane = threadIdx.x & (lanes - 1u), in_block = threadIdx.x / lanes, per_block = blockDim.x / lanes;
+    const float width = (float)a.width;
+    uint32_t column[PARTS];
+    float weight[PARTS][8], dw[PARTS][8], db[PARTS][8];
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+        column[p] = ((uint32_t)p * lanes + lane) * kGroup;
+        load_params(weight[p], a.weight, a.weight_dtype, column[p], a.width, 1.0f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) dw[p][k] = db[p][k] = 0.0f;
+    }
+    const uint64_t stride = (uint64_t)gridDim.x * per_block;
+    uint64_t row = (uint64_t)blockIdx.x * per_block + in_block;
+    Raw8<T> dy[PARTS], t[PARTS], dt[PARTS], next_dy[PARTS], next_t[PARTS], next_dt[PARTS];
+    float mean = 0.0f, rstd = 0.0f, next_mean = 0.0f, next_rstd = 0.0f;
+    const auto fetch = [&](uint64_t which) {
+        if (which >= a.rows) return;
+        next_mean = a.mean[which];
+        next_rstd = a.rstd[which];
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            if (column[p] >= a.width) continue;
+            load_part<T, EVEN>(next_dy[p], a.dy, which * a.width, column[p], a.width);
+            load_part<T, EVEN>(next_t[p], a.t, which * a.width, column[p], a.width);
+            if constexpr (EDGE != kNone)
+                if (a.dtotal != nullptr)
+                    load_part<T, EVEN>(next_dt[p], a.dtotal, which * a.width, column[p], a.width);
+        }
+    };
+    fetch(row);
+    for (; row < a.rows; row += stride) {
+        const uint64_t base = row * a.width;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            dy[p] = next_dy[p];
+            t[p] = next_t[p];
+            dt[p] = next_dt[p];
+        }
+        mean = next_mean;
+        rstd = next_rstd;
+        fetch(row + stride);
+        float level = 0.0f, along = 0.0f;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            if (column[p] >= a.width) continue;
+            float g[8], h[8];
+            widen8<T>(g, dy[p]);
+            widen8<T>(h, t[p]);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                // Past a ragged end: dy reads as zero, and so does h.
+                h[k] = EVEN || column[p] + (uint32_t)k < a.width ? (h[k] - mean) * rstd : 0.0f;
+                dw[p][k] = __builtin_fmaf(g[k], h[k], dw[p][k]);
+                db[p][k] += g[k];
+                g[k] *= weight[p][k];
+                level += g[k];
+                along = __builtin_fmaf(g[k], h[k], along);
+            }
+        }
+        level = row_sum(level) / width;
+        along = row_sum(along) / width;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            if (column[p] >= a.width) continue;
+            float g[8], h[8];
+            widen8<T>(g, dy[p]);
+            widen8<T>(h, t[p]);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                g[k] = rstd * (g[k] * weight[p][k] - level - (h[k] - mean) * rstd * along);
+            Raw8<T> out;
+            if constexpr (EDGE != kNone) {
+                if (a.dtotal != nullptr) {
+                    widen8<T>(h, dt[p]);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) g[k] += h[k];
+                }
+                narrow8<T>(out, g);
+                store_part<T, EVEN>(a.dresidual, base, column[p], a.width, out);
+                if constexpr (EDGE == kDropAdd) drop8(g, numbers8<EVEN>(base + column[p], a.mask), a.mask);
+            }
+            narrow8<T>(out, g);
+            store_part<T, EVEN>(a.dx, base, column[p], a.width, out);
+        }
+    }
+    if (a.partials == nullptr) return;
+    if constexpr (THREADS <= kRowThreads) {
+        if (lanes <= 64u) {
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    for (uint32_t off = lanes; off < 64u; off <<= 1) {
+                        dw[p][k] += __shfl_xor(dw[p][k], (int)off, 64);
+                        db[p][k] += __shfl_xor(db[p][k], (int)off, 64);
+                    }
+                }
+            const uint32_t wave = threadIdx.x >> 6, waves = blockDim.x >> 6, at = threadIdx.x & 63u;
+            for (uint32_t k = 0; k + 1u < waves; ++k) {          // wave k hands its sums to wave k + 1
+                if (wave == k) {
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            join[(p * 16 + j) * 64 + at] = dw[p][j];
+                            join[(p * 16 + 8 + j) * 64 + at] = db[p][j];
+                        }
+                }
+                __syncthreads();
+                if (wave == k + 1u) {
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            dw[p][j] += join[(p * 16 + j) * 64 + at];
+                            db[p][j] += join[(p * 16 + 8 + j) * 64 + at];
+                        }
+                }
+            }
+            if (wave + 1u != waves || at >= lanes) return;
+        }
+    }
+    float *out = a.partials + (uint64_t)blockIdx.x * 2u * a.width;
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) {
+            if (column[p] + k >= a.width) continue;
+            out[column[p] + k] = dw[p][k];
+            out[a.width + column[p] + k] = db[p][k];
+        }
+    }
 }
 
 // ---- rows of any width: a workgroup per row, the row read once per pass ---------------------
@@ -172,41 +584,93 @@ __global__ __launch_bounds__(kBlock) void norm_columns_kernel(NormBackward a) {
     out[a.width + c] = db;
 }
 
-// dw and db from the partial sums, rounded to the weight's dtype.
+// dw and db from the partial sums, rounded to the weight's dtype: 32 columns
+// and 32 slices of the groups per workgroup, the slices joined in order.
+constexpr uint32_t kFinalColumns = 32, kFinalSlices = 32;
+
 template <class T>
-__global__ __launch_bounds__(kBlock) void norm_finalize_kernel(const float *partials, uint32_t groups, uint32_t width,
-                                                               typename T::raw *dw, typename T::raw *db) {
-    const uint64_t c = (uint64_t)blockIdx.x * kBlock + threadIdx.x;
-    if (c >= 2u * (uint64_t)width) return;
-    typename T::raw *out = c < width ? dw : db;
-    if (out == nullptr) return;
+__global__ __launch_bounds__(kFinalColumns * kFinalSlices) void norm_finalize_kernel(const float *partials,
+                                                                                      uint32_t groups, uint32_t width,
+                                                                                      typename T::raw *dw,
+                                                                                      typename T::raw *db) {
+    __shared__ float shared[kFinalSlices][kFinalColumns + 1];
+    const uint32_t column = threadIdx.x % kFinalColumns, slice = threadIdx.x / kFinalColumns;
+    const uint64_t c = (uint64_t)blockIdx.x * kFinalColumns + column;
     float sum = 0.0f;
-    for (uint32_t k = 0; k < groups; ++k) sum += partials[(uint64_t)k * 2u * width + c];
-    store1<T>(out, c < width ? c : c - width, sum);
+    if (c < 2u * (uint64_t)width) {
+#pragma unroll 8
+        for (uint32_t k = slice; k < groups; k += kFinalSlices) sum += partials[(uint64_t)k * 2u * width + c];
+    }
+    shared[slice][column] = sum;
+    __syncthreads();
+    if (slice != 0 || c >= 2u * (uint64_t)width) return;
+    sum = 0.0f;
+#pragma unroll
+    for (uint32_t k = 0; k < kFinalSlices; ++k) sum += shared[k][column];
+    typename T::raw *out = c < width ? dw : db;
+    if (out != nullptr) store1<T>(out, c < width ? c : c - width, sum);
 }
 
 // ---- dropout over a flat tensor ----------------------------------------------------------------
-template <class T>
-__global__ __launch_bounds__(kBlock) void dropout_kernel(const typename T::raw *x, typename T::raw *y, uint64_t n,
-                                                         Mask mask) {
-    const uint64_t groups = (n + 7) >> 3;
-    for (uint64_t g = (uint64_t)blockIdx.x * kBlock + threadIdx.x; g < groups; g += (uint64_t)gridDim.x * kBlock) {
-        const PhiloxWords words = philox(g, mask.offset, mask.seed);
+constexpr int kDropGroups = 2;          // groups of eight per lane, a workgroup's width apart
+
+template <class T, bool EVEN>
+__global__ __launch_bounds__(kBlock) void dropout_kernel(const void *x, void *y, uint64_t n, Mask mask) {
+    constexpr uint64_t kDropTile = (uint64_t)kBlock * kGroup * kDropGroups;
+    for (uint64_t start = blockIdx.x * kDropTile; start < n; start += gridDim.x * kDropTile) {
+        Raw8<T> raw[kDropGroups];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const uint64_t i = (g << 3) + k;
-            if (i < n) {
-                const float v = load1<T>(x, i) * mask.factor;
-                store1<T>(y, i, philox_half(words, k) >= mask.threshold ? v : 0.0f);
-            }
+        for (int u = 0; u < kDropGroups; ++u) {
+            const uint64_t i = start + ((uint64_t)u * kBlock + threadIdx.x) * kGroup;
+            if (i + kGroup <= n) load8<T, EVEN>(raw[u], x, i);
+            else if (i < n) load_end<T>(raw[u], x, i, (uint32_t)(n - i));
+        }
+#pragma unroll
+        for (int u = 0; u < kDropGroups; ++u) {
+            const uint64_t i = start + ((uint64_t)u * kBlock + threadIdx.x) * kGroup;
+            if (i >= n) continue;
+            float v[8];
+            widen8<T>(v, raw[u]);
+            drop8(v, philox(i >> 3, mask.offset, mask.seed), mask);
+            narrow8<T>(raw[u], v);
+            if (i + kGroup <= n) store8<T, EVEN>(y, i, raw[u]);
+            else store_end<T>(y, i, raw[u], (uint32_t)(n - i));
         }
     }
 }
 
 // ---- launches ------------------------------------------------------------------------------------
-constexpr uint32_t kColumnGroups = 256;                 // row groups of the column sums
+constexpr uint32_t kColumnGroups = 256;                 // row groups of the column sums of rows past the tilings
 constexpr uint64_t kMaxPartials = 256ull << 20;         // bytes of their workspace
-constexpr uint64_t kMaxWidth = 1ull << 30;              // 2 width lanes of the finalize stay below 2**32
+constexpr uint64_t kMaxWidth = 1ull << 24;              // exact in float32, and the finalize stays below 2**32 lanes
+constexpr uint32_t kForwardGroups = 2048, kBackwardGroups = 768;       // workgroups of a launch that strides over rows
+
+// How a row is laid over lanes (norm_kernel); parts == 0: it does not fit.
+struct RowTiling {
+    uint32_t lanes, parts, threads;
+};
+
+static RowTiling row_tiling(uint32_t width) {
+    const uint32_t groups = (width + kGroup - 1) / kGroup;
+    RowTiling best{0, 0, 0};
+    for (uint32_t parts = 3; parts >= 1; --parts) {
+        uint32_t lanes = 1;
+        while (lanes * parts < groups) lanes <<= 1;
+        if (lanes > (uint32_t)kWideThreads || (lanes > (uint32_t)kRowThreads && parts > 2)) continue;
+        if (best.parts == 0 || lanes * parts < best.lanes * best.parts)
+            best = RowTiling{lanes, parts, lanes <= 64u ? (uint32_t)kRowThreads : lanes};
+    }
+    return best;
+}
+
+// Workgroups for `rows` rows, `per_block` at a time: at most `most`, all with
+// the same number of rounds but the last.
+static uint32_t row_grid(uint64_t rows, uint32_t per_block, uint32_t most) {
+    const uint64_t blocks = (rows + per_block - 1) / per_block;
+    if (blocks <= most) return blocks < 1 ? 1u : (uint32_t)blocks;
+    const uint64_t rounds = (blocks + most - 1) / most;
+    return (uint32_t)((blocks + rounds - 1) / rounds);
+}
 
 static uint32_t column_groups(uint64_t rows, uint64_t width) {
     uint64_t groups = rows < kColumnGroups ? rows : kColumnGroups;
@@ -215,39 +679,100 @@ static uint32_t column_groups(uint64_t rows, uint64_t width) {
     return groups < 1 ? 1u : (uint32_t)groups;
 }
 
-template <class T>
-static void launch_forward(const NormForward &a, int edge, hipStream_t s) {
-    const dim3 grid(strided_grid(a.rows, kBlock)), block(kBlock);
-    if (edge == kNone) norm_rows_kernel<T, kNone><<<grid, block, 0, s>>>(a);
-    else if (edge == kAdd) norm_rows_kernel<T, kAdd><<<grid, block, 0, s>>>(a);
-    else norm_rows_kernel<T, kDropAdd><<<grid, block, 0, s>>>(a);
+static uint32_t partial_groups(uint64_t rows, uint32_t width) {
+    const RowTiling tiling = row_tiling(width);
+    if (tiling.parts == 0) return column_groups(rows, width);
+    return row_grid(rows, tiling.threads / tiling.lanes, kBackwardGroups);
+}
+
+static bool aligned16(std::initializer_list<const void *> arrays) {
+    uintptr_t bits = 0;
+    for (const void *p : arrays) bits |= (uintptr_t)p;
+    return bits % 16 == 0;
+}
+
+template <class T, int EDGE, int PARTS, bool EVEN>
+static void launch_norm(const NormForward &a, const RowTiling &g, hipStream_t s) {
+    const dim3 grid(row_grid(a.rows, g.threads / g.lanes, kForwardGroups)), block(g.threads);
+    if (g.threads <= (uint32_t)kRowThreads)
+        norm_kernel<T, EDGE, PARTS, EVEN, kRowThreads><<<grid, block, 0, s>>>(a, g.lanes);
+    else if constexpr (PARTS <= 2) norm_kernel<T, EDGE, PARTS, EVEN, kWideThreads><<<grid, block, 0, s>>>(a, g.lanes);
+}
+
+template <class T, int EDGE, int PARTS, bool EVEN>
+static void launch_norm_backward(const NormBackward &a, const RowTiling &g, uint32_t groups, hipStream_t s) {
+    const dim3 grid(groups), block(g.threads);
+    if (g.threads <= (uint32_t)kRowThreads)
+        norm_backward_kernel<T, EDGE, PARTS, EVEN, kRowThreads><<<grid, block, 0, s>>>(a, g.lanes);
+    else if constexpr (PARTS <= 2)
+        norm_backward_kernel<T, EDGE, PARTS, EVEN, kWideThreads><<<grid, block, 0, s>>>(a, g.lanes);
+}
+
+// Calls launch(parts, even) with both as constants.
+template <class F>
+static void with_tiling(const RowTiling &g, bool even, F &&launch) {
+    using std::integral_constant;
+    const auto with_parts = [&](auto e) {
+        if (g.parts == 1) launch(integral_constant<int, 1>{}, e);
+        else if (g.parts == 2) launch(integral_constant<int, 2>{}, e);
+        else launch(integral_constant<int, 3>{}, e);
+    };
+    if (even) with_parts(integral_constant<bool, true>{});
+    else with_parts(integral_constant<bool, false>{});
+}
+
+template <class T, int EDGE>
+static void launch_forward_edge(const NormForward &a, hipStream_t s) {
+    const RowTiling g = row_tiling(a.width);
+    if (g.parts == 0) {
+        norm_rows_kernel<T, EDGE><<<dim3(strided_grid(a.rows, kBlock)), dim3(kBlock), 0, s>>>(a);
+        return;
+    }
+    const bool even = a.width % kGroup == 0 && aligned16({a.x, a.residual, a.total, a.y});
+    with_tiling(g, even, [&](auto parts, auto e) { launch_norm<T, EDGE, parts.value, e.value>(a, g, s); });
+}
+
+template <class T, int EDGE>
+static void launch_backward_edge(const NormBackward &a, uint32_t groups, hipStream_t s) {
+    const RowTiling g = row_tiling(a.width);
+    if (g.parts == 0) {
+        norm_rows_backward_kernel<T, EDGE><<<dim3(strided_grid(a.rows, kBlock)), dim3(kBlock), 0, s>>>(a);
+        if (a.partials != nullptr)
+            norm_columns_kernel<T><<<dim3((a.width + kBlock - 1) / kBlock, groups), dim3(kBlock), 0, s>>>(a);
+        return;
+    }
+    const bool even = a.width % kGroup == 0 && aligned16({a.dy, a.dtotal, a.t, a.dx, a.dresidual});
+    with_tiling(g, even,
+                [&](auto parts, auto e) { launch_norm_backward<T, EDGE, parts.value, e.value>(a, g, groups, s); });
 }
 
 template <class T>
-static void launch_backward(const NormBackward &a, int edge, bool columns, hipStream_t s) {
-    const dim3 grid(strided_grid(a.rows, kBlock)), block(kBlock);
-    if (edge == kNone) norm_rows_backward_kernel<T, kNone><<<grid, block, 0, s>>>(a);
-    else if (edge == kAdd) norm_rows_backward_kernel<T, kAdd><<<grid, block, 0, s>>>(a);
-    else norm_rows_backward_kernel<T, kDropAdd><<<grid, block, 0, s>>>(a);
-    if (columns) {
-        const dim3 tiles((a.width + kBlock - 1) / kBlock, column_groups(a.rows, a.width));
-        norm_columns_kernel<T><<<tiles, block, 0, s>>>(a);
-    }
+static void launch_forward(const NormForward &a, int edge, hipStream_t s) {
+    if (edge == kNone) launch_forward_edge<T, kNone>(a, s);
+    else if (edge == kAdd) launch_forward_edge<T, kAdd>(a, s);
+    else launch_forward_edge<T, kDropAdd>(a, s);
+}
+
+template <class T>
+static void launch_backward(const NormBackward &a, int edge, uint32_t groups, hipStream_t s) {
+    if (edge == kNone) launch_backward_edge<T, kNone>(a, groups, s);
+    else if (edge == kAdd) launch_backward_edge<T, kAdd>(a, groups, s);
+    else launch_backward_edge<T, kDropAdd>(a, groups, s);
 }
 
 template <class T>
 static void launch_finalize(const NormBackward &a, uint32_t groups, void *dw, void *db, hipStream_t s) {
-    const dim3 grid((unsigned)((2u * (uint64_t)a.width + kBlock - 1) / kBlock));
-    norm_finalize_kernel<T><<<grid, dim3(kBlock), 0, s>>>(a.partials, groups, a.width,
-                                                          static_cast<typename T::raw *>(dw),
-                                                          static_cast<typename T::raw *>(db));
+    const dim3 grid((unsigned)((2u * (uint64_t)a.width + kFinalColumns - 1) / kFinalColumns));
+    norm_finalize_kernel<T><<<grid, dim3(kFinalColumns * kFinalSlices), 0, s>>>(
+        a.partials, groups, a.width, static_cast<typename T::raw *>(dw), static_cast<typename T::raw *>(db));
 }
 
 template <class T>
 static void launch_dropout(const void *x, void *y, uint64_t n, const Mask &mask, hipStream_t s) {
-    const dim3 grid(strided_grid(((n + 7) / 8 + kBlock - 1) / kBlock, kBlock));
-    dropout_kernel<T><<<grid, dim3(kBlock), 0, s>>>(static_cast<const typename T::raw *>(x),
-                                                    static_cast<typename T::raw *>(y), n, mask);
+    const uint64_t tile = (uint64_t)kBlock * kGroup * kDropGroups;
+    const dim3 grid(strided_grid((n + tile - 1) / tile, kBlock)), block(kBlock);
+    if (aligned16({x, y})) dropout_kernel<T, true><<<grid, block, 0, s>>>(x, y, n, mask);
+    else dropout_kernel<T, false><<<grid, block, 0, s>>>(x, y, n, mask);
 }
 
 // ---- argument checks --------------------------------------------------------------------------------
@@ -259,7 +784,7 @@ static int32_t check_rows(const char *entry, int32_t dtype, int32_t weight_dtype
     if (!half_or_float(dtype)) return fail(NT_ERR_TYPE, name + ": activations must be float32, float16 or bfloat16");
     if (has_params && weight_dtype != dtype && weight_dtype != NT_F32)
         return fail(NT_ERR_TYPE, name + ": weight and bias must have the activations' dtype or float32");
-    if (width == 0 || width > kMaxWidth) return fail(NT_ERR_VALUE, name + ": the width must be 1..2**30");
+    if (width == 0 || width > kMaxWidth) return fail(NT_ERR_VALUE, name + ": the width must be 1..2**24");
     if (rows > 0xffffffffffffull / width) return fail(NT_ERR_VALUE, name + ": too many elements");
     if (threshold > 65536u) return fail(NT_ERR_VALUE, name + ": the drop threshold must be 0..65536");
     return NT_OK;
@@ -317,7 +842,7 @@ static int32_t backward(const char *entry, int32_t device, NormBackward a, int32
     if (!guard.ok()) return hip_check(guard.error(), "hipSetDevice");
     hipStream_t s = (hipStream_t)stream;
     const bool columns = dw != nullptr || db != nullptr;
-    const uint32_t groups = column_groups(a.rows, a.width);
+    const uint32_t groups = partial_groups(a.rows, a.width);
     void *workspace = nullptr;
     if (columns) {
         // The workspace goes back to the pool as soon as the kernels are queued: the pool reuses it on this
@@ -334,9 +859,9 @@ static int32_t backward(const char *entry, int32_t device, NormBackward a, int32
         a.partials = static_cast<float *>(workspace);
     }
     switch (dtype) {
-        case NT_F32: launch_backward<TF32>(a, edge, columns, s); break;
-        case NT_F16: launch_backward<TF16>(a, edge, columns, s); break;
-        default: launch_backward<TBF16>(a, edge, columns, s); break;
+        case NT_F32: launch_backward<TF32>(a, edge, groups, s); break;
+        case NT_F16: launch_backward<TF16>(a, edge, groups, s); break;
+        default: launch_backward<TBF16>(a, edge, groups, s); break;
     }
     hipError_t status = hipGetLastError();
     if (columns && status == hipSuccess) {
