@@ -100,13 +100,13 @@ template <class T> struct Raw8 {
     u32x4 w[kWords];
 };
 
-template <class T, bool EVEN>
+template <class T, bool EVEN, bool NT = false>
 __device__ __forceinline__ void load8(Raw8<T> &out, const void *base, uint64_t i) {
     const auto *p = reinterpret_cast<const typename T::raw *>(base) + i;
 #pragma unroll
     for (int k = 0; k < Raw8<T>::kWords; ++k) {
-        if constexpr (EVEN) out.w[k] = gload<true, u32x4, gu32x4>(p + k * 4);
-        else out.w[k] = gload<true, u32x4, gu32x4_any>(p + k * 4);
+        if constexpr (EVEN) out.w[k] = gload<NT, u32x4, gu32x4>(p + k * 4);
+        else out.w[k] = gload<NT, u32x4, gu32x4_any>(p + k * 4);
     }
 }
 
@@ -240,47 +240,74 @@ __device__ __forceinline__ void drop8(float (&v)[8], const PhiloxWords &words, c
 // waves and workgroups and need no barrier; wider ones have a workgroup of
 // their own.  The row is read once, all sums come from registers, and the
 // next row is on its way while this one is summed.
-constexpr int kRowThreads = 256;        // lanes of a workgroup of rows that are at most as wide
+constexpr int kRowThreads = 512;        // lanes of a workgroup of rows that are at most as wide
+constexpr int kBackwardThreads = 512;   // the same of the backward pass
 constexpr int kWideThreads = 1024;      // at most, for wider rows
 
 // Sum over the `lanes` lanes of a row, the same on each.  Rows of several
 // waves go through `shared`, of which consecutive sums use the two halves in
 // turn: a wave that writes a half again has passed the barrier of the sum in
 // between, which no wave reaches before it has read that half.
+//
+// Within a wave the halves of 2, 4, 8 and 16 lanes are exchanged by the
+// operand paths of the vector ALU (quad permutations, then mirrors: all lanes
+// of a half hold the same sum by then), those of 32 and 64 by the row swaps.
+template <int CTRL>
+__device__ __forceinline__ float add_moved(float v) {
+    return v + bits_f32((uint32_t)__builtin_amdgcn_mov_dpp((int)f32_bits(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float lanes_sum(float v, uint32_t lanes) {
+    if (lanes > 1u) v = add_moved<0xB1>(v);             // lane ^ 1
+    if (lanes > 2u) v = add_moved<0x4E>(v);             // lane ^ 2
+    if (lanes > 4u) v = add_moved<0x141>(v);            // 7 - lane of eight
+    if (lanes > 8u) v = add_moved<0x140>(v);            // 15 - lane of sixteen
+    if (lanes > 16u) {
+        const auto pair = __builtin_amdgcn_permlane16_swap(f32_bits(v), f32_bits(v), false, false);
+        v = bits_f32(pair[0]) + bits_f32(pair[1]);
+    }
+    if (lanes > 32u) {
+        const auto pair = __builtin_amdgcn_permlane32_swap(f32_bits(v), f32_bits(v), false, false);
+        v = bits_f32(pair[0]) + bits_f32(pair[1]);
+    }
+    return v;
+}
+
 template <int MAX_WAVES>
 struct RowSum {
     float (*shared)[MAX_WAVES];
     uint32_t lanes;
     uint32_t half = 0;
     __device__ __forceinline__ float operator()(float v) {
-#pragma unroll
-        for (uint32_t off = 1; off < 64u; off <<= 1)
-            if (off < lanes) v += __shfl_xor(v, (int)off, 64);
+        v = lanes_sum(v, lanes);
         if (lanes <= 64u) return v;
         float *slot = shared[half];
         half ^= 1u;
-        if ((threadIdx.x & 63u) == 0u) slot[threadIdx.x >> 6] = v;
+        const uint32_t wave = threadIdx.x >> 6, waves = lanes / 64u, first = wave & ~(waves - 1u);
+        if ((threadIdx.x & 63u) == 0u) slot[wave] = v;
         __syncthreads();
         float total = 0.0f;
-        for (uint32_t k = 0; k < lanes / 64u; ++k) total += slot[k];
+        for (uint32_t k = first; k < first + waves; ++k) total += slot[k];
         return total;
     }
 };
 
+// Waves per SIMD that the forward pass's registers leave room for.
+template <class T, int EDGE, int PARTS>
+constexpr int forward_waves() {
+    return EDGE == kNone && PARTS <= 2 && T::code != NT_F32 ? 8 : 4;
+}
+
 template <class T, int EDGE, int PARTS, bool EVEN, int THREADS>
-__global__ __launch_bounds__(THREADS) void norm_kernel(NormForward a, uint32_t lanes) {
+__global__ __launch_bounds__(THREADS, (forward_waves<T, EDGE, PARTS>())) void norm_kernel(NormForward a,
+                                                                                       uint32_t lanes) {
+    extern __shared__ float4 room[];                    // weight, then bias
     __shared__ float shared[2][THREADS / 64];
     RowSum<THREADS / 64> row_sum{shared, lanes};
-    const uint32_t lane = threadIdx.x & (lanes - 1u), in_block = threadIdx.x / lanes, per_block = blockDim.x / lanes;
+    const uint32_t lane = threadIdx.x & (lanes - 1u), in_block = threadIdx.x / lanes, per_block = THREADS / lanes;
     const float width = (float)a.width;
     uint32_t column[PARTS];
-    float weight[PARTS][8], bias[PARTS][8];
 #pragma unroll
-    for (int p = 0; p < PARTS; ++p) {
-        column[p] = ((uint32_t)p * lanes + lane) * kGroup;
-        load_params(weight[p], a.weight, a.weight_dtype, column[p], a.width, 1.0f);
-        load_params(bias[p], a.bias, a.weight_dtype, column[p], a.width, 0.0f);
-    }
+    for (int p = 0; p < PARTS; ++p) column[p] = ((uint32_t)p * lanes + lane) * kGroup;
     const uint64_t stride = (uint64_t)gridDim.x * per_block;
     uint64_t row = (uint64_t)blockIdx.x * per_block + in_block;
     Raw8<T> x[PARTS], r[PARTS];
@@ -292,14 +319,36 @@ __global__ __launch_bounds__(THREADS) void norm_kernel(NormForward a, uint32_t l
             if constexpr (EDGE != kNone) load_part<T, EVEN>(r[p], a.residual, which * a.width, column[p], a.width);
         }
     };
+    float w[PARTS][8], b[PARTS][8];                     // asked for first: they are there before the rows
+    if (in_block == 0u) {
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            load_params(w[p], a.weight, a.weight_dtype, column[p], a.width, 1.0f);
+            load_params(b[p], a.bias, a.weight_dtype, column[p], a.width, 0.0f);
+        }
+    }
     fetch(row);
-    for (; row < a.rows; row += stride) {
+    if (in_block == 0u) {
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                room[(2 * p + q) * lanes + lane] =
+                    make_float4(w[p][4 * q], w[p][4 * q + 1], w[p][4 * q + 2], w[p][4 * q + 3]);
+                room[(2 * PARTS + 2 * p + q) * lanes + lane] =
+                    make_float4(b[p][4 * q], b[p][4 * q + 1], b[p][4 * q + 2], b[p][4 * q + 3]);
+            }
+        }
+    }
+    __syncthreads();
+    for (uint64_t first = (uint64_t)blockIdx.x * per_block; first < a.rows; first += stride) {
         const uint64_t base = row * a.width;
+        const bool active = row < a.rows;
         float t[PARTS][8];
         float sum = 0.0f;
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
-            const bool mine = column[p] < a.width;
+            const bool mine = active && column[p] < a.width;
             if (mine) {
                 widen8<T>(t[p], x[p]);
                 if constexpr (EDGE == kDropAdd) drop8(t[p], numbers8<EVEN>(base + column[p], a.mask), a.mask);
@@ -312,7 +361,7 @@ __global__ __launch_bounds__(THREADS) void norm_kernel(NormForward a, uint32_t l
             }
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const bool in_row = EVEN ? mine : column[p] + (uint32_t)k < a.width;
+                const bool in_row = EVEN ? mine : mine && column[p] + (uint32_t)k < a.width;
                 t[p][k] = in_row ? t[p][k] : 0.0f;
                 sum += t[p][k];
             }
@@ -331,7 +380,7 @@ __global__ __launch_bounds__(THREADS) void norm_kernel(NormForward a, uint32_t l
         const float rstd = 1.0f / __builtin_sqrtf(row_sum(squares) / width + a.eps);
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
-            if (column[p] >= a.width) continue;
+            if (!active || column[p] >= a.width) continue;
             Raw8<T> out;
             if constexpr (EDGE != kNone) {
                 narrow8<T>(out, t[p]);
@@ -339,71 +388,109 @@ __global__ __launch_bounds__(THREADS) void norm_kernel(NormForward a, uint32_t l
             }
             float y[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) y[k] = __builtin_fmaf((t[p][k] - mean) * rstd, weight[p][k], bias[p][k]);
+            for (int q = 0; q < 2; ++q) {
+                const float4 w = room[(2 * p + q) * lanes + lane], b = room[(2 * PARTS + 2 * p + q) * lanes + lane];
+                y[4 * q] = __builtin_fmaf((t[p][4 * q] - mean) * rstd, w.x, b.x);
+                y[4 * q + 1] = __builtin_fmaf((t[p][4 * q + 1] - mean) * rstd, w.y, b.y);
+                y[4 * q + 2] = __builtin_fmaf((t[p][4 * q + 2] - mean) * rstd, w.z, b.z);
+                y[4 * q + 3] = __builtin_fmaf((t[p][4 * q + 3] - mean) * rstd, w.w, b.w);
+            }
             narrow8<T>(out, y);
             store_part<T, EVEN>(a.y, base, column[p], a.width, out);
         }
-        if (a.mean != nullptr && lane == 0) {
+        if (active && a.mean != nullptr && lane == 0) {
             a.mean[row] = mean;
             a.rstd[row] = rstd;
         }
+        row += stride;
     }
 }
 
+// Sums of two values over the lanes of a row, for workgroups that hold
+// several rows of more than a wave: as RowSum, with a slot per wave and half.
+template <int WAVES>
+struct RowSum2 {
+    float (*shared)[2][WAVES];
+    uint32_t lanes;
+    uint32_t half = 0;
+    __device__ __forceinline__ void operator()(float &u, float &v) {
+        u = lanes_sum(u, lanes);
+        v = lanes_sum(v, lanes);
+        if (lanes <= 64u) return;
+        float (*slot)[WAVES] = shared[half];
+        half ^= 1u;
+        const uint32_t wave = threadIdx.x >> 6, waves = lanes / 64u, first = wave & ~(waves - 1u);
+        if ((threadIdx.x & 63u) == 0u) {
+            slot[0][wave] = u;
+            slot[1][wave] = v;
+        }
+        __syncthreads();
+        u = v = 0.0f;
+        for (uint32_t k = first; k < first + waves; ++k) {
+            u += slot[0][k];
+            v += slot[1][k];
+        }
+    }
+};
+
 // The backward pass of the same tiling.  dw and db of a lane's columns stay
-// in registers over all rows of the workgroup; rows that share a workgroup
-// are joined at the end, and each workgroup writes one row of partial sums.
+// in registers over all rows of the workgroup; the rows that share a
+// workgroup are joined at the end, halving them in turn, and each workgroup
+// writes one row of partial sums.  Four waves per SIMD hide the loads (128
+// vector registers each), so no row is fetched ahead, and the weights wait in
+// LDS.  Every workgroup makes the same number of rounds; a round past the last
+// row reads zeros.
 template <class T, int EDGE, int PARTS, bool EVEN, int THREADS>
-__global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormBackward a, uint32_t lanes) {
-    __shared__ float shared[2][2 * (THREADS / 64)];
-    __shared__ float join[THREADS > kRowThreads ? 1 : PARTS * 16 * 64];
-    RowSum<2 * (THREADS / 64)> row_sum{shared, lanes};
-    const uint32_t lane = threadIdx.x & (lanes - 1u), in_block = threadIdx.x / lanes, per_block = blockDim.x / lanes;
+__global__ __launch_bounds__(THREADS, 4) void norm_backward_kernel(NormBackward a, uint32_t lanes) {
+    extern __shared__ float4 room[];                    // the weights, then the rows that are joined
+    __shared__ float shared[2][2][THREADS / 64];
+    RowSum2<THREADS / 64> row_sum{shared, lanes};
+    const uint32_t lane = threadIdx.x & (lanes - 1u), in_block = threadIdx.x / lanes, per_block = THREADS / lanes;
     const float width = (float)a.width;
     uint32_t column[PARTS];
-    float weight[PARTS][8], dw[PARTS][8], db[PARTS][8];
 #pragma unroll
-    for (int p = 0; p < PARTS; ++p) {
-        column[p] = ((uint32_t)p * lanes + lane) * kGroup;
-        load_params(weight[p], a.weight, a.weight_dtype, column[p], a.width, 1.0f);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) dw[p][k] = db[p][k] = 0.0f;
-    }
+    for (int p = 0; p < PARTS; ++p) column[p] = ((uint32_t)p * lanes + lane) * kGroup;
     const uint64_t stride = (uint64_t)gridDim.x * per_block;
     uint64_t row = (uint64_t)blockIdx.x * per_block + in_block;
-    Raw8<T> dy[PARTS], t[PARTS], dt[PARTS], next_dy[PARTS], next_t[PARTS], next_dt[PARTS];
-    float mean = 0.0f, rstd = 0.0f, next_mean = 0.0f, next_rstd = 0.0f;
-    const auto fetch = [&](uint64_t which) {
-        if (which >= a.rows) return;
-        next_mean = a.mean[which];
-        next_rstd = a.rstd[which];
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
-            if (column[p] >= a.width) continue;
-            load_part<T, EVEN>(next_dy[p], a.dy, which * a.width, column[p], a.width);
-            load_part<T, EVEN>(next_t[p], a.t, which * a.width, column[p], a.width);
-            if constexpr (EDGE != kNone)
-                if (a.dtotal != nullptr)
-                    load_part<T, EVEN>(next_dt[p], a.dtotal, which * a.width, column[p], a.width);
-        }
+    Raw8<T> dy[PARTS], t[PARTS], dt[PARTS];
+    const auto fetch = [&](uint64_t which, int p) {
+        if (which >= a.rows || column[p] >= a.width) return;
+        load_part<T, EVEN>(dy[p], a.dy, which * a.width, column[p], a.width);
+        load_part<T, EVEN>(t[p], a.t, which * a.width, column[p], a.width);
+        if constexpr (EDGE != kNone)
+            if (a.dtotal != nullptr) load_part<T, EVEN>(dt[p], a.dtotal, which * a.width, column[p], a.width);
     };
-    fetch(row);
-    for (; row < a.rows; row += stride) {
-        const uint64_t base = row * a.width;
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
-            dy[p] = next_dy[p];
-            t[p] = next_t[p];
-            dt[p] = next_dt[p];
+    for (int p = 0; p < PARTS; ++p) fetch(row, p);
+    float next_mean = row < a.rows ? a.mean[row] : 0.0f, next_rstd = row < a.rows ? a.rstd[row] : 0.0f;
+    float dw[PARTS][8], db[PARTS][8];
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) dw[p][k] = db[p][k] = 0.0f;
+        if (in_block == 0u) {
+            float w[8];
+            load_params(w, a.weight, a.weight_dtype, column[p], a.width, 1.0f);
+            room[(2 * p) * lanes + lane] = make_float4(w[0], w[1], w[2], w[3]);
+            room[(2 * p + 1) * lanes + lane] = make_float4(w[4], w[5], w[6], w[7]);
         }
-        mean = next_mean;
-        rstd = next_rstd;
-        fetch(row + stride);
+    }
+    __syncthreads();
+    const auto weights = [&](float (&w)[8], int p) {
+        const float4 low = room[(2 * p) * lanes + lane], high = room[(2 * p + 1) * lanes + lane];
+        w[0] = low.x; w[1] = low.y; w[2] = low.z; w[3] = low.w;
+        w[4] = high.x; w[5] = high.y; w[6] = high.z; w[7] = high.w;
+    };
+    for (uint64_t first = (uint64_t)blockIdx.x * per_block; first < a.rows; first += stride) {
+        const uint64_t base = row * a.width, next = row + stride;
+        const bool active = row < a.rows;
+        const float mean = next_mean, rstd = next_rstd;
         float level = 0.0f, along = 0.0f;
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
-            if (column[p] >= a.width) continue;
-            float g[8], h[8];
+            if (!active || column[p] >= a.width) continue;
+            float g[8], h[8], w[8];
+            weights(w, p);
             widen8<T>(g, dy[p]);
             widen8<T>(h, t[p]);
 #pragma unroll
@@ -412,29 +499,37 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormBackward a, 
                 h[k] = EVEN || column[p] + (uint32_t)k < a.width ? (h[k] - mean) * rstd : 0.0f;
                 dw[p][k] = __builtin_fmaf(g[k], h[k], dw[p][k]);
                 db[p][k] += g[k];
-                g[k] *= weight[p][k];
+                g[k] *= w[k];
                 level += g[k];
                 along = __builtin_fmaf(g[k], h[k], along);
             }
         }
-        level = row_sum(level) / width;
-        along = row_sum(along) / width;
+        if (next < a.rows) {
+            next_mean = a.mean[next];
+            next_rstd = a.rstd[next];
+        }
+        row_sum(level, along);
+        level /= width;
+        along /= width;
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
-            if (column[p] >= a.width) continue;
-            float g[8], h[8];
+            if (!active || column[p] >= a.width) continue;
+            float g[8], h[8], w[8];
+            weights(w, p);
             widen8<T>(g, dy[p]);
             widen8<T>(h, t[p]);
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                g[k] = rstd * (g[k] * weight[p][k] - level - (h[k] - mean) * rstd * along);
-            Raw8<T> out;
+            for (int k = 0; k < 8; ++k) g[k] = rstd * (g[k] * w[k] - level - (h[k] - mean) * rstd * along);
             if constexpr (EDGE != kNone) {
                 if (a.dtotal != nullptr) {
                     widen8<T>(h, dt[p]);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) g[k] += h[k];
                 }
+            }
+            fetch(next, p);                             // into the registers that were just read
+            Raw8<T> out;
+            if constexpr (EDGE != kNone) {
                 narrow8<T>(out, g);
                 store_part<T, EVEN>(a.dresidual, base, column[p], a.width, out);
                 if constexpr (EDGE == kDropAdd) drop8(g, numbers8<EVEN>(base + column[p], a.mask), a.mask);
@@ -442,53 +537,52 @@ __global__ __launch_bounds__(THREADS) void norm_backward_kernel(NormBackward a, 
             narrow8<T>(out, g);
             store_part<T, EVEN>(a.dx, base, column[p], a.width, out);
         }
+        row = next;
     }
     if (a.partials == nullptr) return;
-    if constexpr (THREADS <= kRowThreads) {
-        if (lanes <= 64u) {
+    const auto each = [&](auto &&use) {                 // the lane's sums, four at a time
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    for (uint32_t off = lanes; off < 64u; off <<= 1) {
-                        dw[p][k] += __shfl_xor(dw[p][k], (int)off, 64);
-                        db[p][k] += __shfl_xor(db[p][k], (int)off, 64);
-                    }
-                }
-            const uint32_t wave = threadIdx.x >> 6, waves = blockDim.x >> 6, at = threadIdx.x & 63u;
-            for (uint32_t k = 0; k + 1u < waves; ++k) {          // wave k hands its sums to wave k + 1
-                if (wave == k) {
-#pragma unroll
-                    for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            join[(p * 16 + j) * 64 + at] = dw[p][j];
-                            join[(p * 16 + 8 + j) * 64 + at] = db[p][j];
-                        }
-                }
-                __syncthreads();
-                if (wave == k + 1u) {
-#pragma unroll
-                    for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            dw[p][j] += join[(p * 16 + j) * 64 + at];
-                            db[p][j] += join[(p * 16 + 8 + j) * 64 + at];
-                        }
-                }
-            }
-            if (wave + 1u != waves || at >= lanes) return;
+        for (int p = 0; p < PARTS; ++p) {
+            use(4 * p, dw[p][0], dw[p][1], dw[p][2], dw[p][3]);
+            use(4 * p + 1, dw[p][4], dw[p][5], dw[p][6], dw[p][7]);
+            use(4 * p + 2, db[p][0], db[p][1], db[p][2], db[p][3]);
+            use(4 * p + 3, db[p][4], db[p][5], db[p][6], db[p][7]);
         }
+    };
+    for (uint32_t off = lanes; off < 64u; off <<= 1)    // rows of one wave
+        each([&](int, float &x, float &y, float &z, float &w) {
+            x += __shfl_xor(x, (int)off, 64);
+            y += __shfl_xor(y, (int)off, 64);
+            z += __shfl_xor(z, (int)off, 64);
+            w += __shfl_xor(w, (int)off, 64);
+        });
+    const uint32_t span = lanes < 64u ? 64u : lanes, member = threadIdx.x / span, at = threadIdx.x & (span - 1u);
+    for (uint32_t half = THREADS / span / 2u; half > 0u; half >>= 1) {
+        __syncthreads();                                // the weights, or the last half, are read
+        if (member >= half && member < 2u * half && at < lanes)
+            each([&](int q, float x, float y, float z, float w) {
+                room[((member - half) * 4 * PARTS + q) * lanes + at] = make_float4(x, y, z, w);
+            });
+        __syncthreads();
+        if (member < half && at < lanes)
+            each([&](int q, float &x, float &y, float &z, float &w) {
+                const float4 other = room[(member * 4 * PARTS + q) * lanes + at];
+                x += other.x;
+                y += other.y;
+                z += other.z;
+                w += other.w;
+            });
     }
+    if (member != 0u || at >= lanes) return;
     float *out = a.partials + (uint64_t)blockIdx.x * 2u * a.width;
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) {
-#pragma unroll
-        for (uint32_t k = 0; k < 8; ++k) {
-            if (column[p] + k >= a.width) continue;
-            out[column[p] + k] = dw[p][k];
-            out[a.width + column[p] + k] = db[p][k];
-        }
+        if (column[p] >= a.width) continue;
+        Raw8<TF32> sums;
+        narrow8<TF32>(sums, dw[p]);
+        store_part<TF32, false>(out, 0, column[p], a.width, sums);
+        narrow8<TF32>(sums, db[p]);
+        store_part<TF32, false>(out + a.width, 0, column[p], a.width, sums);
     }
 }
 
@@ -612,9 +706,10 @@ __global__ __launch_bounds__(kFinalColumns * kFinalSlices) void norm_finalize_ke
 }
 
 // ---- dropout over a flat tensor ----------------------------------------------------------------
+constexpr uint64_t kCachedBytes = 64ull << 20;
 constexpr int kDropGroups = 2;          // groups of eight per lane, a workgroup's width apart
 
-template <class T, bool EVEN>
+template <class T, bool EVEN, bool NT>
 __global__ __launch_bounds__(kBlock) void dropout_kernel(const void *x, void *y, uint64_t n, Mask mask) {
     constexpr uint64_t kDropTile = (uint64_t)kBlock * kGroup * kDropGroups;
     for (uint64_t start = blockIdx.x * kDropTile; start < n; start += gridDim.x * kDropTile) {
@@ -622,7 +717,7 @@ __global__ __launch_bounds__(kBlock) void dropout_kernel(const void *x, void *y,
 #pragma unroll
         for (int u = 0; u < kDropGroups; ++u) {
             const uint64_t i = start + ((uint64_t)u * kBlock + threadIdx.x) * kGroup;
-            if (i + kGroup <= n) load8<T, EVEN>(raw[u], x, i);
+            if (i + kGroup <= n) load8<T, EVEN, NT>(raw[u], x, i);
             else if (i < n) load_end<T>(raw[u], x, i, (uint32_t)(n - i));
         }
 #pragma unroll
@@ -643,24 +738,53 @@ __global__ __launch_bounds__(kBlock) void dropout_kernel(const void *x, void *y,
 constexpr uint32_t kColumnGroups = 256;                 // row groups of the column sums of rows past the tilings
 constexpr uint64_t kMaxPartials = 256ull << 20;         // bytes of their workspace
 constexpr uint64_t kMaxWidth = 1ull << 24;              // exact in float32, and the finalize stays below 2**32 lanes
-constexpr uint32_t kForwardGroups = 2048, kBackwardGroups = 768;       // workgroups of a launch that strides over rows
+constexpr uint32_t kSimds = 256 * 4;                    // launches stride over rows with as many waves as are resident
+constexpr uint32_t kBackwardWaves = 4;                  // per SIMD
+constexpr uint64_t kFewLanes = 256 * 64 * 4;
 
-// How a row is laid over lanes (norm_kernel); parts == 0: it does not fit.
+// How a row is laid over lanes; parts == 0: it does not fit.
 struct RowTiling {
     uint32_t lanes, parts, threads;
 };
 
-static RowTiling row_tiling(uint32_t width) {
+// The forward pass: the tiling that leaves the fewest lanes idle, of equals
+// the one with the fewest lanes.  Where the rows do not fill the chip, one
+// group a lane: a row's latency counts, not its share of a workgroup.
+static RowTiling forward_tiling(uint64_t rows, uint32_t width, int32_t dtype) {
     const uint32_t groups = (width + kGroup - 1) / kGroup;
     RowTiling best{0, 0, 0};
-    for (uint32_t parts = 3; parts >= 1; --parts) {
+    for (uint32_t parts = dtype == NT_F32 ? 2 : 3; parts >= 1; --parts) {
         uint32_t lanes = 1;
         while (lanes * parts < groups) lanes <<= 1;
         if (lanes > (uint32_t)kWideThreads || (lanes > (uint32_t)kRowThreads && parts > 2)) continue;
-        if (best.parts == 0 || lanes * parts < best.lanes * best.parts)
-            best = RowTiling{lanes, parts, lanes <= 64u ? (uint32_t)kRowThreads : lanes};
+        const bool few = parts == 1 && rows * lanes <= kFewLanes;
+        if (best.parts == 0 || few || lanes * parts < best.lanes * best.parts)
+            best = RowTiling{lanes, parts, lanes <= (uint32_t)kRowThreads ? (uint32_t)kRowThreads : (uint32_t)kWideThreads};
     }
     return best;
+}
+
+// The backward pass: as above among what 128 registers a lane hold (three
+// groups of a 16-bit type, two of float32), in workgroups of kBackwardThreads.
+static RowTiling backward_tiling(uint32_t width, int32_t dtype) {
+    const uint32_t groups = (width + kGroup - 1) / kGroup;
+    RowTiling best{0, 0, 0};
+    for (uint32_t parts = 2; parts >= 1; --parts) {
+        uint32_t lanes = 1;
+        while (lanes * parts < groups) lanes <<= 1;
+        if (lanes > (uint32_t)kWideThreads) continue;
+        if (best.parts == 0 || lanes * parts < best.lanes * best.parts || dtype == NT_F32)
+            best = RowTiling{lanes, parts, lanes <= (uint32_t)kBackwardThreads ? (uint32_t)kBackwardThreads : lanes};
+    }
+    return best;
+}
+
+// LDS of norm_backward_kernel: the weights, or half of the rows that are joined.
+static uint32_t backward_room(const RowTiling &g) {
+    const uint32_t span = g.lanes < 64u ? 64u : g.lanes;
+    const uint32_t weights = g.lanes * g.parts * kGroup * 4u;
+    const uint32_t joined = g.threads / span / 2u * g.lanes * g.parts * 2u * kGroup * 4u;
+    return weights > joined ? weights : joined;
 }
 
 // Workgroups for `rows` rows, `per_block` at a time: at most `most`, all with
@@ -679,10 +803,10 @@ static uint32_t column_groups(uint64_t rows, uint64_t width) {
     return groups < 1 ? 1u : (uint32_t)groups;
 }
 
-static uint32_t partial_groups(uint64_t rows, uint32_t width) {
-    const RowTiling tiling = row_tiling(width);
-    if (tiling.parts == 0) return column_groups(rows, width);
-    return row_grid(rows, tiling.threads / tiling.lanes, kBackwardGroups);
+static uint32_t partial_groups(uint64_t rows, uint32_t width, int32_t dtype) {
+    const RowTiling g = backward_tiling(width, dtype);
+    if (g.parts == 0) return column_groups(rows, width);
+    return row_grid(rows, g.threads / g.lanes, kSimds * kBackwardWaves * 64u / g.threads);
 }
 
 static bool aligned16(std::initializer_list<const void *> arrays) {
@@ -693,29 +817,31 @@ static bool aligned16(std::initializer_list<const void *> arrays) {
 
 template <class T, int EDGE, int PARTS, bool EVEN>
 static void launch_norm(const NormForward &a, const RowTiling &g, hipStream_t s) {
-    const dim3 grid(row_grid(a.rows, g.threads / g.lanes, kForwardGroups)), block(g.threads);
-    if (g.threads <= (uint32_t)kRowThreads)
-        norm_kernel<T, EDGE, PARTS, EVEN, kRowThreads><<<grid, block, 0, s>>>(a, g.lanes);
-    else if constexpr (PARTS <= 2) norm_kernel<T, EDGE, PARTS, EVEN, kWideThreads><<<grid, block, 0, s>>>(a, g.lanes);
+    const dim3 grid(row_grid(a.rows, g.threads / g.lanes,
+                                   (uint32_t)(kSimds * forward_waves<T, EDGE, PARTS>()) * 64u / g.threads)), block(g.threads);
+    const uint32_t room = g.lanes * g.parts * kGroup * 8u;
+    if (g.threads == (uint32_t)kRowThreads)
+        norm_kernel<T, EDGE, PARTS, EVEN, kRowThreads><<<grid, block, room, s>>>(a, g.lanes);
+    else if constexpr (PARTS <= 2) norm_kernel<T, EDGE, PARTS, EVEN, kWideThreads><<<grid, block, room, s>>>(a, g.lanes);
 }
 
 template <class T, int EDGE, int PARTS, bool EVEN>
 static void launch_norm_backward(const NormBackward &a, const RowTiling &g, uint32_t groups, hipStream_t s) {
     const dim3 grid(groups), block(g.threads);
-    if (g.threads <= (uint32_t)kRowThreads)
-        norm_backward_kernel<T, EDGE, PARTS, EVEN, kRowThreads><<<grid, block, 0, s>>>(a, g.lanes);
-    else if constexpr (PARTS <= 2)
-        norm_backward_kernel<T, EDGE, PARTS, EVEN, kWideThreads><<<grid, block, 0, s>>>(a, g.lanes);
+    const uint32_t room = backward_room(g);
+    if (g.threads == (uint32_t)kBackwardThreads)
+        norm_backward_kernel<T, EDGE, PARTS, EVEN, kBackwardThreads><<<grid, block, room, s>>>(a, g.lanes);
+    else norm_backward_kernel<T, EDGE, PARTS, EVEN, kWideThreads><<<grid, block, room, s>>>(a, g.lanes);
 }
 
 // Calls launch(parts, even) with both as constants.
-template <class F>
+template <int MAX_PARTS, class F>
 static void with_tiling(const RowTiling &g, bool even, F &&launch) {
     using std::integral_constant;
     const auto with_parts = [&](auto e) {
         if (g.parts == 1) launch(integral_constant<int, 1>{}, e);
         else if (g.parts == 2) launch(integral_constant<int, 2>{}, e);
-        else launch(integral_constant<int, 3>{}, e);
+        else if constexpr (MAX_PARTS > 2) launch(integral_constant<int, 3>{}, e);
     };
     if (even) with_parts(integral_constant<bool, true>{});
     else with_parts(integral_constant<bool, false>{});
@@ -723,18 +849,19 @@ static void with_tiling(const RowTiling &g, bool even, F &&launch) {
 
 template <class T, int EDGE>
 static void launch_forward_edge(const NormForward &a, hipStream_t s) {
-    const RowTiling g = row_tiling(a.width);
+    const RowTiling g = forward_tiling(a.rows, a.width, T::code);
     if (g.parts == 0) {
         norm_rows_kernel<T, EDGE><<<dim3(strided_grid(a.rows, kBlock)), dim3(kBlock), 0, s>>>(a);
         return;
     }
     const bool even = a.width % kGroup == 0 && aligned16({a.x, a.residual, a.total, a.y});
-    with_tiling(g, even, [&](auto parts, auto e) { launch_norm<T, EDGE, parts.value, e.value>(a, g, s); });
+    with_tiling<T::code == NT_F32 ? 2 : 3>(
+        g, even, [&](auto parts, auto e) { launch_norm<T, EDGE, parts.value, e.value>(a, g, s); });
 }
 
 template <class T, int EDGE>
 static void launch_backward_edge(const NormBackward &a, uint32_t groups, hipStream_t s) {
-    const RowTiling g = row_tiling(a.width);
+    const RowTiling g = backward_tiling(a.width, T::code);
     if (g.parts == 0) {
         norm_rows_backward_kernel<T, EDGE><<<dim3(strided_grid(a.rows, kBlock)), dim3(kBlock), 0, s>>>(a);
         if (a.partials != nullptr)
@@ -742,8 +869,8 @@ static void launch_backward_edge(const NormBackward &a, uint32_t groups, hipStre
         return;
     }
     const bool even = a.width % kGroup == 0 && aligned16({a.dy, a.dtotal, a.t, a.dx, a.dresidual});
-    with_tiling(g, even,
-                [&](auto parts, auto e) { launch_norm_backward<T, EDGE, parts.value, e.value>(a, g, groups, s); });
+    with_tiling<2>(g, even,
+                   [&](auto parts, auto e) { launch_norm_backward<T, EDGE, parts.value, e.value>(a, g, groups, s); });
 }
 
 template <class T>
@@ -771,8 +898,11 @@ template <class T>
 static void launch_dropout(const void *x, void *y, uint64_t n, const Mask &mask, hipStream_t s) {
     const uint64_t tile = (uint64_t)kBlock * kGroup * kDropGroups;
     const dim3 grid(strided_grid((n + tile - 1) / tile, kBlock)), block(kBlock);
-    if (aligned16({x, y})) dropout_kernel<T, true><<<grid, block, 0, s>>>(x, y, n, mask);
-    else dropout_kernel<T, false><<<grid, block, 0, s>>>(x, y, n, mask);
+    const bool even = aligned16({x, y}), past = n * sizeof(typename T::raw) > kCachedBytes;
+    if (even && past) dropout_kernel<T, true, true><<<grid, block, 0, s>>>(x, y, n, mask);
+    else if (even) dropout_kernel<T, true, false><<<grid, block, 0, s>>>(x, y, n, mask);
+    else if (past) dropout_kernel<T, false, true><<<grid, block, 0, s>>>(x, y, n, mask);
+    else dropout_kernel<T, false, false><<<grid, block, 0, s>>>(x, y, n, mask);
 }
 
 // ---- argument checks --------------------------------------------------------------------------------
@@ -842,7 +972,7 @@ static int32_t backward(const char *entry, int32_t device, NormBackward a, int32
     if (!guard.ok()) return hip_check(guard.error(), "hipSetDevice");
     hipStream_t s = (hipStream_t)stream;
     const bool columns = dw != nullptr || db != nullptr;
-    const uint32_t groups = partial_groups(a.rows, a.width);
+    const uint32_t groups = partial_groups(a.rows, a.width, dtype);
     void *workspace = nullptr;
     if (columns) {
         // The workspace goes back to the pool as soon as the kernels are queued: the pool reuses it on this
