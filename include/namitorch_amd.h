@@ -551,8 +551,9 @@ int32_t nt_any_negative(const void *array, int32_t dtype, uint64_t count,
  * once, when stored.  A row holding an infinity or NaN gives NaN outputs.
  * Outputs overlap neither inputs nor one another.  Work is queued on
  * `stream` of `device`; the backward entries take their workspace from the
- * library's pool in that stream's order and refuse (NT_ERR_RUNTIME) a stream
- * in capture when they need it.  With no rows the forward entries do
+ * library's pool in that stream's order.  They, and what draws a mask, refuse
+ * (NT_ERR_RUNTIME) a stream in capture: a replay would use a workspace handed
+ * to others since, or repeat the mask.  With no rows the forward entries do
  * nothing, the backward entries write zero dweight and dbias.
  */
 int32_t nt_layer_norm(int32_t device, const void *x, int32_t dtype, const void *weight,

@@ -15,6 +15,7 @@
 // change from run to run.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <initializer_list>
 #include <type_traits>
 
@@ -42,11 +43,13 @@ struct NormBackward {
     const void *dy, *dtotal, *t, *weight;
     const float *mean, *rstd;
     void *dx, *dresidual;       // the edge writes both, the norm dx alone
-    float *partials;            // [groups][2][width]
+    float *partials;            // [row_blocks][2][width], or null
     uint64_t rows;
     uint32_t width;
     int32_t weight_dtype;
     Mask mask;
+    uint32_t row_blocks;        // workgroups of the launch that take rows; the others take columns (few rows)
+    void *dw, *db;              // what those write
 };
 
 __device__ __forceinline__ float load_param(const void *base, int32_t dtype, uint64_t i, float absent) {
@@ -433,24 +436,87 @@ struct RowSum2 {
     }
 };
 
+__device__ __forceinline__ void store_param(void *base, int32_t dtype, uint64_t i, float v) {
+    switch (dtype) {
+        case NT_F32: reinterpret_cast<float *>(base)[i] = v; break;
+        case NT_F16: reinterpret_cast<uint16_t *>(base)[i] = f32_to_f16(v); break;
+        default: reinterpret_cast<uint16_t *>(base)[i] = f32_to_bf16(v); break;
+    }
+}
+
+// dw and db of 64 columns over all rows: eight lanes to a row's columns, the
+// rows over the rest of the workgroup, joined in a fixed order.
+template <class T, bool EVEN, int THREADS>
+__device__ __forceinline__ void column_tile(const NormBackward &a, uint32_t tile, float4 *room) {
+    const uint32_t c = tile * 64u + (threadIdx.x & 7u) * kGroup;
+    float dw[8] = {}, db[8] = {};
+    if (c < a.width) {
+#pragma unroll 2
+        for (uint64_t row = threadIdx.x >> 3; row < a.rows; row += THREADS / 8) {
+            Raw8<T> dy, t;
+            load_part<T, EVEN>(dy, a.dy, row * a.width, c, a.width);
+            load_part<T, EVEN>(t, a.t, row * a.width, c, a.width);
+            const float mean = a.mean[row], rstd = a.rstd[row];
+            float g[8], h[8];
+            widen8<T>(g, dy);
+            widen8<T>(h, t);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                dw[k] = __builtin_fmaf(g[k], (h[k] - mean) * rstd, dw[k]);
+                db[k] += g[k];
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+#pragma unroll
+        for (int off = 8; off < 64; off <<= 1) {
+            dw[k] += __shfl_xor(dw[k], off, 64);
+            db[k] += __shfl_xor(db[k], off, 64);
+        }
+    }
+    float *sums = reinterpret_cast<float *>(room);      // [wave][dw, db][64]
+    if ((threadIdx.x & 63u) < 8u) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            sums[(threadIdx.x >> 6) * 128u + (threadIdx.x & 7u) * 8u + k] = dw[k];
+            sums[(threadIdx.x >> 6) * 128u + 64u + (threadIdx.x & 7u) * 8u + k] = db[k];
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x >= 128u) return;
+    float sum = 0.0f;
+#pragma unroll
+    for (uint32_t k = 0; k < THREADS / 64; ++k) sum += sums[k * 128u + threadIdx.x];
+    const uint32_t column = tile * 64u + (threadIdx.x & 63u);
+    void *out = threadIdx.x < 64u ? a.dw : a.db;
+    if (out != nullptr && column < a.width) store_param(out, a.weight_dtype, column, sum);
+}
+
 // The backward pass of the same tiling.  dw and db of a lane's columns stay
 // in registers over all rows of the workgroup; the rows that share a
 // workgroup are joined at the end, halving them in turn, and each workgroup
 // writes one row of partial sums.  Four waves per SIMD hide the loads (128
 // vector registers each), so no row is fetched ahead, and the weights wait in
 // LDS.  Every workgroup makes the same number of rounds; a round past the last
-// row reads zeros.
+// row reads zeros.  With few rows, partial sums would be as large as the rows
+// themselves: then workgroups of the same launch take columns instead, and
+// read the rows once more from the caches.
 template <class T, int EDGE, int PARTS, bool EVEN, int THREADS>
 __global__ __launch_bounds__(THREADS, 4) void norm_backward_kernel(NormBackward a, uint32_t lanes) {
     extern __shared__ float4 room[];                    // the weights, then the rows that are joined
     __shared__ float shared[2][2][THREADS / 64];
+    if (blockIdx.x >= a.row_blocks) {
+        column_tile<T, EVEN, THREADS>(a, blockIdx.x - a.row_blocks, room);
+        return;
+    }
     RowSum2<THREADS / 64> row_sum{shared, lanes};
     const uint32_t lane = threadIdx.x & (lanes - 1u), in_block = threadIdx.x / lanes, per_block = THREADS / lanes;
     const float width = (float)a.width;
     uint32_t column[PARTS];
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) column[p] = ((uint32_t)p * lanes + lane) * kGroup;
-    const uint64_t stride = (uint64_t)gridDim.x * per_block;
+    const uint64_t stride = (uint64_t)a.row_blocks * per_block;
     uint64_t row = (uint64_t)blockIdx.x * per_block + in_block;
     Raw8<T> dy[PARTS], t[PARTS], dt[PARTS];
     const auto fetch = [&](uint64_t which, int p) {
@@ -740,6 +806,7 @@ constexpr uint64_t kMaxPartials = 256ull << 20;         // bytes of their worksp
 constexpr uint64_t kMaxWidth = 1ull << 24;              // exact in float32, and the finalize stays below 2**32 lanes
 constexpr uint32_t kSimds = 256 * 4;                    // launches stride over rows with as many waves as are resident
 constexpr uint32_t kBackwardWaves = 4;                  // per SIMD
+constexpr uint64_t kFewRows = 512;
 constexpr uint64_t kFewLanes = 256 * 64 * 4;
 
 // How a row is laid over lanes; parts == 0: it does not fit.
@@ -759,7 +826,7 @@ static RowTiling forward_tiling(uint64_t rows, uint32_t width, int32_t dtype) {
         if (lanes > (uint32_t)kWideThreads || (lanes > (uint32_t)kRowThreads && parts > 2)) continue;
         const bool few = parts == 1 && rows * lanes <= kFewLanes;
         if (best.parts == 0 || few || lanes * parts < best.lanes * best.parts)
-            best = RowTiling{lanes, parts, lanes <= (uint32_t)kRowThreads ? (uint32_t)kRowThreads : (uint32_t)kWideThreads};
+            best = RowTiling{lanes, parts, uint32_t(lanes <= (uint32_t)kRowThreads ? kRowThreads : kWideThreads)};
     }
     return best;
 }
@@ -774,18 +841,23 @@ static RowTiling backward_tiling(uint32_t width, int32_t dtype) {
         while (lanes * parts < groups) lanes <<= 1;
         if (lanes > (uint32_t)kWideThreads) continue;
         if (best.parts == 0 || lanes * parts < best.lanes * best.parts || dtype == NT_F32)
-            best = RowTiling{lanes, parts, lanes <= (uint32_t)kBackwardThreads ? (uint32_t)kBackwardThreads : lanes};
+            best = RowTiling{lanes, parts, uint32_t(lanes <= (uint32_t)kBackwardThreads ? kBackwardThreads : kWideThreads)};
     }
     return best;
 }
 
-// LDS of norm_backward_kernel: the weights, or half of the rows that are joined.
+// LDS of norm_backward_kernel: the weights, half of the rows that are joined,
+// or a column tile's sums of each wave.
 static uint32_t backward_room(const RowTiling &g) {
     const uint32_t span = g.lanes < 64u ? 64u : g.lanes;
     const uint32_t weights = g.lanes * g.parts * kGroup * 4u;
     const uint32_t joined = g.threads / span / 2u * g.lanes * g.parts * 2u * kGroup * 4u;
-    return weights > joined ? weights : joined;
+    const uint32_t tile = g.threads / 64u * 128u * 4u;
+    return std::max(weights, std::max(joined, tile));
 }
+
+// Whether the backward launch of `rows` rows sums columns in workgroups of its own.
+static bool takes_columns(uint64_t rows, const RowTiling &g) { return g.parts != 0 && rows <= kFewRows; }
 
 // Workgroups for `rows` rows, `per_block` at a time: at most `most`, all with
 // the same number of rounds but the last.
@@ -817,17 +889,19 @@ static bool aligned16(std::initializer_list<const void *> arrays) {
 
 template <class T, int EDGE, int PARTS, bool EVEN>
 static void launch_norm(const NormForward &a, const RowTiling &g, hipStream_t s) {
-    const dim3 grid(row_grid(a.rows, g.threads / g.lanes,
-                                   (uint32_t)(kSimds * forward_waves<T, EDGE, PARTS>()) * 64u / g.threads)), block(g.threads);
+    constexpr uint32_t waves = kSimds * (uint32_t)forward_waves<T, EDGE, PARTS>();
+    const dim3 grid(row_grid(a.rows, g.threads / g.lanes, waves * 64u / g.threads)), block(g.threads);
     const uint32_t room = g.lanes * g.parts * kGroup * 8u;
     if (g.threads == (uint32_t)kRowThreads)
         norm_kernel<T, EDGE, PARTS, EVEN, kRowThreads><<<grid, block, room, s>>>(a, g.lanes);
-    else if constexpr (PARTS <= 2) norm_kernel<T, EDGE, PARTS, EVEN, kWideThreads><<<grid, block, room, s>>>(a, g.lanes);
+    else if constexpr (PARTS <= 2)
+        norm_kernel<T, EDGE, PARTS, EVEN, kWideThreads><<<grid, block, room, s>>>(a, g.lanes);
 }
 
 template <class T, int EDGE, int PARTS, bool EVEN>
-static void launch_norm_backward(const NormBackward &a, const RowTiling &g, uint32_t groups, hipStream_t s) {
-    const dim3 grid(groups), block(g.threads);
+static void launch_norm_backward(const NormBackward &a, const RowTiling &g, hipStream_t s) {
+    const bool columns = a.partials == nullptr && (a.dw != nullptr || a.db != nullptr);
+    const dim3 grid(a.row_blocks + (columns ? (a.width + 63u) / 64u : 0u)), block(g.threads);
     const uint32_t room = backward_room(g);
     if (g.threads == (uint32_t)kBackwardThreads)
         norm_backward_kernel<T, EDGE, PARTS, EVEN, kBackwardThreads><<<grid, block, room, s>>>(a, g.lanes);
@@ -860,17 +934,17 @@ static void launch_forward_edge(const NormForward &a, hipStream_t s) {
 }
 
 template <class T, int EDGE>
-static void launch_backward_edge(const NormBackward &a, uint32_t groups, hipStream_t s) {
+static void launch_backward_edge(const NormBackward &a, hipStream_t s) {
     const RowTiling g = backward_tiling(a.width, T::code);
     if (g.parts == 0) {
         norm_rows_backward_kernel<T, EDGE><<<dim3(strided_grid(a.rows, kBlock)), dim3(kBlock), 0, s>>>(a);
         if (a.partials != nullptr)
-            norm_columns_kernel<T><<<dim3((a.width + kBlock - 1) / kBlock, groups), dim3(kBlock), 0, s>>>(a);
+            norm_columns_kernel<T><<<dim3((a.width + kBlock - 1) / kBlock, a.row_blocks), dim3(kBlock), 0, s>>>(a);
         return;
     }
     const bool even = a.width % kGroup == 0 && aligned16({a.dy, a.dtotal, a.t, a.dx, a.dresidual});
     with_tiling<2>(g, even,
-                   [&](auto parts, auto e) { launch_norm_backward<T, EDGE, parts.value, e.value>(a, g, groups, s); });
+                   [&](auto parts, auto e) { launch_norm_backward<T, EDGE, parts.value, e.value>(a, g, s); });
 }
 
 template <class T>
@@ -881,17 +955,17 @@ static void launch_forward(const NormForward &a, int edge, hipStream_t s) {
 }
 
 template <class T>
-static void launch_backward(const NormBackward &a, int edge, uint32_t groups, hipStream_t s) {
-    if (edge == kNone) launch_backward_edge<T, kNone>(a, groups, s);
-    else if (edge == kAdd) launch_backward_edge<T, kAdd>(a, groups, s);
-    else launch_backward_edge<T, kDropAdd>(a, groups, s);
+static void launch_backward(const NormBackward &a, int edge, hipStream_t s) {
+    if (edge == kNone) launch_backward_edge<T, kNone>(a, s);
+    else if (edge == kAdd) launch_backward_edge<T, kAdd>(a, s);
+    else launch_backward_edge<T, kDropAdd>(a, s);
 }
 
 template <class T>
-static void launch_finalize(const NormBackward &a, uint32_t groups, void *dw, void *db, hipStream_t s) {
+static void launch_finalize(const NormBackward &a, hipStream_t s) {
     const dim3 grid((unsigned)((2u * (uint64_t)a.width + kFinalColumns - 1) / kFinalColumns));
     norm_finalize_kernel<T><<<grid, dim3(kFinalColumns * kFinalSlices), 0, s>>>(
-        a.partials, groups, a.width, static_cast<typename T::raw *>(dw), static_cast<typename T::raw *>(db));
+        a.partials, a.row_blocks, a.width, static_cast<typename T::raw *>(a.dw), static_cast<typename T::raw *>(a.db));
 }
 
 template <class T>
@@ -950,12 +1024,25 @@ static int32_t check_arrays(const char *entry, std::initializer_list<Array> arra
     return NT_OK;
 }
 
+// NT_ERR_RUNTIME while `stream` is captured: a replay would repeat a mask, or
+// use a workspace that the pool has handed to others since.
+static int32_t refuse_capture(const char *entry, void *stream) {
+    int32_t capturing = 0;
+    const int32_t rc = nt_stream_capturing(stream, &capturing);
+    if (rc != NT_OK) return rc;
+    return capturing ? fail(NT_ERR_RUNTIME, std::string(entry) + ": not supported in stream capture") : NT_OK;
+}
+
 static int32_t forward(const char *entry, int32_t device, const NormForward &a, int32_t dtype, int edge, void *stream) {
     if ((a.mean == nullptr) != (a.rstd == nullptr))
         return fail(NT_ERR_VALUE, std::string(entry) + ": mean and rstd are given together");
     if (a.rows == 0) return NT_OK;
     DeviceGuard guard(device);
     if (!guard.ok()) return hip_check(guard.error(), "hipSetDevice");
+    if (edge == kDropAdd) {
+        const int32_t rc = refuse_capture(entry, stream);
+        if (rc != NT_OK) return rc;
+    }
     hipStream_t s = (hipStream_t)stream;
     switch (dtype) {
         case NT_F32: launch_forward<TF32>(a, edge, s); break;
@@ -966,46 +1053,41 @@ static int32_t forward(const char *entry, int32_t device, const NormForward &a, 
     return NT_OK;
 }
 
-static int32_t backward(const char *entry, int32_t device, NormBackward a, int32_t dtype, int edge, void *dw, void *db,
-                        void *stream) {
+static int32_t backward(const char *entry, int32_t device, NormBackward a, int32_t dtype, int edge, void *stream) {
     DeviceGuard guard(device);
     if (!guard.ok()) return hip_check(guard.error(), "hipSetDevice");
+    const int32_t refused = refuse_capture(entry, stream);
+    if (refused != NT_OK) return refused;
     hipStream_t s = (hipStream_t)stream;
-    const bool columns = dw != nullptr || db != nullptr;
-    const uint32_t groups = partial_groups(a.rows, a.width, dtype);
-    void *workspace = nullptr;
-    if (columns) {
-        // The workspace goes back to the pool as soon as the kernels are queued: the pool reuses it on this
-        // stream only.  Captured work would keep using it after that.
-        int32_t capturing = 0;
-        const int32_t queried = nt_stream_capturing(stream, &capturing);
-        if (queried != NT_OK) return queried;
-        if (capturing)
-            return fail(NT_ERR_RUNTIME, std::string(entry) + ": not supported in stream capture");
+    a.row_blocks = partial_groups(a.rows, a.width, dtype);
+    const bool partial =
+        (a.dw != nullptr || a.db != nullptr) && !takes_columns(a.rows, backward_tiling(a.width, dtype));
+    if (partial) {
+        // Goes back to the pool as soon as the kernels are queued: the pool reuses it on this stream only.
+        void *workspace = nullptr;
         std::string error;
-        const int32_t rc = device_pool().allocate(device, (uint64_t)groups * 2u * a.width * sizeof(float), stream,
-                                                  &workspace, error);
+        const int32_t rc = device_pool().allocate(device, (uint64_t)a.row_blocks * 2u * a.width * sizeof(float),
+                                                  stream, &workspace, error);
         if (rc != NT_OK) return fail(rc, error);
         a.partials = static_cast<float *>(workspace);
     }
     switch (dtype) {
-        case NT_F32: launch_backward<TF32>(a, edge, groups, s); break;
-        case NT_F16: launch_backward<TF16>(a, edge, groups, s); break;
-        default: launch_backward<TBF16>(a, edge, groups, s); break;
+        case NT_F32: launch_backward<TF32>(a, edge, s); break;
+        case NT_F16: launch_backward<TF16>(a, edge, s); break;
+        default: launch_backward<TBF16>(a, edge, s); break;
     }
     hipError_t status = hipGetLastError();
-    if (columns && status == hipSuccess) {
+    if (!partial) return hip_check(status, "layer norm backward launch");
+    if (status == hipSuccess) {
         switch (a.weight_dtype) {
-            case NT_F32: launch_finalize<TF32>(a, groups, dw, db, s); break;
-            case NT_F16: launch_finalize<TF16>(a, groups, dw, db, s); break;
-            default: launch_finalize<TBF16>(a, groups, dw, db, s); break;
+            case NT_F32: launch_finalize<TF32>(a, s); break;
+            case NT_F16: launch_finalize<TF16>(a, s); break;
+            default: launch_finalize<TBF16>(a, s); break;
         }
         status = hipGetLastError();
     }
-    if (workspace != nullptr) {
-        std::string error;
-        (void)device_pool().release(workspace, error);
-    }
+    std::string error;
+    (void)device_pool().release(a.partials, error);
     return hip_check(status, "layer norm backward launch");
 }
 
@@ -1046,8 +1128,9 @@ int32_t nt_layer_norm_backward(int32_t device, const void *dy, const void *x, in
                        {dx, dtype, n, true, any}, {dweight, weight_dtype, width, true, false},
                        {dbias, weight_dtype, width, true, false}});
     if (rc != NT_OK) return rc;
-    const NormBackward a{dy, nullptr, x, weight, mean, rstd, dx, nullptr, nullptr, rows, (uint32_t)width, weight_dtype, {}};
-    return backward("nt_layer_norm_backward", device, a, dtype, kNone, dweight, dbias, stream);
+    const NormBackward a{dy, nullptr, x, weight, mean, rstd, dx, nullptr, nullptr, rows, (uint32_t)width,
+                         weight_dtype, {}, 0, dweight, dbias};
+    return backward("nt_layer_norm_backward", device, a, dtype, kNone, stream);
 }
 
 int32_t nt_dropout(int32_t device, const void *x, int32_t dtype, void *y, uint64_t count, uint32_t threshold,
@@ -1058,10 +1141,12 @@ int32_t nt_dropout(int32_t device, const void *x, int32_t dtype, void *y, uint64
     if (count == 0) return NT_OK;
     if (count > 0xffffffffffffull) return fail(NT_ERR_VALUE, "nt_dropout: too many elements");
     // In place (y == x) each lane reads its elements before it writes them.
-    int32_t rc = check_arrays("nt_dropout", {{x, dtype, x == y ? 0 : count, false, true}, {y, dtype, count, true, true}});
+    int32_t rc = check_arrays("nt_dropout",
+                              {{x, dtype, x == y ? 0 : count, false, true}, {y, dtype, count, true, true}});
     if (rc != NT_OK) return rc;
     DeviceGuard guard(device);
     if (!guard.ok()) return hip_check(guard.error(), "hipSetDevice");
+    if (threshold != 0 && (rc = refuse_capture("nt_dropout", stream)) != NT_OK) return rc;
     const Mask mask = make_mask(threshold, seed, offset);
     hipStream_t s = (hipStream_t)stream;
     switch (dtype) {
@@ -1112,8 +1197,8 @@ int32_t nt_dropout_add_layer_norm_backward(int32_t device, const void *dy, const
                               {dweight, weight_dtype, width, true, false}, {dbias, weight_dtype, width, true, false}});
     if (rc != NT_OK) return rc;
     const NormBackward a{dy, dtotal, total, weight, mean, rstd, dx, dresidual, nullptr, rows, (uint32_t)width,
-                         weight_dtype, make_mask(threshold, seed, offset)};
-    return backward(entry, device, a, dtype, threshold == 0 ? kAdd : kDropAdd, dweight, dbias, stream);
+                         weight_dtype, make_mask(threshold, seed, offset), 0, dweight, dbias};
+    return backward(entry, device, a, dtype, threshold == 0 ? kAdd : kDropAdd, stream);
 }
 
 }  // extern "C"

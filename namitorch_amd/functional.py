@@ -39,11 +39,12 @@ from __future__ import annotations
 import math
 from numbers import Integral, Real
 
-from . import _native, runtime
+from . import _native
 from .array import DeviceArray
-from .backends import ensure_same_device, get_backend
+from .backends import _backends, ensure_same_device, get_backend
 from .backends._graph_capture import reject_during_capture
 from .dtype import bfloat16, float16, float32
+from .runtime import current_stream
 from .tensor import Tensor, device_views
 
 _DTYPES = frozenset((float16, bfloat16, float32))
@@ -56,9 +57,10 @@ def _activation(value, name: str, like: Tensor | None = None) -> int:
     if not isinstance(value, Tensor):
         raise TypeError(f"{name} must be a NamiTorch Tensor, got {type(value).__name__}.")
     if like is None:
-        backend = get_backend(value)         # a device's backend also puts it under the capture checks
-        if value._ptr is None:
-            backend._unsupported("Layer norm and dropout")
+        if value._device not in _backends or value._ptr is None:
+            backend = get_backend(value)     # which also puts a device under the capture checks
+            if value._ptr is None:
+                backend._unsupported("Layer norm and dropout")
         if value._dtype not in _DTYPES:
             raise TypeError(f"{name} must be float16, bfloat16 or float32, got {value._dtype.name}.")
     else:
@@ -115,7 +117,9 @@ def _statistic(value, name: str, shape: tuple, like: Tensor) -> int:
 
 def _normalized(value: Tensor, normalized_shape) -> tuple:
     """(leading shape, normalized shape, rows, width)."""
-    shape = (normalized_shape,) if isinstance(normalized_shape, Integral) else tuple(normalized_shape)
+    shape = normalized_shape
+    if type(shape) is not tuple:
+        shape = (int(shape),) if isinstance(shape, Integral) else tuple(shape)
     lead = len(value._shape) - len(shape)
     if not shape or lead < 0 or value._shape[lead:] != shape:
         raise ValueError(f"normalized_shape {shape} must be the trailing dimensions of {value._shape}.")
@@ -131,9 +135,10 @@ def _split(value: Tensor, lead: int) -> tuple:
 
 
 def _epsilon(eps) -> float:
-    if isinstance(eps, bool) or not isinstance(eps, Real):
-        raise TypeError("eps must be a real number.")
-    eps = float(eps)
+    if type(eps) is not float:
+        if isinstance(eps, bool) or not isinstance(eps, Real):
+            raise TypeError("eps must be a real number.")
+        eps = float(eps)
     if not 0.0 <= eps < math.inf:
         raise ValueError(f"eps must be finite and nonnegative, got {eps}.")
     return eps
@@ -141,26 +146,32 @@ def _epsilon(eps) -> float:
 
 def _threshold(p) -> int:
     """Drop threshold of the 16-bit numbers: p rounded to a multiple of 2**-16."""
-    if isinstance(p, bool) or not isinstance(p, Real):
-        raise TypeError("p must be a real number.")
-    p = float(p)
+    if type(p) is not float:
+        if isinstance(p, bool) or not isinstance(p, Real):
+            raise TypeError("p must be a real number.")
+        p = float(p)
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"p must be between 0 and 1, got {p}.")
     return round(p * 65536)
 
 
 def _counter(value, name: str) -> int:
-    if isinstance(value, bool) or not isinstance(value, Integral):
-        raise TypeError(f"{name} must be an integer.")
+    if type(value) is not int:
+        if isinstance(value, bool) or not isinstance(value, Integral):
+            raise TypeError(f"{name} must be an integer.")
+        value = int(value)
     if not 0 <= value < _MAX_SEED:
         raise ValueError(f"{name} must be in [0, 2**64), got {value}.")
-    return int(value)
-
-
-def _flag(value) -> bool:
-    if type(value) is not bool:
-        raise TypeError("training must be a Python bool.")
     return value
+
+
+def _training_threshold(p, training) -> int:
+    threshold = _threshold(p)
+    if training is True:
+        return threshold
+    if training is not False:
+        raise TypeError("training must be a Python bool.")
+    return 0
 
 
 # ---- results ------------------------------------------------------------------------------------
@@ -191,9 +202,12 @@ def _result(given, name: str, shape: tuple, dtype, like: Tensor) -> Tensor:
     return given
 
 
-def _written(*tensors) -> None:
-    """In-place bookkeeping of given Tensors that a launch has overwritten."""
-    for tensor in tensors:
+def _launch(status: int, given: tuple) -> None:
+    """Raise what the library refused; otherwise the in-place bookkeeping of
+    the given Tensors that the launch overwrites."""
+    if status:
+        _native.check(status)
+    for tensor in given:
         if tensor is not None:
             tensor._pending = tensor._incoming = tensor._known_item = None
             tensor._version_counter.increment()
@@ -226,10 +240,9 @@ def _layer_norm(x, normalized_shape, weight, bias, eps, given, stats: bool) -> t
         mean = _result(given[1], "mean", lead, float32, x)
         rstd = _result(given[2], "rstd", lead, float32, x)
     device = x._device.index
-    _native.call("nt_layer_norm", device, source, x._dtype._code, scale, shift, code, eps, y._ptr,
-                 mean._ptr if stats else None, rstd._ptr if stats else None, rows, width,
-                 runtime.current_stream(device))
-    _written(*given)
+    _launch(_native.load().nt_layer_norm(
+        device, source, x._dtype._code, scale, shift, code, eps, y._ptr, mean._ptr if stats else None,
+        rstd._ptr if stats else None, rows, width, current_stream(device)), given)
     return (y, mean, rstd)
 
 
@@ -243,14 +256,14 @@ def layer_norm_backward(grad_output, input, mean, rstd, weight=None, bias=None, 
     dy = _activation(grad_output, "grad_output", input)
     _, shape, rows, width, mean_at, rstd_at = _kept(input, mean, rstd)
     scale, _, code = _affine_pair(weight, bias, shape, input)
-    reject_during_capture("Layer norm backward")
+    if None in given:
+        reject_during_capture("Layer norm backward")
     dx = _result(given[0], "grad_input", input._shape, input._dtype, input)
     dw, db = _affine_results(given[1:], weight, bias, input)
     device = input._device.index
-    _native.call("nt_layer_norm_backward", device, dy, x, input._dtype._code, mean_at, rstd_at, scale, code, dx._ptr,
-                 None if dw is None else dw._ptr, None if db is None else db._ptr, rows, width,
-                 runtime.current_stream(device))
-    _written(*given)
+    _launch(_native.load().nt_layer_norm_backward(
+        device, dy, x, input._dtype._code, mean_at, rstd_at, scale, code, dx._ptr, None if dw is None else dw._ptr,
+        None if db is None else db._ptr, rows, width, current_stream(device)), given)
     return dx, dw, db
 
 
@@ -292,19 +305,18 @@ def dropout_backward(grad_output, p=0.5, training=True, *, seed, offset=0, out=N
 
 
 def _dropout(x, p, training, seed, offset, out, name: str) -> Tensor:
-    given = _given(out, 1)[0]
+    given, = outs = _given(out, 1)
     source = _activation(x, name)
-    threshold = _threshold(p) if _flag(training) else _threshold(p) * 0
+    threshold = _training_threshold(p, training)
     seed, offset = _counter(seed, "seed"), _counter(offset, "offset")
-    if threshold:
+    if given is None:
+        if threshold == 0:
+            return x
         reject_during_capture("Dropout")
-    elif given is None:
-        return x
     y = _result(given, "output", x._shape, x._dtype, x)
     device = x._device.index
-    _native.call("nt_dropout", device, source, x._dtype._code, y._ptr, x._numel, threshold, seed, offset,
-                 runtime.current_stream(device))
-    _written(given)
+    _launch(_native.load().nt_dropout(
+        device, source, x._dtype._code, y._ptr, x._numel, threshold, seed, offset, current_stream(device)), outs)
     return y
 
 
@@ -331,12 +343,10 @@ def _edge(x, residual, normalized_shape, weight, bias, p, eps, training, seed, o
     lead, shape, rows, width = _normalized(x, normalized_shape)
     scale, shift, code = _affine_pair(weight, bias, shape, x)
     eps = _epsilon(eps)
-    threshold = _threshold(p) if _flag(training) else _threshold(p) * 0
+    threshold = _training_threshold(p, training)
     seed, offset = _counter(seed, "seed"), _counter(offset, "offset")
-    if threshold:
-        reject_during_capture("Dropout")
-    elif None in given:
-        reject_during_capture("Layer norm without out")
+    if None in given:
+        reject_during_capture("Dropout" if threshold else "Layer norm without out")
     y = _result(given[0], "output", x._shape, x._dtype, x)
     total = _result(given[1], "total", x._shape, x._dtype, x)
     mean = rstd = None
@@ -344,10 +354,9 @@ def _edge(x, residual, normalized_shape, weight, bias, p, eps, training, seed, o
         mean = _result(given[2], "mean", lead, float32, x)
         rstd = _result(given[3], "rstd", lead, float32, x)
     device = x._device.index
-    _native.call("nt_dropout_add_layer_norm", device, source, stream_in, x._dtype._code, scale, shift, code, eps,
-                 threshold, seed, offset, total._ptr, y._ptr, mean._ptr if stats else None,
-                 rstd._ptr if stats else None, rows, width, runtime.current_stream(device))
-    _written(*given)
+    _launch(_native.load().nt_dropout_add_layer_norm(
+        device, source, stream_in, x._dtype._code, scale, shift, code, eps, threshold, seed, offset, total._ptr, y._ptr,
+        mean._ptr if stats else None, rstd._ptr if stats else None, rows, width, current_stream(device)), given)
     return (y, total, mean, rstd)
 
 
@@ -362,17 +371,17 @@ def dropout_add_layer_norm_backward(grad_output, grad_total, total, mean, rstd, 
     dt = None if grad_total is None else _activation(grad_total, "grad_total", total)
     _, shape, rows, width, mean_at, rstd_at = _kept(total, mean, rstd)
     scale, _, code = _affine_pair(weight, bias, shape, total)
-    threshold = _threshold(p) if _flag(training) else _threshold(p) * 0
+    threshold = _training_threshold(p, training)
     seed, offset = _counter(seed, "seed"), _counter(offset, "offset")
-    reject_during_capture("Layer norm backward")
+    if None in given:
+        reject_during_capture("Layer norm backward")
     dx = _result(given[0], "grad_input", total._shape, total._dtype, total)
     dr = _result(given[1], "grad_residual", total._shape, total._dtype, total)
     dw, db = _affine_results(given[2:], weight, bias, total)
     device = total._device.index
-    _native.call("nt_dropout_add_layer_norm_backward", device, dy, dt, t, total._dtype._code, mean_at, rstd_at, scale,
-                 code, threshold, seed, offset, dx._ptr, dr._ptr, None if dw is None else dw._ptr,
-                 None if db is None else db._ptr, rows, width, runtime.current_stream(device))
-    _written(*given)
+    _launch(_native.load().nt_dropout_add_layer_norm_backward(
+        device, dy, dt, t, total._dtype._code, mean_at, rstd_at, scale, code, threshold, seed, offset, dx._ptr, dr._ptr,
+        None if dw is None else dw._ptr, None if db is None else db._ptr, rows, width, current_stream(device)), given)
     return dx, dr, dw, db
 
 
