@@ -178,15 +178,32 @@ __device__ __forceinline__ void store_end(void *base, uint64_t i, const Raw8<T> 
     }
 }
 
-// Elements [c, c + 8) of the row that starts at `base + row`, c < width.
+// The group of a lane: eight columns from `column` on (the width where the
+// lane has none).  The last group of a row whose width is no multiple of
+// eight ends at the row's end and starts inside the group before it: its
+// elements below `first` are the other lane's, computed alike by both.  So it
+// too is loaded and stored whole, without a wait for single elements; only
+// rows of less than eight are.
+struct Columns {
+    uint32_t column, first;
+    __device__ __forceinline__ Columns() {}
+    __device__ __forceinline__ Columns(uint32_t c, uint32_t width)
+        : column(c < width && c + kGroup > width && width >= kGroup ? width - kGroup : c < width ? c : width),
+          first(c - column) {}
+    template <bool EVEN>
+    __device__ __forceinline__ bool has(uint32_t k, uint32_t width) const {
+        return EVEN ? column < width : k >= first && column + k < width;
+    }
+};
+
 template <class T, bool EVEN>
 __device__ __forceinline__ void load_part(Raw8<T> &out, const void *base, uint64_t row, uint32_t c, uint32_t width) {
-    if (EVEN || c + kGroup <= width) load8<T, EVEN>(out, base, row + c);
+    if (EVEN || width >= kGroup) load8<T, EVEN>(out, base, row + c);
     else load_end<T>(out, base, row + c, width - c);
 }
 template <class T, bool EVEN>
 __device__ __forceinline__ void store_part(void *base, uint64_t row, uint32_t c, uint32_t width, const Raw8<T> &in) {
-    if (EVEN || c + kGroup <= width) store8<T, EVEN>(base, row + c, in);
+    if (EVEN || width >= kGroup) store8<T, EVEN>(base, row + c, in);
     else store_end<T>(base, row + c, in, width - c);
 }
 
@@ -297,7 +314,7 @@ struct RowSum {
 // Waves per SIMD that the forward pass's registers leave room for.
 template <class T, int EDGE, int PARTS>
 constexpr int forward_waves() {
-    return EDGE == kNone && PARTS <= 2 && T::code != NT_F32 ? 8 : 4;
+    return EDGE != kNone || PARTS > 2 || (T::code == NT_F32 && PARTS == 2) ? 4 : 8;
 }
 
 template <class T, int EDGE, int PARTS, bool EVEN, int THREADS>
@@ -308,26 +325,26 @@ __global__ __launch_bounds__(THREADS, (forward_waves<T, EDGE, PARTS>())) void no
     RowSum<THREADS / 64> row_sum{shared, lanes};
     const uint32_t lane = threadIdx.x & (lanes - 1u), in_block = threadIdx.x / lanes, per_block = THREADS / lanes;
     const float width = (float)a.width;
-    uint32_t column[PARTS];
+    Columns at[PARTS];
 #pragma unroll
-    for (int p = 0; p < PARTS; ++p) column[p] = ((uint32_t)p * lanes + lane) * kGroup;
+    for (int p = 0; p < PARTS; ++p) at[p] = Columns(((uint32_t)p * lanes + lane) * kGroup, a.width);
     const uint64_t stride = (uint64_t)gridDim.x * per_block;
     uint64_t row = (uint64_t)blockIdx.x * per_block + in_block;
     Raw8<T> x[PARTS], r[PARTS];
     const auto fetch = [&](uint64_t which) {
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
-            if (which >= a.rows || column[p] >= a.width) continue;
-            load_part<T, EVEN>(x[p], a.x, which * a.width, column[p], a.width);
-            if constexpr (EDGE != kNone) load_part<T, EVEN>(r[p], a.residual, which * a.width, column[p], a.width);
+            if (which >= a.rows || at[p].column >= a.width) continue;
+            load_part<T, EVEN>(x[p], a.x, which * a.width, at[p].column, a.width);
+            if constexpr (EDGE != kNone) load_part<T, EVEN>(r[p], a.residual, which * a.width, at[p].column, a.width);
         }
     };
     float w[PARTS][8], b[PARTS][8];                     // asked for first: they are there before the rows
     if (in_block == 0u) {
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
-            load_params(w[p], a.weight, a.weight_dtype, column[p], a.width, 1.0f);
-            load_params(b[p], a.bias, a.weight_dtype, column[p], a.width, 0.0f);
+            load_params(w[p], a.weight, a.weight_dtype, at[p].column, a.width, 1.0f);
+            load_params(b[p], a.bias, a.weight_dtype, at[p].column, a.width, 0.0f);
         }
     }
     fetch(row);
@@ -351,10 +368,10 @@ __global__ __launch_bounds__(THREADS, (forward_waves<T, EDGE, PARTS>())) void no
         float sum = 0.0f;
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
-            const bool mine = active && column[p] < a.width;
+            const bool mine = active && at[p].column < a.width;
             if (mine) {
                 widen8<T>(t[p], x[p]);
-                if constexpr (EDGE == kDropAdd) drop8(t[p], numbers8<EVEN>(base + column[p], a.mask), a.mask);
+                if constexpr (EDGE == kDropAdd) drop8(t[p], numbers8<EVEN>(base + at[p].column, a.mask), a.mask);
                 if constexpr (EDGE != kNone) {
                     float add[8];
                     widen8<T>(add, r[p]);
@@ -364,9 +381,9 @@ __global__ __launch_bounds__(THREADS, (forward_waves<T, EDGE, PARTS>())) void no
             }
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const bool in_row = EVEN ? mine : mine && column[p] + (uint32_t)k < a.width;
-                t[p][k] = in_row ? t[p][k] : 0.0f;
-                sum += t[p][k];
+                const bool in_row = active && at[p].template has<EVEN>(k, a.width);
+                t[p][k] = mine ? t[p][k] : 0.0f;
+                sum += EVEN || in_row ? t[p][k] : 0.0f;
             }
         }
         fetch(row + stride);
@@ -376,18 +393,18 @@ __global__ __launch_bounds__(THREADS, (forward_waves<T, EDGE, PARTS>())) void no
         for (int p = 0; p < PARTS; ++p)
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const bool in_row = EVEN ? column[p] < a.width : column[p] + (uint32_t)k < a.width;
+                const bool in_row = at[p].template has<EVEN>(k, a.width);
                 const float d = t[p][k] - mean;
                 squares = in_row ? __builtin_fmaf(d, d, squares) : squares;
             }
         const float rstd = 1.0f / __builtin_sqrtf(row_sum(squares) / width + a.eps);
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
-            if (!active || column[p] >= a.width) continue;
+            if (!active || at[p].column >= a.width) continue;
             Raw8<T> out;
             if constexpr (EDGE != kNone) {
                 narrow8<T>(out, t[p]);
-                store_part<T, EVEN>(a.total, base, column[p], a.width, out);
+                store_part<T, EVEN>(a.total, base, at[p].column, a.width, out);
             }
             float y[8];
 #pragma unroll
@@ -399,7 +416,7 @@ __global__ __launch_bounds__(THREADS, (forward_waves<T, EDGE, PARTS>())) void no
                 y[4 * q + 3] = __builtin_fmaf((t[p][4 * q + 3] - mean) * rstd, w.w, b.w);
             }
             narrow8<T>(out, y);
-            store_part<T, EVEN>(a.y, base, column[p], a.width, out);
+            store_part<T, EVEN>(a.y, base, at[p].column, a.width, out);
         }
         if (active && a.mean != nullptr && lane == 0) {
             a.mean[row] = mean;
@@ -448,7 +465,8 @@ __device__ __forceinline__ void store_param(void *base, int32_t dtype, uint64_t 
 // rows over the rest of the workgroup, joined in a fixed order.
 template <class T, bool EVEN, int THREADS>
 __device__ __forceinline__ void column_tile(const NormBackward &a, uint32_t tile, float4 *room) {
-    const uint32_t c = tile * 64u + (threadIdx.x & 7u) * kGroup;
+    const Columns at(tile * 64u + (threadIdx.x & 7u) * kGroup, a.width);
+    const uint32_t c = at.column;
     float dw[8] = {}, db[8] = {};
     if (c < a.width) {
 #pragma unroll 2
@@ -477,10 +495,12 @@ __device__ __forceinline__ void column_tile(const NormBackward &a, uint32_t tile
     }
     float *sums = reinterpret_cast<float *>(room);      // [wave][dw, db][64]
     if ((threadIdx.x & 63u) < 8u) {
+        const uint32_t place = (threadIdx.x >> 6) * 128u + (threadIdx.x & 7u) * 8u;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            sums[(threadIdx.x >> 6) * 128u + (threadIdx.x & 7u) * 8u + k] = dw[k];
-            sums[(threadIdx.x >> 6) * 128u + 64u + (threadIdx.x & 7u) * 8u + k] = db[k];
+        for (uint32_t k = 0; k < 8; ++k) {
+            if (k < at.first) continue;                 // a last group's element `first` is the first of its place
+            sums[place + k - at.first] = dw[k];
+            sums[place + 64u + k - at.first] = db[k];
         }
     }
     __syncthreads();
@@ -513,18 +533,18 @@ __global__ __launch_bounds__(THREADS, 4) void norm_backward_kernel(NormBackward 
     RowSum2<THREADS / 64> row_sum{shared, lanes};
     const uint32_t lane = threadIdx.x & (lanes - 1u), in_block = threadIdx.x / lanes, per_block = THREADS / lanes;
     const float width = (float)a.width;
-    uint32_t column[PARTS];
+    Columns at[PARTS];
 #pragma unroll
-    for (int p = 0; p < PARTS; ++p) column[p] = ((uint32_t)p * lanes + lane) * kGroup;
+    for (int p = 0; p < PARTS; ++p) at[p] = Columns(((uint32_t)p * lanes + lane) * kGroup, a.width);
     const uint64_t stride = (uint64_t)a.row_blocks * per_block;
     uint64_t row = (uint64_t)blockIdx.x * per_block + in_block;
     Raw8<T> dy[PARTS], t[PARTS], dt[PARTS];
     const auto fetch = [&](uint64_t which, int p) {
-        if (which >= a.rows || column[p] >= a.width) return;
-        load_part<T, EVEN>(dy[p], a.dy, which * a.width, column[p], a.width);
-        load_part<T, EVEN>(t[p], a.t, which * a.width, column[p], a.width);
+        if (which >= a.rows || at[p].column >= a.width) return;
+        load_part<T, EVEN>(dy[p], a.dy, which * a.width, at[p].column, a.width);
+        load_part<T, EVEN>(t[p], a.t, which * a.width, at[p].column, a.width);
         if constexpr (EDGE != kNone)
-            if (a.dtotal != nullptr) load_part<T, EVEN>(dt[p], a.dtotal, which * a.width, column[p], a.width);
+            if (a.dtotal != nullptr) load_part<T, EVEN>(dt[p], a.dtotal, which * a.width, at[p].column, a.width);
     };
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) fetch(row, p);
@@ -536,7 +556,7 @@ __global__ __launch_bounds__(THREADS, 4) void norm_backward_kernel(NormBackward 
         for (int k = 0; k < 8; ++k) dw[p][k] = db[p][k] = 0.0f;
         if (in_block == 0u) {
             float w[8];
-            load_params(w, a.weight, a.weight_dtype, column[p], a.width, 1.0f);
+            load_params(w, a.weight, a.weight_dtype, at[p].column, a.width, 1.0f);
             room[(2 * p) * lanes + lane] = make_float4(w[0], w[1], w[2], w[3]);
             room[(2 * p + 1) * lanes + lane] = make_float4(w[4], w[5], w[6], w[7]);
         }
@@ -554,15 +574,16 @@ __global__ __launch_bounds__(THREADS, 4) void norm_backward_kernel(NormBackward 
         float level = 0.0f, along = 0.0f;
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
-            if (!active || column[p] >= a.width) continue;
+            if (!active || at[p].column >= a.width) continue;
             float g[8], h[8], w[8];
             weights(w, p);
             widen8<T>(g, dy[p]);
             widen8<T>(h, t[p]);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                // Past a ragged end: dy reads as zero, and so does h.
-                h[k] = EVEN || column[p] + (uint32_t)k < a.width ? (h[k] - mean) * rstd : 0.0f;
+                const bool in_row = EVEN || at[p].template has<EVEN>(k, a.width);
+                g[k] = in_row ? g[k] : 0.0f;
+                h[k] = in_row ? (h[k] - mean) * rstd : 0.0f;
                 dw[p][k] = __builtin_fmaf(g[k], h[k], dw[p][k]);
                 db[p][k] += g[k];
                 g[k] *= w[k];
@@ -579,7 +600,7 @@ __global__ __launch_bounds__(THREADS, 4) void norm_backward_kernel(NormBackward 
         along /= width;
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
-            if (!active || column[p] >= a.width) continue;
+            if (!active || at[p].column >= a.width) continue;
             float g[8], h[8], w[8];
             weights(w, p);
             widen8<T>(g, dy[p]);
@@ -597,11 +618,11 @@ __global__ __launch_bounds__(THREADS, 4) void norm_backward_kernel(NormBackward 
             Raw8<T> out;
             if constexpr (EDGE != kNone) {
                 narrow8<T>(out, g);
-                store_part<T, EVEN>(a.dresidual, base, column[p], a.width, out);
-                if constexpr (EDGE == kDropAdd) drop8(g, numbers8<EVEN>(base + column[p], a.mask), a.mask);
+                store_part<T, EVEN>(a.dresidual, base, at[p].column, a.width, out);
+                if constexpr (EDGE == kDropAdd) drop8(g, numbers8<EVEN>(base + at[p].column, a.mask), a.mask);
             }
             narrow8<T>(out, g);
-            store_part<T, EVEN>(a.dx, base, column[p], a.width, out);
+            store_part<T, EVEN>(a.dx, base, at[p].column, a.width, out);
         }
         row = next;
     }
@@ -622,33 +643,42 @@ __global__ __launch_bounds__(THREADS, 4) void norm_backward_kernel(NormBackward 
             z += __shfl_xor(z, (int)off, 64);
             w += __shfl_xor(w, (int)off, 64);
         });
-    const uint32_t span = lanes < 64u ? 64u : lanes, member = threadIdx.x / span, at = threadIdx.x & (span - 1u);
+    const uint32_t span = lanes < 64u ? 64u : lanes, member = threadIdx.x / span, place = threadIdx.x & (span - 1u);
     for (uint32_t half = THREADS / span / 2u; half > 0u; half >>= 1) {
         __syncthreads();                                // the weights, or the last half, are read
-        if (member >= half && member < 2u * half && at < lanes)
+        if (member >= half && member < 2u * half && place < lanes)
             each([&](int q, float x, float y, float z, float w) {
-                room[((member - half) * 4 * PARTS + q) * lanes + at] = make_float4(x, y, z, w);
+                room[((member - half) * 4 * PARTS + q) * lanes + place] = make_float4(x, y, z, w);
             });
         __syncthreads();
-        if (member < half && at < lanes)
+        if (member < half && place < lanes)
             each([&](int q, float &x, float &y, float &z, float &w) {
-                const float4 other = room[(member * 4 * PARTS + q) * lanes + at];
+                const float4 other = room[(member * 4 * PARTS + q) * lanes + place];
                 x += other.x;
                 y += other.y;
                 z += other.z;
                 w += other.w;
             });
     }
-    if (member != 0u || at >= lanes) return;
+    if (member != 0u || place >= lanes) return;
     float *out = a.partials + (uint64_t)blockIdx.x * 2u * a.width;
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) {
-        if (column[p] >= a.width) continue;
+        if (at[p].column >= a.width) continue;
         Raw8<TF32> sums;
+        if (at[p].first != 0u || at[p].column + kGroup > a.width) {
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) {
+                if (!at[p].template has<false>(k, a.width)) continue;
+                out[at[p].column + k] = dw[p][k];
+                out[a.width + at[p].column + k] = db[p][k];
+            }
+            continue;
+        }
         narrow8<TF32>(sums, dw[p]);
-        store_part<TF32, false>(out, 0, column[p], a.width, sums);
+        store8<TF32, false>(out, at[p].column, sums);
         narrow8<TF32>(sums, db[p]);
-        store_part<TF32, false>(out + a.width, 0, column[p], a.width, sums);
+        store8<TF32, false>(out, a.width + at[p].column, sums);
     }
 }
 
@@ -824,8 +854,8 @@ static RowTiling forward_tiling(uint64_t rows, uint32_t width, int32_t dtype) {
         uint32_t lanes = 1;
         while (lanes * parts < groups) lanes <<= 1;
         if (lanes > (uint32_t)kWideThreads || (lanes > (uint32_t)kRowThreads && parts > 2)) continue;
-        const bool few = parts == 1 && rows * lanes <= kFewLanes;
-        if (best.parts == 0 || few || lanes * parts < best.lanes * best.parts)
+        const bool one = parts == 1 && (dtype == NT_F32 || rows * lanes <= kFewLanes);
+        if (best.parts == 0 || one || lanes * parts < best.lanes * best.parts)
             best = RowTiling{lanes, parts, uint32_t(lanes <= (uint32_t)kRowThreads ? kRowThreads : kWideThreads)};
     }
     return best;
@@ -841,7 +871,8 @@ static RowTiling backward_tiling(uint32_t width, int32_t dtype) {
         while (lanes * parts < groups) lanes <<= 1;
         if (lanes > (uint32_t)kWideThreads) continue;
         if (best.parts == 0 || lanes * parts < best.lanes * best.parts || dtype == NT_F32)
-            best = RowTiling{lanes, parts, uint32_t(lanes <= (uint32_t)kBackwardThreads ? kBackwardThreads : kWideThreads)};
+            best = RowTiling{lanes, parts,
+                             uint32_t(lanes <= (uint32_t)kBackwardThreads ? kBackwardThreads : kWideThreads)};
     }
     return best;
 }
