@@ -5,6 +5,9 @@ entry points refuse before any device is asked."""
 from __future__ import annotations
 
 import math
+import shutil
+import subprocess
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -119,3 +122,12 @@ def test_scalar_arguments():
         with pytest.raises(ValueError, match="eps must be finite and nonnegative"):
             F._epsilon(bad)
     assert F._counter(np.uint64((1 << 64) - 1), "seed") == (1 << 64) - 1
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_generator_header_on_the_host(tmp_path):
+    source = Path(__file__).resolve().parent / "host" / "philox_test.cpp"
+    binary = tmp_path / "philox_test"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", str(source), "-o", str(binary)], check=True)
+    result = subprocess.run([str(binary)], capture_output=True, text=True)
+    assert result.returncode == 0, result.stdout + result.stderr
