@@ -837,7 +837,7 @@ constexpr uint64_t kMaxWidth = 1ull << 24;              // exact in float32, and
 constexpr uint32_t kSimds = 256 * 4;                    // launches stride over rows with as many waves as are resident
 constexpr uint32_t kBackwardWaves = 4;                  // per SIMD
 constexpr uint64_t kFewRows = 512;
-constexpr uint64_t kFewLanes = 256 * 64 * 4;
+constexpr uint64_t kFewLanes = kSimds * 4 * 64;        // of rows: a workgroup's worth of waves on every SIMD pair
 
 // How a row is laid over lanes; parts == 0: it does not fit.
 struct RowTiling {
@@ -1003,7 +1003,7 @@ template <class T>
 static void launch_dropout(const void *x, void *y, uint64_t n, const Mask &mask, hipStream_t s) {
     const uint64_t tile = (uint64_t)kBlock * kGroup * kDropGroups;
     const dim3 grid(strided_grid((n + tile - 1) / tile, kBlock)), block(kBlock);
-    const bool even = aligned16({x, y}), past = n * sizeof(typename T::raw) > kCachedBytes;
+    const bool even = aligned16({x, y}), past = T::code != NT_F32 && n * sizeof(typename T::raw) > kCachedBytes;
     if (even && past) dropout_kernel<T, true, true><<<grid, block, 0, s>>>(x, y, n, mask);
     else if (even) dropout_kernel<T, true, false><<<grid, block, 0, s>>>(x, y, n, mask);
     else if (past) dropout_kernel<T, false, true><<<grid, block, 0, s>>>(x, y, n, mask);

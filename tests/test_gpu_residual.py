@@ -19,7 +19,7 @@ import pytest
 import torch
 
 import namitorch_amd as nt
-from namitorch_amd import functional as F
+from namitorch_amd import _native, functional as F
 from oracle import residual
 
 pytestmark = pytest.mark.gpu
@@ -504,3 +504,127 @@ def test_results_feed_a_step():
     for parameter, old, gradient in zip(params, before, (dw, db)):
         moved = old - parameter.numpy()
         assert (np.sign(moved) == np.sign(gradient.numpy()))[np.abs(gradient.numpy()) > 1e-3].all()
+
+
+# ---- launch shapes: few and many rows, every tiling, both dropout paths -----------------------------------
+MANY = [(512, 768), (513, 768), (600, 5), (2000, 33), (1100, 1001), (520, 4096), (514, 8200), (520, 1531), (4099, 16)]
+
+
+@pytest.mark.parametrize("dtype, weight_dtype", [("float32", "float32"), ("bfloat16", "float32"), ("float16", "float16")])
+@pytest.mark.parametrize("rows, width", MANY)
+def test_edge_of_many_rows(rows, width, dtype, weight_dtype):
+    """Past 512 rows the weight's gradient goes through partial sums; up to there the launch sums columns."""
+    rng = _rng(20, rows, width)
+    t, w, b = _inputs(rng, rows, width, dtype, weight_dtype)
+    dy, dt = (_tensor(0.1 * rng.standard_normal((rows, width)), dtype) for _ in range(2))
+    _, mean, rstd = F.layer_norm_forward(t, width, w, b)
+    call = dict(p=0.25, seed=width, offset=rows)
+    dx, dr, dw, db = F.dropout_add_layer_norm_backward(dy, dt, t, mean, rstd, w, b, **call)
+    expected, allowed = _backward_bounds(_values(dy), _values(t), _values(mean), _values(rstd), _values(w))
+    want, more = expected[0] + _values(dt), np.abs(expected[0]) + np.abs(_values(dt))
+    _near(dr, want, allowed[0] + E * more, dtype, "grad_residual")
+    factor = residual.mask((rows, width), 0.25, width, rows)
+    _near(dx, want * factor, (allowed[0] + E * more + 2 * E * np.abs(want)) * factor, dtype, "grad_input")
+    _near(dw, expected[1], allowed[1], weight_dtype, "grad_weight")
+    _near(db, expected[2], allowed[2], weight_dtype, "grad_bias")
+    x = _tensor(0.5 * rng.standard_normal((rows, width)), dtype)
+    y, total, mean, rstd = F.dropout_add_layer_norm_forward(x, dy, width, w, b, **call)
+    t, t_error = _total(_values(x), _values(dy), 0.25, width, rows)
+    _near(total, t, t_error, dtype, "total")
+    _check_forward(t, t_error, y, mean, rstd, _values(w), _values(b), dtype)
+
+
+@pytest.mark.parametrize("width", list(range(1, 34)) + [63, 65, 127, 129, 255, 257, 383, 385, 513, 767, 1023, 1025, 1537])
+def test_every_tiling(width):
+    rng = _rng(21, width)
+    for rows in (3, 700):
+        x, w, b = _inputs(rng, rows, width, "bfloat16", "float32")
+        dy = _tensor(rng.standard_normal((rows, width)), "bfloat16")
+        y, mean, rstd = F.layer_norm_forward(x, width, w, b)
+        _check_forward(_values(x), np.zeros((rows, width)), y, mean, rstd, _values(w), _values(b), "bfloat16")
+        made = F.layer_norm_backward(dy, x, mean, rstd, w, b)
+        expected, allowed = _backward_bounds(_values(dy), _values(x), _values(mean), _values(rstd), _values(w))
+        for got, want, bound, kind in zip(made, expected, allowed, ("bfloat16", "float32", "float32")):
+            _near(got, want, bound, kind)
+
+
+@pytest.mark.parametrize("shift", [0, 1])
+def test_dropout_of_a_large_tensor(shift):
+    """Past 64 MiB, where a 16-bit input is read around the caches."""
+    count = (33 << 20) + 5
+    room = nt.DeviceArray.empty((count + shift,), "bfloat16", DEV)
+    room.fill_bits(0x4040)                                  # 3.0
+    x = nt.Tensor._from_storage(room.narrow(shift, count))
+    y = F.dropout(x, 0.1, seed=8, offset=9)
+    for first, size in ((0, 5000), (count // 2 + 3, 5000), (count - 5000, 5000)):
+        got = nt.Tensor._from_storage(y._data.narrow(first, size))
+        expected = residual.dropout(np.full(size, 3.0), 0.1, 8, 9, first)
+        assert np.array_equal(got.numpy() == 0, expected == 0)
+        _near(got, expected, 2 * E * np.abs(expected), "bfloat16")
+
+
+def test_one_row_without_leading_dimensions():
+    x, w, b = _inputs(_rng(22), 1, 96, "float32", "float32")
+    flat = nt.Tensor._from_storage(x._data.reshape((96,)))
+    y, mean, rstd = F.layer_norm_forward(flat, 96, w, b)
+    assert y.shape == (96,) and mean.shape == rstd.shape == ()
+    assert np.array_equal(y.bits(), F.layer_norm(x, 96, w, b).bits()[0])
+    dx, dw, db = F.layer_norm_backward(flat, flat, mean, rstd, w, b)
+    assert dx.shape == dw.shape == (96,) and np.array_equal(db.bits(), flat.bits())
+
+
+def test_deferred_transforms_are_seen():
+    """A gradient whose unscaling is still pending is read as the unscaled values; written as `out`, it holds what the
+    call wrote."""
+    rng = _rng(23)
+    parameter = nt.Parameter(rng.standard_normal((4, 40)).astype(np.float32), device=DEV)
+    optimizer = nt.optim.AdamW([parameter], lr=1e-3)
+    scaler = nt.GradScaler(init_scale=1024.0)
+    scaled = rng.standard_normal((4, 40)).astype(np.float32)
+    for write in (False, True):
+        scaler.scale(nt.Tensor(np.float32(1.0), device=DEV))
+        parameter.grad = nt.Tensor(scaled, device=DEV)
+        assert scaler.unscale_(optimizer)
+        if write:
+            y = F.layer_norm(nt.Tensor(scaled, device=DEV), 40, out=parameter.grad)
+            assert y is parameter.grad
+            assert np.array_equal(y.bits(), F.layer_norm(nt.Tensor(scaled, device=DEV), 40).bits())
+        else:
+            y = F.dropout(parameter.grad, 0.5, seed=1)
+            expected = F.dropout(nt.Tensor(scaled / np.float32(1024), device=DEV), 0.5, seed=1)
+            assert np.array_equal(y.bits(), expected.bits())
+        scaler.step(optimizer)
+        scaler.update()
+
+
+def test_library_refusals():
+    """The C entries' own checks (a caller without this package's Python layer)."""
+    call = _native.call
+    x = torch.zeros(64, device=DEV)
+    p, out = x.data_ptr(), torch.zeros(64, device=DEV).data_ptr()
+    F32, F64 = _native.NT_F32, _native.NT_F64
+    cases = [
+        (TypeError, "float32, float16 or bfloat16", ("nt_dropout", 0, p, F64, out, 8, 1, 0, 0, None)),
+        (ValueError, "0..65536", ("nt_dropout", 0, p, F32, out, 8, 65537, 0, 0, None)),
+        (ValueError, "NULL", ("nt_dropout", 0, p, F32, None, 8, 1, 0, 0, None)),
+        (ValueError, "not aligned", ("nt_dropout", 0, p + 2, F32, out, 8, 1, 0, 0, None)),
+        (ValueError, "overlaps", ("nt_dropout", 0, p, F32, p + 4, 8, 1, 0, 0, None)),
+        (ValueError, "1..2\\*\\*24", ("nt_layer_norm", 0, p, F32, None, None, F32, 1e-5, out, None, None, 1, 0, None)),
+        (ValueError, "1..2\\*\\*24", ("nt_layer_norm", 0, p, F32, None, None, F32, 1e-5, out, None, None, 1,
+                                      (1 << 24) + 1, None)),
+        (ValueError, "too many", ("nt_layer_norm", 0, p, F32, None, None, F32, 1e-5, out, None, None, 1 << 60, 8, None)),
+        (ValueError, "together", ("nt_layer_norm", 0, p, F32, None, None, F32, 1e-5, out, p + 128, None, 1, 8, None)),
+        (TypeError, "weight and bias", ("nt_layer_norm", 0, p, F32, p + 64, None, _native.NT_F16, 1e-5, out, None,
+                                        None, 1, 8, None)),
+        (ValueError, "NULL", ("nt_layer_norm_backward", 0, p, p, F32, None, None, None, F32, out, None, None, 1, 8, None)),
+        (ValueError, "overlaps", ("nt_dropout_add_layer_norm", 0, p, p, F32, None, None, F32, 1e-5, 0, 0, 0, out, out,
+                                  None, None, 1, 8, None)),
+        (ValueError, "0..65536", ("nt_dropout_add_layer_norm_backward", 0, p, None, p, F32, p, p, None, F32, 1 << 20, 0,
+                                  0, out, out + 64, None, None, 1, 8, None)),
+    ]
+    for kind, message, arguments in cases:
+        with pytest.raises(kind, match=message):
+            call(*arguments)
+    call("nt_dropout", 0, None, F32, None, 0, 1, 0, 0, None)
+    call("nt_layer_norm", 0, None, F32, None, None, F32, 1e-5, None, None, None, 0, 8, None)
+    assert _native.load().nt_last_error() == b""
