@@ -666,7 +666,7 @@ __global__ __launch_bounds__(THREADS, 4) void norm_backward_kernel(NormBackward 
     for (int p = 0; p < PARTS; ++p) {
         if (at[p].column >= a.width) continue;
         Raw8<TF32> sums;
-        if (at[p].first != 0u || at[p].column + kGroup > a.width) {
+        if (!EVEN && (at[p].first != 0u || at[p].column + kGroup > a.width)) {
 #pragma unroll
             for (uint32_t k = 0; k < 8; ++k) {
                 if (!at[p].template has<false>(k, a.width)) continue;
