@@ -11,8 +11,14 @@
 //   dw   = sum over rows of dy h,   db = sum over rows of dy.
 //
 // Every sum and statistic is float32; values are rounded once, when stored.
-// The sums over rows run in two stages of fixed order, so gradients do not
-// change from run to run.
+// The sums over rows run in a fixed order, so gradients do not change from
+// run to run.
+//
+// All of it is bound by memory once a launch is large: 8 to 35 vector
+// operations per element (the generator is half of the latter) against 4 to 20
+// bytes.  Times here are kernel times on one MI355X, by kernel trace over
+// three sets of tensors in turn; a stream of one read and one write of the
+// same size runs at 6.6 TB/s, one of two and two at 6.0 (268 MB) to 6.3 TB/s.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -88,7 +94,9 @@ __device__ __forceinline__ float block_sum_f32(float v, float *shared) {
 // What a lane holds of a row at a time: one 16-byte access of a 16-bit type,
 // two of float32, and one call of the mask's generator.  Where rows do not
 // start on 16 bytes the same accesses run unaligned (gfx950 takes any
-// alignment), and the lane at a row's ragged end goes element by element.
+// alignment).  Norms read through the caches: their inputs were just written
+// by a product or an earlier edge (8192 x 768 bfloat16 forward: 6.9 us, with
+// nontemporal loads 10.8), and store around them (temporal stores 8.2 us).
 constexpr int kGroup = 8;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
@@ -153,7 +161,7 @@ __device__ __forceinline__ void narrow8(Raw8<T> &out, const float (&in)[8]) {
     }
 }
 
-// The `left` (< 8) elements of a row's ragged end; the others read as zero.
+// The `left` (< 8) elements of a ragged end; the others read as zero.
 template <class T>
 __device__ __forceinline__ void load_end(Raw8<T> &out, const void *base, uint64_t i, uint32_t left) {
     const auto *p = reinterpret_cast<const typename T::raw *>(base) + i;
@@ -182,8 +190,9 @@ __device__ __forceinline__ void store_end(void *base, uint64_t i, const Raw8<T> 
 // lane has none).  The last group of a row whose width is no multiple of
 // eight ends at the row's end and starts inside the group before it: its
 // elements below `first` are the other lane's, computed alike by both.  So it
-// too is loaded and stored whole, without a wait for single elements; only
-// rows of less than eight are.
+// too is loaded and stored whole; only rows of less than eight go element by
+// element.  Element loads at every end made each wave wait before it asked for
+// its next row (10006 x 1001 bfloat16: norm 14.4 -> 12.8 us, edge 26.0 -> 22.6).
 struct Columns {
     uint32_t column, first;
     __device__ __forceinline__ Columns() {}
@@ -230,6 +239,8 @@ __device__ __forceinline__ void load_params(float (&out)[8], const void *base, i
 
 // Numbers of the eight elements from flat index i on: one call where i is a
 // multiple of eight, else the two groups they straddle, shifted together.
+// (Taking the second group from the next lane, and the last lane's from a call
+// on the scalar unit, was no faster: 26.8 against 26.0 us for the edge above.)
 template <bool EVEN>
 __device__ __forceinline__ PhiloxWords numbers8(uint64_t i, const Mask &m) {
     PhiloxWords words = philox(i >> 3, m.offset, m.seed);
@@ -256,13 +267,16 @@ __device__ __forceinline__ void drop8(float (&v)[8], const PhiloxWords &words, c
 
 // ---- rows that fit in registers ----------------------------------------------------------------------
 // `lanes` (a power of two) lanes hold a row in `parts` groups of eight each,
-// group k of lane l at column 8 (k lanes + l).  Rows of at most 64 lanes share
-// waves and workgroups and need no barrier; wider ones have a workgroup of
-// their own.  The row is read once, all sums come from registers, and the
-// next row is on its way while this one is summed.
-constexpr int kRowThreads = 512;        // lanes of a workgroup of rows that are at most as wide
+// group k of lane l at column 8 (k lanes + l).  Several rows share a workgroup
+// (and a wave, below 64 lanes), which makes as many rounds as its rows need; a
+// round past the last row computes nothing that is kept.  The row is read
+// once, the variance is that of centred values in registers, and the next row
+// is on its way while this one is summed.  Weight and bias wait in LDS: in
+// registers they left room for five waves per SIMD instead of eight (16384 x
+// 4096 float16 forward: 59 us with them, 49 without).
+constexpr int kRowThreads = 512;        // lanes of a workgroup, for rows of at most as many
 constexpr int kBackwardThreads = 512;   // the same of the backward pass
-constexpr int kWideThreads = 1024;      // at most, for wider rows
+constexpr int kWideThreads = 1024;      // of a workgroup, for rows of more
 
 // Sum over the `lanes` lanes of a row, the same on each.  Rows of several
 // waves go through `shared`, of which consecutive sums use the two halves in
@@ -271,7 +285,8 @@ constexpr int kWideThreads = 1024;      // at most, for wider rows
 //
 // Within a wave the halves of 2, 4, 8 and 16 lanes are exchanged by the
 // operand paths of the vector ALU (quad permutations, then mirrors: all lanes
-// of a half hold the same sum by then), those of 32 and 64 by the row swaps.
+// of a half hold the same sum by then), those of 32 and 64 by the row swaps
+// (64 rows of 2048 in the forward pass: 4.8 us with permutes through LDS, 4.4 so).
 template <int CTRL>
 __device__ __forceinline__ float add_moved(float v) {
     return v + bits_f32((uint32_t)__builtin_amdgcn_mov_dpp((int)f32_bits(v), CTRL, 0xf, 0xf, true));
@@ -311,7 +326,9 @@ struct RowSum {
     }
 };
 
-// Waves per SIMD that the forward pass's registers leave room for.
+// Waves per SIMD that the forward pass's registers leave room for, and that a
+// launch has: more only queue up (65536 x 768 float16: 38.9 us with the
+// resident waves, 41.6 with twice as many).
 template <class T, int EDGE, int PARTS>
 constexpr int forward_waves() {
     return EDGE != kNone || PARTS > 2 || (T::code == NT_F32 && PARTS == 2) ? 4 : 8;
@@ -339,26 +356,29 @@ __global__ __launch_bounds__(THREADS, (forward_waves<T, EDGE, PARTS>())) void no
             if constexpr (EDGE != kNone) load_part<T, EVEN>(r[p], a.residual, which * a.width, at[p].column, a.width);
         }
     };
-    float w[PARTS][8], b[PARTS][8];                     // asked for first: they are there before the rows
-    if (in_block == 0u) {
+    // The first row's lanes bring the weight, the second's the bias (or the
+    // first's again), asked for before the rows: they are there before them.
+    float param[PARTS][8];
+    const auto ask = [&](bool is_bias) {
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p)
+            load_params(param[p], is_bias ? a.bias : a.weight, a.weight_dtype, at[p].column, a.width,
+                        is_bias ? 0.0f : 1.0f);
+    };
+    const auto keep = [&](bool is_bias) {
+        float4 *to = room + (is_bias ? 2 * PARTS * lanes : 0u) + lane;
 #pragma unroll
         for (int p = 0; p < PARTS; ++p) {
-            load_params(w[p], a.weight, a.weight_dtype, at[p].column, a.width, 1.0f);
-            load_params(b[p], a.bias, a.weight_dtype, at[p].column, a.width, 0.0f);
+            to[2 * p * lanes] = make_float4(param[p][0], param[p][1], param[p][2], param[p][3]);
+            to[(2 * p + 1) * lanes] = make_float4(param[p][4], param[p][5], param[p][6], param[p][7]);
         }
-    }
+    };
+    if (in_block < 2u) ask(in_block == 1u);
     fetch(row);
-    if (in_block == 0u) {
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                room[(2 * p + q) * lanes + lane] =
-                    make_float4(w[p][4 * q], w[p][4 * q + 1], w[p][4 * q + 2], w[p][4 * q + 3]);
-                room[(2 * PARTS + 2 * p + q) * lanes + lane] =
-                    make_float4(b[p][4 * q], b[p][4 * q + 1], b[p][4 * q + 2], b[p][4 * q + 3]);
-            }
-        }
+    if (in_block < 2u) keep(in_block == 1u);
+    if (per_block == 1u) {
+        ask(true);
+        keep(true);
     }
     __syncthreads();
     for (uint64_t first = (uint64_t)blockIdx.x * per_block; first < a.rows; first += stride) {
@@ -461,8 +481,8 @@ __device__ __forceinline__ void store_param(void *base, int32_t dtype, uint64_t 
     }
 }
 
-// dw and db of 64 columns over all rows: eight lanes to a row's columns, the
-// rows over the rest of the workgroup, joined in a fixed order.
+// dw and db of 64 columns over all rows, for few rows: eight lanes to a row's
+// columns, the rows over the rest of the workgroup, joined in a fixed order.
 template <class T, bool EVEN, int THREADS>
 __device__ __forceinline__ void column_tile(const NormBackward &a, uint32_t tile, float4 *room) {
     const Columns at(tile * 64u + (threadIdx.x & 7u) * kGroup, a.width);
@@ -516,12 +536,19 @@ __device__ __forceinline__ void column_tile(const NormBackward &a, uint32_t tile
 // The backward pass of the same tiling.  dw and db of a lane's columns stay
 // in registers over all rows of the workgroup; the rows that share a
 // workgroup are joined at the end, halving them in turn, and each workgroup
-// writes one row of partial sums.  Four waves per SIMD hide the loads (128
-// vector registers each), so no row is fetched ahead, and the weights wait in
-// LDS.  Every workgroup makes the same number of rounds; a round past the last
-// row reads zeros.  With few rows, partial sums would be as large as the rows
-// themselves: then workgroups of the same launch take columns instead, and
-// read the rows once more from the caches.
+// writes one row of partial sums, which norm_finalize_kernel adds.  With few
+// rows, partial sums would be as large as the rows themselves: then workgroups
+// of the same launch take columns instead (column_tile), and read the rows
+// once more from the caches.
+//
+// Four waves per SIMD (128 registers) hide the loads; a row's successor is
+// read into the registers of each group as soon as that group is done.  Twice
+// the registers for it were no faster (norm 16384 x 4096 float16: 80 against
+// 77 us), nor were 256 (136 us for the edge of that size, against 126) or 1024
+// lanes (129).  It runs at what its accesses allow: with the sums and the
+// arithmetic taken out the same kernel takes 73 us instead of 76 (norm, 16384 x
+// 4096 float16, no weights), 39.1 instead of 39.5 (8192 x 2048 float32) and 124
+// instead of 119 (edge, p = 0), that is 5.2 to 5.5 TB/s.
 template <class T, int EDGE, int PARTS, bool EVEN, int THREADS>
 __global__ __launch_bounds__(THREADS, 4) void norm_backward_kernel(NormBackward a, uint32_t lanes) {
     extern __shared__ float4 room[];                    // the weights, then the rows that are joined
@@ -683,6 +710,8 @@ __global__ __launch_bounds__(THREADS, 4) void norm_backward_kernel(NormBackward 
 }
 
 // ---- rows of any width: a workgroup per row, the row read once per pass ---------------------
+// For rows past the tilings (16384 columns).  Bound by the three passes over
+// the row, an element at a time, from the caches.
 template <class T, int EDGE>
 __device__ __forceinline__ float row_value(const NormForward &a, uint64_t i) {
     float v = load1<T>(reinterpret_cast<const typename T::raw *>(a.x), i);
@@ -775,7 +804,9 @@ __global__ __launch_bounds__(kBlock) void norm_columns_kernel(NormBackward a) {
 }
 
 // dw and db from the partial sums, rounded to the weight's dtype: 32 columns
-// and 32 slices of the groups per workgroup, the slices joined in order.
+// and 32 slices of the groups per workgroup, the slices joined in order.  3.9
+// us for 512 groups of 768 columns, of which a launch alone is near 3; 64
+// columns to a workgroup took 4.4, 16 took 4.0 (and 8.0 instead of 5.1 at 4096).
 constexpr uint32_t kFinalColumns = 32, kFinalSlices = 32;
 
 template <class T>
@@ -802,8 +833,16 @@ __global__ __launch_bounds__(kFinalColumns * kFinalSlices) void norm_finalize_ke
 }
 
 // ---- dropout over a flat tensor ----------------------------------------------------------------
-constexpr uint64_t kCachedBytes = 64ull << 20;
-constexpr int kDropGroups = 2;          // groups of eight per lane, a workgroup's width apart
+// 8192 x 8192 bfloat16: 45 us, 5.9 TB/s.  The generator's 18 wide multiplies per
+// eight elements take some 34 us of the vector ALU, which the accesses hide.
+// Two groups of eight per lane, a workgroup's width apart: 44.6 us, with one
+// 46.7, with four 47.0 (16384 x 4096 float16).
+constexpr int kDropGroups = 2;
+// A 16-bit input larger than this is read around the caches, where little of
+// it would be found: 134 MB 45.0 against 46.3 us, but 67 MB 24.5 against 22.0
+// and 13 MB 7.2 against 6.4.  Float32, whose lanes touch a line twice, always
+// reads through them (134 MB: 51.2 against 53.0 us).
+constexpr uint64_t kCachedBytes = 96ull << 20;
 
 template <class T, bool EVEN, bool NT>
 __global__ __launch_bounds__(kBlock) void dropout_kernel(const void *x, void *y, uint64_t n, Mask mask) {
@@ -834,10 +873,18 @@ __global__ __launch_bounds__(kBlock) void dropout_kernel(const void *x, void *y,
 constexpr uint32_t kColumnGroups = 256;                 // row groups of the column sums of rows past the tilings
 constexpr uint64_t kMaxPartials = 256ull << 20;         // bytes of their workspace
 constexpr uint64_t kMaxWidth = 1ull << 24;              // exact in float32, and the finalize stays below 2**32 lanes
-constexpr uint32_t kSimds = 256 * 4;                    // launches stride over rows with as many waves as are resident
-constexpr uint32_t kBackwardWaves = 4;                  // per SIMD
+constexpr uint32_t kSimds = 256 * 4;
+constexpr uint32_t kBackwardWaves = 4;                  // per SIMD; with 2, the edge of 16384 x 4096: 145 us, not 126
+// Up to this many rows the backward launch sums columns in workgroups of its
+// own.  Kernel times with them and with partial sums: 129 x 8192 float16 5.8
+// and 13.6 us, 512 x 776 bfloat16 5.5 and 10.1, 512 x 4096 9.2 and 13.7; but
+// 1024 x 784 11.3 and 10.1.
 constexpr uint64_t kFewRows = 512;
-constexpr uint64_t kFewLanes = kSimds * 4 * 64;        // of rows: a workgroup's worth of waves on every SIMD pair
+// A forward launch of at most this many lanes at one group a lane (16 waves a
+// CU) takes one group a lane: 1 x 768 2.8 us (three groups 3.6), 512 x 760 4.3
+// (5.5), 2048 x 744 5.2 (5.6); past it the idle lanes cost more, 8192 x 768
+// 10.2 (6.6).
+constexpr uint64_t kFewLanes = kSimds * 4 * 64;
 
 // How a row is laid over lanes; parts == 0: it does not fit.
 struct RowTiling {
@@ -846,7 +893,9 @@ struct RowTiling {
 
 // The forward pass: the tiling that leaves the fewest lanes idle, of equals
 // the one with the fewest lanes.  Where the rows do not fill the chip, one
-// group a lane: a row's latency counts, not its share of a workgroup.
+// group a lane: a row's latency counts, not its share of a workgroup.  Float32
+// takes one group (32 bytes) a lane as far as that reaches: edge 8192 x 2048
+// 52.9 us, with two 58.9.
 static RowTiling forward_tiling(uint64_t rows, uint32_t width, int32_t dtype) {
     const uint32_t groups = (width + kGroup - 1) / kGroup;
     RowTiling best{0, 0, 0};
@@ -861,8 +910,9 @@ static RowTiling forward_tiling(uint64_t rows, uint32_t width, int32_t dtype) {
     return best;
 }
 
-// The backward pass: as above among what 128 registers a lane hold (three
-// groups of a 16-bit type, two of float32), in workgroups of kBackwardThreads.
+// The backward pass: as above with at most two groups a lane, which 128
+// registers hold (8192 x 768 bfloat16: 12.7 us, with three groups 14.5), and
+// one of float32 (8192 x 2048: 39.4 us, with two 41.4).
 static RowTiling backward_tiling(uint32_t width, int32_t dtype) {
     const uint32_t groups = (width + kGroup - 1) / kGroup;
     RowTiling best{0, 0, 0};

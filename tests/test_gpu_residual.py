@@ -550,8 +550,8 @@ def test_every_tiling(width):
 
 @pytest.mark.parametrize("shift", [0, 1])
 def test_dropout_of_a_large_tensor(shift):
-    """Past 64 MiB, where a 16-bit input is read around the caches."""
-    count = (33 << 20) + 5
+    """Past 96 MiB, where a 16-bit input is read around the caches."""
+    count = (52 << 20) + 5
     room = nt.DeviceArray.empty((count + shift,), "bfloat16", DEV)
     room.fill_bits(0x4040)                                  # 3.0
     x = nt.Tensor._from_storage(room.narrow(shift, count))
