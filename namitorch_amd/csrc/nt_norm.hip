@@ -97,6 +97,10 @@ __device__ __forceinline__ float block_sum_f32(float v, float *shared) {
 // alignment).  Norms read through the caches: their inputs were just written
 // by a product or an earlier edge (8192 x 768 bfloat16 forward: 6.9 us, with
 // nontemporal loads 10.8), and store around them (temporal stores 8.2 us).
+// Float32's two accesses each leave half of a line, which the caches join:
+// its aligned stores go through them (edge 8192 x 2048: 49.4 us, around them
+// 53.6; dropout of 25 MB 10.8 and 12.4), unaligned ones do not (norm backward
+// 8192 x 1001: 23.0 us through them, 19.8 around).
 constexpr int kGroup = 8;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
@@ -126,7 +130,7 @@ __device__ __forceinline__ void store8(void *base, uint64_t i, const Raw8<T> &in
     auto *p = reinterpret_cast<typename T::raw *>(base) + i;
 #pragma unroll
     for (int k = 0; k < Raw8<T>::kWords; ++k) {
-        if constexpr (EVEN) gstore<true, u32x4, gu32x4>(p + k * 4, in.w[k]);
+        if constexpr (EVEN) gstore<T::code != NT_F32, u32x4, gu32x4>(p + k * 4, in.w[k]);
         else gstore<true, u32x4, gu32x4_any>(p + k * 4, in.w[k]);
     }
 }
@@ -895,7 +899,7 @@ struct RowTiling {
 // the one with the fewest lanes.  Where the rows do not fill the chip, one
 // group a lane: a row's latency counts, not its share of a workgroup.  Float32
 // takes one group (32 bytes) a lane as far as that reaches: edge 8192 x 2048
-// 52.9 us, with two 58.9.
+// 52.9 us, with two 58.9 (before its stores went through the caches).
 static RowTiling forward_tiling(uint64_t rows, uint32_t width, int32_t dtype) {
     const uint32_t groups = (width + kGroup - 1) / kGroup;
     RowTiling best{0, 0, 0};
