@@ -1,10 +1,10 @@
 """Build recipe of the gfx950 shared library ``libnamitorch_amd.so``.
 
-One ``hipcc`` invocation compiles every ``csrc/*.hip`` file for gfx950 (and the
-host-only ``csrc/*.cpp``) and
-links them into ``namitorch_amd/_lib/libnamitorch_amd.so`` (in-tree, so the
-built library travels with the source tree).  The flags fix the numerics the
-kernels rely on:
+``hipcc`` compiles every ``csrc/*.hip`` file for gfx950 (and the host-only
+``csrc/*.cpp``), several at a time, and links them into
+``namitorch_amd/_lib/libnamitorch_amd.so`` (in-tree, so the built library
+travels with the source tree).  The flags fix the numerics the kernels rely
+on:
 
 * ``-ffp-contract=off`` — no FMA contraction: each fp32 multiply and add
   rounds separately, as NumPy's ufuncs do;
@@ -23,6 +23,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PACKAGE_DIR = Path(__file__).resolve().parent
@@ -51,36 +53,48 @@ def sources() -> list[Path]:
     return sorted(SOURCE_DIR.glob("*.hip")) + sorted(SOURCE_DIR.glob("*.cpp"))
 
 
-def command(output: Path = LIB_PATH) -> list[str]:
+def compile_command(source: Path, output: Path) -> list[str]:
     return [
         hipcc(),
         f"--offload-arch={ARCH}",
         "-O3",
         "-std=c++17",
         "-fPIC",
-        "-shared",
         *NUMERIC_FLAGS,
         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
         "-Wall",
         "-Wno-unused-function",
         f"-I{INCLUDE_DIR}",
-        *(str(path) for path in sources()),
+        "-c", str(source),
         "-o", str(output),
     ]
+
+
+def link_command(objects: list[Path], output: Path = LIB_PATH) -> list[str]:
+    return [hipcc(), f"--offload-arch={ARCH}", "-fPIC", "-shared", *map(str, objects), "-o", str(output)]
+
+
+def _run(cmd: list[str], verbose: bool) -> None:
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    result = subprocess.run(cmd, capture_output=True, text=True)
+    if result.returncode != 0:
+        raise RuntimeError(f"hipcc failed ({result.returncode}):\n{result.stdout}\n{result.stderr}")
 
 
 def build(verbose: bool = False) -> Path:
     """Compile the library for gfx950; returns the path of the built .so."""
     LIB_DIR.mkdir(exist_ok=True)
     temporary = LIB_PATH.with_name(LIB_PATH.name + f".tmp{os.getpid()}")
-    cmd = command(temporary)
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    result = subprocess.run(cmd, capture_output=True, text=True)
-    if result.returncode != 0:
-        temporary.unlink(missing_ok=True)
-        raise RuntimeError(f"hipcc failed ({result.returncode}):\n{result.stdout}\n{result.stderr}")
-    os.replace(temporary, LIB_PATH)
+    with tempfile.TemporaryDirectory() as folder:
+        jobs = [(source, Path(folder) / (source.name + ".o")) for source in sources()]
+        with ThreadPoolExecutor(max_workers=8) as pool:
+            list(pool.map(lambda job: _run(compile_command(*job), verbose), jobs))
+        try:
+            _run(link_command([output for _, output in jobs], temporary), verbose)
+            os.replace(temporary, LIB_PATH)
+        finally:
+            temporary.unlink(missing_ok=True)
     return LIB_PATH
 
 
