@@ -944,13 +944,13 @@ static uint32_t backward_room(const RowTiling &g) {
 // Whether the backward launch of `rows` rows sums columns in workgroups of its own.
 static bool takes_columns(uint64_t rows, const RowTiling &g) { return g.parts != 0 && rows <= kFewRows; }
 
-// Workgroups for `rows` rows, `per_block` at a time: at most `most`, all with
-// the same number of rounds but the last.
+// Workgroups for `rows` rows, `per_block` at a time: all that are resident
+// (`most`) where there is work for them.  Fewer with the same number of rounds
+// each leave some CUs a workgroup short: 5003 x 1001 float32 11.3 us with 626,
+// 10.5 with 1024; 40001 x 512 float16 15.3 and 14.1.
 static uint32_t row_grid(uint64_t rows, uint32_t per_block, uint32_t most) {
     const uint64_t blocks = (rows + per_block - 1) / per_block;
-    if (blocks <= most) return blocks < 1 ? 1u : (uint32_t)blocks;
-    const uint64_t rounds = (blocks + most - 1) / most;
-    return (uint32_t)((blocks + rounds - 1) / rounds);
+    return blocks > most ? most : blocks < 1 ? 1u : (uint32_t)blocks;
 }
 
 static uint32_t column_groups(uint64_t rows, uint64_t width) {
