@@ -31,7 +31,8 @@ the order of the results (``None`` entries are allocated).  They overlap
 neither inputs nor one another; ``dropout`` may write its own input.  Launches
 go to the calling thread's current stream.  In a stream capture the forward
 calls run when ``out`` names every result and nothing is dropped (a replay
-would repeat the mask); the others raise.
+would repeat the mask); the others raise, and so does a call that is given a
+gradient whose accumulation or unscaling is still deferred.
 """
 
 from __future__ import annotations
@@ -52,6 +53,16 @@ _MAX_SEED = 1 << 64
 
 
 # ---- arguments ----------------------------------------------------------------------------------
+def _current(value: Tensor) -> Tensor:
+    """`value` with its deferred accumulation and transform written back.  In
+    a capture that write would be recorded instead of run, while the marker
+    that asks for it is gone: refused, as every in-place write there."""
+    if value._pending is not None or value._incoming is not None:
+        reject_during_capture("In-place Tensor updates")
+        value._materialize()
+    return value
+
+
 def _activation(value, name: str, like: Tensor | None = None) -> int:
     """Address of an activation (or gradient) Tensor, of `like`'s shape, dtype and device."""
     if not isinstance(value, Tensor):
@@ -70,9 +81,7 @@ def _activation(value, name: str, like: Tensor | None = None) -> int:
             raise TypeError(f"{name} has dtype {value._dtype.name}; expected {like._dtype.name}.")
         if value._device is not like._device:
             ensure_same_device(like, value)
-    if value._pending is not None or value._incoming is not None:
-        value._materialize()
-    return value._ptr
+    return _current(value)._ptr
 
 
 def _affine(value, name: str, shape: tuple, like: Tensor) -> int | None:
@@ -87,9 +96,7 @@ def _affine(value, name: str, shape: tuple, like: Tensor) -> int | None:
         raise TypeError(f"{name} must be {like._dtype.name} or float32, got {value._dtype.name}.")
     if value._device is not like._device:
         ensure_same_device(like, value)
-    if value._pending is not None or value._incoming is not None:
-        value._materialize()
-    return value._ptr
+    return _current(value)._ptr
 
 
 def _affine_pair(weight, bias, shape: tuple, like: Tensor) -> tuple:
@@ -110,9 +117,7 @@ def _statistic(value, name: str, shape: tuple, like: Tensor) -> int:
         raise TypeError(f"{name} must be float32, got {value._dtype.name}.")
     if value._device is not like._device:
         ensure_same_device(like, value)
-    if value._pending is not None or value._incoming is not None:
-        value._materialize()
-    return value._ptr
+    return _current(value)._ptr
 
 
 def _normalized(value: Tensor, normalized_shape) -> tuple:
@@ -199,6 +204,9 @@ def _result(given, name: str, shape: tuple, dtype, like: Tensor) -> Tensor:
     if given._device is not like._device:
         ensure_same_device(like, given)
     given._check_inplace()
+    if given._pending is not None or given._incoming is not None:
+        # The launch replaces what is deferred; one that is only recorded does not yet.
+        reject_during_capture("In-place Tensor updates")
     return given
 
 
