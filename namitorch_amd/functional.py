@@ -179,6 +179,19 @@ def _training_threshold(p, training) -> int:
     return 0
 
 
+def _edge_mask(x: Tensor, p, training, seed, offset) -> tuple:
+    """(threshold, seed, offset) of an edge's dropout.  A call that draws
+    numbers names its seed: with a common default every edge of every step
+    would drop the same elements."""
+    threshold = _training_threshold(p, training)
+    if seed is None:
+        if threshold and x._numel:
+            reject_during_capture("Dropout")
+            raise TypeError("seed is needed where elements are dropped (p > 0 in training).")
+        seed = 0
+    return threshold, _counter(seed, "seed"), _counter(offset, "offset")
+
+
 # ---- results ------------------------------------------------------------------------------------
 def _given(out, count: int) -> tuple:
     """The `out` argument as `count` entries."""
@@ -330,16 +343,16 @@ def _dropout(x, p, training, seed, offset, out, name: str) -> Tensor:
 
 # ---- the residual edge ------------------------------------------------------------------------------
 def dropout_add_layer_norm(input, residual, normalized_shape, weight=None, bias=None, p=0.0, eps=1e-5,
-                           training=True, *, seed=0, offset=0, out=None) -> tuple:
+                           training=True, *, seed=None, offset=0, out=None) -> tuple:
     """``(output, total)`` with ``total = dropout(input) + residual`` and
     ``output`` the layer norm of it.  The norm is taken before ``total`` is
-    rounded to its dtype."""
+    rounded to its dtype.  ``seed`` is needed where elements are dropped."""
     return _edge(input, residual, normalized_shape, weight, bias, p, eps, training, seed, offset, _given(out, 2),
                  False)[:2]
 
 
 def dropout_add_layer_norm_forward(input, residual, normalized_shape, weight=None, bias=None, p=0.0, eps=1e-5,
-                                   training=True, *, seed=0, offset=0, out=None) -> tuple:
+                                   training=True, *, seed=None, offset=0, out=None) -> tuple:
     """``(output, total, mean, rstd)``: :func:`dropout_add_layer_norm` with
     the statistics that its backward call reads."""
     return _edge(input, residual, normalized_shape, weight, bias, p, eps, training, seed, offset, _given(out, 4), True)
@@ -351,8 +364,7 @@ def _edge(x, residual, normalized_shape, weight, bias, p, eps, training, seed, o
     lead, shape, rows, width = _normalized(x, normalized_shape)
     scale, shift, code = _affine_pair(weight, bias, shape, x)
     eps = _epsilon(eps)
-    threshold = _training_threshold(p, training)
-    seed, offset = _counter(seed, "seed"), _counter(offset, "offset")
+    threshold, seed, offset = _edge_mask(x, p, training, seed, offset)
     if None in given:
         reject_during_capture("Dropout" if threshold else "Layer norm without out")
     y = _result(given[0], "output", x._shape, x._dtype, x)
@@ -369,7 +381,7 @@ def _edge(x, residual, normalized_shape, weight, bias, p, eps, training, seed, o
 
 
 def dropout_add_layer_norm_backward(grad_output, grad_total, total, mean, rstd, weight=None, bias=None, p=0.0,
-                                    training=True, *, seed=0, offset=0, out=None) -> tuple:
+                                    training=True, *, seed=None, offset=0, out=None) -> tuple:
     """``(grad_input, grad_residual, grad_weight, grad_bias)`` of
     :func:`dropout_add_layer_norm_forward`, from the gradients of its two
     results (``grad_total`` None: nothing else reads ``total``)."""
@@ -379,8 +391,7 @@ def dropout_add_layer_norm_backward(grad_output, grad_total, total, mean, rstd, 
     dt = None if grad_total is None else _activation(grad_total, "grad_total", total)
     _, shape, rows, width, mean_at, rstd_at = _kept(total, mean, rstd)
     scale, _, code = _affine_pair(weight, bias, shape, total)
-    threshold = _training_threshold(p, training)
-    seed, offset = _counter(seed, "seed"), _counter(offset, "offset")
+    threshold, seed, offset = _edge_mask(total, p, training, seed, offset)
     if None in given:
         reject_during_capture("Layer norm backward")
     dx = _result(given[0], "grad_input", total._shape, total._dtype, total)
