@@ -50,6 +50,9 @@ from .tensor import Tensor, device_views
 
 _DTYPES = frozenset((float16, bfloat16, float32))
 _MAX_SEED = 1 << 64
+# Of float32, in which the kernels add it: past the most rstd would be zero, and
+# below the least a constant row, which is its bias, would be NaN.
+_LEAST_EPS, _MOST_EPS = 2.0 ** -149, (2.0 - 2.0 ** -23) * 2.0 ** 127
 
 
 # ---- arguments ----------------------------------------------------------------------------------
@@ -144,8 +147,8 @@ def _epsilon(eps) -> float:
         if isinstance(eps, bool) or not isinstance(eps, Real):
             raise TypeError("eps must be a real number.")
         eps = float(eps)
-    if not 0.0 <= eps < math.inf:
-        raise ValueError(f"eps must be finite and nonnegative, got {eps}.")
+    if eps != 0.0 and not _LEAST_EPS <= eps <= _MOST_EPS:
+        raise ValueError(f"eps must be finite and nonnegative as a float32, got {eps}.")
     return eps
 
 
