@@ -715,7 +715,10 @@ __global__ __launch_bounds__(THREADS, 4) void norm_backward_kernel(NormBackward 
 
 // ---- rows of any width: a workgroup per row, the row read once per pass ---------------------
 // For rows past the tilings (16384 columns).  Bound by the three passes over
-// the row, an element at a time, from the caches.
+// the row, an element at a time, from the caches.  A lane's share of a row is
+// summed in 64 bits: it is one chain of width / 256 additions (65536 at the
+// widest), which in float32 put the mean of 2^20 values of 0.1 off by 4e-5 of
+// it, and the outputs of 2^24 of them, which are the bias, off by 0.02.
 template <class T, int EDGE>
 __device__ __forceinline__ float row_value(const NormForward &a, uint64_t i) {
     float v = load1<T>(reinterpret_cast<const typename T::raw *>(a.x), i);
@@ -730,19 +733,19 @@ __global__ __launch_bounds__(kBlock) void norm_rows_kernel(NormForward a) {
     const float width = (float)a.width;
     for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const uint64_t base = row * a.width;
-        float sum = 0.0f;
+        double sum = 0.0;
         for (uint32_t c = threadIdx.x; c < a.width; c += kBlock) {
             const float v = row_value<T, EDGE>(a, base + c);
             if constexpr (EDGE != kNone) store1<T>(reinterpret_cast<typename T::raw *>(a.total), base + c, v);
             sum += v;
         }
-        const float mean = block_sum_f32(sum, shared) / width;
-        float squares = 0.0f;
+        const float mean = block_sum_f32((float)sum, shared) / width;
+        double squares = 0.0;
         for (uint32_t c = threadIdx.x; c < a.width; c += kBlock) {
             const float d = row_value<T, EDGE>(a, base + c) - mean;
-            squares = __builtin_fmaf(d, d, squares);
+            squares = __builtin_fma((double)d, (double)d, squares);
         }
-        const float rstd = 1.0f / __builtin_sqrtf(block_sum_f32(squares, shared) / width + a.eps);
+        const float rstd = 1.0f / __builtin_sqrtf(block_sum_f32((float)squares, shared) / width + a.eps);
         for (uint32_t c = threadIdx.x; c < a.width; c += kBlock) {
             const float h = (row_value<T, EDGE>(a, base + c) - mean) * rstd;
             store1<T>(reinterpret_cast<typename T::raw *>(a.y), base + c,
@@ -766,14 +769,14 @@ __global__ __launch_bounds__(kBlock) void norm_rows_backward_kernel(NormBackward
     for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const uint64_t base = row * a.width;
         const float mean = a.mean[row], rstd = a.rstd[row];
-        float level = 0.0f, along = 0.0f;
+        double levels = 0.0, alongs = 0.0;
         for (uint32_t c = threadIdx.x; c < a.width; c += kBlock) {
             const float g = load1<T>(dy, base + c) * load_param(a.weight, a.weight_dtype, c, 1.0f);
-            level += g;
-            along = __builtin_fmaf(g, (load1<T>(t, base + c) - mean) * rstd, along);
+            levels += g;
+            alongs = __builtin_fma((double)g, (double)((load1<T>(t, base + c) - mean) * rstd), alongs);
         }
-        level = block_sum_f32(level, shared) / width;
-        along = block_sum_f32(along, shared) / width;
+        const float level = block_sum_f32((float)levels, shared) / width;
+        const float along = block_sum_f32((float)alongs, shared) / width;
         for (uint32_t c = threadIdx.x; c < a.width; c += kBlock) {
             const float g = load1<T>(dy, base + c) * load_param(a.weight, a.weight_dtype, c, 1.0f);
             const float h = (load1<T>(t, base + c) - mean) * rstd;
