@@ -28,6 +28,7 @@
 #include "nt_internal.hpp"
 #include "nt_philox.hpp"
 #include "nt_pool.hpp"
+#include "nt_rows.hpp"
 
 namespace nt {
 
@@ -101,7 +102,6 @@ __device__ __forceinline__ float block_sum_f32(float v, float *shared) {
 // its aligned stores go through them (edge 8192 x 2048: 49.4 us, around them
 // 53.6; dropout of 25 MB 10.8 and 12.4), unaligned ones do not (norm backward
 // 8192 x 1001: 23.0 us through them, 19.8 around).
-constexpr int kGroup = 8;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 typedef __attribute__((address_space(1))) u32x4 gu32x4;
@@ -190,25 +190,6 @@ __device__ __forceinline__ void store_end(void *base, uint64_t i, const Raw8<T> 
     }
 }
 
-// The group of a lane: eight columns from `column` on (the width where the
-// lane has none).  The last group of a row whose width is no multiple of
-// eight ends at the row's end and starts inside the group before it: its
-// elements below `first` are the other lane's, computed alike by both.  So it
-// too is loaded and stored whole; only rows of less than eight go element by
-// element.  Element loads at every end made each wave wait before it asked for
-// its next row (10006 x 1001 bfloat16: norm 14.4 -> 12.8 us, edge 26.0 -> 22.6).
-struct Columns {
-    uint32_t column, first;
-    __device__ __forceinline__ Columns() {}
-    __device__ __forceinline__ Columns(uint32_t c, uint32_t width)
-        : column(c < width && c + kGroup > width && width >= kGroup ? width - kGroup : c < width ? c : width),
-          first(c - column) {}
-    template <bool EVEN>
-    __device__ __forceinline__ bool has(uint32_t k, uint32_t width) const {
-        return EVEN ? column < width : k >= first && column + k < width;
-    }
-};
-
 template <class T, bool EVEN>
 __device__ __forceinline__ void load_part(Raw8<T> &out, const void *base, uint64_t row, uint32_t c, uint32_t width) {
     if (EVEN || width >= kGroup) load8<T, EVEN>(out, base, row + c);
@@ -278,9 +259,6 @@ __device__ __forceinline__ void drop8(float (&v)[8], const PhiloxWords &words, c
 // is on its way while this one is summed.  Weight and bias wait in LDS: in
 // registers they left room for five waves per SIMD instead of eight (16384 x
 // 4096 float16 forward: 59 us with them, 49 without).
-constexpr int kRowThreads = 512;        // lanes of a workgroup, for rows of at most as many
-constexpr int kBackwardThreads = 512;   // the same of the backward pass
-constexpr int kWideThreads = 1024;      // of a workgroup, for rows of more
 
 // Sum over the `lanes` lanes of a row, the same on each.  Rows of several
 // waves go through `shared`, of which consecutive sums use the two halves in
@@ -880,60 +858,12 @@ __global__ __launch_bounds__(kBlock) void dropout_kernel(const void *x, void *y,
 constexpr uint32_t kColumnGroups = 256;                 // row groups of the column sums of rows past the tilings
 constexpr uint64_t kMaxPartials = 256ull << 20;         // bytes of their workspace
 constexpr uint64_t kMaxWidth = 1ull << 24;              // exact in float32, and the finalize stays below 2**32 lanes
-constexpr uint32_t kSimds = 256 * 4;
 constexpr uint32_t kBackwardWaves = 4;                  // per SIMD; with 2, the edge of 16384 x 4096: 145 us, not 126
 // Up to this many rows the backward launch sums columns in workgroups of its
 // own.  Kernel times with them and with partial sums: 129 x 8192 float16 5.8
 // and 13.6 us, 512 x 776 bfloat16 5.5 and 10.1, 512 x 4096 9.2 and 13.7; but
 // 1024 x 784 11.3 and 10.1.
 constexpr uint64_t kFewRows = 512;
-// A forward launch of at most this many lanes at one group a lane (16 waves a
-// CU) takes one group a lane: 1 x 768 2.8 us (three groups 3.6), 512 x 760 4.3
-// (5.5), 2048 x 744 5.2 (5.6); past it the idle lanes cost more, 8192 x 768
-// 10.2 (6.6).
-constexpr uint64_t kFewLanes = kSimds * 4 * 64;
-
-// How a row is laid over lanes; parts == 0: it does not fit.
-struct RowTiling {
-    uint32_t lanes, parts, threads;
-};
-
-// The forward pass: the tiling that leaves the fewest lanes idle, of equals
-// the one with the fewest lanes.  Where the rows do not fill the chip, one
-// group a lane: a row's latency counts, not its share of a workgroup.  Float32
-// takes one group (32 bytes) a lane as far as that reaches: edge 8192 x 2048
-// 52.9 us, with two 58.9 (before its stores went through the caches).
-static RowTiling forward_tiling(uint64_t rows, uint32_t width, int32_t dtype) {
-    const uint32_t groups = (width + kGroup - 1) / kGroup;
-    RowTiling best{0, 0, 0};
-    for (uint32_t parts = dtype == NT_F32 ? 2 : 3; parts >= 1; --parts) {
-        uint32_t lanes = 1;
-        while (lanes * parts < groups) lanes <<= 1;
-        if (lanes > (uint32_t)kWideThreads || (lanes > (uint32_t)kRowThreads && parts > 2)) continue;
-        const bool one = parts == 1 && (dtype == NT_F32 || rows * lanes <= kFewLanes);
-        if (best.parts == 0 || one || lanes * parts < best.lanes * best.parts)
-            best = RowTiling{lanes, parts, uint32_t(lanes <= (uint32_t)kRowThreads ? kRowThreads : kWideThreads)};
-    }
-    return best;
-}
-
-// The backward pass: as above with at most two groups a lane, which 128
-// registers hold (8192 x 768 bfloat16: 12.7 us, with three groups 14.5), and
-// one of float32 (8192 x 2048: 39.4 us, with two 41.4).
-static RowTiling backward_tiling(uint32_t width, int32_t dtype) {
-    const uint32_t groups = (width + kGroup - 1) / kGroup;
-    RowTiling best{0, 0, 0};
-    for (uint32_t parts = 2; parts >= 1; --parts) {
-        uint32_t lanes = 1;
-        while (lanes * parts < groups) lanes <<= 1;
-        if (lanes > (uint32_t)kWideThreads) continue;
-        if (best.parts == 0 || lanes * parts < best.lanes * best.parts || dtype == NT_F32)
-            best = RowTiling{lanes, parts,
-                             uint32_t(lanes <= (uint32_t)kBackwardThreads ? kBackwardThreads : kWideThreads)};
-    }
-    return best;
-}
-
 // LDS of norm_backward_kernel: the weights, half of the rows that are joined,
 // or a column tile's sums of each wave.
 static uint32_t backward_room(const RowTiling &g) {
@@ -980,10 +910,13 @@ static void launch_norm(const NormForward &a, const RowTiling &g, hipStream_t s)
     constexpr uint32_t waves = kSimds * (uint32_t)forward_waves<T, EDGE, PARTS>();
     const dim3 grid(row_grid(a.rows, g.threads / g.lanes, waves * 64u / g.threads)), block(g.threads);
     const uint32_t room = g.lanes * g.parts * kGroup * 8u;
-    if (g.threads == (uint32_t)kRowThreads)
-        norm_kernel<T, EDGE, PARTS, EVEN, kRowThreads><<<grid, block, room, s>>>(a, g.lanes);
-    else if constexpr (PARTS <= 2)
-        norm_kernel<T, EDGE, PARTS, EVEN, kWideThreads><<<grid, block, room, s>>>(a, g.lanes);
+    if (g.threads == (uint32_t)kRowThreads) {
+        if constexpr (forward_makes<T::code, PARTS, kRowThreads>())
+            norm_kernel<T, EDGE, PARTS, EVEN, kRowThreads><<<grid, block, room, s>>>(a, g.lanes);
+    } else {
+        if constexpr (forward_makes<T::code, PARTS, kWideThreads>())
+            norm_kernel<T, EDGE, PARTS, EVEN, kWideThreads><<<grid, block, room, s>>>(a, g.lanes);
+    }
 }
 
 template <class T, int EDGE, int PARTS, bool EVEN>
@@ -991,9 +924,13 @@ static void launch_norm_backward(const NormBackward &a, const RowTiling &g, hipS
     const bool columns = a.partials == nullptr && (a.dw != nullptr || a.db != nullptr);
     const dim3 grid(a.row_blocks + (columns ? (a.width + 63u) / 64u : 0u)), block(g.threads);
     const uint32_t room = backward_room(g);
-    if (g.threads == (uint32_t)kBackwardThreads)
-        norm_backward_kernel<T, EDGE, PARTS, EVEN, kBackwardThreads><<<grid, block, room, s>>>(a, g.lanes);
-    else norm_backward_kernel<T, EDGE, PARTS, EVEN, kWideThreads><<<grid, block, room, s>>>(a, g.lanes);
+    if (g.threads == (uint32_t)kBackwardThreads) {
+        if constexpr (backward_makes<T::code, PARTS, kBackwardThreads>())
+            norm_backward_kernel<T, EDGE, PARTS, EVEN, kBackwardThreads><<<grid, block, room, s>>>(a, g.lanes);
+    } else {
+        if constexpr (backward_makes<T::code, PARTS, kWideThreads>())
+            norm_backward_kernel<T, EDGE, PARTS, EVEN, kWideThreads><<<grid, block, room, s>>>(a, g.lanes);
+    }
 }
 
 // Calls launch(parts, even) with both as constants.
@@ -1060,10 +997,15 @@ template <class T>
 static void launch_dropout(const void *x, void *y, uint64_t n, const Mask &mask, hipStream_t s) {
     const uint64_t tile = (uint64_t)kBlock * kGroup * kDropGroups;
     const dim3 grid(strided_grid((n + tile - 1) / tile, kBlock)), block(kBlock);
-    const bool even = aligned16({x, y}), past = T::code != NT_F32 && n * sizeof(typename T::raw) > kCachedBytes;
-    if (even && past) dropout_kernel<T, true, true><<<grid, block, 0, s>>>(x, y, n, mask);
-    else if (even) dropout_kernel<T, true, false><<<grid, block, 0, s>>>(x, y, n, mask);
-    else if (past) dropout_kernel<T, false, true><<<grid, block, 0, s>>>(x, y, n, mask);
+    const bool even = aligned16({x, y});
+    if constexpr (T::code != NT_F32) {
+        if (n * sizeof(typename T::raw) > kCachedBytes) {
+            if (even) dropout_kernel<T, true, true><<<grid, block, 0, s>>>(x, y, n, mask);
+            else dropout_kernel<T, false, true><<<grid, block, 0, s>>>(x, y, n, mask);
+            return;
+        }
+    }
+    if (even) dropout_kernel<T, true, false><<<grid, block, 0, s>>>(x, y, n, mask);
     else dropout_kernel<T, false, false><<<grid, block, 0, s>>>(x, y, n, mask);
 }
 
