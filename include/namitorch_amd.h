@@ -547,10 +547,10 @@ int32_t nt_any_negative(const void *array, int32_t dtype, uint64_t count,
  * weight, bias and their gradients; NULL weight is ones, NULL bias zeros.
  * mean and rstd (float32, one per row) are written when not NULL (both or
  * neither) and are what the backward entry reads.  A NULL dweight or dbias
- * is not computed.  Sums are float32 in a fixed order; values are rounded
- * once, when stored.  A row holding an infinity or NaN gives NaN outputs.
- * Outputs overlap neither inputs nor one another.  Work is queued on
- * `stream` of `device`; the backward entries take their workspace from the
+ * is not computed.  Sums are float32 (a lane's share of a row past 16384
+ * columns 64 bits) in a fixed order; values are rounded once, when stored.
+ * A row holding an infinity or NaN gives NaN outputs.  Outputs overlap
+ * neither inputs nor one another.  Work is queued on `stream` of `device`; the backward entries take their workspace from the
  * library's pool in that stream's order.  They, and what draws a mask, refuse
  * (NT_ERR_RUNTIME) a stream in capture: a replay would use a workspace handed
  * to others since, or repeat the mask.  With no rows the forward entries do

@@ -10,7 +10,8 @@
 //   dt   = rstd (g - sum g / W - h sum(g h) / W)   (+ the gradient that the sum gets from elsewhere)
 //   dw   = sum over rows of dy h,   db = sum over rows of dy.
 //
-// Every sum and statistic is float32; values are rounded once, when stored.
+// Every sum and statistic is float32 (a lane's share of a very long row 64
+// bits); values are rounded once, when stored.
 // The sums over rows run in a fixed order, so gradients do not change from
 // run to run.
 //
@@ -308,9 +309,15 @@ struct RowSum {
     }
 };
 
-// Waves per SIMD that the forward pass's registers leave room for, and that a
-// launch has: more only queue up (65536 x 768 float16: 38.9 us with the
-// resident waves, 41.6 with twice as many).
+// Waves per SIMD that the compiler leaves registers for, and that the grid of
+// a launch is made for: more only queue up, each loading weight and bias again
+// (65536 x 768 float16: 38.9 us with the resident waves, 41.6 with twice as
+// many).  It is a floor: edges of one group a lane take 64 to 78 registers,
+// room for 6 or 7.  It does not look at LDS, of which weight and bias take 8
+// bytes a column: 16-bit norms of 6145 to 8192 columns (64 KB) run 4 waves per
+// SIMD, 16-bit rows of 8193 to 12288 (96 KB, 512 lanes) 2 and 16-bit norms of
+// 12289 to 16384 4, on grids made for twice as many and more (2048 rows of
+// bfloat16: 6144 columns 11.1 us, 8192 17.9, 12288 30.1, 16384 37.8).
 template <class T, int EDGE, int PARTS>
 constexpr int forward_waves() {
     return EDGE != kNone || PARTS > 2 || (T::code == NT_F32 && PARTS == 2) ? 4 : 8;
@@ -693,10 +700,12 @@ __global__ __launch_bounds__(THREADS, 4) void norm_backward_kernel(NormBackward 
 
 // ---- rows of any width: a workgroup per row, the row read once per pass ---------------------
 // For rows past the tilings (16384 columns).  Bound by the three passes over
-// the row, an element at a time, from the caches.  A lane's share of a row is
-// summed in 64 bits: it is one chain of width / 256 additions (65536 at the
-// widest), which in float32 put the mean of 2^20 values of 0.1 off by 4e-5 of
-// it, and the outputs of 2^24 of them, which are the bias, off by 0.02.
+// the row, an element at a time, from the caches, and in edges that drop by a
+// whole call of the generator for every element of every pass (512 x 32768
+// bfloat16: norm 115 us, backward 142, edge 185 and 182).  A lane's share of a
+// row is summed in 64 bits: it is one chain of width / 256 additions (65536 at
+// the widest), which in float32 put the mean of 2^20 values of 0.1 off by 4e-5
+// of it, and the outputs of 2^24 of them, which are the bias, off by 0.02.
 template <class T, int EDGE>
 __device__ __forceinline__ float row_value(const NormForward &a, uint64_t i) {
     float v = load1<T>(reinterpret_cast<const typename T::raw *>(a.x), i);
@@ -862,7 +871,10 @@ constexpr uint32_t kBackwardWaves = 4;                  // per SIMD; with 2, the
 // Up to this many rows the backward launch sums columns in workgroups of its
 // own.  Kernel times with them and with partial sums: 129 x 8192 float16 5.8
 // and 13.6 us, 512 x 776 bfloat16 5.5 and 10.1, 512 x 4096 9.2 and 13.7; but
-// 1024 x 784 11.3 and 10.1.
+// 1024 x 784 11.3 and 10.1.  The rule looks at rows alone, and wider ones would
+// gain past it: a workgroup holds one row of more than 4096 columns, so that
+// 513 x 8192 float16 has 512 rows of partial sums, 34 MB beside 25 MB of data
+// (a whole call 25.0 us; with 512 rows 12.6).
 constexpr uint64_t kFewRows = 512;
 // LDS of norm_backward_kernel: the weights, half of the rows that are joined,
 // or a column tile's sums of each wave.
@@ -877,10 +889,10 @@ static uint32_t backward_room(const RowTiling &g) {
 // Whether the backward launch of `rows` rows sums columns in workgroups of its own.
 static bool takes_columns(uint64_t rows, const RowTiling &g) { return g.parts != 0 && rows <= kFewRows; }
 
-// Workgroups for `rows` rows, `per_block` at a time: all that are resident
-// (`most`) where there is work for them.  Fewer with the same number of rounds
-// each leave some CUs a workgroup short: 5003 x 1001 float32 11.3 us with 626,
-// 10.5 with 1024; 40001 x 512 float16 15.3 and 14.1.
+// Workgroups for `rows` rows, `per_block` at a time: as many as the registers
+// leave resident (`most`) where there is work for them.  Fewer with the same
+// number of rounds each leave some CUs a workgroup short: 5003 x 1001 float32
+// 11.3 us with 626, 10.5 with 1024; 40001 x 512 float16 15.3 and 14.1.
 static uint32_t row_grid(uint64_t rows, uint32_t per_block, uint32_t most) {
     const uint64_t blocks = (rows + per_block - 1) / per_block;
     return blocks > most ? most : blocks < 1 ? 1u : (uint32_t)blocks;

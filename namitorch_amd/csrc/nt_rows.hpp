@@ -77,9 +77,12 @@ constexpr bool forward_makes() {
     return THREADS == kRowThreads ? PARTS == 1 || DTYPE != NT_F32 : PARTS <= 2;
 }
 
-// The backward pass: as above with at most two groups a lane, which 128
-// registers hold (8192 x 768 bfloat16: 12.7 us, with three groups 14.5), and
-// one of float32 (8192 x 2048: 39.4 us, with two 41.4).
+// The backward pass: as above with at most two groups a lane (8192 x 768
+// bfloat16: 12.7 us, with three groups 14.5), and one of float32 (8192 x 2048:
+// 39.4 us, with two 41.4).  128 registers hold them but for the float32 edge of
+// 8193 to 16384 columns, two groups a lane: 8 registers are spilled where it
+// drops, on ragged rows 129 (1 without dropout).  2048 x 12288 takes 122 us, x
+// 12289 147; float16, which spills none, 84 there.
 inline RowTiling backward_tiling(uint32_t width, int32_t dtype) {
     const uint32_t groups = (width + kGroup - 1) / kGroup;
     RowTiling best{0, 0, 0};
