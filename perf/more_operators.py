@@ -9,9 +9,9 @@ matrix products and its optimizer:
   the norm of ``total`` for the next block, and ``gated_grad``: its backward pass.
 
 With ``z = x W^T`` (rows ``i``, classes ``v``), target ``t_i`` and ``c`` rows that are not ignored:
-``lse_i = log sum_v exp z_iv``, ``loss_i = lse_i - z_i,t_i``, of which the mean (over ``c``) or each is returned;
-``dz_iv = g_i (exp(z_iv - lse_i) - [v = t_i])`` with ``g_i = grad_loss / c`` (or the row's own) and zero in ignored
-rows; ``dx = dz W``, ``dW = dz^T x``.
+``lse_i = log sum_v exp z_iv``, ``loss_i = lse_i - z_i,t_i``, both zero in ignored rows, of which the mean (over
+``c``), the sum or each is returned; ``dz_iv = g_i (exp(z_iv - lse_i) - [v = t_i])`` with ``g_i = grad_loss / c`` (or
+the sum's or the row's own) and zero in ignored rows; ``dx = dz W``, ``dW = dz^T x``.
 
 With ``N(x; w, b) = (x - mean) rstd w + b`` (``rms``: no mean): ``total = s r + a N(x; u, k)``, ``y = N(total; w, b)``
 and, given ``dy`` and what ``total`` gets from elsewhere, the gradients of ``x``, ``r``, ``u``, ``k``, ``a``, ``w``
@@ -30,6 +30,7 @@ _TORCH = {"float16": torch.float16, "bfloat16": torch.bfloat16, "float32": torch
 _SIZE = {"float16": 2, "bfloat16": 2, "float32": 4}
 _EPS = 1e-5
 _IGNORED = -100
+_SHARE_IGNORED = 0.1
 _MOST_WORK = 6 * 8192 * 32000 * 4096        # operations of the largest listed loss
 _MOST_LOGITS = 8192 * 50257                 # what the plain form holds at a time
 _MOST_WEIGHT = 32000 * 4096
@@ -133,7 +134,7 @@ def _loss_inputs(case, seed):
     x = torch.randn(rows, width, generator=generator, device="cuda").addcmul_(weight[target], lift)
     given = {"input": x.to(dtype), "weight": weight.to(dtype)}
     if rows > 1:
-        target[torch.rand(rows, generator=generator, device="cuda") < 0.1] = _IGNORED
+        target[torch.rand(rows, generator=generator, device="cuda") < _SHARE_IGNORED] = _IGNORED
     given["target"] = target
     if case["kind"] == "loss_grad":
         lse = torch.empty(rows, device="cuda", dtype=torch.float32)
@@ -255,7 +256,7 @@ def _plain_loss(case, given):
     counted = target != _IGNORED
     picked = logits.gather(1, target.clamp(min=0)[:, None])[:, 0]
     lse = logits.sub_(most).exp_().sum(dim=1).log_() + most[:, 0]
-    loss = torch.where(counted, lse - picked, 0.0)
+    loss, lse = torch.where(counted, lse - picked, 0.0), torch.where(counted, lse, 0.0)
     if case["reduction"] != "none":
         loss = loss.double().sum()
         if case["reduction"] == "mean":
@@ -378,7 +379,7 @@ def _exact_loss(case, given, rows_at_once=1024):
             own_logit[part] = z[torch.arange(z.shape[0], device=z.device), index[part]]
     if backward:
         return {"grad_input": dx, "grad_weight": dw}
-    loss = (lse - own_logit) * known.double()
+    loss, lse = (lse - own_logit) * known.double(), lse * known.double()
     if case["reduction"] == "sum":
         loss = loss.sum()
     elif case["reduction"] == "mean":
@@ -446,7 +447,8 @@ def work(case):
     kind, rows, width, size = case["kind"], case["rows"], case["width"], _SIZE[case["dtype"]]
     if kind in ("loss", "loss_grad"):
         factors = (rows + case["classes"]) * width * size
-        product = 2 * rows * case["classes"] * width
+        counted = rows if rows == 1 else round(rows * (1 - _SHARE_IGNORED))
+        product = 2 * counted * case["classes"] * width
         per_row = rows * (8 + 4)                        # target and lse
         if kind == "loss":
             return {"bytes": factors + per_row + 4 * (rows if case["reduction"] == "none" else 1), "flops": product}
