@@ -597,6 +597,45 @@ int32_t nt_dropout_add_layer_norm_backward(int32_t device, const void *dy, const
                                            void *dweight, void *dbias, uint64_t rows,
                                            uint64_t width, void *stream);
 
+/* ---- the loss ----------------------------------------------------------- */
+
+/*
+ * Softmax cross entropy of the linear layer z = x weight^T (x: rows x width,
+ * weight: classes x width, both of `dtype`: float32, float16, bfloat16),
+ * whose logits are never in memory:
+ *
+ *   lse = log sum exp z, loss = lse - z[target]         of each row
+ *
+ * `target` has `target_size` bytes an entry (4: int32, 8: int64).  A row whose
+ * target is `ignore_index` is not counted: its loss and lse are zero and what
+ * x holds there takes no part in anything.  A target that is no class makes
+ * that row's loss NaN and the gradients that it reaches.  `reduction` 0: a
+ * loss for each row; 1: the mean over the counted rows (0 if there are none);
+ * 2: their sum.  `lse` (one per row) may be NULL.
+ *
+ * Backward: with g the gradient of each row's loss (reduction 0: grad_loss[row];
+ * otherwise *grad_loss, or `grad_value` where that is NULL, for the mean
+ * divided by the number of counted rows),
+ *
+ *   dz = g (exp(z - lse) - [class = target]), dx = dz weight, dweight = dz^T x
+ *
+ * with dz rounded once to `dtype`.  Both take workspace of the library's pool
+ * in the order of `stream` (about the size of x for the forward pass, and for
+ * the backward pass up to 512 MiB for a piece of dz and two to six times x)
+ * and refuse a stream in capture.  Rows: fewer than 2**24; classes: fewer than
+ * 2**30; width: at most 2**21.  No counterpart in the reference's kernels.
+ */
+int32_t nt_linear_cross_entropy(int32_t device, const void *x, const void *weight, int32_t dtype,
+                                const void *target, int32_t target_size, int64_t ignore_index,
+                                int32_t reduction, float *loss, float *lse, uint64_t rows,
+                                uint64_t classes, uint64_t width, void *stream);
+int32_t nt_linear_cross_entropy_backward(int32_t device, const float *grad_loss, float grad_value,
+                                         const void *x, const void *weight, int32_t dtype,
+                                         const void *target, int32_t target_size,
+                                         int64_t ignore_index, int32_t reduction, const float *lse,
+                                         void *dx, void *dweight, uint64_t rows, uint64_t classes,
+                                         uint64_t width, void *stream);
+
 /* ---- measurement ------------------------------------------------------- */
 
 /*

@@ -176,6 +176,11 @@ SIGNATURES = {
     "nt_dropout_add_layer_norm_backward": (c_int32, [c_int32, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p,
                                                      c_void_p, c_int32, c_uint32, c_uint64, c_uint64, c_void_p,
                                                      c_void_p, c_void_p, c_void_p, c_uint64, c_uint64, c_void_p]),
+    "nt_linear_cross_entropy": (c_int32, [c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_int32, c_int64, c_int32,
+                                          c_void_p, c_void_p, c_uint64, c_uint64, c_uint64, c_void_p]),
+    "nt_linear_cross_entropy_backward": (c_int32, [c_int32, c_void_p, c_float, c_void_p, c_void_p, c_int32, c_void_p,
+                                                   c_int32, c_int64, c_int32, c_void_p, c_void_p, c_void_p, c_uint64,
+                                                   c_uint64, c_uint64, c_void_p]),
     "nt_stream_probe": (c_int32, [ctypes.POINTER(c_void_p), c_int32, c_int32, ctypes.POINTER(c_void_p), c_int32, c_int32,
                                   c_uint64, c_void_p]),
     "nt_malloc": (c_int32, [c_int32, c_uint64, c_void_p, ctypes.POINTER(c_void_p)]),

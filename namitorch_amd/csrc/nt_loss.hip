@@ -1,0 +1,776 @@
+// nt_loss.hip — softmax cross entropy of a linear layer's outputs over a large
+// vocabulary, whose logits are never in memory, and its backward pass.
+//
+// With x of N rows and W of V, both H wide, z = x W^T, target t_i:
+//   lse_i  = log sum_v exp z_iv,   loss_i = lse_i - z_i,t
+//   dz_iv  = g_i (exp(z_iv - lse_i) - [v = t_i])
+//   dx     = dz W,   dW = dz^T x
+// with g_i the gradient of row i's loss (that of the mean over the counted
+// rows, divided by their number).  Rows with the ignored target are taken out
+// before anything else: what they hold is never multiplied.
+//
+// Forward: the product's tiles end as a maximum and a sum of exponentials of
+// each row (and the target's logit), from which a second kernel makes lse and
+// loss.  Backward: the product is made once more, a piece of the vocabulary at
+// a time, and its tiles end as dz in the operands' type; two products of the
+// piece follow.  The sums over the vocabulary that dx needs are float32 in
+// memory from piece to piece.
+//
+// dz is rounded once, to the operands' type: half a unit in its last place,
+// as the stored gradients themselves are.  A factor that all rows share is
+// multiplied into the products instead, so that dz is exp(z - lse) - [v = t]
+// and most targets' -1 is exact: rounded together with that factor, which is
+// as far off for each of them, the gradient of 8192 rows by 50257 classes was
+// 1.7 times as far from the 64-bit one as a single rounding.  In float16 dz is
+// multiplied by a power of two first, such that the largest |g_i| comes to
+// 2**14 to 2**15: exp(z - lse) is some 1 / V, which float16 alone would hold
+// with few digits or none.  Float32 is three bfloat16 planes (nt_product.hpp).
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <initializer_list>
+#include <string>
+
+#include "nt_internal.hpp"
+#include "nt_pool.hpp"
+#include "nt_product.hpp"
+
+namespace nt {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kInfinity = __builtin_huge_valf();
+
+enum Reduction { kEach = 0, kMean = 1, kSum = 2 };
+
+// What the rows' targets are; class_of gives the class, kIgnored or kOutside.
+struct Targets {
+    const void *at;
+    int64_t ignored;
+    uint32_t classes;
+    int32_t size;               // bytes of a target: 4 or 8
+};
+constexpr int32_t kIgnored = -1, kOutside = -2;
+
+__device__ __forceinline__ int32_t class_of(const Targets &t, uint64_t i) {
+    const int64_t v = t.size == 8 ? reinterpret_cast<const int64_t *>(t.at)[i]
+                                  : (int64_t) reinterpret_cast<const int32_t *>(t.at)[i];
+    if (v == t.ignored) return kIgnored;
+    return v >= 0 && v < (int64_t)t.classes ? (int32_t)v : kOutside;
+}
+
+// The counted rows in order, made by rows_kernel.
+struct Rows {
+    uint32_t *count;            // how many
+    float *unscale;             // what the products of dz are multiplied by
+    uint32_t *row;              // of counted row j: its row,
+    int32_t *target;            // its class or kOutside,
+    float *weight;              // (backward) what its dz is multiplied by
+};
+
+// ---- counted rows ----------------------------------------------------------------------------------
+constexpr int kRowsBlock = 1024;
+
+// One workgroup: each lane takes a run of consecutive rows.
+template <bool BACKWARD>
+__global__ __launch_bounds__(kRowsBlock) void rows_kernel(Targets t, uint32_t rows, Rows out, const float *grad,
+                                                          float grad_value, int32_t reduction, bool scaled) {
+    __shared__ uint32_t counts[kRowsBlock / 64];
+    __shared__ float most[kRowsBlock / 64];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t each = (rows + kRowsBlock - 1) / kRowsBlock;
+    const uint32_t begin = threadIdx.x * each < rows ? threadIdx.x * each : rows;
+    const uint32_t end = rows - begin < each ? rows : begin + each;
+    uint32_t mine = 0;
+    float largest = 0.0f;
+    for (uint32_t i = begin; i < end; ++i) {
+        if (class_of(t, i) == kIgnored) continue;
+        ++mine;
+        if (BACKWARD && reduction == kEach) largest = fmaxf(largest, fabsf(grad[i]));
+    }
+    uint32_t before = mine;                                // inclusive sums over the wave
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t other = __shfl_up(before, off, 64);
+        if (lane >= (uint32_t)off) before += other;
+        if (BACKWARD) largest = fmaxf(largest, __shfl_xor(largest, off, 64));
+    }
+    if (lane == 63u) {
+        counts[wave] = before;
+        most[wave] = largest;
+    }
+    __syncthreads();
+    uint32_t count = 0;
+    for (uint32_t k = 0; k < kRowsBlock / 64; ++k) {
+        if (k < wave) before += counts[k];
+        count += counts[k];
+        if (BACKWARD) largest = fmaxf(largest, most[k]);
+    }
+    float common = 0.0f, scale = 1.0f;
+    if constexpr (BACKWARD) {
+        if (reduction != kEach) {
+            common = grad != nullptr ? *grad : grad_value;
+            if (reduction == kMean) common = common / (float)(count > 0 ? count : 1u);
+            largest = 1.0f;
+        }
+        if (scaled && largest > 0.0f && largest < kInfinity) {
+            int exponent;
+            frexpf(largest, &exponent);
+            exponent = 15 - exponent;
+            scale = ldexpf(1.0f, exponent > 126 ? 126 : exponent < -126 ? -126 : exponent);
+        }
+    }
+    if (threadIdx.x == 0) {
+        *out.count = count;
+        if (BACKWARD) *out.unscale = (reduction == kEach ? 1.0f : common) / scale;
+    }
+    uint32_t j = before - mine;
+    for (uint32_t i = begin; i < end; ++i) {
+        const int32_t c = class_of(t, i);
+        if (c == kIgnored) continue;
+        out.row[j] = i;
+        out.target[j] = c;
+        if constexpr (BACKWARD)
+            out.weight[j] = c == kOutside ? __builtin_nanf("") : (reduction == kEach ? grad[i] : 1.0f) * scale;
+        ++j;
+    }
+}
+
+// ---- operands as the products take them --------------------------------------------------------------
+// Float32 as three bfloat16 values whose sum it is (or nearly: the last is
+// rounded where float32's exponent ends).  What is not finite is the first
+// alone.
+__device__ __forceinline__ void three_planes(float v, uint16_t (&plane)[3]) {
+    uint32_t high = f32_to_bf16(v);
+    if ((high & 0x7fffu) == 0x7f80u) high = f32_bits(v) >> 16;           // rounded up to infinity, or infinite
+    const bool finite = (f32_bits(v) & 0x7f800000u) != 0x7f800000u;
+    plane[0] = (uint16_t)high;
+    const float left = v - bf16_to_f32((uint16_t)high);
+    plane[1] = finite ? f32_to_bf16(left) : (uint16_t)0;
+    plane[2] = finite ? f32_to_bf16(left - bf16_to_f32(plane[1])) : (uint16_t)0;
+}
+
+// Rows of `width` elements at any address to rows of `pitch` (a multiple of
+// 8), the end of each zero.  `row` and `live`: a row each from there, as many
+// as `live` says.
+template <class T>
+__global__ __launch_bounds__(kBlock) void pack_kernel(const void *from, uint32_t width, uint16_t *to, uint32_t pitch,
+                                                      uint64_t plane, uint32_t rows, const uint32_t *row,
+                                                      const uint32_t *live) {
+    if (live != nullptr) rows = *live;
+    const uint64_t groups = pitch / 8u, all = rows * groups;
+    for (uint64_t g = blockIdx.x * (uint64_t)kBlock + threadIdx.x; g < all; g += (uint64_t)gridDim.x * kBlock) {
+        const uint32_t r = (uint32_t)(g / groups), c = (uint32_t)(g % groups) * 8u;
+        const uint64_t source = (row != nullptr ? row[r] : r) * (uint64_t)width + c;
+        const auto *in = reinterpret_cast<const typename T::raw *>(from) + source;
+        uint16_t *out = to + r * (uint64_t)pitch + c;
+        if constexpr (T::code == NT_F32) {
+            uint16_t planes[3][8];
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) {
+                uint16_t one[3];
+                three_planes(c + k < width ? in[k] : 0.0f, one);
+                planes[0][k] = one[0];
+                planes[1][k] = one[1];
+                planes[2][k] = one[2];
+            }
+            for (int k = 0; k < 3; ++k)
+                *reinterpret_cast<u32x4_t *>(out + k * plane) = __builtin_bit_cast(u32x4_t, planes[k]);
+        } else {
+            uint16_t group[8];
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) group[k] = c + k < width ? in[k] : (uint16_t)0;
+            *reinterpret_cast<u32x4_t *>(out) = __builtin_bit_cast(u32x4_t, group);
+        }
+    }
+}
+
+// ---- what becomes of the products' tiles ------------------------------------------------------------------
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
+
+// Two halves' maximum m and sum of exp(z - m), joined.
+struct Partial2 {
+    float most, sum;
+};
+__device__ __forceinline__ Partial2 join(Partial2 a, Partial2 b) {
+    const float most = fmaxf(a.most, b.most);
+    const float fa = a.most == most ? 1.0f : exp_of(a.most - most), fb = b.most == most ? 1.0f : exp_of(b.most - most);
+    return Partial2{most, a.sum * fa + b.sum * fb};
+}
+
+// Logits to a maximum and sum of each row's part of a wave's tile, and the target's logit.
+struct FinishLoss {
+    Partial2 *partials;         // [slot][rows]
+    float *target_logit;        // [rows]
+    const int32_t *target;
+    const uint32_t *live;
+    uint32_t first, classes;    // of the piece: its first class, and their number
+    uint32_t first_slot;
+    uint64_t rows;              // length of a slot
+
+    template <class T>
+    __device__ __forceinline__ void operator()(const f32x4 (&acc)[T::TP][T::TQ], uint32_t p_first, uint32_t q_first,
+                                               uint32_t, uint32_t lane) const {
+        const uint32_t count = *live, slot = first_slot + p_first / T::kWaveP, up = p_first + 4u * (lane >> 4);
+        const bool whole = p_first + T::kWaveP <= classes;
+#pragma unroll
+        for (int j = 0; j < T::TQ; ++j) {
+            const uint32_t q = q_first + 16u * j + (lane & 15u);
+            const uint32_t place = q < count ? (uint32_t)target[q] - first - up : ~0u;
+            float most = -kInfinity;
+            f32x4 z[T::TP];
+#pragma unroll
+            for (int i = 0; i < T::TP; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    z[i][r] = whole || up + 16u * i + r < classes ? acc[i][j][r] : -kInfinity;
+                    most = fmaxf(most, z[i][r]);
+                }
+            if (__builtin_amdgcn_ballot_w64(place < 16u * T::TP) != 0) {
+#pragma unroll
+                for (int i = 0; i < T::TP; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (place == 16u * i + r) target_logit[q] = z[i][r];
+            }
+            most = fmaxf(most, __shfl_xor(most, 16, 64));
+            most = fmaxf(most, __shfl_xor(most, 32, 64));
+            const float from = most == -kInfinity ? 0.0f : most;
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < T::TP; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sum += exp_of(z[i][r] - from);
+            sum += __shfl_xor(sum, 16, 64);
+            sum += __shfl_xor(sum, 32, 64);
+            if (lane < 16u && q < count) partials[slot * rows + q] = Partial2{most, sum};
+        }
+    }
+};
+
+// Logits to dz.  The columns from the piece's last class to the line's end are zero.
+template <bool HALF, int PLANES>
+struct FinishGrad {
+    uint16_t *dz;
+    uint64_t plane;
+    uint32_t pitch;
+    const float *lse, *weight;  // lse by row, the others by counted row
+    const int32_t *target;
+    const uint32_t *row, *live;
+    uint32_t first, classes;
+
+    template <class T>
+    __device__ __forceinline__ void operator()(const f32x4 (&acc)[T::TP][T::TQ], uint32_t p_first, uint32_t q_first,
+                                               uint32_t, uint32_t lane) const {
+        const uint32_t count = *live, up = p_first + 4u * (lane >> 4);
+#pragma unroll
+        for (int j = 0; j < T::TQ; ++j) {
+            const uint32_t q = q_first + 16u * j + (lane & 15u);
+            if (q >= count) continue;
+            const float from = lse[row[q]], by = weight[q];
+            const uint32_t place = (uint32_t)target[q] - first - up;
+            uint16_t *line = dz + q * (uint64_t)pitch + up;
+#pragma unroll
+            for (int i = 0; i < T::TP; ++i) {
+                if (up + 16u * i >= pitch) continue;
+                float v[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    v[r] = exp_of(acc[i][j][r] - from);
+                    if (place == 16u * i + r) v[r] -= 1.0f;
+                    v[r] = up + 16u * i + r < classes ? v[r] * by : 0.0f;
+                }
+                if constexpr (PLANES == 1) {
+                    uint16_t e[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) e[r] = HALF ? f32_to_f16(v[r]) : f32_to_bf16(v[r]);
+                    *reinterpret_cast<u32x2 *>(line + 16 * i) = __builtin_bit_cast(u32x2, e);
+                } else {
+                    uint16_t e[3][4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        uint16_t one[3];
+                        three_planes(v[r], one);
+                        e[0][r] = one[0];
+                        e[1][r] = one[1];
+                        e[2][r] = one[2];
+                    }
+                    for (int k = 0; k < 3; ++k)
+                        *reinterpret_cast<u32x2 *>(line + k * plane + 16 * i) = __builtin_bit_cast(u32x2, e[k]);
+                }
+            }
+        }
+    }
+};
+
+// A piece's part of dx, in float32: stored, or added to the pieces before.
+struct FinishSum {
+    float *sums;                // [split][rows][width]
+    uint64_t split_stride;
+    uint32_t width;             // a multiple of 8
+    const uint32_t *live;
+    bool add;
+
+    template <class T>
+    __device__ __forceinline__ void operator()(const f32x4 (&acc)[T::TP][T::TQ], uint32_t p_first, uint32_t q_first,
+                                               uint32_t split, uint32_t lane) const {
+        const uint32_t count = *live, up = p_first + 4u * (lane >> 4);
+#pragma unroll
+        for (int j = 0; j < T::TQ; ++j) {
+            const uint32_t q = q_first + 16u * j + (lane & 15u);
+            if (q >= count) continue;
+            float *line = sums + split * split_stride + q * (uint64_t)width + up;
+#pragma unroll
+            for (int i = 0; i < T::TP; ++i) {
+                if (up + 16u * i >= width) continue;
+                f32x4 v = acc[i][j];
+                if (add) v += *reinterpret_cast<const f32x4 *>(line + 16 * i);
+                *reinterpret_cast<f32x4 *>(line + 16 * i) = v;
+            }
+        }
+    }
+};
+
+// A piece's rows of dW.
+template <class S>
+struct FinishWeight {
+    typename S::raw *to;
+    const float *unscale;
+    uint32_t width, classes;
+    bool even;                  // four elements can be stored at once
+
+    template <class T>
+    __device__ __forceinline__ void operator()(const f32x4 (&acc)[T::TP][T::TQ], uint32_t p_first, uint32_t q_first,
+                                               uint32_t, uint32_t lane) const {
+        const float by = *unscale;
+        const uint32_t up = p_first + 4u * (lane >> 4);
+#pragma unroll
+        for (int j = 0; j < T::TQ; ++j) {
+            const uint32_t q = q_first + 16u * j + (lane & 15u);
+            if (q >= classes) continue;
+            typename S::raw *line = to + q * (uint64_t)width;
+#pragma unroll
+            for (int i = 0; i < T::TP; ++i) {
+                const uint32_t c = up + 16u * i;
+                float v[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r] * by;
+                if (even && c + 4u <= width) {
+                    Vec4IO<S, false>::store(line, c, v);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (c + r < width) store1<S>(line, c + r, v[r]);
+                }
+            }
+        }
+    }
+};
+
+// ---- the ends of both passes -----------------------------------------------------------------------------
+// lse and loss of 16 rows a workgroup: 16 lanes share out a row's slots.
+__global__ __launch_bounds__(kBlock) void loss_rows_kernel(const Partial2 *partials, uint32_t slots, uint64_t stride,
+                                                           const float *target_logit, Rows rows, float *lse,
+                                                           float *loss) {
+    __shared__ Partial2 shared[16][17];
+    const uint32_t count = *rows.count, r = threadIdx.x & 15u, slice = threadIdx.x >> 4;
+    for (uint32_t first = blockIdx.x * 16u; first < count; first += gridDim.x * 16u) {
+        const uint32_t j = first + r;
+        Partial2 p{-kInfinity, 0.0f};
+        if (j < count)
+            for (uint32_t k = slice; k < slots; k += 16u) p = join(p, partials[k * stride + j]);
+        __syncthreads();
+        shared[slice][r] = p;
+        __syncthreads();
+        if (slice == 0 && j < count) {
+            for (uint32_t k = 1; k < 16; ++k) p = join(p, shared[k][r]);
+            const float value = p.most + __builtin_amdgcn_logf(p.sum) * kLn2;
+            const uint32_t row = rows.row[j];
+            if (lse != nullptr) lse[row] = value;
+            if (loss != nullptr) loss[row] = rows.target[j] == kOutside ? __builtin_nanf("") : value - target_logit[j];
+        }
+    }
+}
+
+// Rows that are not counted have loss and lse zero.
+__global__ __launch_bounds__(kBlock) void loss_ignored_kernel(Targets t, uint32_t rows, float *lse, float *loss) {
+    for (uint32_t i = blockIdx.x * kBlock + threadIdx.x; i < rows; i += gridDim.x * kBlock) {
+        if (class_of(t, i) != kIgnored) continue;
+        if (lse != nullptr) lse[i] = 0.0f;
+        if (loss != nullptr) loss[i] = 0.0f;
+    }
+}
+
+// Sum or mean of the rows' losses, in 64 bits and a fixed order.
+__global__ __launch_bounds__(kRowsBlock) void loss_sum_kernel(const float *each, uint32_t rows, const uint32_t *count,
+                                                              bool mean, float *loss) {
+    __shared__ double shared[kRowsBlock / 64];
+    double sum = 0.0;
+    for (uint32_t i = threadIdx.x; i < rows; i += kRowsBlock) sum += (double)each[i];
+    sum = wave_sum(sum);
+    if ((threadIdx.x & 63u) == 0u) shared[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int k = 1; k < kRowsBlock / 64; ++k) sum += shared[k];
+        const uint32_t n = *count;
+        *loss = (float)(mean ? sum / (double)(n > 0 ? n : 1u) : sum);
+    }
+}
+
+// dx from its sums; rows that are not counted are zero.  `row` is in order, so
+// row i is counted row j where row[j] == i, found by halving.
+template <class T>
+__global__ __launch_bounds__(kBlock) void grad_input_kernel(const float *sums, uint64_t split_stride, uint32_t splits,
+                                                            uint32_t pitch, Rows rows, uint32_t all, uint32_t width,
+                                                            typename T::raw *dx) {
+    const uint32_t count = *rows.count;
+    const float by = *rows.unscale;
+    for (uint32_t i = blockIdx.x; i < all; i += gridDim.x) {
+        uint32_t low = 0, high = count;
+        while (low < high) {
+            const uint32_t middle = (low + high) / 2u;
+            if (rows.row[middle] < i) low = middle + 1u;
+            else high = middle;
+        }
+        const bool counted = low < count && rows.row[low] == i;
+        for (uint32_t c = threadIdx.x; c < width; c += kBlock) {
+            float v = 0.0f;
+            if (counted) {
+                for (uint32_t s = 0; s < splits; ++s) v += sums[s * split_stride + low * (uint64_t)pitch + c];
+                v *= by;
+            }
+            store1<T>(dx, i * (uint64_t)width + c, v);
+        }
+    }
+}
+
+// ---- launches ----------------------------------------------------------------------------------------
+constexpr uint64_t kPieceBytes = 512ull << 20;       // of dz, and of packed weights, at a time
+constexpr uint32_t kSumTiles = 512;                  // dx: tiles and splits to fill the chip with
+
+using Large = Tile<128, 128, 2, 2>;
+
+struct Problem {
+    const void *x, *w;
+    int32_t dtype;
+    uint32_t rows, classes, width;
+    Targets targets;
+    int32_t reduction;
+};
+
+// Memory of the pool for one call, in parts; goes back as soon as the kernels
+// are queued (the pool reuses it on this stream only).
+class Workspace {
+  public:
+    template <class V>
+    void want(V **at, uint64_t count) {
+        entries_[used_++] = {reinterpret_cast<void **>(at), bytes_};
+        bytes_ += (count * sizeof(V) + 255u) & ~255ull;
+    }
+    int32_t allocate(int32_t device, void *stream) {
+        std::string error;
+        const int32_t rc = device_pool().allocate(device, bytes_ > 0 ? bytes_ : 256u, stream, &base_, error);
+        if (rc != NT_OK) return fail(rc, error);
+        for (int k = 0; k < used_; ++k) *entries_[k].at = static_cast<char *>(base_) + entries_[k].offset;
+        return NT_OK;
+    }
+    ~Workspace() {
+        std::string error;
+        if (base_ != nullptr) (void)device_pool().release(base_, error);
+    }
+
+  private:
+    struct Entry {
+        void **at;
+        uint64_t offset;
+    };
+    Entry entries_[16];
+    int used_ = 0;
+    uint64_t bytes_ = 0;
+    void *base_ = nullptr;
+};
+
+static uint32_t blocks_of(uint64_t items, uint32_t each) {
+    const uint64_t blocks = (items + each - 1) / each;
+    return blocks < 1 ? 1u : blocks > 8192u ? 8192u : (uint32_t)blocks;
+}
+
+template <class T> struct Kind {            // how the products take a type
+    static constexpr bool kHalf = T::code == NT_F16;
+    static constexpr int kPlanes = T::code == NT_F32 ? 3 : 1;
+};
+
+// The pieces of the vocabulary: as few as keep dz and the packed weights
+// within their bytes, of whole tiles.
+static uint32_t piece_of(const Problem &a, uint32_t pitch, int planes, bool packed, bool backward) {
+    uint64_t most = a.classes;
+    if (backward) most = std::min<uint64_t>(most, kPieceBytes / (2ull * planes * a.rows));
+    if (packed) most = std::min<uint64_t>(most, kPieceBytes / (2ull * planes * pitch));
+    if (most >= a.classes) return a.classes;
+    const uint64_t pieces = (a.classes + std::max<uint64_t>(most, 256u) - 1) / std::max<uint64_t>(most, 256u);
+    const uint64_t each = (a.classes + pieces - 1) / pieces;
+    return (uint32_t)((each + 255u) / 256u * 256u);
+}
+
+template <class T>
+static int32_t forward_of(const Problem &a, int32_t device, float *loss, float *lse, void *stream) {
+    constexpr int planes = Kind<T>::kPlanes;
+    constexpr bool half = Kind<T>::kHalf;
+    hipStream_t s = (hipStream_t)stream;
+    const uint32_t pitch = (a.width + 7u) / 8u * 8u;
+    const bool pack_w = planes > 1 || pitch != a.width || (uintptr_t)a.w % 16u != 0;
+    const uint32_t piece = piece_of(a, pitch, planes, pack_w, false);
+    using Shape = Large;
+    const uint32_t slots_piece = (piece + Shape::BP - 1) / Shape::BP * Shape::WP;
+    const uint32_t pieces = (a.classes + piece - 1) / piece;
+    const uint64_t slots = (uint64_t)slots_piece * pieces;
+
+    Rows rows{};
+    uint16_t *px = nullptr, *pw = nullptr;
+    Partial2 *partials = nullptr;
+    float *target_logit = nullptr, *each = nullptr;
+    Workspace room;
+    room.want(&rows.count, 1);
+    room.want(&rows.row, a.rows);
+    room.want(&rows.target, a.rows);
+    room.want(&target_logit, a.rows);
+    room.want(&partials, slots * a.rows);
+    room.want(&px, (uint64_t)planes * a.rows * pitch);
+    if (pack_w) room.want(&pw, (uint64_t)planes * piece * pitch);
+    if (a.reduction != kEach) room.want(&each, a.rows);
+    int32_t rc = room.allocate(device, stream);
+    if (rc != NT_OK) return rc;
+    float *to = a.reduction == kEach ? loss : each;
+
+    rows_kernel<false><<<1, kRowsBlock, 0, s>>>(a.targets, a.rows, rows, nullptr, 0.0f, a.reduction, false);
+    loss_ignored_kernel<<<blocks_of(a.rows, kBlock), kBlock, 0, s>>>(a.targets, a.rows, lse, to);
+    const uint64_t plane_x = (uint64_t)a.rows * pitch, plane_w = (uint64_t)piece * pitch;
+    pack_kernel<T><<<blocks_of(a.rows * (uint64_t)(pitch / 8u), kBlock), kBlock, 0, s>>>(
+        a.x, a.width, px, pitch, plane_x, a.rows, rows.row, rows.count);
+    for (uint32_t k = 0; k < pieces; ++k) {
+        const uint32_t first = k * piece, classes = std::min(piece, a.classes - first);
+        const void *weights = static_cast<const typename T::raw *>(a.w) + (uint64_t)first * a.width;
+        if (pack_w)
+            pack_kernel<T><<<blocks_of(classes * (uint64_t)(pitch / 8u), kBlock), kBlock, 0, s>>>(
+                weights, a.width, pw, pitch, plane_w, classes, nullptr, nullptr);
+        Product product{};
+        product.p = Operand{pack_w ? pw : static_cast<const uint16_t *>(weights), pitch, plane_w, classes, pitch};
+        product.q = Operand{px, pitch, plane_x, a.rows, pitch};
+        product.tiles_p = (classes + Shape::BP - 1) / Shape::BP;
+        product.tiles_q = (a.rows + Shape::BQ - 1) / Shape::BQ;
+        product.splits = 1;
+        product.depth = pitch;
+        product.live = rows.count;
+        const FinishLoss finish{partials, target_logit, rows.target, rows.count, first, classes, k * slots_piece, a.rows};
+        launch_product<half, Shape, true, true, planes>(product, finish, s);
+    }
+    const uint32_t last = (a.classes - (pieces - 1) * piece + Shape::BP - 1) / Shape::BP * Shape::WP;
+    loss_rows_kernel<<<blocks_of(a.rows, 16), kBlock, 0, s>>>(partials, (pieces - 1) * slots_piece + last, a.rows,
+                                                               target_logit, rows, lse, to);
+    if (a.reduction != kEach)
+        loss_sum_kernel<<<1, kRowsBlock, 0, s>>>(each, a.rows, rows.count, a.reduction == kMean, loss);
+    return hip_check(hipGetLastError(), "linear cross entropy launch");
+}
+
+template <class T>
+static int32_t backward_of(const Problem &a, int32_t device, const float *grad, float grad_value, const float *lse,
+                           void *dx, void *dw, void *stream) {
+    constexpr int planes = Kind<T>::kPlanes;
+    constexpr bool half = Kind<T>::kHalf;
+    using Shape = Large;
+    using Raw = typename T::raw;
+    hipStream_t s = (hipStream_t)stream;
+    const uint32_t pitch = (a.width + 7u) / 8u * 8u;
+    const bool pack_w = planes > 1 || pitch != a.width || (uintptr_t)a.w % 16u != 0;
+    const uint32_t piece = piece_of(a, pitch, planes, pack_w, true);
+    const uint32_t pieces = (a.classes + piece - 1) / piece;
+    const uint32_t dz_pitch = (piece + 63u) / 64u * 64u;
+    const uint32_t tiles_h = (pitch + Shape::BP - 1) / Shape::BP, tiles_n = (a.rows + Shape::BQ - 1) / Shape::BQ;
+    const uint32_t depth = (piece + kDepth - 1) / kDepth;
+    uint32_t splits = std::max(1u, kSumTiles / std::max(1u, tiles_h * tiles_n));
+    splits = std::min(splits, std::max(1u, depth / 8u));
+
+    Rows rows{};
+    uint16_t *px = nullptr, *pw = nullptr, *dz = nullptr;
+    float *sums = nullptr;
+    Workspace room;
+    room.want(&rows.count, 1);
+    room.want(&rows.unscale, 1);
+    room.want(&rows.row, a.rows);
+    room.want(&rows.target, a.rows);
+    room.want(&rows.weight, a.rows);
+    room.want(&px, (uint64_t)planes * a.rows * pitch);
+    if (pack_w) room.want(&pw, (uint64_t)planes * piece * pitch);
+    room.want(&dz, (uint64_t)planes * a.rows * dz_pitch);
+    room.want(&sums, (uint64_t)splits * a.rows * pitch);
+    int32_t rc = room.allocate(device, stream);
+    if (rc != NT_OK) return rc;
+
+    rows_kernel<true><<<1, kRowsBlock, 0, s>>>(a.targets, a.rows, rows, grad, grad_value, a.reduction, half);
+    const uint64_t plane_x = (uint64_t)a.rows * pitch, plane_w = (uint64_t)piece * pitch;
+    const uint64_t plane_dz = (uint64_t)a.rows * dz_pitch;
+    pack_kernel<T><<<blocks_of(a.rows * (uint64_t)(pitch / 8u), kBlock), kBlock, 0, s>>>(
+        a.x, a.width, px, pitch, plane_x, a.rows, rows.row, rows.count);
+    for (uint32_t k = 0; k < pieces; ++k) {
+        const uint32_t first = k * piece, classes = std::min(piece, a.classes - first);
+        const uint32_t line = (classes + 63u) / 64u * 64u;
+        const void *weights = static_cast<const Raw *>(a.w) + (uint64_t)first * a.width;
+        if (pack_w)
+            pack_kernel<T><<<blocks_of(classes * (uint64_t)(pitch / 8u), kBlock), kBlock, 0, s>>>(
+                weights, a.width, pw, pitch, plane_w, classes, nullptr, nullptr);
+        const uint16_t *w = pack_w ? pw : static_cast<const uint16_t *>(weights);
+        Product logits{};
+        logits.p = Operand{w, pitch, plane_w, classes, pitch};
+        logits.q = Operand{px, pitch, plane_x, a.rows, pitch};
+        logits.tiles_p = (line + Shape::BP - 1) / Shape::BP;
+        logits.tiles_q = tiles_n;
+        logits.splits = 1;
+        logits.depth = pitch;
+        logits.live = rows.count;
+        const FinishGrad<half, planes> grads{dz,         plane_dz,    line,     lse, rows.weight, rows.target,
+                                             rows.row, rows.count, first, classes};
+        launch_product<half, Shape, true, true, planes>(logits, grads, s);
+
+        Product input{};                    // dx[i][h] = sum over v of dz[i][v] W[v][h]
+        input.p = Operand{w, pitch, plane_w, pitch, classes};
+        input.q = Operand{dz, line, plane_dz, a.rows, line};
+        input.tiles_p = tiles_h;
+        input.tiles_q = tiles_n;
+        input.splits = splits;
+        input.depth = line;
+        input.live = rows.count;
+        const FinishSum sum{sums, (uint64_t)a.rows * pitch, pitch, rows.count, k > 0};
+        launch_product<half, Shape, false, true, planes>(input, sum, s);
+
+        Product weight{};                   // dW[v][h] = sum over i of dz[i][v] x[i][h]
+        weight.p = Operand{px, pitch, plane_x, pitch, a.rows};
+        weight.q = Operand{dz, line, plane_dz, line, a.rows};
+        weight.tiles_p = tiles_h;
+        weight.tiles_q = (classes + Shape::BQ - 1) / Shape::BQ;
+        weight.splits = 1;
+        weight.depth = a.rows;
+        weight.live = rows.count;
+        weight.live_depth = true;
+        Raw *to = static_cast<Raw *>(dw) + (uint64_t)first * a.width;
+        const bool even = a.width % 4u == 0 && (uintptr_t)dw % (4u * sizeof(Raw)) == 0;
+        const FinishWeight<T> last{to, rows.unscale, a.width, classes, even};
+        launch_product<half, Shape, false, false, planes>(weight, last, s);
+    }
+    grad_input_kernel<T><<<std::min(a.rows, 8192u), kBlock, 0, s>>>(sums, (uint64_t)a.rows * pitch, splits, pitch, rows,
+                                                                    a.rows, a.width, static_cast<Raw *>(dx));
+    return hip_check(hipGetLastError(), "linear cross entropy backward launch");
+}
+
+// ---- argument checks -----------------------------------------------------------------------------------
+static int32_t check_problem(const char *entry, int32_t dtype, int32_t target_size, int32_t reduction, uint64_t rows,
+                             uint64_t classes, uint64_t width) {
+    const std::string name(entry);
+    if (dtype != NT_F32 && dtype != NT_F16 && dtype != NT_BF16)
+        return fail(NT_ERR_TYPE, name + ": input and weight must be float32, float16 or bfloat16");
+    if (target_size != 4 && target_size != 8) return fail(NT_ERR_TYPE, name + ": targets must be int32 or int64");
+    if (reduction < kEach || reduction > kSum) return fail(NT_ERR_VALUE, name + ": unknown reduction");
+    if (width == 0 || width > kMostPitch / 2u) return fail(NT_ERR_VALUE, name + ": the width must be 1..2**21");
+    if (classes == 0 || classes >= 1u << 30) return fail(NT_ERR_VALUE, name + ": there must be 1..2**30 - 1 classes");
+    if (rows >= 1u << 24) return fail(NT_ERR_VALUE, name + ": there must be fewer than 2**24 rows");
+    return NT_OK;
+}
+
+struct LossArray {
+    const void *ptr;
+    uint64_t size, count;       // bytes of an element, elements
+    bool written, needed;
+};
+
+static int32_t check_loss_arrays(const char *entry, std::initializer_list<LossArray> arrays) {
+    for (const LossArray &a : arrays) {
+        if (a.ptr == nullptr) {
+            if (a.needed && a.count > 0) return fail(NT_ERR_VALUE, std::string(entry) + ": NULL array");
+            continue;
+        }
+        const uintptr_t start = (uintptr_t)a.ptr;
+        if (start % a.size != 0) return fail(NT_ERR_VALUE, std::string(entry) + ": an array is not aligned to its dtype");
+        if (!a.written) continue;
+        for (const LossArray &b : arrays) {
+            if (&a == &b || b.ptr == nullptr) continue;
+            const uintptr_t other = (uintptr_t)b.ptr;
+            if (start < other + b.count * b.size && other < start + a.count * a.size)
+                return fail(NT_ERR_VALUE, std::string(entry) + ": an output overlaps another array");
+        }
+    }
+    return NT_OK;
+}
+
+static int32_t refuse_loss_capture(const char *entry, void *stream) {
+    int32_t capturing = 0;
+    const int32_t rc = nt_stream_capturing(stream, &capturing);
+    if (rc != NT_OK) return rc;
+    return capturing ? fail(NT_ERR_RUNTIME, std::string(entry) + ": not supported in stream capture") : NT_OK;
+}
+
+}  // namespace nt
+
+using namespace nt;
+
+extern "C" {
+
+int32_t nt_linear_cross_entropy(int32_t device, const void *x, const void *weight, int32_t dtype, const void *target,
+                                int32_t target_size, int64_t ignore_index, int32_t reduction, float *loss, float *lse,
+                                uint64_t rows, uint64_t classes, uint64_t width, void *stream) {
+    clear_error();
+    const char *entry = "nt_linear_cross_entropy";
+    int32_t rc = check_problem(entry, dtype, target_size, reduction, rows, classes, width);
+    if (rc != NT_OK) return rc;
+    const uint64_t size = dtype == NT_F32 ? 4u : 2u;
+    rc = check_loss_arrays(entry, {{x, size, rows * width, false, true},
+                                   {weight, size, classes * width, false, true},
+                                   {target, (uint64_t)target_size, rows, false, true},
+                                   {loss, 4, reduction == kEach ? rows : 1, true, true},
+                                   {lse, 4, rows, true, false}});
+    if (rc != NT_OK) return rc;
+    if (rows == 0 && reduction == kEach) return NT_OK;
+    DeviceGuard guard(device);
+    if (!guard.ok()) return hip_check(guard.error(), "hipSetDevice");
+    rc = refuse_loss_capture(entry, stream);
+    if (rc != NT_OK) return rc;
+    if (rows == 0) return nt_fill(loss, 1, 4, 0, stream);
+    const Problem a{x, weight, dtype, (uint32_t)rows, (uint32_t)classes, (uint32_t)width,
+                    {target, ignore_index, (uint32_t)classes, target_size}, reduction};
+    switch (dtype) {
+        case NT_F32: return forward_of<TF32>(a, device, loss, lse, stream);
+        case NT_F16: return forward_of<TF16>(a, device, loss, lse, stream);
+        default: return forward_of<TBF16>(a, device, loss, lse, stream);
+    }
+}
+
+int32_t nt_linear_cross_entropy_backward(int32_t device, const float *grad_loss, float grad_value, const void *x,
+                                         const void *weight, int32_t dtype, const void *target, int32_t target_size,
+                                         int64_t ignore_index, int32_t reduction, const float *lse, void *dx,
+                                         void *dweight, uint64_t rows, uint64_t classes, uint64_t width, void *stream) {
+    clear_error();
+    const char *entry = "nt_linear_cross_entropy_backward";
+    int32_t rc = check_problem(entry, dtype, target_size, reduction, rows, classes, width);
+    if (rc != NT_OK) return rc;
+    const uint64_t size = dtype == NT_F32 ? 4u : 2u;
+    rc = check_loss_arrays(entry, {{grad_loss, 4, reduction == kEach ? rows : 1, false, reduction == kEach},
+                                   {x, size, rows * width, false, true},
+                                   {weight, size, classes * width, false, true},
+                                   {target, (uint64_t)target_size, rows, false, true},
+                                   {lse, 4, rows, false, true},
+                                   {dx, size, rows * width, true, true},
+                                   {dweight, size, classes * width, true, true}});
+    if (rc != NT_OK) return rc;
+    DeviceGuard guard(device);
+    if (!guard.ok()) return hip_check(guard.error(), "hipSetDevice");
+    rc = refuse_loss_capture(entry, stream);
+    if (rc != NT_OK) return rc;
+    if (rows == 0) return nt_fill(dweight, classes * width, (int32_t)size, 0, stream);
+    const Problem a{x, weight, dtype, (uint32_t)rows, (uint32_t)classes, (uint32_t)width,
+                    {target, ignore_index, (uint32_t)classes, target_size}, reduction};
+    switch (dtype) {
+        case NT_F32: return backward_of<TF32>(a, device, grad_loss, grad_value, lse, dx, dweight, stream);
+        case NT_F16: return backward_of<TF16>(a, device, grad_loss, grad_value, lse, dx, dweight, stream);
+        default: return backward_of<TBF16>(a, device, grad_loss, grad_value, lse, dx, dweight, stream);
+    }
+}
+
+}  // extern "C"

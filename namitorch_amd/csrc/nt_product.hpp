@@ -1,0 +1,264 @@
+// nt_product.hpp — matrix products of 16-bit operands on the matrix cores,
+// with what becomes of a product's tile left to the caller.
+//
+//   C[q][p] = sum over k of Q(q, k) P(p, k)
+//
+// Either operand lies in memory as [row][k] ("deep": k runs along a line) or
+// as [k][row].  A workgroup makes one tile of BP x BQ elements, in steps of 64
+// along k: a step's slices of both operands go straight from memory to LDS
+// while the slices before are multiplied, so there are two such rooms.  Sums
+// are float32 in the matrix cores' accumulators.
+//
+// A 16-byte group of a slice does not lie where its place in memory says, but
+// with its index in the line changed by an exclusive or, so that the lanes
+// that read a column of groups at once find them in different banks.  The
+// change is made in the address that a lane loads from, since a wave's loads
+// into LDS lie in the order of its lanes.
+//
+// Float32 operands come as three bfloat16 planes whose sum they are (8 + 8 + 8
+// significand bits): of the nine products of planes the six largest are made,
+// one after the other at each step, and what is left out is below 2^-24 of the
+// product.  The matrix cores' own float32 instructions reach 157 TFLOP/s, a
+// sixth of the bfloat16 rate more.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "nt_common.hpp"
+
+namespace nt {
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef short s16x8_t __attribute__((ext_vector_type(8)));
+
+constexpr uint32_t kDepth = 64;             // elements along k in a step
+constexpr uint32_t kMostPitch = 1u << 22;   // elements of a line: a tile's offsets stay below 2**32 bytes
+
+struct Operand {
+    const uint16_t *base;       // 16-byte aligned
+    uint64_t pitch;             // elements from line to line, a multiple of 8
+    uint64_t plane;             // elements from plane to plane
+    uint32_t rows;              // deep: rows; otherwise columns, a multiple of 8
+    uint32_t depth;             // along k; a multiple of 8 when deep
+};
+
+// How many rows there are may be known on the device alone (`live`, at most
+// what the grid is made for): then they are operand q's rows, or, with
+// `live_depth`, the length of k of both.
+struct Product {
+    Operand p, q;
+    uint32_t tiles_p, tiles_q, splits, depth;   // depth: along k, in steps of 64 that are shared out among the splits
+    const uint32_t *live;
+    bool live_depth;
+};
+
+// Shape of a workgroup's tile and of the waves in it.
+template <int BP_, int BQ_, int WP_, int WQ_>
+struct Tile {
+    static constexpr int BP = BP_, BQ = BQ_, WP = WP_, WQ = WQ_;
+    static constexpr int kWaves = WP * WQ, kThreads = kWaves * 64;
+    static constexpr int kWaveP = BP / WP, kWaveQ = BQ / WQ;        // a wave's part
+    static constexpr int TP = kWaveP / 16, TQ = kWaveQ / 16;        // in tiles of the matrix instruction
+};
+
+__device__ __attribute__((aligned(16))) const uint32_t kZeroGroup[4] = {0u, 0u, 0u, 0u};
+
+// The exclusive or of a line of the [k][row] slices, in 32-byte groups: the 16
+// lines that a wave's transposed read touches at once get different ones.
+__device__ __forceinline__ uint32_t turn_of(uint32_t k) { return (k & 3u) | (((k >> 3) & 3u) << 2); }
+
+// One operand's way into LDS.
+template <int B, int WAVES, bool DEEP>
+struct Loader {
+    static constexpr int kLoads = B * 128 / 1024 / WAVES;       // 1 KB each, a wave's share
+    static_assert(kLoads * WAVES * 1024 == B * 128, "a slice is shared out among the waves");
+    const char *base;
+    uint64_t pitch, plane;
+    uint32_t depth;
+    uint32_t offset[kLoads];
+    uint32_t line[kLoads];              // deep: the group's first k; otherwise the line's k
+
+    __device__ __forceinline__ void init(const Operand &o, uint32_t first, uint32_t wave, uint32_t lane) {
+        pitch = o.pitch * 2u;
+        plane = o.plane * 2u;
+        depth = o.depth;
+        base = reinterpret_cast<const char *>(o.base) + (DEEP ? first * pitch : (uint64_t)first * 2u);
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const uint32_t part = (uint32_t)j * WAVES + wave;
+            if constexpr (DEEP) {
+                // Rows past the last are the last again: what they give is not kept.
+                uint32_t row = part * 8u + (lane >> 3);
+                const uint32_t last = o.rows - 1u - first;
+                row = row < last ? row : last;
+                const uint32_t group = (lane & 7u) ^ (lane >> 3);
+                offset[j] = row * (uint32_t)pitch + group * 16u;
+                line[j] = group * 8u;
+            } else {
+                constexpr uint32_t lanes = B / 8;               // of a line
+                const uint32_t k = part * (64u / lanes) + lane / lanes;
+                const uint32_t group = lane % lanes;
+                const uint32_t turned = (((group >> 1) ^ (turn_of(k) & (B / 16u - 1u))) << 1) | (group & 1u);
+                uint32_t column = turned * 8u;
+                const uint32_t last = o.rows - 8u - first;
+                column = column < last ? column : last;
+                offset[j] = k * (uint32_t)pitch + column * 2u;
+                line[j] = k;
+            }
+        }
+    }
+
+    // Queue the slice from k on; groups past the end of k are zeros.
+    __device__ __forceinline__ void load(uint16_t *room, uint32_t k, uint32_t which, uint32_t wave) const {
+        const char *from = base + which * plane + (DEEP ? (uint64_t)k * 2u : k * pitch);
+        const bool whole = k + kDepth <= depth;
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const char *at = from + offset[j];
+            if (!whole) at = k + line[j] < depth ? at : reinterpret_cast<const char *>(kZeroGroup);
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)at,
+                                             (__attribute__((address_space(3))) void *)(room + (j * WAVES + wave) * 512u),
+                                             16, 0, 0);
+        }
+    }
+};
+
+// The eight elements along k of a lane, one for each matrix instruction: lane
+// l has row l % 16 of a 16-row tile and k = 8 (l / 16) on.
+template <int B, bool DEEP>
+struct Reader {
+    uint32_t first;             // element of the wave's first row
+    uint32_t lane;
+    __device__ __forceinline__ s16x8_t read(const uint16_t *room, int t, int half) const {
+        const uint32_t g = lane >> 4;
+        if constexpr (DEEP) {
+            const uint32_t row = first + (uint32_t)t * 16u + (lane & 15u);
+            const uint32_t group = ((uint32_t)half * 4u + g) ^ (lane & 7u);
+            return *reinterpret_cast<const s16x8_t *>(room + row * 64u + group * 8u);
+        } else {
+            // Two transposed reads of four lines each: the 16 lanes of a group bring 4 lines of 16
+            // elements, and each gets a column of them.
+            const uint32_t k = (uint32_t)half * 32u + g * 8u + ((lane & 15u) >> 2);
+            const uint32_t turned = (first / 16u + (uint32_t)t) ^ (turn_of(k) & (B / 16u - 1u));
+            const uint16_t *at = room + k * B + turned * 16u + (lane & 3u) * 4u;
+            const s16x4_t low = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4_t *)(at));
+            const s16x4_t high = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4_t *)(at + 4u * B));
+            return __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+};
+
+template <bool HALF>
+__device__ __forceinline__ f32x4 multiply(s16x8_t a, s16x8_t b, f32x4 c) {
+    if constexpr (HALF)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c,
+                                                      0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
+                                                       c, 0, 0, 0);
+}
+
+// Workgroup b of n as a place in the order of the tiles: the ones that an XCD
+// gets (every eighth) are neighbours there, so that they share its L2.
+__device__ __forceinline__ uint32_t xcd_order(uint32_t b, uint32_t n) {
+    const uint32_t xcd = b & 7u, left = n & 7u;
+    return xcd * (n >> 3) + (xcd < left ? xcd : left) + (b >> 3);
+}
+
+// PLANES: 1, or 3 of float32.  `finish` gets the wave's accumulators: element
+// [tp][tq][r] is p = p_first + 16 tp + 4 (lane / 16) + r, q = q_first + 16 tq + lane % 16.
+template <bool HALF, class T, bool P_DEEP, bool Q_DEEP, int PLANES, class Finish>
+__global__ __launch_bounds__(T::kThreads) void product_kernel(Product a, Finish finish) {
+    __shared__ __attribute__((aligned(16))) uint16_t room0[(T::BP + T::BQ) * kDepth];
+    __shared__ __attribute__((aligned(16))) uint16_t room1[(T::BP + T::BQ) * kDepth];
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+    // Tiles go in bands of 8 along q, in each band along p.
+    if (a.live != nullptr) {
+        const uint32_t live = __builtin_amdgcn_readfirstlane(*a.live);
+        if (a.live_depth) {
+            a.p.depth = a.q.depth = a.depth = live;
+        } else {
+            a.q.rows = live;
+            a.tiles_q = (live + T::BQ - 1u) / T::BQ;
+        }
+    }
+    const uint32_t tiles = a.tiles_p * a.tiles_q;
+    if (blockIdx.x >= tiles * a.splits) return;
+    const uint32_t place = xcd_order(blockIdx.x, tiles * a.splits), split = place / tiles, tile = place % tiles;
+    const uint32_t band = tile / (8u * a.tiles_p), in_band = tile % (8u * a.tiles_p);
+    const uint32_t high = a.tiles_q - band * 8u < 8u ? a.tiles_q - band * 8u : 8u;
+    const uint32_t tile_q = band * 8u + in_band % high, tile_p = in_band / high;
+
+    Loader<T::BP, T::kWaves, P_DEEP> load_p;
+    Loader<T::BQ, T::kWaves, Q_DEEP> load_q;
+    load_p.init(a.p, tile_p * T::BP, wave, lane);
+    load_q.init(a.q, tile_q * T::BQ, wave, lane);
+    const uint32_t wave_p = wave % T::WP, wave_q = wave / T::WP;
+    const Reader<T::BP, P_DEEP> read_p{wave_p * T::kWaveP, lane};
+    const Reader<T::BQ, Q_DEEP> read_q{wave_q * T::kWaveQ, lane};
+
+    f32x4 acc[T::TP][T::TQ];
+#pragma unroll
+    for (int i = 0; i < T::TP; ++i)
+#pragma unroll
+        for (int j = 0; j < T::TQ; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    constexpr uint32_t products = PLANES == 1 ? 1u : 6u;
+    const uint32_t steps = (a.depth + kDepth - 1u) / kDepth;
+    const uint32_t begin = (uint32_t)((uint64_t)steps * split / a.splits);
+    const uint32_t end = (uint32_t)((uint64_t)steps * (split + 1u) / a.splits);
+    const uint32_t total = (end - begin) * products;
+    const auto stage = [&](uint16_t *room, uint32_t s) {
+        uint32_t k = begin + s, plane_p = 0, plane_q = 0;
+        if constexpr (PLANES == 3) {
+            const uint32_t which = s % 6u;          // (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
+            k = begin + s / 6u;
+            plane_p = (0x010120u >> (4u * which)) & 15u;
+            plane_q = (0x001102u >> (4u * which)) & 15u;
+        }
+        load_p.load(room, k * kDepth, plane_p, wave);
+        load_q.load(room + T::BP * kDepth, k * kDepth, plane_q, wave);
+    };
+    const auto compute = [&](const uint16_t *room) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            s16x8_t fp[T::TP], fq[T::TQ];
+#pragma unroll
+            for (int i = 0; i < T::TP; ++i) fp[i] = read_p.read(room, i, half);
+#pragma unroll
+            for (int j = 0; j < T::TQ; ++j) fq[j] = read_q.read(room + T::BP * kDepth, j, half);
+#pragma unroll
+            for (int i = 0; i < T::TP; ++i)
+#pragma unroll
+                for (int j = 0; j < T::TQ; ++j) acc[i][j] = multiply<HALF>(fp[i], fq[j], acc[i][j]);
+        }
+    };
+    if (total > 0) stage(room0, 0);
+    __syncthreads();
+    for (uint32_t s = 0; s < total; s += 2) {
+        if (s + 1 < total) stage(room1, s + 1);
+        compute(room0);
+        __syncthreads();
+        if (s + 1 >= total) break;
+        if (s + 2 < total) stage(room0, s + 2);
+        compute(room1);
+        __syncthreads();
+    }
+    finish.template operator()<T>(acc, tile_p * T::BP + wave_p * T::kWaveP, tile_q * T::BQ + wave_q * T::kWaveQ, split,
+                                  lane);
+}
+
+template <bool HALF, class T, bool P_DEEP, bool Q_DEEP, int PLANES, class Finish>
+static void launch_product(Product a, const Finish &finish, hipStream_t s) {
+    const dim3 grid(a.tiles_p * a.tiles_q * a.splits);
+    product_kernel<HALF, T, P_DEEP, Q_DEEP, PLANES, Finish><<<grid, dim3(T::kThreads), 0, s>>>(a, finish);
+}
+
+}  // namespace nt

@@ -44,7 +44,7 @@ from . import _native
 from .array import DeviceArray
 from .backends import _backends, ensure_same_device, get_backend
 from .backends._graph_capture import reject_during_capture
-from .dtype import bfloat16, float16, float32
+from .dtype import bfloat16, float16, float32, int32, int64
 from .runtime import current_stream
 from .tensor import Tensor, device_views
 
@@ -66,7 +66,7 @@ def _current(value: Tensor) -> Tensor:
     return value
 
 
-def _activation(value, name: str, like: Tensor | None = None) -> int:
+def _activation(value, name: str, like: Tensor | None = None, what: str = "Layer norm and dropout") -> int:
     """Address of an activation (or gradient) Tensor, of `like`'s shape, dtype and device."""
     if not isinstance(value, Tensor):
         raise TypeError(f"{name} must be a NamiTorch Tensor, got {type(value).__name__}.")
@@ -74,7 +74,7 @@ def _activation(value, name: str, like: Tensor | None = None) -> int:
         if value._device not in _backends or value._ptr is None:
             backend = get_backend(value)     # which also puts a device under the capture checks
             if value._ptr is None:
-                backend._unsupported("Layer norm and dropout")
+                backend._unsupported(what)
         if value._dtype not in _DTYPES:
             raise TypeError(f"{name} must be float16, bfloat16 or float32, got {value._dtype.name}.")
     else:
@@ -407,5 +407,118 @@ def dropout_add_layer_norm_backward(grad_output, grad_total, total, mean, rstd, 
     return dx, dr, dw, db
 
 
+# ---- the loss -----------------------------------------------------------------------------------------
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def linear_cross_entropy(input, weight, target, *, ignore_index=-100, reduction="mean", out=None) -> Tensor:
+    """Softmax cross entropy of the logits ``input @ weight.T`` against the
+    class indices ``target``, without the logits ever being in memory.
+
+    ``input``: ``(..., width)``; ``weight``: ``(classes, width)`` of the same
+    dtype; ``target``: int64 or int32 of the leading shape.  Rows whose target
+    is ``ignore_index`` are not counted: whatever their input holds, their
+    loss is zero and they give no gradient.  ``reduction``: the ``"mean"`` over
+    the counted rows (zero where there are none), their ``"sum"``, or
+    ``"none"``, a loss for each row; float32 in every case.  A target that is
+    no class makes its row's loss NaN, and the gradients."""
+    return _linear_cross_entropy(input, weight, target, ignore_index, reduction, _given(out, 1), False)[0]
+
+
+def linear_cross_entropy_forward(input, weight, target, *, ignore_index=-100, reduction="mean", out=None) -> tuple:
+    """``(loss, lse)``: :func:`linear_cross_entropy` and the float32
+    ``log(sum(exp(logits)))`` of each row (zero where it is not counted) that
+    :func:`linear_cross_entropy_backward` reads."""
+    return _linear_cross_entropy(input, weight, target, ignore_index, reduction, _given(out, 2), True)
+
+
+def _linear_cross_entropy(x, weight, target, ignore_index, reduction, given, keep: bool) -> tuple:
+    source = _activation(x, "input", None, "Linear cross entropy")
+    head, classes, width = _head(weight, x)
+    lead, at = x._shape[:-1], _targets(target, x)
+    code, ignored = _reduction(reduction), _ignored(ignore_index)
+    reject_during_capture("Linear cross entropy")
+    loss = _result(given[0], "loss", lead if code == 0 else (), float32, x)
+    lse = _result(given[1], "lse", lead, float32, x) if keep else None
+    device = x._device.index
+    _launch(_native.load().nt_linear_cross_entropy(
+        device, source, head, x._dtype._code, at, target._dtype.itemsize, ignored, code, loss._ptr,
+        lse._ptr if keep else None, math.prod(lead), classes, width, current_stream(device)), given)
+    return loss, lse
+
+
+def linear_cross_entropy_backward(grad_loss, input, weight, target, lse, *, ignore_index=-100, reduction="mean",
+                                  out=None) -> tuple:
+    """``(grad_input, grad_weight)`` of :func:`linear_cross_entropy_forward`
+    with its ``lse`` and the same ``ignore_index`` and ``reduction``.
+    ``grad_loss``, the gradient of the loss: a float32 Tensor of the loss's
+    shape or, for a mean or sum, a number (a loss scale; 1 without one)."""
+    given = _given(out, 2)
+    x = _activation(input, "input", None, "Linear cross entropy")
+    head, classes, width = _head(weight, input)
+    lead, at = input._shape[:-1], _targets(target, input)
+    code, ignored = _reduction(reduction), _ignored(ignore_index)
+    kept = _statistic(lse, "lse", lead, input)
+    value, grad = 0.0, None
+    if isinstance(grad_loss, Tensor):
+        grad = _statistic(grad_loss, "grad_loss", lead if code == 0 else (), input)
+    elif isinstance(grad_loss, bool) or not isinstance(grad_loss, Real) or code == 0:
+        raise TypeError("grad_loss must be a float32 Tensor of the loss's shape" +
+                        (", as each row has a loss." if code == 0 else " or a real number."))
+    else:
+        value = float(grad_loss)
+    reject_during_capture("Linear cross entropy backward")
+    dx = _result(given[0], "grad_input", input._shape, input._dtype, input)
+    dw = _result(given[1], "grad_weight", weight._shape, weight._dtype, input)
+    device = input._device.index
+    _launch(_native.load().nt_linear_cross_entropy_backward(
+        device, grad, value, x, head, input._dtype._code, at, target._dtype.itemsize, ignored, code, kept, dx._ptr,
+        dw._ptr, math.prod(lead), classes, width, current_stream(device)), given)
+    return dx, dw
+
+
+def _head(weight, x: Tensor) -> tuple:
+    """(address of the weight, classes, width)."""
+    if not x._shape:
+        raise ValueError("input must have at least one dimension.")
+    if not isinstance(weight, Tensor):
+        raise TypeError(f"weight must be a NamiTorch Tensor, got {type(weight).__name__}.")
+    if len(weight._shape) != 2 or weight._shape[1] != x._shape[-1] or 0 in weight._shape:
+        raise ValueError(f"weight has shape {weight._shape}; expected (classes, {x._shape[-1]}), neither of them zero.")
+    if weight._dtype is not x._dtype:
+        raise TypeError(f"weight has dtype {weight._dtype.name}; expected {x._dtype.name}.")
+    if weight._device is not x._device:
+        ensure_same_device(x, weight)
+    return _current(weight)._ptr, *weight._shape
+
+
+def _targets(target, x: Tensor) -> int:
+    if not isinstance(target, Tensor):
+        raise TypeError(f"target must be a NamiTorch Tensor, got {type(target).__name__}.")
+    if target._dtype not in (int32, int64):
+        raise TypeError(f"target must be int64 or int32, got {target._dtype.name}.")
+    if target._shape != x._shape[:-1]:
+        raise ValueError(f"target has shape {target._shape}; expected {x._shape[:-1]}.")
+    if target._device is not x._device:
+        ensure_same_device(x, target)
+    return target._ptr
+
+
+def _reduction(value) -> int:
+    code = _REDUCTIONS.get(value) if isinstance(value, str) else None
+    if code is None:
+        raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {value!r}.")
+    return code
+
+
+def _ignored(value) -> int:
+    if isinstance(value, bool) or not isinstance(value, Integral):
+        raise TypeError("ignore_index must be an integer.")
+    if not -(1 << 63) <= value < 1 << 63:
+        raise ValueError(f"ignore_index must be in [-2**63, 2**63), got {value}.")
+    return int(value)
+
+
 __all__ = ["layer_norm", "layer_norm_forward", "layer_norm_backward", "dropout", "dropout_backward",
-           "dropout_add_layer_norm", "dropout_add_layer_norm_forward", "dropout_add_layer_norm_backward"]
+           "dropout_add_layer_norm", "dropout_add_layer_norm_forward", "dropout_add_layer_norm_backward",
+           "linear_cross_entropy", "linear_cross_entropy_forward", "linear_cross_entropy_backward"]
