@@ -597,6 +597,43 @@ int32_t nt_dropout_add_layer_norm_backward(int32_t device, const void *dy, const
                                            void *dweight, void *dbias, uint64_t rows,
                                            uint64_t width, void *stream);
 
+/*
+ * The edge after a block that is normalized before and after it.  With
+ * N(x; w, b) = (x - mean) rstd w + b as in nt_layer_norm, or with `rms` the
+ * root mean square instead of the deviation and no mean:
+ *
+ *   total = residual_scale residual + gate N(x; inner_weight, inner_bias)
+ *   y     = N(total; weight, bias)
+ *
+ * y is of total before its rounding.  NULL weights are ones, NULL biases
+ * zeros, a NULL gate is one.  The gate (`gate_dtype`: the activations' or
+ * float32) has `gate_rows` rows of `width`, each for rows / gate_rows
+ * consecutive rows.  The four statistics (float32, one per row) are given
+ * together or not at all, without the means for `rms`; the backward entry
+ * takes NULL means as rms.  It writes dx, dresidual and, where not NULL, the
+ * gradients of the vectors and the gate (sums over rows in a fixed order).
+ * dtotal, the gradient total receives elsewhere, may be NULL.  Types, widths,
+ * overlaps, captures and empty batches as in nt_layer_norm.
+ */
+int32_t nt_norm_gate_add_norm(int32_t device, const void *x, const void *residual, int32_t dtype,
+                              const void *inner_weight, const void *inner_bias, const void *gate,
+                              int32_t gate_dtype, uint64_t gate_rows, const void *weight,
+                              const void *bias, int32_t weight_dtype, float residual_scale,
+                              float eps, int32_t rms, void *total, void *y, float *inner_mean,
+                              float *inner_rstd, float *mean, float *rstd, uint64_t rows,
+                              uint64_t width, void *stream);
+int32_t nt_norm_gate_add_norm_backward(int32_t device, const void *dy, const void *dtotal,
+                                       const void *x, const void *total, int32_t dtype,
+                                       const float *inner_mean, const float *inner_rstd,
+                                       const float *mean, const float *rstd,
+                                       const void *inner_weight, const void *inner_bias,
+                                       const void *gate, int32_t gate_dtype, uint64_t gate_rows,
+                                       const void *weight, int32_t weight_dtype,
+                                       float residual_scale, void *dx, void *dresidual,
+                                       void *dinner_weight, void *dinner_bias, void *dgate,
+                                       void *dweight, void *dbias, uint64_t rows, uint64_t width,
+                                       void *stream);
+
 /* ---- the loss ----------------------------------------------------------- */
 
 /*

@@ -176,6 +176,14 @@ SIGNATURES = {
     "nt_dropout_add_layer_norm_backward": (c_int32, [c_int32, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p,
                                                      c_void_p, c_int32, c_uint32, c_uint64, c_uint64, c_void_p,
                                                      c_void_p, c_void_p, c_void_p, c_uint64, c_uint64, c_void_p]),
+    "nt_norm_gate_add_norm": (c_int32, [c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_int32,
+                                        c_uint64, c_void_p, c_void_p, c_int32, c_float, c_float, c_int32, c_void_p,
+                                        c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_uint64, c_uint64, c_void_p]),
+    "nt_norm_gate_add_norm_backward": (c_int32, [c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p,
+                                                 c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32,
+                                                 c_uint64, c_void_p, c_int32, c_float, c_void_p, c_void_p, c_void_p,
+                                                 c_void_p, c_void_p, c_void_p, c_void_p, c_uint64, c_uint64,
+                                                 c_void_p]),
     "nt_linear_cross_entropy": (c_int32, [c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_int32, c_int64, c_int32,
                                           c_void_p, c_void_p, c_uint64, c_uint64, c_uint64, c_void_p]),
     "nt_linear_cross_entropy_backward": (c_int32, [c_int32, c_void_p, c_float, c_void_p, c_void_p, c_int32, c_void_p,

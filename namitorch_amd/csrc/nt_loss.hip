@@ -28,9 +28,9 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <initializer_list>
 #include <string>
 
+#include "nt_entry.hpp"
 #include "nt_internal.hpp"
 #include "nt_pool.hpp"
 #include "nt_product.hpp"
@@ -458,38 +458,6 @@ struct Problem {
     int32_t reduction;
 };
 
-// Memory of the pool for one call, in parts; goes back as soon as the kernels
-// are queued (the pool reuses it on this stream only).
-class Workspace {
-  public:
-    template <class V>
-    void want(V **at, uint64_t count) {
-        entries_[used_++] = {reinterpret_cast<void **>(at), bytes_};
-        bytes_ += (count * sizeof(V) + 255u) & ~255ull;
-    }
-    int32_t allocate(int32_t device, void *stream) {
-        std::string error;
-        const int32_t rc = device_pool().allocate(device, bytes_ > 0 ? bytes_ : 256u, stream, &base_, error);
-        if (rc != NT_OK) return fail(rc, error);
-        for (int k = 0; k < used_; ++k) *entries_[k].at = static_cast<char *>(base_) + entries_[k].offset;
-        return NT_OK;
-    }
-    ~Workspace() {
-        std::string error;
-        if (base_ != nullptr) (void)device_pool().release(base_, error);
-    }
-
-  private:
-    struct Entry {
-        void **at;
-        uint64_t offset;
-    };
-    Entry entries_[16];
-    int used_ = 0;
-    uint64_t bytes_ = 0;
-    void *base_ = nullptr;
-};
-
 static uint32_t blocks_of(uint64_t items, uint32_t each) {
     const uint64_t blocks = (items + each - 1) / each;
     return blocks < 1 ? 1u : blocks > 8192u ? 8192u : (uint32_t)blocks;
@@ -665,7 +633,7 @@ static int32_t backward_of(const Problem &a, int32_t device, const float *grad, 
 static int32_t check_problem(const char *entry, int32_t dtype, int32_t target_size, int32_t reduction, uint64_t rows,
                              uint64_t classes, uint64_t width) {
     const std::string name(entry);
-    if (dtype != NT_F32 && dtype != NT_F16 && dtype != NT_BF16)
+    if (!half_or_float(dtype))
         return fail(NT_ERR_TYPE, name + ": input and weight must be float32, float16 or bfloat16");
     if (target_size != 4 && target_size != 8) return fail(NT_ERR_TYPE, name + ": targets must be int32 or int64");
     if (reduction < kEach || reduction > kSum) return fail(NT_ERR_VALUE, name + ": unknown reduction");
@@ -673,38 +641,6 @@ static int32_t check_problem(const char *entry, int32_t dtype, int32_t target_si
     if (classes == 0 || classes >= 1u << 30) return fail(NT_ERR_VALUE, name + ": there must be 1..2**30 - 1 classes");
     if (rows >= 1u << 24) return fail(NT_ERR_VALUE, name + ": there must be fewer than 2**24 rows");
     return NT_OK;
-}
-
-struct LossArray {
-    const void *ptr;
-    uint64_t size, count;       // bytes of an element, elements
-    bool written, needed;
-};
-
-static int32_t check_loss_arrays(const char *entry, std::initializer_list<LossArray> arrays) {
-    for (const LossArray &a : arrays) {
-        if (a.ptr == nullptr) {
-            if (a.needed && a.count > 0) return fail(NT_ERR_VALUE, std::string(entry) + ": NULL array");
-            continue;
-        }
-        const uintptr_t start = (uintptr_t)a.ptr;
-        if (start % a.size != 0) return fail(NT_ERR_VALUE, std::string(entry) + ": an array is not aligned to its dtype");
-        if (!a.written) continue;
-        for (const LossArray &b : arrays) {
-            if (&a == &b || b.ptr == nullptr) continue;
-            const uintptr_t other = (uintptr_t)b.ptr;
-            if (start < other + b.count * b.size && other < start + a.count * a.size)
-                return fail(NT_ERR_VALUE, std::string(entry) + ": an output overlaps another array");
-        }
-    }
-    return NT_OK;
-}
-
-static int32_t refuse_loss_capture(const char *entry, void *stream) {
-    int32_t capturing = 0;
-    const int32_t rc = nt_stream_capturing(stream, &capturing);
-    if (rc != NT_OK) return rc;
-    return capturing ? fail(NT_ERR_RUNTIME, std::string(entry) + ": not supported in stream capture") : NT_OK;
 }
 
 }  // namespace nt
@@ -720,17 +656,17 @@ int32_t nt_linear_cross_entropy(int32_t device, const void *x, const void *weigh
     const char *entry = "nt_linear_cross_entropy";
     int32_t rc = check_problem(entry, dtype, target_size, reduction, rows, classes, width);
     if (rc != NT_OK) return rc;
-    const uint64_t size = dtype == NT_F32 ? 4u : 2u;
-    rc = check_loss_arrays(entry, {{x, size, rows * width, false, true},
-                                   {weight, size, classes * width, false, true},
-                                   {target, (uint64_t)target_size, rows, false, true},
-                                   {loss, 4, reduction == kEach ? rows : 1, true, true},
-                                   {lse, 4, rows, true, false}});
+    const int32_t index = target_size == 8 ? kInt64 : kInt32;
+    rc = check_arrays(entry, {{x, dtype, rows * width, false, rows > 0},
+                              {weight, dtype, classes * width, false, true},
+                              {target, index, rows, false, rows > 0},
+                              {loss, NT_F32, reduction == kEach ? rows : 1, true, reduction != kEach || rows > 0},
+                              {lse, NT_F32, rows, true, false}});
     if (rc != NT_OK) return rc;
     if (rows == 0 && reduction == kEach) return NT_OK;
     DeviceGuard guard(device);
     if (!guard.ok()) return hip_check(guard.error(), "hipSetDevice");
-    rc = refuse_loss_capture(entry, stream);
+    rc = refuse_capture(entry, stream);
     if (rc != NT_OK) return rc;
     if (rows == 0) return nt_fill(loss, 1, 4, 0, stream);
     const Problem a{x, weight, dtype, (uint32_t)rows, (uint32_t)classes, (uint32_t)width,
@@ -750,20 +686,20 @@ int32_t nt_linear_cross_entropy_backward(int32_t device, const float *grad_loss,
     const char *entry = "nt_linear_cross_entropy_backward";
     int32_t rc = check_problem(entry, dtype, target_size, reduction, rows, classes, width);
     if (rc != NT_OK) return rc;
-    const uint64_t size = dtype == NT_F32 ? 4u : 2u;
-    rc = check_loss_arrays(entry, {{grad_loss, 4, reduction == kEach ? rows : 1, false, reduction == kEach},
-                                   {x, size, rows * width, false, true},
-                                   {weight, size, classes * width, false, true},
-                                   {target, (uint64_t)target_size, rows, false, true},
-                                   {lse, 4, rows, false, true},
-                                   {dx, size, rows * width, true, true},
-                                   {dweight, size, classes * width, true, true}});
+    const int32_t index = target_size == 8 ? kInt64 : kInt32;
+    rc = check_arrays(entry, {{grad_loss, NT_F32, reduction == kEach ? rows : 1, false, reduction == kEach && rows > 0},
+                              {x, dtype, rows * width, false, rows > 0},
+                              {weight, dtype, classes * width, false, true},
+                              {target, index, rows, false, rows > 0},
+                              {lse, NT_F32, rows, false, rows > 0},
+                              {dx, dtype, rows * width, true, rows > 0},
+                              {dweight, dtype, classes * width, true, true}});
     if (rc != NT_OK) return rc;
     DeviceGuard guard(device);
     if (!guard.ok()) return hip_check(guard.error(), "hipSetDevice");
-    rc = refuse_loss_capture(entry, stream);
+    rc = refuse_capture(entry, stream);
     if (rc != NT_OK) return rc;
-    if (rows == 0) return nt_fill(dweight, classes * width, (int32_t)size, 0, stream);
+    if (rows == 0) return nt_fill(dweight, classes * width, dtype == NT_F32 ? 4 : 2, 0, stream);
     const Problem a{x, weight, dtype, (uint32_t)rows, (uint32_t)classes, (uint32_t)width,
                     {target, ignore_index, (uint32_t)classes, target_size}, reduction};
     switch (dtype) {

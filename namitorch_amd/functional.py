@@ -407,6 +407,165 @@ def dropout_add_layer_norm_backward(grad_output, grad_total, total, mean, rstd, 
     return dx, dr, dw, db
 
 
+# ---- the edge after a block that is normalized on both sides --------------------------------------------
+_NORMS = {"layer": 0, "rms": 1}
+
+
+def norm_gate_add_norm(input, residual, normalized_shape, inner_weight=None, inner_bias=None, gate=None, weight=None,
+                       bias=None, residual_scale=1.0, eps=1e-5, *, norm="layer", out=None) -> tuple:
+    """``(output, total)`` with ``total = residual_scale * residual + gate *
+    N(input)`` and ``output = N(total)``: the norm after a block, its gate, the
+    residual stream and the norm before the next block, in one pass.
+
+    ``N`` is layer norm over the trailing dimensions ``normalized_shape`` or,
+    with ``norm="rms"``, the root mean square norm ``x / sqrt(mean(x**2) + eps)
+    * weight + bias``; the first has ``inner_weight`` and ``inner_bias``, the
+    second ``weight`` and ``bias`` (one dtype for all).  ``gate``, of the input's
+    dtype or float32, has the normalized shape (one gate for all rows), or
+    leading dimensions of the input before it, of which the last ones may be 1
+    (one for each sequence of a batch, or for each row).  The second norm is
+    taken before ``total`` is rounded to its dtype."""
+    return _gated(input, residual, normalized_shape, inner_weight, inner_bias, gate, weight, bias, residual_scale, eps,
+                  norm, _given(out, 2), False)[:2]
+
+
+def norm_gate_add_norm_forward(input, residual, normalized_shape, inner_weight=None, inner_bias=None, gate=None,
+                               weight=None, bias=None, residual_scale=1.0, eps=1e-5, *, norm="layer",
+                               out=None) -> tuple:
+    """``(output, total, inner_mean, inner_rstd, mean, rstd)``:
+    :func:`norm_gate_add_norm` with the float32 statistics that its backward
+    call reads.  With ``norm="rms"`` the means are None."""
+    return _gated(input, residual, normalized_shape, inner_weight, inner_bias, gate, weight, bias, residual_scale, eps,
+                  norm, _given(out, 6), True)
+
+
+def _gated(x, residual, normalized_shape, inner_weight, inner_bias, gate, weight, bias, residual_scale, eps, norm, given,
+           stats: bool) -> tuple:
+    source = _activation(x, "input")
+    stream_in = _activation(residual, "residual", x)
+    lead, shape, rows, width = _normalized(x, normalized_shape)
+    vectors, code = _vectors((inner_weight, inner_bias, weight, bias), shape, x)
+    gate_at, gate_code, gate_rows = _gate(gate, lead, shape, x)
+    scale, eps, rms = _scale(residual_scale), _epsilon(eps), _norm_kind(norm)
+    if stats and rms and (given[2] is not None or given[4] is not None):
+        raise ValueError("out: a mean was given, but root mean square norms have none.")
+    needed = given if not (stats and rms) else (given[0], given[1], given[3], given[5])
+    if None in needed:
+        reject_during_capture("Layer norm without out")
+    y = _result(given[0], "output", x._shape, x._dtype, x)
+    total = _result(given[1], "total", x._shape, x._dtype, x)
+    kept = [None] * 4
+    if stats:
+        for place, name in enumerate(("inner_mean", "inner_rstd", "mean", "rstd")):
+            if not rms or place % 2:
+                kept[place] = _result(given[2 + place], name, lead, float32, x)
+    device = x._device.index
+    _launch(_native.load().nt_norm_gate_add_norm(
+        device, source, stream_in, x._dtype._code, vectors[0], vectors[1], gate_at, gate_code, gate_rows, vectors[2],
+        vectors[3], code, scale, eps, rms, total._ptr, y._ptr, *(None if k is None else k._ptr for k in kept), rows,
+        width, current_stream(device)), given)
+    return (y, total, *kept)
+
+
+def norm_gate_add_norm_backward(grad_output, grad_total, input, total, inner_mean, inner_rstd, mean, rstd,
+                                inner_weight=None, inner_bias=None, gate=None, weight=None, bias=None,
+                                residual_scale=1.0, *, out=None) -> tuple:
+    """``(grad_input, grad_residual, grad_inner_weight, grad_inner_bias,
+    grad_gate, grad_weight, grad_bias)`` of :func:`norm_gate_add_norm_forward`
+    at ``input`` with its ``total`` and statistics (means None: root mean
+    square norms), from the gradients of its two results (``grad_total`` None:
+    nothing else reads ``total``).  A parameter's gradient has its shape and
+    dtype, and is None where the parameter is None."""
+    given = _given(out, 7)
+    t = _activation(total, "total")
+    source = _activation(input, "input", total)
+    dy = _activation(grad_output, "grad_output", total)
+    dt = None if grad_total is None else _activation(grad_total, "grad_total", total)
+    if (mean is None) != (inner_mean is None):
+        raise ValueError("inner_mean and mean are given together, or both are None (root mean square norms).")
+    if not isinstance(rstd, Tensor):
+        raise TypeError(f"rstd must be a NamiTorch Tensor, got {type(rstd).__name__}.")
+    lead = len(rstd._shape)
+    if lead >= len(total._shape) or rstd._shape != total._shape[:lead]:
+        raise ValueError(f"rstd has shape {rstd._shape}, which is not the leading shape of {total._shape}.")
+    lead, shape, rows, width = _split(total, lead)
+    stats = [None if value is None else _statistic(value, name, lead, total) for value, name in (
+        (inner_mean, "inner_mean"), (inner_rstd, "inner_rstd"), (mean, "mean"), (rstd, "rstd"))]
+    if stats[1] is None and inner_rstd is None:
+        raise TypeError("inner_rstd must be a NamiTorch Tensor, got NoneType.")
+    vectors, code = _vectors((inner_weight, inner_bias, weight, bias), shape, total)
+    gate_at, gate_code, gate_rows = _gate(gate, lead, shape, total)
+    scale = _scale(residual_scale)
+    if None in given:
+        reject_during_capture("Layer norm backward")
+    dx = _result(given[0], "grad_input", total._shape, total._dtype, total)
+    dr = _result(given[1], "grad_residual", total._shape, total._dtype, total)
+    made = []
+    for parameter, name, result in zip((inner_weight, inner_bias, gate, weight, bias),
+                                       ("grad_inner_weight", "grad_inner_bias", "grad_gate", "grad_weight", "grad_bias"),
+                                       given[2:]):
+        if parameter is not None:
+            made.append(_result(result, name, parameter._shape, parameter._dtype, total))
+        elif result is None:
+            made.append(None)
+        else:
+            raise ValueError(f"out: {name} was given, but the edge has no such parameter.")
+    device = total._device.index
+    _launch(_native.load().nt_norm_gate_add_norm_backward(
+        device, dy, dt, source, t, total._dtype._code, *stats, vectors[0], vectors[1], gate_at, gate_code, gate_rows,
+        vectors[2], code, scale, dx._ptr, dr._ptr, *(None if v is None else v._ptr for v in made), rows, width,
+        current_stream(device)), given)
+    return (dx, dr, *made)
+
+
+def _vectors(values, shape: tuple, like: Tensor) -> tuple:
+    """(addresses of the weights and biases, their dtype code)."""
+    names = ("inner_weight", "inner_bias", "weight", "bias")
+    at = [_affine(value, name, shape, like) for value, name in zip(values, names)]
+    kinds = {value._dtype for value in values if value is not None}
+    if len(kinds) > 1:
+        raise TypeError(f"weights and biases must have one dtype, got {' and '.join(sorted(k.name for k in kinds))}.")
+    return at, (kinds.pop() if kinds else like._dtype)._code
+
+
+def _gate(value, lead: tuple, shape: tuple, like: Tensor) -> tuple:
+    """(address, dtype code, rows) of a gate; 0 rows where there is none."""
+    if value is None:
+        return None, like._dtype._code, 0
+    if not isinstance(value, Tensor):
+        raise TypeError(f"gate must be a NamiTorch Tensor, got {type(value).__name__}.")
+    own = len(value._shape) - len(shape)
+    before = value._shape[:own] if own >= 0 else None
+    same = 0
+    if before:
+        while same < own and same < len(lead) and before[same] == lead[same]:
+            same += 1
+    if before is None or value._shape[own:] != shape or own not in (0, len(lead)) or any(n != 1 for n in before[same:]):
+        raise ValueError(f"gate has shape {value._shape}; expected {shape}, or leading dimensions of {lead} before it, "
+                         "the last of which may be 1.")
+    if value._dtype is not like._dtype and value._dtype is not float32:
+        raise TypeError(f"gate must be {like._dtype.name} or float32, got {value._dtype.name}.")
+    if value._device is not like._device:
+        ensure_same_device(like, value)
+    return _current(value)._ptr, value._dtype._code, math.prod(before)
+
+
+def _scale(value) -> float:
+    if isinstance(value, bool) or not isinstance(value, Real):
+        raise TypeError("residual_scale must be a real number.")
+    value = float(value)
+    if not abs(value) <= _MOST_EPS:
+        raise ValueError(f"residual_scale must be finite as a float32, got {value}.")
+    return value
+
+
+def _norm_kind(value) -> int:
+    code = _NORMS.get(value) if isinstance(value, str) else None
+    if code is None:
+        raise ValueError(f"norm must be 'layer' or 'rms', got {value!r}.")
+    return code
+
+
 # ---- the loss -----------------------------------------------------------------------------------------
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
@@ -521,4 +680,5 @@ def _ignored(value) -> int:
 
 __all__ = ["layer_norm", "layer_norm_forward", "layer_norm_backward", "dropout", "dropout_backward",
            "dropout_add_layer_norm", "dropout_add_layer_norm_forward", "dropout_add_layer_norm_backward",
+           "norm_gate_add_norm", "norm_gate_add_norm_forward", "norm_gate_add_norm_backward",
            "linear_cross_entropy", "linear_cross_entropy_forward", "linear_cross_entropy_backward"]
