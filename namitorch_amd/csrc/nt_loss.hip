@@ -151,17 +151,18 @@ __device__ __forceinline__ void three_planes(float v, uint16_t (&plane)[3]) {
 }
 
 // Rows of `width` elements at any address to rows of `pitch` (a multiple of
-// 8), the end of each zero.  `row` and `live`: a row each from there, as many
-// as `live` says.
+// 64), the end of each zero, and to the next multiple of 64 rows of zeros.
+// `row` and `live`: a row each from there, as many as `live` says.
 template <class T>
 __global__ __launch_bounds__(kBlock) void pack_kernel(const void *from, uint32_t width, uint16_t *to, uint32_t pitch,
                                                       uint64_t plane, uint32_t rows, const uint32_t *row,
                                                       const uint32_t *live) {
     if (live != nullptr) rows = *live;
-    const uint64_t groups = pitch / 8u, all = rows * groups;
+    const uint64_t groups = pitch / 8u, all = whole_steps(rows) * groups;
     for (uint64_t g = blockIdx.x * (uint64_t)kBlock + threadIdx.x; g < all; g += (uint64_t)gridDim.x * kBlock) {
         const uint32_t r = (uint32_t)(g / groups), c = (uint32_t)(g % groups) * 8u;
-        const uint64_t source = (row != nullptr ? row[r] : r) * (uint64_t)width + c;
+        const uint64_t source = (row == nullptr || r >= rows ? r : row[r]) * (uint64_t)width + c;
+        const uint32_t end = r < rows ? width : 0u;
         const auto *in = reinterpret_cast<const typename T::raw *>(from) + source;
         uint16_t *out = to + r * (uint64_t)pitch + c;
         if constexpr (T::code == NT_F32) {
@@ -169,7 +170,7 @@ __global__ __launch_bounds__(kBlock) void pack_kernel(const void *from, uint32_t
 #pragma unroll
             for (uint32_t k = 0; k < 8; ++k) {
                 uint16_t one[3];
-                three_planes(c + k < width ? in[k] : 0.0f, one);
+                three_planes(c + k < end ? in[k] : 0.0f, one);
                 planes[0][k] = one[0];
                 planes[1][k] = one[1];
                 planes[2][k] = one[2];
@@ -179,7 +180,7 @@ __global__ __launch_bounds__(kBlock) void pack_kernel(const void *from, uint32_t
         } else {
             uint16_t group[8];
 #pragma unroll
-            for (uint32_t k = 0; k < 8; ++k) group[k] = c + k < width ? in[k] : (uint16_t)0;
+            for (uint32_t k = 0; k < 8; ++k) group[k] = c + k < end ? in[k] : (uint16_t)0;
             *reinterpret_cast<u32x4_t *>(out) = __builtin_bit_cast(u32x4_t, group);
         }
     }
@@ -248,7 +249,8 @@ struct FinishLoss {
     }
 };
 
-// Logits to dz.  The columns from the piece's last class to the line's end are zero.
+// Logits to dz.  The columns from the piece's last class to the line's end and
+// the rows from the last counted one to a whole step are zero.
 template <bool HALF, int PLANES>
 struct FinishGrad {
     uint16_t *dz;
@@ -262,13 +264,14 @@ struct FinishGrad {
     template <class T>
     __device__ __forceinline__ void operator()(const f32x4 (&acc)[T::TP][T::TQ], uint32_t p_first, uint32_t q_first,
                                                uint32_t, uint32_t lane) const {
-        const uint32_t count = *live, up = p_first + 4u * (lane >> 4);
+        const uint32_t count = *live, padded = whole_steps(count), up = p_first + 4u * (lane >> 4);
 #pragma unroll
         for (int j = 0; j < T::TQ; ++j) {
             const uint32_t q = q_first + 16u * j + (lane & 15u);
-            if (q >= count) continue;
-            const float from = lse[row[q]], by = weight[q];
-            const uint32_t place = (uint32_t)target[q] - first - up;
+            if (q >= padded) continue;
+            const bool there = q < count;
+            const float from = there ? lse[row[q]] : 0.0f, by = there ? weight[q] : 0.0f;
+            const uint32_t place = there ? (uint32_t)target[q] - first - up : ~0u;
             uint16_t *line = dz + q * (uint64_t)pitch + up;
 #pragma unroll
             for (int i = 0; i < T::TP; ++i) {
@@ -278,7 +281,7 @@ struct FinishGrad {
                 for (int r = 0; r < 4; ++r) {
                     v[r] = exp_of(acc[i][j][r] - from);
                     if (place == 16u * i + r) v[r] -= 1.0f;
-                    v[r] = up + 16u * i + r < classes ? v[r] * by : 0.0f;
+                    v[r] = there && up + 16u * i + r < classes ? v[r] * by : 0.0f;
                 }
                 if constexpr (PLANES == 1) {
                     uint16_t e[4];
@@ -448,7 +451,7 @@ __global__ __launch_bounds__(kBlock) void grad_input_kernel(const float *sums, u
 constexpr uint64_t kPieceBytes = 512ull << 20;       // of dz, and of packed weights, at a time
 constexpr uint32_t kSumTiles = 512;                  // dx: tiles and splits to fill the chip with
 
-using Large = Tile<128, 128, 2, 2>;
+using Large = Tile<256, 256, 2, 4>;
 
 struct Problem {
     const void *x, *w;
@@ -485,7 +488,7 @@ static int32_t forward_of(const Problem &a, int32_t device, float *loss, float *
     constexpr int planes = Kind<T>::kPlanes;
     constexpr bool half = Kind<T>::kHalf;
     hipStream_t s = (hipStream_t)stream;
-    const uint32_t pitch = (a.width + 7u) / 8u * 8u;
+    const uint32_t pitch = whole_steps(a.width), padded = whole_steps(a.rows);
     const bool pack_w = planes > 1 || pitch != a.width || (uintptr_t)a.w % 16u != 0;
     const uint32_t piece = piece_of(a, pitch, planes, pack_w, false);
     using Shape = Large;
@@ -503,8 +506,8 @@ static int32_t forward_of(const Problem &a, int32_t device, float *loss, float *
     room.want(&rows.target, a.rows);
     room.want(&target_logit, a.rows);
     room.want(&partials, slots * a.rows);
-    room.want(&px, (uint64_t)planes * a.rows * pitch);
-    if (pack_w) room.want(&pw, (uint64_t)planes * piece * pitch);
+    room.want(&px, (uint64_t)planes * padded * pitch);
+    if (pack_w) room.want(&pw, (uint64_t)planes * whole_steps(piece) * pitch);
     if (a.reduction != kEach) room.want(&each, a.rows);
     int32_t rc = room.allocate(device, stream);
     if (rc != NT_OK) return rc;
@@ -512,8 +515,8 @@ static int32_t forward_of(const Problem &a, int32_t device, float *loss, float *
 
     rows_kernel<false><<<1, kRowsBlock, 0, s>>>(a.targets, a.rows, rows, nullptr, 0.0f, a.reduction, false);
     loss_ignored_kernel<<<blocks_of(a.rows, kBlock), kBlock, 0, s>>>(a.targets, a.rows, lse, to);
-    const uint64_t plane_x = (uint64_t)a.rows * pitch, plane_w = (uint64_t)piece * pitch;
-    pack_kernel<T><<<blocks_of(a.rows * (uint64_t)(pitch / 8u), kBlock), kBlock, 0, s>>>(
+    const uint64_t plane_x = (uint64_t)padded * pitch, plane_w = (uint64_t)whole_steps(piece) * pitch;
+    pack_kernel<T><<<blocks_of(padded * (uint64_t)(pitch / 8u), kBlock), kBlock, 0, s>>>(
         a.x, a.width, px, pitch, plane_x, a.rows, rows.row, rows.count);
     for (uint32_t k = 0; k < pieces; ++k) {
         const uint32_t first = k * piece, classes = std::min(piece, a.classes - first);
@@ -522,10 +525,10 @@ static int32_t forward_of(const Problem &a, int32_t device, float *loss, float *
             pack_kernel<T><<<blocks_of(classes * (uint64_t)(pitch / 8u), kBlock), kBlock, 0, s>>>(
                 weights, a.width, pw, pitch, plane_w, classes, nullptr, nullptr);
         Product product{};
-        product.p = Operand{pack_w ? pw : static_cast<const uint16_t *>(weights), pitch, plane_w, classes, pitch};
-        product.q = Operand{px, pitch, plane_x, a.rows, pitch};
+        product.p = Operand{pack_w ? pw : static_cast<const uint16_t *>(weights), nullptr, pitch, plane_w, classes};
+        product.q = Operand{px, nullptr, pitch, plane_x, a.rows};
         product.tiles_p = (classes + Shape::BP - 1) / Shape::BP;
-        product.tiles_q = (a.rows + Shape::BQ - 1) / Shape::BQ;
+        product.tiles_q = (padded + Shape::BQ - 1) / Shape::BQ;
         product.splits = 1;
         product.depth = pitch;
         product.live = rows.count;
@@ -548,12 +551,12 @@ static int32_t backward_of(const Problem &a, int32_t device, const float *grad, 
     using Shape = Large;
     using Raw = typename T::raw;
     hipStream_t s = (hipStream_t)stream;
-    const uint32_t pitch = (a.width + 7u) / 8u * 8u;
+    const uint32_t pitch = whole_steps(a.width), padded = whole_steps(a.rows);
     const bool pack_w = planes > 1 || pitch != a.width || (uintptr_t)a.w % 16u != 0;
     const uint32_t piece = piece_of(a, pitch, planes, pack_w, true);
     const uint32_t pieces = (a.classes + piece - 1) / piece;
-    const uint32_t dz_pitch = (piece + 63u) / 64u * 64u;
-    const uint32_t tiles_h = (pitch + Shape::BP - 1) / Shape::BP, tiles_n = (a.rows + Shape::BQ - 1) / Shape::BQ;
+    const uint32_t dz_pitch = whole_steps(piece);
+    const uint32_t tiles_h = (pitch + Shape::BP - 1) / Shape::BP, tiles_n = (padded + Shape::BQ - 1) / Shape::BQ;
     const uint32_t depth = (piece + kDepth - 1) / kDepth;
     uint32_t splits = std::max(1u, kSumTiles / std::max(1u, tiles_h * tiles_n));
     splits = std::min(splits, std::max(1u, depth / 8u));
@@ -567,29 +570,38 @@ static int32_t backward_of(const Problem &a, int32_t device, const float *grad, 
     room.want(&rows.row, a.rows);
     room.want(&rows.target, a.rows);
     room.want(&rows.weight, a.rows);
-    room.want(&px, (uint64_t)planes * a.rows * pitch);
-    if (pack_w) room.want(&pw, (uint64_t)planes * piece * pitch);
-    room.want(&dz, (uint64_t)planes * a.rows * dz_pitch);
+    room.want(&px, (uint64_t)planes * padded * pitch);
+    // The weights' last lines, where those are read in place and do not fill a step.
+    const bool ragged = !pack_w && a.classes % kDepth != 0;
+    if (pack_w) room.want(&pw, (uint64_t)planes * whole_steps(piece) * pitch);
+    else if (ragged) room.want(&pw, (uint64_t)kDepth * pitch);
+    room.want(&dz, (uint64_t)planes * padded * dz_pitch);
     room.want(&sums, (uint64_t)splits * a.rows * pitch);
     int32_t rc = room.allocate(device, stream);
     if (rc != NT_OK) return rc;
 
     rows_kernel<true><<<1, kRowsBlock, 0, s>>>(a.targets, a.rows, rows, grad, grad_value, a.reduction, half);
-    const uint64_t plane_x = (uint64_t)a.rows * pitch, plane_w = (uint64_t)piece * pitch;
-    const uint64_t plane_dz = (uint64_t)a.rows * dz_pitch;
-    pack_kernel<T><<<blocks_of(a.rows * (uint64_t)(pitch / 8u), kBlock), kBlock, 0, s>>>(
+    const uint64_t plane_x = (uint64_t)padded * pitch, plane_w = (uint64_t)whole_steps(piece) * pitch;
+    const uint64_t plane_dz = (uint64_t)padded * dz_pitch;
+    pack_kernel<T><<<blocks_of(padded * (uint64_t)(pitch / 8u), kBlock), kBlock, 0, s>>>(
         a.x, a.width, px, pitch, plane_x, a.rows, rows.row, rows.count);
+    if (ragged) {
+        const uint32_t lines = a.classes % kDepth;
+        pack_kernel<T><<<blocks_of(kDepth * (uint64_t)(pitch / 8u), kBlock), kBlock, 0, s>>>(
+            static_cast<const Raw *>(a.w) + (uint64_t)(a.classes - lines) * a.width, a.width, pw, pitch, 0, lines,
+            nullptr, nullptr);
+    }
     for (uint32_t k = 0; k < pieces; ++k) {
         const uint32_t first = k * piece, classes = std::min(piece, a.classes - first);
-        const uint32_t line = (classes + 63u) / 64u * 64u;
+        const uint32_t line = whole_steps(classes);
         const void *weights = static_cast<const Raw *>(a.w) + (uint64_t)first * a.width;
         if (pack_w)
             pack_kernel<T><<<blocks_of(classes * (uint64_t)(pitch / 8u), kBlock), kBlock, 0, s>>>(
                 weights, a.width, pw, pitch, plane_w, classes, nullptr, nullptr);
         const uint16_t *w = pack_w ? pw : static_cast<const uint16_t *>(weights);
         Product logits{};
-        logits.p = Operand{w, pitch, plane_w, classes, pitch};
-        logits.q = Operand{px, pitch, plane_x, a.rows, pitch};
+        logits.p = Operand{w, nullptr, pitch, plane_w, classes};
+        logits.q = Operand{px, nullptr, pitch, plane_x, a.rows};
         logits.tiles_p = (line + Shape::BP - 1) / Shape::BP;
         logits.tiles_q = tiles_n;
         logits.splits = 1;
@@ -600,8 +612,8 @@ static int32_t backward_of(const Problem &a, int32_t device, const float *grad, 
         launch_product<half, Shape, true, true, planes>(logits, grads, s);
 
         Product input{};                    // dx[i][h] = sum over v of dz[i][v] W[v][h]
-        input.p = Operand{w, pitch, plane_w, pitch, classes};
-        input.q = Operand{dz, line, plane_dz, a.rows, line};
+        input.p = Operand{w, ragged && k + 1u == pieces ? pw : nullptr, pitch, plane_w, pitch};
+        input.q = Operand{dz, nullptr, line, plane_dz, a.rows};
         input.tiles_p = tiles_h;
         input.tiles_q = tiles_n;
         input.splits = splits;
@@ -611,8 +623,8 @@ static int32_t backward_of(const Problem &a, int32_t device, const float *grad, 
         launch_product<half, Shape, false, true, planes>(input, sum, s);
 
         Product weight{};                   // dW[v][h] = sum over i of dz[i][v] x[i][h]
-        weight.p = Operand{px, pitch, plane_x, pitch, a.rows};
-        weight.q = Operand{dz, line, plane_dz, line, a.rows};
+        weight.p = Operand{px, nullptr, pitch, plane_x, pitch};
+        weight.q = Operand{dz, nullptr, line, plane_dz, line};
         weight.tiles_p = tiles_h;
         weight.tiles_q = (classes + Shape::BQ - 1) / Shape::BQ;
         weight.splits = 1;

@@ -38,17 +38,22 @@ typedef short s16x8_t __attribute__((ext_vector_type(8)));
 constexpr uint32_t kDepth = 64;             // elements along k in a step
 constexpr uint32_t kMostPitch = 1u << 22;   // elements of a line: a tile's offsets stay below 2**32 bytes
 
+// There is no end of k inside a step: deep lines are padded with zeros to
+// whole steps, and so is one operand's number of lines otherwise, where the
+// other has `tail`, a copy of its last lines that fills a step.
 struct Operand {
     const uint16_t *base;       // 16-byte aligned
+    const uint16_t *tail;       // lines of the last step, if that is not whole in `base`; or null
     uint64_t pitch;             // elements from line to line, a multiple of 8
     uint64_t plane;             // elements from plane to plane
     uint32_t rows;              // deep: rows; otherwise columns, a multiple of 8
-    uint32_t depth;             // along k; a multiple of 8 when deep
 };
 
 // How many rows there are may be known on the device alone (`live`, at most
 // what the grid is made for): then they are operand q's rows, or, with
 // `live_depth`, the length of k of both.
+__host__ __device__ __forceinline__ uint32_t whole_steps(uint32_t n) { return (n + kDepth - 1u) / kDepth * kDepth; }
+
 struct Product {
     Operand p, q;
     uint32_t tiles_p, tiles_q, splits, depth;   // depth: along k, in steps of 64 that are shared out among the splits
@@ -57,15 +62,14 @@ struct Product {
 };
 
 // Shape of a workgroup's tile and of the waves in it.
-template <int BP_, int BQ_, int WP_, int WQ_>
+template <int BP_, int BQ_, int WP_, int WQ_, int PER_SIMD_ = 2>
 struct Tile {
     static constexpr int BP = BP_, BQ = BQ_, WP = WP_, WQ = WQ_;
+    static constexpr int PER_SIMD = PER_SIMD_;                      // waves that the registers leave room for
     static constexpr int kWaves = WP * WQ, kThreads = kWaves * 64;
     static constexpr int kWaveP = BP / WP, kWaveQ = BQ / WQ;        // a wave's part
     static constexpr int TP = kWaveP / 16, TQ = kWaveQ / 16;        // in tiles of the matrix instruction
 };
-
-__device__ __attribute__((aligned(16))) const uint32_t kZeroGroup[4] = {0u, 0u, 0u, 0u};
 
 // The exclusive or of a line of the [k][row] slices, in 32-byte groups: the 16
 // lines that a wave's transposed read touches at once get different ones.
@@ -76,28 +80,25 @@ template <int B, int WAVES, bool DEEP>
 struct Loader {
     static constexpr int kLoads = B * 128 / 1024 / WAVES;       // 1 KB each, a wave's share
     static_assert(kLoads * WAVES * 1024 == B * 128, "a slice is shared out among the waves");
-    const char *base;
+    const char *base, *tail;
     uint64_t pitch, plane;
-    uint32_t depth;
     uint32_t offset[kLoads];
-    uint32_t line[kLoads];              // deep: the group's first k; otherwise the line's k
 
     __device__ __forceinline__ void init(const Operand &o, uint32_t first, uint32_t wave, uint32_t lane) {
         pitch = o.pitch * 2u;
         plane = o.plane * 2u;
-        depth = o.depth;
-        base = reinterpret_cast<const char *>(o.base) + (DEEP ? first * pitch : (uint64_t)first * 2u);
+        const uint64_t start = DEEP ? first * pitch : (uint64_t)first * 2u;
+        base = reinterpret_cast<const char *>(o.base) + start;
+        tail = o.tail == nullptr ? nullptr : reinterpret_cast<const char *>(o.tail) + start;
 #pragma unroll
         for (int j = 0; j < kLoads; ++j) {
             const uint32_t part = (uint32_t)j * WAVES + wave;
             if constexpr (DEEP) {
                 // Rows past the last are the last again: what they give is not kept.
                 uint32_t row = part * 8u + (lane >> 3);
-                const uint32_t last = o.rows - 1u - first;
+                const uint32_t last = o.rows > first ? o.rows - 1u - first : 0u;
                 row = row < last ? row : last;
-                const uint32_t group = (lane & 7u) ^ (lane >> 3);
-                offset[j] = row * (uint32_t)pitch + group * 16u;
-                line[j] = group * 8u;
+                offset[j] = row * (uint32_t)pitch + ((lane & 7u) ^ (lane >> 3)) * 16u;
             } else {
                 constexpr uint32_t lanes = B / 8;               // of a line
                 const uint32_t k = part * (64u / lanes) + lane / lanes;
@@ -107,23 +108,22 @@ struct Loader {
                 const uint32_t last = o.rows - 8u - first;
                 column = column < last ? column : last;
                 offset[j] = k * (uint32_t)pitch + column * 2u;
-                line[j] = k;
             }
         }
     }
 
-    // Queue the slice from k on; groups past the end of k are zeros.
-    __device__ __forceinline__ void load(uint16_t *room, uint32_t k, uint32_t which, uint32_t wave) const {
-        const char *from = base + which * plane + (DEEP ? (uint64_t)k * 2u : k * pitch);
-        const bool whole = k + kDepth <= depth;
+    // Queue the slice of step `step`, of which there are `steps`.
+    __device__ __forceinline__ void load(uint16_t *room, uint32_t step, uint32_t steps, uint32_t which,
+                                         uint32_t wave) const {
+        const char *from = base + (DEEP ? (uint64_t)step * (2u * kDepth) : step * (kDepth * pitch)) + which * plane;
+        if constexpr (!DEEP) from = tail != nullptr && step + 1u == steps ? tail : from;
+        // A buffer from the tile's place on: 32-bit offsets of the lanes, and no address arithmetic in them.
+        const auto buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(from), 0, -1, 0x00027000);
 #pragma unroll
-        for (int j = 0; j < kLoads; ++j) {
-            const char *at = from + offset[j];
-            if (!whole) at = k + line[j] < depth ? at : reinterpret_cast<const char *>(kZeroGroup);
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)at,
-                                             (__attribute__((address_space(3))) void *)(room + (j * WAVES + wave) * 512u),
-                                             16, 0, 0);
-        }
+        for (int j = 0; j < kLoads; ++j)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                buffer, (__attribute__((address_space(3))) void *)(room + (j * WAVES + wave) * 512u), 16, (int)offset[j],
+                0, 0, 0);
     }
 };
 
@@ -131,24 +131,29 @@ struct Loader {
 // l has row l % 16 of a 16-row tile and k = 8 (l / 16) on.
 template <int B, bool DEEP>
 struct Reader {
-    uint32_t first;             // element of the wave's first row
-    uint32_t lane;
-    __device__ __forceinline__ s16x8_t read(const uint16_t *room, int t, int half) const {
+    uint32_t at;                // byte of the wave's first tile; otherwise than deep, before its exclusive or
+    __device__ __forceinline__ Reader(uint32_t first, uint32_t lane) {
         const uint32_t g = lane >> 4;
         if constexpr (DEEP) {
-            const uint32_t row = first + (uint32_t)t * 16u + (lane & 15u);
-            const uint32_t group = ((uint32_t)half * 4u + g) ^ (lane & 7u);
-            return *reinterpret_cast<const s16x8_t *>(room + row * 64u + group * 8u);
+            at = (first + (lane & 15u)) * 128u + ((g ^ (lane & 7u)) << 4);
         } else {
-            // Two transposed reads of four lines each: the 16 lanes of a group bring 4 lines of 16
-            // elements, and each gets a column of them.
-            const uint32_t k = (uint32_t)half * 32u + g * 8u + ((lane & 15u) >> 2);
-            const uint32_t turned = (first / 16u + (uint32_t)t) ^ (turn_of(k) & (B / 16u - 1u));
-            const uint16_t *at = room + k * B + turned * 16u + (lane & 3u) * 4u;
-            const s16x4_t low = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4_t *)(at));
-            const s16x4_t high = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4_t *)(at + 4u * B));
+            // A transposed read: the 16 lanes of a group bring 4 lines of 16 elements, and each gets a column.
+            const uint32_t k = g * 8u + ((lane & 15u) >> 2);
+            at = k * (2u * B) + (((first / 16u) ^ (turn_of(k) & (B / 16u - 1u))) << 5) + (lane & 3u) * 8u;
+        }
+    }
+    // Keeps the compiler from holding every tile's address in a register of its own.
+    __device__ __forceinline__ void hide() { __asm__ volatile("" : "+v"(at)); }
+    __device__ __forceinline__ s16x8_t read(const uint16_t *room, int t, int half) const {
+        const auto *from = (const __attribute__((address_space(3))) char *)room;
+        if constexpr (DEEP) {
+            // The second half's group is the first's with bit 2 changed.
+            return *(const __attribute__((address_space(3))) s16x8_t *)(from + (half ? at ^ 64u : at) + t * 2048);
+        } else {
+            const auto *place = from + (at ^ ((uint32_t)t << 5)) + half * (64 * B);
+            const s16x4_t low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t *)place);
+            const s16x4_t high =
+                __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t *)(place + 8 * B));
             return __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
@@ -174,7 +179,7 @@ __device__ __forceinline__ uint32_t xcd_order(uint32_t b, uint32_t n) {
 // PLANES: 1, or 3 of float32.  `finish` gets the wave's accumulators: element
 // [tp][tq][r] is p = p_first + 16 tp + 4 (lane / 16) + r, q = q_first + 16 tq + lane % 16.
 template <bool HALF, class T, bool P_DEEP, bool Q_DEEP, int PLANES, class Finish>
-__global__ __launch_bounds__(T::kThreads) void product_kernel(Product a, Finish finish) {
+__global__ __launch_bounds__(T::kThreads, T::PER_SIMD) void product_kernel(Product a, Finish finish) {
     __shared__ __attribute__((aligned(16))) uint16_t room0[(T::BP + T::BQ) * kDepth];
     __shared__ __attribute__((aligned(16))) uint16_t room1[(T::BP + T::BQ) * kDepth];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -183,10 +188,10 @@ __global__ __launch_bounds__(T::kThreads) void product_kernel(Product a, Finish 
     if (a.live != nullptr) {
         const uint32_t live = __builtin_amdgcn_readfirstlane(*a.live);
         if (a.live_depth) {
-            a.p.depth = a.q.depth = a.depth = live;
+            a.depth = live;
         } else {
             a.q.rows = live;
-            a.tiles_q = (live + T::BQ - 1u) / T::BQ;
+            a.tiles_q = (whole_steps(live) + T::BQ - 1u) / T::BQ;     // what a padding to whole steps takes too
         }
     }
     const uint32_t tiles = a.tiles_p * a.tiles_q;
@@ -201,8 +206,8 @@ __global__ __launch_bounds__(T::kThreads) void product_kernel(Product a, Finish 
     load_p.init(a.p, tile_p * T::BP, wave, lane);
     load_q.init(a.q, tile_q * T::BQ, wave, lane);
     const uint32_t wave_p = wave % T::WP, wave_q = wave / T::WP;
-    const Reader<T::BP, P_DEEP> read_p{wave_p * T::kWaveP, lane};
-    const Reader<T::BQ, Q_DEEP> read_q{wave_q * T::kWaveQ, lane};
+    Reader<T::BP, P_DEEP> read_p(wave_p * T::kWaveP, lane);
+    Reader<T::BQ, Q_DEEP> read_q(wave_q * T::kWaveQ, lane);
 
     f32x4 acc[T::TP][T::TQ];
 #pragma unroll
@@ -216,6 +221,7 @@ __global__ __launch_bounds__(T::kThreads) void product_kernel(Product a, Finish 
     const uint32_t end = (uint32_t)((uint64_t)steps * (split + 1u) / a.splits);
     const uint32_t total = (end - begin) * products;
     const auto stage = [&](uint16_t *room, uint32_t s) {
+        s = s < total ? s : total - 1u;
         uint32_t k = begin + s, plane_p = 0, plane_q = 0;
         if constexpr (PLANES == 3) {
             const uint32_t which = s % 6u;          // (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
@@ -223,10 +229,13 @@ __global__ __launch_bounds__(T::kThreads) void product_kernel(Product a, Finish 
             plane_p = (0x010120u >> (4u * which)) & 15u;
             plane_q = (0x001102u >> (4u * which)) & 15u;
         }
-        load_p.load(room, k * kDepth, plane_p, wave);
-        load_q.load(room + T::BP * kDepth, k * kDepth, plane_q, wave);
+        load_p.load(room, k, steps, plane_p, wave);
+        load_q.load(room + T::BP * kDepth, k, steps, plane_q, wave);
     };
     const auto compute = [&](const uint16_t *room) {
+        __builtin_amdgcn_sched_barrier(0);          // the loads before are under way first
+        read_p.hide();
+        read_q.hide();
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             s16x8_t fp[T::TP], fq[T::TQ];
@@ -240,16 +249,19 @@ __global__ __launch_bounds__(T::kThreads) void product_kernel(Product a, Finish 
                 for (int j = 0; j < T::TQ; ++j) acc[i][j] = multiply<HALF>(fp[i], fq[j], acc[i][j]);
         }
     };
-    if (total > 0) stage(room0, 0);
-    __syncthreads();
-    for (uint32_t s = 0; s < total; s += 2) {
-        if (s + 1 < total) stage(room1, s + 1);
-        compute(room0);
+    if (total > 0) {
+        // Past the last step the last is queued again, so that the loop has no branches.
+        stage(room0, 0);
         __syncthreads();
-        if (s + 1 >= total) break;
-        if (s + 2 < total) stage(room0, s + 2);
-        compute(room1);
-        __syncthreads();
+        for (uint32_t s = 0; s + 1 < total; s += 2) {
+            stage(room1, s + 1);
+            compute(room0);
+            __syncthreads();
+            stage(room0, s + 2);
+            compute(room1);
+            __syncthreads();
+        }
+        if (total & 1u) compute(room0);
     }
     finish.template operator()<T>(acc, tile_p * T::BP + wave_p * T::kWaveP, tile_q * T::BQ + wave_q * T::kWaveQ, split,
                                   lane);
