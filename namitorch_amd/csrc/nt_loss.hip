@@ -249,6 +249,14 @@ struct FinishLoss {
     }
 };
 
+// Four values rounded to a 16-bit type, one rounding to nearest even each (the
+// packed conversions of gfx950).
+template <bool HALF>
+__device__ __forceinline__ u32x2 narrow4(f32x4 v) {
+    if constexpr (HALF) return __builtin_bit_cast(u32x2, __builtin_convertvector(v, f16x4_t));
+    else return __builtin_bit_cast(u32x2, __builtin_convertvector(v, bf16x4_t));
+}
+
 // Logits to dz.  The columns from the piece's last class to the line's end and
 // the rows from the last counted one to a whole step are zero.
 template <bool HALF, int PLANES>
@@ -265,29 +273,34 @@ struct FinishGrad {
     __device__ __forceinline__ void operator()(const f32x4 (&acc)[T::TP][T::TQ], uint32_t p_first, uint32_t q_first,
                                                uint32_t, uint32_t lane) const {
         const uint32_t count = *live, padded = whole_steps(count), up = p_first + 4u * (lane >> 4);
+        const bool whole = p_first + T::kWaveP <= classes;
 #pragma unroll
         for (int j = 0; j < T::TQ; ++j) {
             const uint32_t q = q_first + 16u * j + (lane & 15u);
             if (q >= padded) continue;
             const bool there = q < count;
-            const float from = there ? lse[row[q]] : 0.0f, by = there ? weight[q] : 0.0f;
+            // A row of padding: exp(z - infinity) is zero, as its sums z are finite.
+            const float from = there ? lse[row[q]] : kInfinity, by = there ? weight[q] : 0.0f;
             const uint32_t place = there ? (uint32_t)target[q] - first - up : ~0u;
+            const bool any = __builtin_amdgcn_ballot_w64(place < 16u * T::TP) != 0;
             uint16_t *line = dz + q * (uint64_t)pitch + up;
 #pragma unroll
             for (int i = 0; i < T::TP; ++i) {
-                if (up + 16u * i >= pitch) continue;
-                float v[4];
+                f32x4 v;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    v[r] = exp_of(acc[i][j][r] - from);
-                    if (place == 16u * i + r) v[r] -= 1.0f;
-                    v[r] = there && up + 16u * i + r < classes ? v[r] * by : 0.0f;
+                for (int r = 0; r < 4; ++r) v[r] = exp_of(acc[i][j][r] - from);
+                if (any) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) v[r] = place == 16u * i + r ? v[r] - 1.0f : v[r];
+                }
+                v *= by;
+                if (!whole) {
+                    if (up + 16u * i >= pitch) continue;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) v[r] = up + 16u * i + r < classes ? v[r] : 0.0f;
                 }
                 if constexpr (PLANES == 1) {
-                    uint16_t e[4];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) e[r] = HALF ? f32_to_f16(v[r]) : f32_to_bf16(v[r]);
-                    *reinterpret_cast<u32x2 *>(line + 16 * i) = __builtin_bit_cast(u32x2, e);
+                    *reinterpret_cast<u32x2 *>(line + 16 * i) = narrow4<HALF>(v);
                 } else {
                     uint16_t e[3][4];
 #pragma unroll
@@ -355,11 +368,10 @@ struct FinishWeight {
 #pragma unroll
             for (int i = 0; i < T::TP; ++i) {
                 const uint32_t c = up + 16u * i;
-                float v[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r] * by;
+                const f32x4 v = acc[i][j] * by;
                 if (even && c + 4u <= width) {
-                    Vec4IO<S, false>::store(line, c, v);
+                    if constexpr (S::code == NT_F32) *reinterpret_cast<f32x4 *>(line + c) = v;
+                    else *reinterpret_cast<u32x2 *>(line + c) = narrow4<S::code == NT_F16>(v);
                 } else {
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
@@ -451,7 +463,10 @@ __global__ __launch_bounds__(kBlock) void grad_input_kernel(const float *sums, u
 constexpr uint64_t kPieceBytes = 512ull << 20;       // of dz, and of packed weights, at a time
 constexpr uint32_t kSumTiles = 512;                  // dx: tiles and splits to fill the chip with
 
-using Large = Tile<256, 256, 2, 4>;
+#ifndef LT
+#define LT 256, 256, 2, 4
+#endif
+using Large = Tile<LT>;
 
 struct Problem {
     const void *x, *w;

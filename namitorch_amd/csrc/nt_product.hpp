@@ -31,6 +31,8 @@ namespace nt {
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef short s16x8_t __attribute__((ext_vector_type(8)));
@@ -232,25 +234,99 @@ __global__ __launch_bounds__(T::kThreads, T::PER_SIMD) void product_kernel(Produ
         load_p.load(room, k, steps, plane_p, wave);
         load_q.load(room + T::BP * kDepth, k, steps, plane_q, wave);
     };
-    const auto compute = [&](const uint16_t *room) {
-        __builtin_amdgcn_sched_barrier(0);          // the loads before are under way first
+    s16x8_t fp[T::TP], fq[T::TQ];
+    const auto fetch = [&](const uint16_t *room, int half) {
         read_p.hide();
         read_q.hide();
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            s16x8_t fp[T::TP], fq[T::TQ];
+        for (int j = 0; j < T::TQ; ++j) fq[j] = read_q.read(room + T::BP * kDepth, j, half);
 #pragma unroll
-            for (int i = 0; i < T::TP; ++i) fp[i] = read_p.read(room, i, half);
-#pragma unroll
-            for (int j = 0; j < T::TQ; ++j) fq[j] = read_q.read(room + T::BP * kDepth, j, half);
-#pragma unroll
-            for (int i = 0; i < T::TP; ++i)
-#pragma unroll
-                for (int j = 0; j < T::TQ; ++j) acc[i][j] = multiply<HALF>(fp[i], fq[j], acc[i][j]);
-        }
+        for (int i = 0; i < T::TP; ++i) fp[i] = read_p.read(room, i, half);
     };
-    if (total > 0) {
-        // Past the last step the last is queued again, so that the loop has no branches.
+    const auto multiply_tiles = [&]() {
+#pragma unroll
+        for (int i = 0; i < T::TP; ++i)
+#pragma unroll
+            for (int j = 0; j < T::TQ; ++j) acc[i][j] = multiply<HALF>(fp[i], fq[j], acc[i][j]);
+    };
+    if constexpr (T::kWaves == 8) {
+        // The two waves of a SIMD take turns: one reads its fragments of half a step from LDS while the
+        // other multiplies its own.  Past the last step the last is queued again, so that the loops have
+        // no branches.
+        const auto turn = [&]() {
+            __asm__ volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            __asm__ volatile("" ::: "memory");
+        };
+        const auto loaded = [&]() { __builtin_amdgcn_s_waitcnt(0x0f70); };      // vmcnt(0)
+        const auto fetched = [&]() { __builtin_amdgcn_s_waitcnt(0xc07f); };     // lgkmcnt(0)
+        const auto multiply_all = [&]() {
+            __builtin_amdgcn_s_setprio(1);
+            multiply_tiles();
+            __builtin_amdgcn_s_setprio(0);
+        };
+        if (total > 0) {
+            stage(room0, 0);
+            loaded();
+            turn();
+            if (wave < 4u) {
+                const auto step = [&](uint16_t *room, uint16_t *other, uint32_t next) {
+                    stage(other, next);
+                    fetch(room, 0);
+                    fetched();
+                    turn();
+                    multiply_all();
+                    turn();
+                    fetch(room, 1);
+                    fetched();
+                    turn();
+                    multiply_all();
+                    loaded();
+                    turn();
+                };
+                for (uint32_t s = 0; s + 1 < total; s += 2) {
+                    step(room0, room1, s + 1);
+                    step(room1, room0, s + 2);
+                }
+                if (total & 1u) step(room0, room1, total);
+            } else {
+#pragma unroll
+                for (int i = 0; i < T::TP; ++i) fp[i] = s16x8_t{0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < T::TQ; ++j) fq[j] = s16x8_t{0, 0, 0, 0, 0, 0, 0, 0};
+                const auto step = [&](uint16_t *room, uint16_t *other, uint32_t next) {
+                    stage(other, next);
+                    multiply_all();
+                    turn();
+                    fetch(room, 0);
+                    fetched();
+                    turn();
+                    multiply_all();
+                    turn();
+                    fetch(room, 1);
+                    fetched();
+                    loaded();
+                    turn();
+                };
+                for (uint32_t s = 0; s + 1 < total; s += 2) {
+                    step(room0, room1, s + 1);
+                    step(room1, room0, s + 2);
+                }
+                if (total & 1u) step(room0, room1, total);
+                multiply_tiles();
+            }
+        }
+    } else if (total > 0) {
+        const auto compute = [&](const uint16_t *room) {
+            __builtin_amdgcn_sched_barrier(0);          // the loads before are under way first
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                fetch(room, half);
+                multiply_tiles();
+            }
+        };
         stage(room0, 0);
         __syncthreads();
         for (uint32_t s = 0; s + 1 < total; s += 2) {
