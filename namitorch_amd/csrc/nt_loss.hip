@@ -189,6 +189,19 @@ __global__ __launch_bounds__(kBlock) void pack_kernel(const void *from, uint32_t
 // ---- what becomes of the products' tiles ------------------------------------------------------------------
 __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
 
+// exp(z - from).  Of 16-bit operands in one operation less, with z - from
+// rounded together with from log2(e): off by 2^-24 |from|, below what their
+// product's sums are off by.
+template <int PLANES>
+struct ExpFrom {
+    float from;
+    __device__ __forceinline__ explicit ExpFrom(float f) : from(PLANES == 1 ? f * -kLog2e : f) {}
+    __device__ __forceinline__ float operator()(float z) const {
+        if constexpr (PLANES == 1) return __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, from));
+        else return exp_of(z - from);
+    }
+};
+
 // Two halves' maximum m and sum of exp(z - m), joined.
 struct Partial2 {
     float most, sum;
@@ -200,6 +213,7 @@ __device__ __forceinline__ Partial2 join(Partial2 a, Partial2 b) {
 }
 
 // Logits to a maximum and sum of each row's part of a wave's tile, and the target's logit.
+template <int PLANES>
 struct FinishLoss {
     Partial2 *partials;         // [slot][rows]
     float *target_logit;        // [rows]
@@ -236,12 +250,12 @@ struct FinishLoss {
             }
             most = fmaxf(most, __shfl_xor(most, 16, 64));
             most = fmaxf(most, __shfl_xor(most, 32, 64));
-            const float from = most == -kInfinity ? 0.0f : most;
+            const ExpFrom<PLANES> exp_from(most == -kInfinity ? 0.0f : most);
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < T::TP; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) sum += exp_of(z[i][r] - from);
+                for (int r = 0; r < 4; ++r) sum += exp_from(z[i][r]);
             sum += __shfl_xor(sum, 16, 64);
             sum += __shfl_xor(sum, 32, 64);
             if (lane < 16u && q < count) partials[slot * rows + q] = Partial2{most, sum};
@@ -280,7 +294,8 @@ struct FinishGrad {
             if (q >= padded) continue;
             const bool there = q < count;
             // A row of padding: exp(z - infinity) is zero, as its sums z are finite.
-            const float from = there ? lse[row[q]] : kInfinity, by = there ? weight[q] : 0.0f;
+            const ExpFrom<PLANES> exp_from(there ? lse[row[q]] : kInfinity);
+            const float by = there ? weight[q] : 0.0f;
             const uint32_t place = there ? (uint32_t)target[q] - first - up : ~0u;
             const bool any = __builtin_amdgcn_ballot_w64(place < 16u * T::TP) != 0;
             uint16_t *line = dz + q * (uint64_t)pitch + up;
@@ -288,7 +303,7 @@ struct FinishGrad {
             for (int i = 0; i < T::TP; ++i) {
                 f32x4 v;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = exp_of(acc[i][j][r] - from);
+                for (int r = 0; r < 4; ++r) v[r] = exp_from(acc[i][j][r]);
                 if (any) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) v[r] = place == 16u * i + r ? v[r] - 1.0f : v[r];
@@ -547,7 +562,7 @@ static int32_t forward_of(const Problem &a, int32_t device, float *loss, float *
         product.splits = 1;
         product.depth = pitch;
         product.live = rows.count;
-        const FinishLoss finish{partials, target_logit, rows.target, rows.count, first, classes, k * slots_piece, a.rows};
+        const FinishLoss<planes> finish{partials, target_logit, rows.target, rows.count, first, classes, k * slots_piece, a.rows};
         launch_product<half, Shape, true, true, planes>(product, finish, s);
     }
     const uint32_t last = (a.classes - (pieces - 1) * piece + Shape::BP - 1) / Shape::BP * Shape::WP;

@@ -234,99 +234,44 @@ __global__ __launch_bounds__(T::kThreads, T::PER_SIMD) void product_kernel(Produ
         load_p.load(room, k, steps, plane_p, wave);
         load_q.load(room + T::BP * kDepth, k, steps, plane_q, wave);
     };
-    s16x8_t fp[T::TP], fq[T::TQ];
-    const auto fetch = [&](const uint16_t *room, int half) {
+    const auto compute = [&](const uint16_t *room) {
+        __builtin_amdgcn_sched_barrier(0);          // the loads before are under way first
         read_p.hide();
         read_q.hide();
+        s16x8_t fp[2][T::TP], fq[2][T::TQ];
 #pragma unroll
-        for (int j = 0; j < T::TQ; ++j) fq[j] = read_q.read(room + T::BP * kDepth, j, half);
+        for (int half = 0; half < 2; ++half) {
 #pragma unroll
-        for (int i = 0; i < T::TP; ++i) fp[i] = read_p.read(room, i, half);
-    };
-    const auto multiply_tiles = [&]() {
+            for (int j = 0; j < T::TQ; ++j) fq[half][j] = read_q.read(room + T::BP * kDepth, j, half);
 #pragma unroll
-        for (int i = 0; i < T::TP; ++i)
-#pragma unroll
-            for (int j = 0; j < T::TQ; ++j) acc[i][j] = multiply<HALF>(fp[i], fq[j], acc[i][j]);
-    };
-    if constexpr (T::kWaves == 8) {
-        // The two waves of a SIMD take turns: one reads its fragments of half a step from LDS while the
-        // other multiplies its own.  Past the last step the last is queued again, so that the loops have
-        // no branches.
-        const auto turn = [&]() {
-            __asm__ volatile("" ::: "memory");
-            __builtin_amdgcn_sched_barrier(0);
-            __builtin_amdgcn_s_barrier();
-            __builtin_amdgcn_sched_barrier(0);
-            __asm__ volatile("" ::: "memory");
-        };
-        const auto loaded = [&]() { __builtin_amdgcn_s_waitcnt(0x0f70); };      // vmcnt(0)
-        const auto fetched = [&]() { __builtin_amdgcn_s_waitcnt(0xc07f); };     // lgkmcnt(0)
-        const auto multiply_all = [&]() {
-            __builtin_amdgcn_s_setprio(1);
-            multiply_tiles();
-            __builtin_amdgcn_s_setprio(0);
-        };
-        if (total > 0) {
-            stage(room0, 0);
-            loaded();
-            turn();
-            if (wave < 4u) {
-                const auto step = [&](uint16_t *room, uint16_t *other, uint32_t next) {
-                    stage(other, next);
-                    fetch(room, 0);
-                    fetched();
-                    turn();
-                    multiply_all();
-                    turn();
-                    fetch(room, 1);
-                    fetched();
-                    turn();
-                    multiply_all();
-                    loaded();
-                    turn();
-                };
-                for (uint32_t s = 0; s + 1 < total; s += 2) {
-                    step(room0, room1, s + 1);
-                    step(room1, room0, s + 2);
-                }
-                if (total & 1u) step(room0, room1, total);
-            } else {
-#pragma unroll
-                for (int i = 0; i < T::TP; ++i) fp[i] = s16x8_t{0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-                for (int j = 0; j < T::TQ; ++j) fq[j] = s16x8_t{0, 0, 0, 0, 0, 0, 0, 0};
-                const auto step = [&](uint16_t *room, uint16_t *other, uint32_t next) {
-                    stage(other, next);
-                    multiply_all();
-                    turn();
-                    fetch(room, 0);
-                    fetched();
-                    turn();
-                    multiply_all();
-                    turn();
-                    fetch(room, 1);
-                    fetched();
-                    loaded();
-                    turn();
-                };
-                for (uint32_t s = 0; s + 1 < total; s += 2) {
-                    step(room0, room1, s + 1);
-                    step(room1, room0, s + 2);
-                }
-                if (total & 1u) step(room0, room1, total);
-                multiply_tiles();
-            }
+            for (int i = 0; i < T::TP; ++i) fp[half][i] = read_p.read(room, i, half);
         }
-    } else if (total > 0) {
-        const auto compute = [&](const uint16_t *room) {
-            __builtin_amdgcn_sched_barrier(0);          // the loads before are under way first
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int i = 0; i < T::TP; ++i)
+#pragma unroll
+                for (int j = 0; j < T::TQ; ++j) acc[i][j] = multiply<HALF>(fp[half][i], fq[half][j], acc[i][j]);
+        // The order of both: a tile of p is read while the one two before it is multiplied.
+        constexpr int rp = P_DEEP ? 1 : 2, rq = T::TQ * (Q_DEEP ? 1 : 2);
+        if constexpr (T::TP > 2) {
+            __builtin_amdgcn_sched_group_barrier(0x100, rq + 2 * rp, 0);        // reads of LDS
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                fetch(room, half);
-                multiply_tiles();
+#pragma unroll
+                for (int i = 0; i < T::TP - 2; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, T::TQ, 0);      // matrix instructions
+                    __builtin_amdgcn_sched_group_barrier(0x100, rp, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x008, T::TQ, 0);
+                if (half == 0) __builtin_amdgcn_sched_group_barrier(0x100, rq, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, T::TQ, 0);
+                if (half == 0) __builtin_amdgcn_sched_group_barrier(0x100, 2 * rp, 0);
             }
-        };
+        }
+    };
+    if (total > 0) {
+        // Past the last step the last is queued again, so that the loop has no branches.
         stage(room0, 0);
         __syncthreads();
         for (uint32_t s = 0; s + 1 < total; s += 2) {
