@@ -63,6 +63,7 @@ __device__ __forceinline__ int32_t class_of(const Targets &t, uint64_t i) {
 struct Rows {
     uint32_t *count;            // how many
     float *unscale;             // what the products of dz are multiplied by
+    uint32_t *place;            // (backward) of each row: which counted row it is, or ~0
     uint32_t *row;              // of counted row j: its row,
     int32_t *target;            // its class or kOutside,
     float *weight;              // (backward) what its dz is multiplied by
@@ -127,6 +128,7 @@ __global__ __launch_bounds__(kRowsBlock) void rows_kernel(Targets t, uint32_t ro
     uint32_t j = before - mine;
     for (uint32_t i = begin; i < end; ++i) {
         const int32_t c = class_of(t, i);
+        if (BACKWARD) out.place[i] = c == kIgnored ? ~0u : j;
         if (c == kIgnored) continue;
         out.row[j] = i;
         out.target[j] = c;
@@ -271,6 +273,22 @@ __device__ __forceinline__ u32x2 narrow4(f32x4 v) {
     else return __builtin_bit_cast(u32x2, __builtin_convertvector(v, bf16x4_t));
 }
 
+// Two tiles' four values a lane, along p, to eight consecutive ones: lanes 16
+// to 31 exchange with the first 16, the last 16 with those before them, so
+// that rows of 16 lanes 0 and 2 hold the first tile's halves and 1 and 3 the
+// second's.  A lane's 16 bytes then lie beside the next lanes' (64 bytes of a
+// line at a time instead of 32).
+struct Pair {
+    u32x4_t words;
+    __device__ __forceinline__ Pair(u32x2 first, u32x2 second) {
+        const auto x = __builtin_amdgcn_permlane16_swap(first.x, second.x, false, false);
+        const auto y = __builtin_amdgcn_permlane16_swap(first.y, second.y, false, false);
+        words = u32x4_t{x[0], y[0], x[1], y[1]};
+    }
+    // Where a lane's elements begin, from the first tile's first on.
+    static __device__ __forceinline__ uint32_t place(uint32_t lane) { return ((lane >> 4) & 1u) * 16u + (lane >> 5) * 8u; }
+};
+
 // Logits to dz.  The columns from the piece's last class to the line's end and
 // the rows from the last counted one to a whole step are zero.
 template <bool HALF, int PLANES>
@@ -298,9 +316,8 @@ struct FinishGrad {
             const float by = there ? weight[q] : 0.0f;
             const uint32_t place = there ? (uint32_t)target[q] - first - up : ~0u;
             const bool any = __builtin_amdgcn_ballot_w64(place < 16u * T::TP) != 0;
-            uint16_t *line = dz + q * (uint64_t)pitch + up;
-#pragma unroll
-            for (int i = 0; i < T::TP; ++i) {
+            uint16_t *line = dz + q * (uint64_t)pitch;
+            const auto tile = [&](int i) {
                 f32x4 v;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) v[r] = exp_from(acc[i][j][r]);
@@ -310,13 +327,23 @@ struct FinishGrad {
                 }
                 v *= by;
                 if (!whole) {
-                    if (up + 16u * i >= pitch) continue;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) v[r] = up + 16u * i + r < classes ? v[r] : 0.0f;
                 }
-                if constexpr (PLANES == 1) {
-                    *reinterpret_cast<u32x2 *>(line + 16 * i) = narrow4<HALF>(v);
-                } else {
+                return v;
+            };
+            if constexpr (PLANES == 1) {
+#pragma unroll
+                for (int i = 0; i < T::TP; i += 2) {
+                    const Pair pair(narrow4<HALF>(tile(i)), narrow4<HALF>(tile(i + 1)));
+                    const uint32_t c = p_first + 16u * i + Pair::place(lane);
+                    if (whole || c < pitch) *reinterpret_cast<u32x4_t *>(line + c) = pair.words;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < T::TP; ++i) {
+                    const f32x4 v = tile(i);
+                    if (!whole && up + 16u * i >= pitch) continue;
                     uint16_t e[3][4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
@@ -327,7 +354,7 @@ struct FinishGrad {
                         e[2][r] = one[2];
                     }
                     for (int k = 0; k < 3; ++k)
-                        *reinterpret_cast<u32x2 *>(line + k * plane + 16 * i) = __builtin_bit_cast(u32x2, e[k]);
+                        *reinterpret_cast<u32x2 *>(line + k * plane + up + 16 * i) = __builtin_bit_cast(u32x2, e[k]);
                 }
             }
         }
@@ -368,7 +395,7 @@ struct FinishWeight {
     typename S::raw *to;
     const float *unscale;
     uint32_t width, classes;
-    bool even;                  // four elements can be stored at once
+    bool even;                  // 16 bytes can be stored at once
 
     template <class T>
     __device__ __forceinline__ void operator()(const f32x4 (&acc)[T::TP][T::TQ], uint32_t p_first, uint32_t q_first,
@@ -380,13 +407,22 @@ struct FinishWeight {
             const uint32_t q = q_first + 16u * j + (lane & 15u);
             if (q >= classes) continue;
             typename S::raw *line = to + q * (uint64_t)width;
+            if (even && S::code != NT_F32) {
+#pragma unroll
+                for (int i = 0; i < T::TP; i += 2) {
+                    const Pair pair(narrow4<S::code == NT_F16>(acc[i][j] * by),
+                                    narrow4<S::code == NT_F16>(acc[i + 1][j] * by));
+                    const uint32_t c = p_first + 16u * i + Pair::place(lane);
+                    if (c < width) *reinterpret_cast<u32x4_t *>(line + c) = pair.words;
+                }
+                continue;
+            }
 #pragma unroll
             for (int i = 0; i < T::TP; ++i) {
                 const uint32_t c = up + 16u * i;
                 const f32x4 v = acc[i][j] * by;
-                if (even && c + 4u <= width) {
-                    if constexpr (S::code == NT_F32) *reinterpret_cast<f32x4 *>(line + c) = v;
-                    else *reinterpret_cast<u32x2 *>(line + c) = narrow4<S::code == NT_F16>(v);
+                if (even) {
+                    if (c < width) *reinterpret_cast<f32x4 *>(line + c) = v;
                 } else {
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
@@ -447,41 +483,94 @@ __global__ __launch_bounds__(kRowsBlock) void loss_sum_kernel(const float *each,
     }
 }
 
-// dx from its sums; rows that are not counted are zero.  `row` is in order, so
-// row i is counted row j where row[j] == i, found by halving.
+// dx from its sums, eight columns a lane; rows that are not counted are zero.
 template <class T>
 __global__ __launch_bounds__(kBlock) void grad_input_kernel(const float *sums, uint64_t split_stride, uint32_t splits,
                                                             uint32_t pitch, Rows rows, uint32_t all, uint32_t width,
-                                                            typename T::raw *dx) {
-    const uint32_t count = *rows.count;
+                                                            bool even, typename T::raw *dx) {
     const float by = *rows.unscale;
-    for (uint32_t i = blockIdx.x; i < all; i += gridDim.x) {
-        uint32_t low = 0, high = count;
-        while (low < high) {
-            const uint32_t middle = (low + high) / 2u;
-            if (rows.row[middle] < i) low = middle + 1u;
-            else high = middle;
-        }
-        const bool counted = low < count && rows.row[low] == i;
-        for (uint32_t c = threadIdx.x; c < width; c += kBlock) {
-            float v = 0.0f;
-            if (counted) {
-                for (uint32_t s = 0; s < splits; ++s) v += sums[s * split_stride + low * (uint64_t)pitch + c];
-                v *= by;
+    const uint32_t groups = (width + 7u) / 8u;
+    const uint64_t items = all * (uint64_t)groups;
+    for (uint64_t g = blockIdx.x * (uint64_t)kBlock + threadIdx.x; g < items; g += (uint64_t)gridDim.x * kBlock) {
+        const uint32_t i = (uint32_t)(g / groups), c = (uint32_t)(g % groups) * 8u, j = rows.place[i];
+        f32x4 v[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+        if (j != ~0u) {
+            const float *from = sums + j * (uint64_t)pitch + c;
+#pragma unroll 4
+            for (uint32_t s = 0; s < splits; ++s) {
+                v[0] += *reinterpret_cast<const f32x4 *>(from + s * split_stride);
+                v[1] += *reinterpret_cast<const f32x4 *>(from + s * split_stride + 4);
             }
-            store1<T>(dx, i * (uint64_t)width + c, v);
+            v[0] *= by;
+            v[1] *= by;
+        }
+        typename T::raw *out = dx + i * (uint64_t)width + c;
+        if (even) {
+            if constexpr (T::code == NT_F32) {
+                *reinterpret_cast<f32x4 *>(out) = v[0];
+                *reinterpret_cast<f32x4 *>(out + 4) = v[1];
+            } else {
+                const u32x2 low = narrow4<T::code == NT_F16>(v[0]), high = narrow4<T::code == NT_F16>(v[1]);
+                *reinterpret_cast<u32x4_t *>(out) = u32x4_t{low.x, low.y, high.x, high.y};
+            }
+        } else {
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k)
+                if (c + k < width) store1<T>(out, k, v[k >> 2][k & 3]);
         }
     }
 }
 
 // ---- launches ----------------------------------------------------------------------------------------
-constexpr uint64_t kPieceBytes = 512ull << 20;       // of dz, and of packed weights, at a time
-constexpr uint32_t kSumTiles = 512;                  // dx: tiles and splits to fill the chip with
+constexpr uint64_t kPieceBytes = 1ull << 30;       // of dz, and of packed weights, at a time
 
-#ifndef LT
-#define LT 256, 256, 2, 4
+constexpr uint32_t kUnits = 256;                     // compute units
+
+using Large = Tile<256, 256, 2, 4>;
+using Middle = Tile<128, 128, 2, 2>;
+using Few = Tile<128, 64, 4, 1>;                     // rows
+
+static uint32_t tiles_of(uint64_t n, uint32_t each) { return (uint32_t)((n + each - 1) / each); }
+
+// Calls launch(shape) with the tile shape for a product of `p` by `q`.
+template <class F>
+static void with_tile(uint64_t p, uint64_t q, F &&launch) {
+    if (q <= 64u) launch(Few{});
+    else if ((uint64_t)tiles_of(p, 256) * tiles_of(q, 256) < kUnits) launch(Middle{});
+    else launch(Large{});
+}
+
+template <class F>
+static void with_input_tile(uint64_t rows, F &&launch) {
+    if (rows <= 64u) launch(Few{});
+    else if (rows <= 128u) launch(Middle{});
+    else launch(Large{});
+}
+
+#ifndef WT
+#define WT 0
 #endif
-using Large = Tile<LT>;
+template <class F>
+static void with_weight_tile(uint64_t p, uint64_t q, uint64_t rows, F &&launch) {
+    if ((uint64_t)tiles_of(p, 256) * tiles_of(q, 256) < kUnits || rows <= WT) launch(Middle{});
+    else launch(Large{});
+}
+
+// Splits of dx's product along k: as many as take the fewest rounds of the
+// chip for their length, with what each adds to the sums' traffic.
+static uint32_t splits_of(uint32_t tiles, uint32_t steps, uint64_t sums) {
+    uint32_t best = 1;
+    double least = 1e30;
+    for (uint32_t s = 1; s <= 64u && s * 4u <= std::max(steps, 4u); ++s) {
+        const double rounds = tiles_of((uint64_t)tiles * s, kUnits);
+        const double us = rounds * (tiles_of(steps, s) + 4u) * 1.6 + s * (double)sums * 8.0 / 4e6;
+        if (us < least) {
+            least = us;
+            best = s;
+        }
+    }
+    return best;
+}
 
 struct Problem {
     const void *x, *w;
@@ -521,10 +610,13 @@ static int32_t forward_of(const Problem &a, int32_t device, float *loss, float *
     const uint32_t pitch = whole_steps(a.width), padded = whole_steps(a.rows);
     const bool pack_w = planes > 1 || pitch != a.width || (uintptr_t)a.w % 16u != 0;
     const uint32_t piece = piece_of(a, pitch, planes, pack_w, false);
-    using Shape = Large;
-    const uint32_t slots_piece = (piece + Shape::BP - 1) / Shape::BP * Shape::WP;
     const uint32_t pieces = (a.classes + piece - 1) / piece;
-    const uint64_t slots = (uint64_t)slots_piece * pieces;
+    uint32_t slots_piece = 0, slots = 0;                  // of a whole piece, of all
+    with_tile(piece, a.rows, [&](auto shape) {
+        using Shape = decltype(shape);
+        slots_piece = tiles_of(piece, Shape::BP) * Shape::WP;
+        slots = (pieces - 1) * slots_piece + tiles_of(a.classes - (pieces - 1) * piece, Shape::BP) * Shape::WP;
+    });
 
     Rows rows{};
     uint16_t *px = nullptr, *pw = nullptr;
@@ -535,7 +627,7 @@ static int32_t forward_of(const Problem &a, int32_t device, float *loss, float *
     room.want(&rows.row, a.rows);
     room.want(&rows.target, a.rows);
     room.want(&target_logit, a.rows);
-    room.want(&partials, slots * a.rows);
+    room.want(&partials, (uint64_t)slots * a.rows);
     room.want(&px, (uint64_t)planes * padded * pitch);
     if (pack_w) room.want(&pw, (uint64_t)planes * whole_steps(piece) * pitch);
     if (a.reduction != kEach) room.want(&each, a.rows);
@@ -557,17 +649,18 @@ static int32_t forward_of(const Problem &a, int32_t device, float *loss, float *
         Product product{};
         product.p = Operand{pack_w ? pw : static_cast<const uint16_t *>(weights), nullptr, pitch, plane_w, classes};
         product.q = Operand{px, nullptr, pitch, plane_x, a.rows};
-        product.tiles_p = (classes + Shape::BP - 1) / Shape::BP;
-        product.tiles_q = (padded + Shape::BQ - 1) / Shape::BQ;
         product.splits = 1;
         product.depth = pitch;
         product.live = rows.count;
         const FinishLoss<planes> finish{partials, target_logit, rows.target, rows.count, first, classes, k * slots_piece, a.rows};
-        launch_product<half, Shape, true, true, planes>(product, finish, s);
+        with_tile(piece, a.rows, [&](auto shape) {
+            using Shape = decltype(shape);
+            product.tiles_p = tiles_of(classes, Shape::BP);
+            product.tiles_q = tiles_of(a.rows, Shape::BQ);
+            launch_product<half, Shape, true, true, planes>(product, finish, s);
+        });
     }
-    const uint32_t last = (a.classes - (pieces - 1) * piece + Shape::BP - 1) / Shape::BP * Shape::WP;
-    loss_rows_kernel<<<blocks_of(a.rows, 16), kBlock, 0, s>>>(partials, (pieces - 1) * slots_piece + last, a.rows,
-                                                               target_logit, rows, lse, to);
+    loss_rows_kernel<<<blocks_of(a.rows, 16), kBlock, 0, s>>>(partials, slots, a.rows, target_logit, rows, lse, to);
     if (a.reduction != kEach)
         loss_sum_kernel<<<1, kRowsBlock, 0, s>>>(each, a.rows, rows.count, a.reduction == kMean, loss);
     return hip_check(hipGetLastError(), "linear cross entropy launch");
@@ -578,7 +671,6 @@ static int32_t backward_of(const Problem &a, int32_t device, const float *grad, 
                            void *dx, void *dw, void *stream) {
     constexpr int planes = Kind<T>::kPlanes;
     constexpr bool half = Kind<T>::kHalf;
-    using Shape = Large;
     using Raw = typename T::raw;
     hipStream_t s = (hipStream_t)stream;
     const uint32_t pitch = whole_steps(a.width), padded = whole_steps(a.rows);
@@ -586,10 +678,12 @@ static int32_t backward_of(const Problem &a, int32_t device, const float *grad, 
     const uint32_t piece = piece_of(a, pitch, planes, pack_w, true);
     const uint32_t pieces = (a.classes + piece - 1) / piece;
     const uint32_t dz_pitch = whole_steps(piece);
-    const uint32_t tiles_h = (pitch + Shape::BP - 1) / Shape::BP, tiles_n = (padded + Shape::BQ - 1) / Shape::BQ;
-    const uint32_t depth = (piece + kDepth - 1) / kDepth;
-    uint32_t splits = std::max(1u, kSumTiles / std::max(1u, tiles_h * tiles_n));
-    splits = std::min(splits, std::max(1u, depth / 8u));
+    uint32_t splits = 1;
+    with_input_tile(a.rows, [&](auto shape) {
+        using Shape = decltype(shape);
+        splits = splits_of(tiles_of(pitch, Shape::BP) * tiles_of(a.rows, Shape::BQ), tiles_of(piece, kDepth),
+                           (uint64_t)a.rows * pitch);
+    });
 
     Rows rows{};
     uint16_t *px = nullptr, *pw = nullptr, *dz = nullptr;
@@ -600,6 +694,7 @@ static int32_t backward_of(const Problem &a, int32_t device, const float *grad, 
     room.want(&rows.row, a.rows);
     room.want(&rows.target, a.rows);
     room.want(&rows.weight, a.rows);
+    room.want(&rows.place, a.rows);
     room.want(&px, (uint64_t)planes * padded * pitch);
     // The weights' last lines, where those are read in place and do not fill a step.
     const bool ragged = !pack_w && a.classes % kDepth != 0;
@@ -632,42 +727,53 @@ static int32_t backward_of(const Problem &a, int32_t device, const float *grad, 
         Product logits{};
         logits.p = Operand{w, nullptr, pitch, plane_w, classes};
         logits.q = Operand{px, nullptr, pitch, plane_x, a.rows};
-        logits.tiles_p = (line + Shape::BP - 1) / Shape::BP;
-        logits.tiles_q = tiles_n;
         logits.splits = 1;
+        logits.pad = true;
         logits.depth = pitch;
         logits.live = rows.count;
         const FinishGrad<half, planes> grads{dz,         plane_dz,    line,     lse, rows.weight, rows.target,
                                              rows.row, rows.count, first, classes};
-        launch_product<half, Shape, true, true, planes>(logits, grads, s);
+        with_tile(piece, padded, [&](auto shape) {
+            using Shape = decltype(shape);
+            logits.tiles_p = tiles_of(line, Shape::BP);
+            logits.tiles_q = tiles_of(padded, Shape::BQ);
+            launch_product<half, Shape, true, true, planes>(logits, grads, s);
+        });
 
         Product input{};                    // dx[i][h] = sum over v of dz[i][v] W[v][h]
         input.p = Operand{w, ragged && k + 1u == pieces ? pw : nullptr, pitch, plane_w, pitch};
         input.q = Operand{dz, nullptr, line, plane_dz, a.rows};
-        input.tiles_p = tiles_h;
-        input.tiles_q = tiles_n;
         input.splits = splits;
         input.depth = line;
         input.live = rows.count;
         const FinishSum sum{sums, (uint64_t)a.rows * pitch, pitch, rows.count, k > 0};
-        launch_product<half, Shape, false, true, planes>(input, sum, s);
+        with_input_tile(a.rows, [&](auto shape) {
+            using Shape = decltype(shape);
+            input.tiles_p = tiles_of(pitch, Shape::BP);
+            input.tiles_q = tiles_of(a.rows, Shape::BQ);
+            launch_product<half, Shape, false, true, planes>(input, sum, s);
+        });
 
         Product weight{};                   // dW[v][h] = sum over i of dz[i][v] x[i][h]
         weight.p = Operand{px, nullptr, pitch, plane_x, pitch};
         weight.q = Operand{dz, nullptr, line, plane_dz, line};
-        weight.tiles_p = tiles_h;
-        weight.tiles_q = (classes + Shape::BQ - 1) / Shape::BQ;
         weight.splits = 1;
         weight.depth = a.rows;
         weight.live = rows.count;
         weight.live_depth = true;
         Raw *to = static_cast<Raw *>(dw) + (uint64_t)first * a.width;
-        const bool even = a.width % 4u == 0 && (uintptr_t)dw % (4u * sizeof(Raw)) == 0;
-        const FinishWeight<T> last{to, rows.unscale, a.width, classes, even};
-        launch_product<half, Shape, false, false, planes>(weight, last, s);
+        const FinishWeight<T> last{to, rows.unscale, a.width, classes,
+                                   a.width % 8u == 0 && (uintptr_t)dw % 16u == 0};
+        with_weight_tile(pitch, classes, a.rows, [&](auto shape) {
+            using Shape = decltype(shape);
+            weight.tiles_p = tiles_of(pitch, Shape::BP);
+            weight.tiles_q = tiles_of(classes, Shape::BQ);
+            launch_product<half, Shape, false, false, planes>(weight, last, s);
+        });
     }
-    grad_input_kernel<T><<<std::min(a.rows, 8192u), kBlock, 0, s>>>(sums, (uint64_t)a.rows * pitch, splits, pitch, rows,
-                                                                    a.rows, a.width, static_cast<Raw *>(dx));
+    const bool even = a.width % 8u == 0 && (uintptr_t)dx % 16u == 0;
+    grad_input_kernel<T><<<blocks_of(a.rows * (uint64_t)((a.width + 7u) / 8u), kBlock), kBlock, 0, s>>>(
+        sums, (uint64_t)a.rows * pitch, splits, pitch, rows, a.rows, a.width, even, static_cast<Raw *>(dx));
     return hip_check(hipGetLastError(), "linear cross entropy backward launch");
 }
 

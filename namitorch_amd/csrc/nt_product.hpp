@@ -61,6 +61,7 @@ struct Product {
     uint32_t tiles_p, tiles_q, splits, depth;   // depth: along k, in steps of 64 that are shared out among the splits
     const uint32_t *live;
     bool live_depth;
+    bool pad;                   // tiles of q reach to a whole step
 };
 
 // Shape of a workgroup's tile and of the waves in it.
@@ -193,7 +194,7 @@ __global__ __launch_bounds__(T::kThreads, T::PER_SIMD) void product_kernel(Produ
             a.depth = live;
         } else {
             a.q.rows = live;
-            a.tiles_q = (whole_steps(live) + T::BQ - 1u) / T::BQ;     // what a padding to whole steps takes too
+            a.tiles_q = ((a.pad ? whole_steps(live) : live) + T::BQ - 1u) / T::BQ;
         }
     }
     const uint32_t tiles = a.tiles_p * a.tiles_q;
