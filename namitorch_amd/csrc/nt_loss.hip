@@ -528,48 +528,34 @@ constexpr uint32_t kUnits = 256;                     // compute units
 
 using Large = Tile<256, 256, 2, 4>;
 using Middle = Tile<128, 128, 2, 2>;
-using Few = Tile<128, 64, 4, 1>;                     // rows
+using Tall = Tile<256, 128, 4, 2, 3>;                // up to 128 rows
+using Few = Tile<128, 64, 4, 1, 3>;                  // up to 64
 
 static uint32_t tiles_of(uint64_t n, uint32_t each) { return (uint32_t)((n + each - 1) / each); }
 
-// Calls launch(shape) with the tile shape for a product of `p` by `q`.
+// Calls launch(shape) with the tile shape of the logits of `rows` and `classes`.
 template <class F>
-static void with_tile(uint64_t p, uint64_t q, F &&launch) {
-    if (q <= 64u) launch(Few{});
-    else if ((uint64_t)tiles_of(p, 256) * tiles_of(q, 256) < kUnits) launch(Middle{});
-    else launch(Large{});
-}
-
-template <class F>
-static void with_input_tile(uint64_t rows, F &&launch) {
+static void with_logits_tile(uint64_t classes, uint64_t rows, F &&launch) {
     if (rows <= 64u) launch(Few{});
-    else if (rows <= 128u) launch(Middle{});
+    else if (rows <= 128u) launch(Tall{});
+    else if ((uint64_t)tiles_of(classes, 256) * tiles_of(rows, 256) < kUnits) launch(Middle{});
     else launch(Large{});
 }
 
-#ifndef WT
-#define WT 0
-#endif
+// The same for the two products of dz.
 template <class F>
-static void with_weight_tile(uint64_t p, uint64_t q, uint64_t rows, F &&launch) {
-    if ((uint64_t)tiles_of(p, 256) * tiles_of(q, 256) < kUnits || rows <= WT) launch(Middle{});
+static void with_grads_tile(uint64_t rows, F &&launch) {
+    if (rows <= 64u) launch(Few{});
+    else if (rows <= 128u) launch(Tall{});
     else launch(Large{});
 }
 
-// Splits of dx's product along k: as many as take the fewest rounds of the
-// chip for their length, with what each adds to the sums' traffic.
-static uint32_t splits_of(uint32_t tiles, uint32_t steps, uint64_t sums) {
-    uint32_t best = 1;
-    double least = 1e30;
-    for (uint32_t s = 1; s <= 64u && s * 4u <= std::max(steps, 4u); ++s) {
-        const double rounds = tiles_of((uint64_t)tiles * s, kUnits);
-        const double us = rounds * (tiles_of(steps, s) + 4u) * 1.6 + s * (double)sums * 8.0 / 4e6;
-        if (us < least) {
-            least = us;
-            best = s;
-        }
-    }
-    return best;
+// Splits of dx's product along k, of which each tile has `steps`, beside
+// `other` steps of tiles: such that no workgroup has more than half of what
+// each compute unit gets, and at least four steps.
+static uint32_t splits_of(uint64_t tiles, uint32_t steps, uint64_t other) {
+    const uint64_t share = std::max<uint64_t>((tiles * steps + other) / (2u * kUnits), 4u);
+    return (uint32_t)std::max<uint64_t>(1u, (steps + share - 1) / share);
 }
 
 struct Problem {
@@ -612,7 +598,7 @@ static int32_t forward_of(const Problem &a, int32_t device, float *loss, float *
     const uint32_t piece = piece_of(a, pitch, planes, pack_w, false);
     const uint32_t pieces = (a.classes + piece - 1) / piece;
     uint32_t slots_piece = 0, slots = 0;                  // of a whole piece, of all
-    with_tile(piece, a.rows, [&](auto shape) {
+    with_logits_tile(piece, a.rows, [&](auto shape) {
         using Shape = decltype(shape);
         slots_piece = tiles_of(piece, Shape::BP) * Shape::WP;
         slots = (pieces - 1) * slots_piece + tiles_of(a.classes - (pieces - 1) * piece, Shape::BP) * Shape::WP;
@@ -653,7 +639,7 @@ static int32_t forward_of(const Problem &a, int32_t device, float *loss, float *
         product.depth = pitch;
         product.live = rows.count;
         const FinishLoss<planes> finish{partials, target_logit, rows.target, rows.count, first, classes, k * slots_piece, a.rows};
-        with_tile(piece, a.rows, [&](auto shape) {
+        with_logits_tile(piece, a.rows, [&](auto shape) {
             using Shape = decltype(shape);
             product.tiles_p = tiles_of(classes, Shape::BP);
             product.tiles_q = tiles_of(a.rows, Shape::BQ);
@@ -679,10 +665,11 @@ static int32_t backward_of(const Problem &a, int32_t device, const float *grad, 
     const uint32_t pieces = (a.classes + piece - 1) / piece;
     const uint32_t dz_pitch = whole_steps(piece);
     uint32_t splits = 1;
-    with_input_tile(a.rows, [&](auto shape) {
+    with_grads_tile(a.rows, [&](auto shape) {
         using Shape = decltype(shape);
-        splits = splits_of(tiles_of(pitch, Shape::BP) * tiles_of(a.rows, Shape::BQ), tiles_of(piece, kDepth),
-                           (uint64_t)a.rows * pitch);
+        const uint32_t tiles_h = tiles_of(pitch, Shape::BP);
+        splits = splits_of((uint64_t)tiles_h * tiles_of(a.rows, Shape::BQ), tiles_of(piece, kDepth),
+                           (uint64_t)tiles_h * tiles_of(piece, Shape::BQ) * tiles_of(a.rows, kDepth));
     });
 
     Rows rows{};
@@ -733,7 +720,7 @@ static int32_t backward_of(const Problem &a, int32_t device, const float *grad, 
         logits.live = rows.count;
         const FinishGrad<half, planes> grads{dz,         plane_dz,    line,     lse, rows.weight, rows.target,
                                              rows.row, rows.count, first, classes};
-        with_tile(piece, padded, [&](auto shape) {
+        with_logits_tile(piece, padded, [&](auto shape) {
             using Shape = decltype(shape);
             logits.tiles_p = tiles_of(line, Shape::BP);
             logits.tiles_q = tiles_of(padded, Shape::BQ);
@@ -747,12 +734,6 @@ static int32_t backward_of(const Problem &a, int32_t device, const float *grad, 
         input.depth = line;
         input.live = rows.count;
         const FinishSum sum{sums, (uint64_t)a.rows * pitch, pitch, rows.count, k > 0};
-        with_input_tile(a.rows, [&](auto shape) {
-            using Shape = decltype(shape);
-            input.tiles_p = tiles_of(pitch, Shape::BP);
-            input.tiles_q = tiles_of(a.rows, Shape::BQ);
-            launch_product<half, Shape, false, true, planes>(input, sum, s);
-        });
 
         Product weight{};                   // dW[v][h] = sum over i of dz[i][v] x[i][h]
         weight.p = Operand{px, nullptr, pitch, plane_x, pitch};
@@ -764,11 +745,12 @@ static int32_t backward_of(const Problem &a, int32_t device, const float *grad, 
         Raw *to = static_cast<Raw *>(dw) + (uint64_t)first * a.width;
         const FinishWeight<T> last{to, rows.unscale, a.width, classes,
                                    a.width % 8u == 0 && (uintptr_t)dw % 16u == 0};
-        with_weight_tile(pitch, classes, a.rows, [&](auto shape) {
+        with_grads_tile(a.rows, [&](auto shape) {
             using Shape = decltype(shape);
-            weight.tiles_p = tiles_of(pitch, Shape::BP);
+            input.tiles_p = weight.tiles_p = tiles_of(pitch, Shape::BP);
+            input.tiles_q = tiles_of(a.rows, Shape::BQ);
             weight.tiles_q = tiles_of(classes, Shape::BQ);
-            launch_product<half, Shape, false, false, planes>(weight, last, s);
+            launch_two_products<half, Shape, planes>(input, sum, weight, last, s);
         });
     }
     const bool even = a.width % 8u == 0 && (uintptr_t)dx % 16u == 0;

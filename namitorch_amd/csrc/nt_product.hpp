@@ -65,10 +65,10 @@ struct Product {
 };
 
 // Shape of a workgroup's tile and of the waves in it.
-template <int BP_, int BQ_, int WP_, int WQ_, int PER_SIMD_ = 2>
+template <int BP_, int BQ_, int WP_, int WQ_, int ROOMS_ = 2>
 struct Tile {
     static constexpr int BP = BP_, BQ = BQ_, WP = WP_, WQ = WQ_;
-    static constexpr int PER_SIMD = PER_SIMD_;                      // waves that the registers leave room for
+    static constexpr int ROOMS = ROOMS_;                            // slices in LDS: one is multiplied, the rest are on their way
     static constexpr int kWaves = WP * WQ, kThreads = kWaves * 64;
     static constexpr int kWaveP = BP / WP, kWaveQ = BQ / WQ;        // a wave's part
     static constexpr int TP = kWaveP / 16, TQ = kWaveQ / 16;        // in tiles of the matrix instruction
@@ -179,12 +179,23 @@ __device__ __forceinline__ uint32_t xcd_order(uint32_t b, uint32_t n) {
     return xcd * (n >> 3) + (xcd < left ? xcd : left) + (b >> 3);
 }
 
-// PLANES: 1, or 3 of float32.  `finish` gets the wave's accumulators: element
-// [tp][tq][r] is p = p_first + 16 tp + 4 (lane / 16) + r, q = q_first + 16 tq + lane % 16.
+// The slices of both operands of a step.
+template <class T>
+struct Room {
+    alignas(16) uint16_t at[(T::BP + T::BQ) * kDepth];
+};
+
+// How many workgroups a product takes at most.
+inline uint32_t workgroups_of(const Product &a) { return a.tiles_p * a.tiles_q * a.splits; }
+
+// Workgroup `block` of a product.  PLANES: 1, or 3 of float32.  `finish` gets
+// the wave's accumulators: element [tp][tq][r] is p = p_first + 16 tp + 4 (lane
+// / 16) + r, q = q_first + 16 tq + lane % 16.  The rooms are arrays of their
+// own: the compiler then knows that a read of one need not wait for what is on
+// its way to another.
 template <bool HALF, class T, bool P_DEEP, bool Q_DEEP, int PLANES, class Finish>
-__global__ __launch_bounds__(T::kThreads, T::PER_SIMD) void product_kernel(Product a, Finish finish) {
-    __shared__ __attribute__((aligned(16))) uint16_t room0[(T::BP + T::BQ) * kDepth];
-    __shared__ __attribute__((aligned(16))) uint16_t room1[(T::BP + T::BQ) * kDepth];
+__device__ __forceinline__ void product(Product a, const Finish &finish, uint32_t block, uint16_t *room0,
+                                        uint16_t *room1, uint16_t *room2) {
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
     // Tiles go in bands of 8 along q, in each band along p.
@@ -198,8 +209,8 @@ __global__ __launch_bounds__(T::kThreads, T::PER_SIMD) void product_kernel(Produ
         }
     }
     const uint32_t tiles = a.tiles_p * a.tiles_q;
-    if (blockIdx.x >= tiles * a.splits) return;
-    const uint32_t place = xcd_order(blockIdx.x, tiles * a.splits), split = place / tiles, tile = place % tiles;
+    if (block >= tiles * a.splits) return;
+    const uint32_t place = xcd_order(block, tiles * a.splits), split = place / tiles, tile = place % tiles;
     const uint32_t band = tile / (8u * a.tiles_p), in_band = tile % (8u * a.tiles_p);
     const uint32_t high = a.tiles_q - band * 8u < 8u ? a.tiles_q - band * 8u : 8u;
     const uint32_t tile_q = band * 8u + in_band % high, tile_p = in_band / high;
@@ -223,6 +234,7 @@ __global__ __launch_bounds__(T::kThreads, T::PER_SIMD) void product_kernel(Produ
     const uint32_t begin = (uint32_t)((uint64_t)steps * split / a.splits);
     const uint32_t end = (uint32_t)((uint64_t)steps * (split + 1u) / a.splits);
     const uint32_t total = (end - begin) * products;
+    // Past the last step the last is queued again, so that the loop has no branches.
     const auto stage = [&](uint16_t *room, uint32_t s) {
         s = s < total ? s : total - 1u;
         uint32_t k = begin + s, plane_p = 0, plane_q = 0;
@@ -236,7 +248,6 @@ __global__ __launch_bounds__(T::kThreads, T::PER_SIMD) void product_kernel(Produ
         load_q.load(room + T::BP * kDepth, k, steps, plane_q, wave);
     };
     const auto compute = [&](const uint16_t *room) {
-        __builtin_amdgcn_sched_barrier(0);          // the loads before are under way first
         read_p.hide();
         read_q.hide();
         s16x8_t fp[2][T::TP], fq[2][T::TQ];
@@ -271,28 +282,90 @@ __global__ __launch_bounds__(T::kThreads, T::PER_SIMD) void product_kernel(Produ
             }
         }
     };
+    // One step: its slice is there, in every wave's part, once the loads before the last ROOMS - 2 slices are
+    // done and all waves say so; that also ends every read of the room that is loaded next.
+    const auto step = [&](const uint16_t *room, uint16_t *free, uint32_t s) {
+        constexpr int ahead = (T::ROOMS - 2) * (decltype(load_p)::kLoads + decltype(load_q)::kLoads);
+        static_assert(ahead < 64, "the counter of loads on their way has six bits");
+        __asm__ volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt((ahead & 15) | (ahead >> 4) << 14 | 0x0f70);     // vmcnt(ahead)
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        __asm__ volatile("" ::: "memory");
+        stage(free, s + T::ROOMS - 1);
+        __builtin_amdgcn_sched_barrier(0);              // the loads are under way first
+        compute(room);
+    };
     if (total > 0) {
-        // Past the last step the last is queued again, so that the loop has no branches.
         stage(room0, 0);
-        __syncthreads();
-        for (uint32_t s = 0; s + 1 < total; s += 2) {
-            stage(room1, s + 1);
-            compute(room0);
-            __syncthreads();
-            stage(room0, s + 2);
-            compute(room1);
-            __syncthreads();
+        if constexpr (T::ROOMS == 2) {
+            uint32_t s = 0;
+            for (; s + 1 < total; s += 2) {
+                step(room0, room1, s);
+                step(room1, room0, s + 1);
+            }
+            if (s < total) step(room0, room1, s);
+        } else {
+            stage(room1, 1);
+            uint32_t s = 0;
+            for (; s + 2 < total; s += 3) {
+                step(room0, room2, s);
+                step(room1, room0, s + 1);
+                step(room2, room1, s + 2);
+            }
+            if (s < total) step(room0, room2, s);
+            if (s + 1 < total) step(room1, room0, s + 1);
         }
-        if (total & 1u) compute(room0);
+        __builtin_amdgcn_s_waitcnt(0x0f70);             // nothing is on its way to LDS when it is given up
     }
     finish.template operator()<T>(acc, tile_p * T::BP + wave_p * T::kWaveP, tile_q * T::BQ + wave_q * T::kWaveQ, split,
                                   lane);
 }
 
 template <bool HALF, class T, bool P_DEEP, bool Q_DEEP, int PLANES, class Finish>
-static void launch_product(Product a, const Finish &finish, hipStream_t s) {
-    const dim3 grid(a.tiles_p * a.tiles_q * a.splits);
-    product_kernel<HALF, T, P_DEEP, Q_DEEP, PLANES, Finish><<<grid, dim3(T::kThreads), 0, s>>>(a, finish);
+__global__ __launch_bounds__(T::kThreads, 2) void product_kernel(Product a, Finish finish) {
+    __shared__ Room<T> room0, room1;
+    if constexpr (T::ROOMS == 2) {
+        product<HALF, T, P_DEEP, Q_DEEP, PLANES>(a, finish, blockIdx.x, room0.at, room1.at, nullptr);
+    } else {
+        __shared__ Room<T> room2;
+        product<HALF, T, P_DEEP, Q_DEEP, PLANES>(a, finish, blockIdx.x, room0.at, room1.at, room2.at);
+    }
+}
+
+// Two products in one launch, the first's workgroups first: the second's fill
+// the units that the first leaves idle at its end.  Both have [k][row] lines
+// for p; the first has deep lines for q.
+template <bool HALF, class T, int PLANES, class FinishA, class FinishB>
+__global__ __launch_bounds__(T::kThreads, 2) void two_products_kernel(Product a, FinishA finish_a, uint32_t first,
+                                                                     Product b, FinishB finish_b) {
+    __shared__ Room<T> room0, room1;
+    const auto run = [&](uint16_t *room2) {
+        if (blockIdx.x < first)
+            product<HALF, T, false, true, PLANES>(a, finish_a, blockIdx.x, room0.at, room1.at, room2);
+        else
+            product<HALF, T, false, false, PLANES>(b, finish_b, blockIdx.x - first, room0.at, room1.at, room2);
+    };
+    if constexpr (T::ROOMS == 2) {
+        run(nullptr);
+    } else {
+        __shared__ Room<T> room2;
+        run(room2.at);
+    }
+}
+
+template <bool HALF, class T, bool P_DEEP, bool Q_DEEP, int PLANES, class Finish>
+static void launch_product(const Product &a, const Finish &finish, hipStream_t s) {
+    product_kernel<HALF, T, P_DEEP, Q_DEEP, PLANES, Finish>
+        <<<dim3(workgroups_of(a)), dim3(T::kThreads), 0, s>>>(a, finish);
+}
+
+template <bool HALF, class T, int PLANES, class FinishA, class FinishB>
+static void launch_two_products(const Product &a, const FinishA &finish_a, const Product &b, const FinishB &finish_b,
+                                hipStream_t s) {
+    const uint32_t first = (workgroups_of(a) + 7u) / 8u * 8u;       // whole rounds of the XCDs
+    two_products_kernel<HALF, T, PLANES, FinishA, FinishB>
+        <<<dim3(first + workgroups_of(b)), dim3(T::kThreads), 0, s>>>(a, finish_a, first, b, finish_b);
 }
 
 }  // namespace nt
