@@ -434,22 +434,38 @@ struct FinishWeight {
 };
 
 // ---- the ends of both passes -----------------------------------------------------------------------------
-// lse and loss of 16 rows a workgroup: 16 lanes share out a row's slots.
-__global__ __launch_bounds__(kBlock) void loss_rows_kernel(const Partial2 *partials, uint32_t slots, uint64_t stride,
-                                                           const float *target_logit, Rows rows, float *lse,
-                                                           float *loss) {
-    __shared__ Partial2 shared[16][17];
-    const uint32_t count = *rows.count, r = threadIdx.x & 15u, slice = threadIdx.x >> 4;
-    for (uint32_t first = blockIdx.x * 16u; first < count; first += gridDim.x * 16u) {
+// lse and loss of ROWS rows a workgroup, over which the lanes share out their
+// slots: 16 rows, or one where there are few, whose slots are read at once.
+template <int ROWS, int THREADS>
+__global__ __launch_bounds__(THREADS) void loss_rows_kernel(const Partial2 *partials, uint32_t slots, uint64_t stride,
+                                                            const float *target_logit, Rows rows, float *lse,
+                                                            float *loss) {
+    constexpr uint32_t slices = THREADS / ROWS;
+    __shared__ Partial2 shared[slices][ROWS + 1];
+    const uint32_t count = *rows.count, r = threadIdx.x % ROWS, slice = threadIdx.x / ROWS;
+    for (uint32_t first = blockIdx.x * ROWS; first < count; first += gridDim.x * ROWS) {
         const uint32_t j = first + r;
         Partial2 p{-kInfinity, 0.0f};
-        if (j < count)
-            for (uint32_t k = slice; k < slots; k += 16u) p = join(p, partials[k * stride + j]);
+        if (j < count) {
+            uint32_t k = slice;
+            for (; k + 7u * slices < slots; k += 8u * slices) {
+                Partial2 part[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) part[u] = partials[(k + u * slices) * stride + j];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) p = join(p, part[u]);
+            }
+            for (; k < slots; k += slices) p = join(p, partials[k * stride + j]);
+        }
         __syncthreads();
         shared[slice][r] = p;
         __syncthreads();
+        for (uint32_t half = slices / 2u; half > 0u; half /= 2u) {
+            if (slice < half) shared[slice][r] = join(shared[slice][r], shared[slice + half][r]);
+            __syncthreads();
+        }
         if (slice == 0 && j < count) {
-            for (uint32_t k = 1; k < 16; ++k) p = join(p, shared[k][r]);
+            p = shared[0][r];
             const float value = p.most + __builtin_amdgcn_logf(p.sum) * kLn2;
             const uint32_t row = rows.row[j];
             if (lse != nullptr) lse[row] = value;
@@ -528,7 +544,7 @@ constexpr uint32_t kUnits = 256;                     // compute units
 
 using Large = Tile<256, 256, 2, 4>;
 using Middle = Tile<128, 128, 2, 2>;
-using Tall = Tile<256, 128, 4, 2, 3>;                // up to 128 rows
+using Tall = Tile<256, 128, 4, 2, 3>;                // up to 256 rows
 using Few = Tile<128, 64, 4, 1, 3>;                  // up to 64
 
 static uint32_t tiles_of(uint64_t n, uint32_t each) { return (uint32_t)((n + each - 1) / each); }
@@ -537,7 +553,7 @@ static uint32_t tiles_of(uint64_t n, uint32_t each) { return (uint32_t)((n + eac
 template <class F>
 static void with_logits_tile(uint64_t classes, uint64_t rows, F &&launch) {
     if (rows <= 64u) launch(Few{});
-    else if (rows <= 128u) launch(Tall{});
+    else if (rows <= 256u) launch(Tall{});
     else if ((uint64_t)tiles_of(classes, 256) * tiles_of(rows, 256) < kUnits) launch(Middle{});
     else launch(Large{});
 }
@@ -546,7 +562,7 @@ static void with_logits_tile(uint64_t classes, uint64_t rows, F &&launch) {
 template <class F>
 static void with_grads_tile(uint64_t rows, F &&launch) {
     if (rows <= 64u) launch(Few{});
-    else if (rows <= 128u) launch(Tall{});
+    else if (rows <= 256u) launch(Tall{});
     else launch(Large{});
 }
 
@@ -646,7 +662,11 @@ static int32_t forward_of(const Problem &a, int32_t device, float *loss, float *
             launch_product<half, Shape, true, true, planes>(product, finish, s);
         });
     }
-    loss_rows_kernel<<<blocks_of(a.rows, 16), kBlock, 0, s>>>(partials, slots, a.rows, target_logit, rows, lse, to);
+    if (a.rows <= kUnits)
+        loss_rows_kernel<1, 1024><<<a.rows, 1024, 0, s>>>(partials, slots, a.rows, target_logit, rows, lse, to);
+    else
+        loss_rows_kernel<16, 512><<<blocks_of(a.rows, 16), 512, 0, s>>>(partials, slots, a.rows, target_logit, rows, lse,
+                                                                        to);
     if (a.reduction != kEach)
         loss_sum_kernel<<<1, kRowsBlock, 0, s>>>(each, a.rows, rows.count, a.reduction == kMean, loss);
     return hip_check(hipGetLastError(), "linear cross entropy launch");
