@@ -29,11 +29,13 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "nt_entry.hpp"
 #include "nt_internal.hpp"
 #include "nt_pool.hpp"
 #include "nt_product.hpp"
+#include "nt_row_ops.hpp"
 
 namespace nt {
 
@@ -72,10 +74,25 @@ struct Rows {
 // ---- counted rows ----------------------------------------------------------------------------------
 constexpr int kRowsBlock = 1024;
 
-// One workgroup: each lane takes a run of consecutive rows.
+// One workgroup: each lane takes a run of consecutive rows, eight of whose
+// targets are read at a time (8192 rows: 11 us one after the other).  Forward,
+// the lse and loss of rows that are not counted are set to zero here.
+template <class F>
+__device__ __forceinline__ void each_class(const Targets &t, uint32_t begin, uint32_t end, F &&use) {
+    for (uint32_t i = begin; i < end; i += 8u) {
+        int32_t c[8];
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) c[k] = class_of(t, i + k < end ? i + k : end - 1u);
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k)
+            if (i + k < end) use(i + k, c[k]);
+    }
+}
+
 template <bool BACKWARD>
 __global__ __launch_bounds__(kRowsBlock) void rows_kernel(Targets t, uint32_t rows, Rows out, const float *grad,
-                                                          float grad_value, int32_t reduction, bool scaled) {
+                                                          float grad_value, int32_t reduction, bool scaled, float *lse,
+                                                          float *loss) {
     __shared__ uint32_t counts[kRowsBlock / 64];
     __shared__ float most[kRowsBlock / 64];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
@@ -84,11 +101,11 @@ __global__ __launch_bounds__(kRowsBlock) void rows_kernel(Targets t, uint32_t ro
     const uint32_t end = rows - begin < each ? rows : begin + each;
     uint32_t mine = 0;
     float largest = 0.0f;
-    for (uint32_t i = begin; i < end; ++i) {
-        if (class_of(t, i) == kIgnored) continue;
+    each_class(t, begin, end, [&](uint32_t i, int32_t c) {
+        if (c == kIgnored) return;
         ++mine;
         if (BACKWARD && reduction == kEach) largest = fmaxf(largest, fabsf(grad[i]));
-    }
+    });
     uint32_t before = mine;                                // inclusive sums over the wave
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
@@ -126,16 +143,19 @@ __global__ __launch_bounds__(kRowsBlock) void rows_kernel(Targets t, uint32_t ro
         if (BACKWARD) *out.unscale = (reduction == kEach ? 1.0f : common) / scale;
     }
     uint32_t j = before - mine;
-    for (uint32_t i = begin; i < end; ++i) {
-        const int32_t c = class_of(t, i);
+    each_class(t, begin, end, [&](uint32_t i, int32_t c) {
         if (BACKWARD) out.place[i] = c == kIgnored ? ~0u : j;
-        if (c == kIgnored) continue;
+        if (c == kIgnored) {
+            if (lse != nullptr) lse[i] = 0.0f;
+            if (loss != nullptr) loss[i] = 0.0f;
+            return;
+        }
         out.row[j] = i;
         out.target[j] = c;
         if constexpr (BACKWARD)
             out.weight[j] = c == kOutside ? __builtin_nanf("") : (reduction == kEach ? grad[i] : 1.0f) * scale;
         ++j;
-    }
+    });
 }
 
 // ---- operands as the products take them --------------------------------------------------------------
@@ -474,15 +494,6 @@ __global__ __launch_bounds__(THREADS) void loss_rows_kernel(const Partial2 *part
     }
 }
 
-// Rows that are not counted have loss and lse zero.
-__global__ __launch_bounds__(kBlock) void loss_ignored_kernel(Targets t, uint32_t rows, float *lse, float *loss) {
-    for (uint32_t i = blockIdx.x * kBlock + threadIdx.x; i < rows; i += gridDim.x * kBlock) {
-        if (class_of(t, i) != kIgnored) continue;
-        if (lse != nullptr) lse[i] = 0.0f;
-        if (loss != nullptr) loss[i] = 0.0f;
-    }
-}
-
 // Sum or mean of the rows' losses, in 64 bits and a fixed order.
 __global__ __launch_bounds__(kRowsBlock) void loss_sum_kernel(const float *each, uint32_t rows, const uint32_t *count,
                                                               bool mean, float *loss) {
@@ -499,6 +510,120 @@ __global__ __launch_bounds__(kRowsBlock) void loss_sum_kernel(const float *each,
     }
 }
 
+// ---- a few rows -----------------------------------------------------------------------------------------
+// Scoring a token or a few: bound by the one read of the weights, which a tile
+// of the matrix cores would spend on rows that are not there, after launches
+// that gather and pack.  A wave takes a run of classes, four at a time, and
+// holds its lanes' part of the sums of all rows; the weights are read where
+// and as they lie.  Two launches.  A call of one row of 50257 x 768 float16:
+// 20.5 us (with 1024 workgroups 23.7), as a tile 27.9; 32000 x 4096 45.1 and
+// 53.4.  Of two rows 29.5 and 27.8, four 41.5 and 27.8: so one row only, but up
+// to four of what the tiles would have to pack first (float32, and widths that
+// are not whole steps), five times the weights' bytes.
+constexpr uint32_t kFewRows = 4, kFewAtOnce = 4, kFewBlocks = 2048;
+
+template <class T>
+__device__ __forceinline__ void load_group(float (&out)[8], const void *base, uint64_t row, uint32_t c, uint32_t width) {
+    Raw8<T> raw;
+    if (c + kGroup <= width) load8<T, false>(raw, base, row + c);
+    else load_end<T>(raw, base, row + c, c < width ? width - c : 0u);
+    widen8<T>(out, raw);
+}
+
+template <class T, int ROWS>
+__global__ __launch_bounds__(kBlock) void few_rows_kernel(const void *x, const void *w, Targets t, uint32_t width,
+                                                          Partial2 *partials, float *target_logit) {
+    __shared__ Partial2 shared[kBlock / 64][ROWS];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint64_t place = blockIdx.x * (uint64_t)(kBlock / 64) + wave, waves = gridDim.x * (uint64_t)(kBlock / 64);
+    const uint32_t begin = (uint32_t)(t.classes * place / waves), end = (uint32_t)(t.classes * (place + 1u) / waves);
+    Partial2 part[ROWS];
+    int32_t target[ROWS];
+#pragma unroll
+    for (int n = 0; n < ROWS; ++n) {
+        part[n] = Partial2{-kInfinity, 0.0f};
+        target[n] = class_of(t, n);
+    }
+    for (uint32_t v = begin; v < end; v += kFewAtOnce) {
+        float z[kFewAtOnce][ROWS];
+#pragma unroll
+        for (uint32_t k = 0; k < kFewAtOnce; ++k)
+#pragma unroll
+            for (int n = 0; n < ROWS; ++n) z[k][n] = 0.0f;
+        for (uint32_t first = 0; first < width; first += 64u * kGroup) {
+            const uint32_t c = first + lane * kGroup;
+            float weights[kFewAtOnce][8];
+#pragma unroll
+            for (uint32_t k = 0; k < kFewAtOnce; ++k)
+                load_group<T>(weights[k], w, (v + k < end ? v + k : end - 1u) * (uint64_t)width, c, width);
+#pragma unroll
+            for (int n = 0; n < ROWS; ++n) {
+                float values[8];
+                load_group<T>(values, x, n * (uint64_t)width, c, width);
+#pragma unroll
+                for (uint32_t k = 0; k < kFewAtOnce; ++k)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) z[k][n] = __builtin_fmaf(weights[k][e], values[e], z[k][n]);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < ROWS; ++n) {
+            float most = part[n].most;
+#pragma unroll
+            for (uint32_t k = 0; k < kFewAtOnce; ++k) {
+                z[k][n] = lanes_sum(z[k][n], 64u);
+                if (v + k >= end) z[k][n] = -kInfinity;
+                else if ((int32_t)(v + k) == target[n] && lane == 0u) target_logit[n] = z[k][n];
+                most = fmaxf(most, z[k][n]);
+            }
+            const float from = most == -kInfinity ? 0.0f : most;
+            float sum = part[n].sum * (part[n].most == most ? 1.0f : exp_of(part[n].most - from));
+#pragma unroll
+            for (uint32_t k = 0; k < kFewAtOnce; ++k) sum += exp_of(z[k][n] - from);
+            part[n] = Partial2{most, sum};
+        }
+    }
+    if (lane == 0u)
+#pragma unroll
+        for (int n = 0; n < ROWS; ++n) shared[wave][n] = part[n];
+    __syncthreads();
+    if (threadIdx.x >= ROWS) return;
+    Partial2 all = shared[0][threadIdx.x];
+    for (uint32_t k = 1; k < kBlock / 64; ++k) all = join(all, shared[k][threadIdx.x]);
+    partials[blockIdx.x * (uint64_t)ROWS + threadIdx.x] = all;
+}
+
+// lse, loss and their reduction for those rows: one workgroup, a lane a slot.
+__global__ __launch_bounds__(kRowsBlock) void few_loss_kernel(const Partial2 *partials, uint32_t slots, Targets t,
+                                                              uint32_t rows, const float *target_logit,
+                                                              int32_t reduction, float *lse, float *loss) {
+    __shared__ Partial2 shared[kRowsBlock / 64];
+    double total = 0.0;
+    uint32_t counted = 0;
+    for (uint32_t n = 0; n < rows; ++n) {
+        Partial2 p{-kInfinity, 0.0f};
+        for (uint32_t k = threadIdx.x; k < slots; k += kRowsBlock) p = join(p, partials[k * (uint64_t)rows + n]);
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1)
+            p = join(p, Partial2{__shfl_xor(p.most, off, 64), __shfl_xor(p.sum, off, 64)});
+        __syncthreads();
+        if ((threadIdx.x & 63u) == 0u) shared[threadIdx.x >> 6] = p;
+        __syncthreads();
+        if (threadIdx.x != 0u) continue;
+        for (uint32_t k = 1; k < kRowsBlock / 64; ++k) p = join(p, shared[k]);
+        const int32_t c = class_of(t, n);
+        const float value = p.most + __builtin_amdgcn_logf(p.sum) * kLn2;
+        const float each = c == kIgnored ? 0.0f : c == kOutside ? __builtin_nanf("") : value - target_logit[n];
+        if (lse != nullptr) lse[n] = c == kIgnored ? 0.0f : value;
+        if (reduction == kEach) loss[n] = each;
+        total += (double)each;
+        counted += c != kIgnored;
+    }
+    if (threadIdx.x == 0u && reduction != kEach)
+        *loss = (float)(reduction == kMean ? total / (double)(counted > 0 ? counted : 1u) : total);
+}
+
+// ---- dx -------------------------------------------------------------------------------------------------
 // dx from its sums, eight columns a lane; rows that are not counted are zero.
 template <class T>
 __global__ __launch_bounds__(kBlock) void grad_input_kernel(const float *sums, uint64_t split_stride, uint32_t splits,
@@ -605,12 +730,36 @@ static uint32_t piece_of(const Problem &a, uint32_t pitch, int planes, bool pack
 }
 
 template <class T>
+static int32_t few_rows_of(const Problem &a, int32_t device, float *loss, float *lse, void *stream) {
+    hipStream_t s = (hipStream_t)stream;
+    const uint32_t blocks = std::min(kFewBlocks, (a.classes + kBlock / 64 - 1) / (kBlock / 64));
+    Partial2 *partials = nullptr;
+    float *target_logit = nullptr;
+    Workspace room;
+    room.want(&partials, (uint64_t)blocks * a.rows);
+    room.want(&target_logit, a.rows);
+    const int32_t rc = room.allocate(device, stream);
+    if (rc != NT_OK) return rc;
+    const auto launch = [&](auto rows) {
+        few_rows_kernel<T, decltype(rows)::value><<<blocks, kBlock, 0, s>>>(a.x, a.w, a.targets, a.width, partials,
+                                                                            target_logit);
+    };
+    if (a.rows == 1u) launch(std::integral_constant<int, 1>{});
+    else if (a.rows == 2u) launch(std::integral_constant<int, 2>{});
+    else if (a.rows == 3u) launch(std::integral_constant<int, 3>{});
+    else launch(std::integral_constant<int, 4>{});
+    few_loss_kernel<<<1, kRowsBlock, 0, s>>>(partials, blocks, a.targets, a.rows, target_logit, a.reduction, lse, loss);
+    return hip_check(hipGetLastError(), "linear cross entropy launch");
+}
+
+template <class T>
 static int32_t forward_of(const Problem &a, int32_t device, float *loss, float *lse, void *stream) {
     constexpr int planes = Kind<T>::kPlanes;
     constexpr bool half = Kind<T>::kHalf;
     hipStream_t s = (hipStream_t)stream;
     const uint32_t pitch = whole_steps(a.width), padded = whole_steps(a.rows);
     const bool pack_w = planes > 1 || pitch != a.width || (uintptr_t)a.w % 16u != 0;
+    if (a.rows <= (planes > 1 || pitch != a.width ? kFewRows : 1u)) return few_rows_of<T>(a, device, loss, lse, stream);
     const uint32_t piece = piece_of(a, pitch, planes, pack_w, false);
     const uint32_t pieces = (a.classes + piece - 1) / piece;
     uint32_t slots_piece = 0, slots = 0;                  // of a whole piece, of all
@@ -637,8 +786,7 @@ static int32_t forward_of(const Problem &a, int32_t device, float *loss, float *
     if (rc != NT_OK) return rc;
     float *to = a.reduction == kEach ? loss : each;
 
-    rows_kernel<false><<<1, kRowsBlock, 0, s>>>(a.targets, a.rows, rows, nullptr, 0.0f, a.reduction, false);
-    loss_ignored_kernel<<<blocks_of(a.rows, kBlock), kBlock, 0, s>>>(a.targets, a.rows, lse, to);
+    rows_kernel<false><<<1, kRowsBlock, 0, s>>>(a.targets, a.rows, rows, nullptr, 0.0f, a.reduction, false, lse, to);
     const uint64_t plane_x = (uint64_t)padded * pitch, plane_w = (uint64_t)whole_steps(piece) * pitch;
     pack_kernel<T><<<blocks_of(padded * (uint64_t)(pitch / 8u), kBlock), kBlock, 0, s>>>(
         a.x, a.width, px, pitch, plane_x, a.rows, rows.row, rows.count);
@@ -712,7 +860,8 @@ static int32_t backward_of(const Problem &a, int32_t device, const float *grad, 
     int32_t rc = room.allocate(device, stream);
     if (rc != NT_OK) return rc;
 
-    rows_kernel<true><<<1, kRowsBlock, 0, s>>>(a.targets, a.rows, rows, grad, grad_value, a.reduction, half);
+    rows_kernel<true><<<1, kRowsBlock, 0, s>>>(a.targets, a.rows, rows, grad, grad_value, a.reduction, half, nullptr,
+                                               nullptr);
     const uint64_t plane_x = (uint64_t)padded * pitch, plane_w = (uint64_t)whole_steps(piece) * pitch;
     const uint64_t plane_dz = (uint64_t)padded * dz_pitch;
     pack_kernel<T><<<blocks_of(padded * (uint64_t)(pitch / 8u), kBlock), kBlock, 0, s>>>(
