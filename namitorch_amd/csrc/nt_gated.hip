@@ -25,6 +25,7 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "nt_entry.hpp"
 #include "nt_internal.hpp"
@@ -76,6 +77,356 @@ __device__ __forceinline__ float block_total(double v, double *shared) {
     double total = 0.0;
     for (uint32_t k = 0; k < blockDim.x / 64u; ++k) total += shared[k];
     return (float)total;
+}
+
+// ---- rows that fit in registers ---------------------------------------------------------------------
+// As in the residual path's norms (nt_rows.hpp): a row lies over `lanes` lanes
+// in `parts` groups of eight, is read once, and variances are of centred
+// values; rows share workgroups, which make as many rounds as they need, and
+// the next row is on its way while this one is summed.  The vectors wait in
+// LDS as float32; a gate that a workgroup's rows share is multiplied into the
+// first norm's weight and bias there.  Rows of less than eight, or of more than
+// 8192 (whose vectors LDS does not hold), take the kernels for any width.
+enum GateKind { kFolded = 0, kOwn = 1, kOwnFloat = 2 };   // none or shared; a row's own, of the data's type or float32
+
+template <class T, int KIND> struct GateType { using type = T; };
+template <class T> struct GateType<T, kOwnFloat> { using type = TF32; };
+
+template <class T>
+__device__ __forceinline__ void store_row(void *base, uint64_t i, bool even, const float (&v)[8]) {
+    Raw8<T> out;
+    narrow8<T>(out, v);
+    if (T::code == NT_F32 && even) store8<T, true>(base, i, out);
+    else store8<T, false>(base, i, out);
+}
+
+// The vectors of a lane's columns in LDS: [vector][half of a group][part][lane].
+template <int PARTS>
+struct Vectors {
+    float4 *room;
+    uint32_t lanes, lane;
+    __device__ __forceinline__ void keep(int vector, int p, const float (&v)[8]) const {
+        float4 *to = room + ((vector * 2 * PARTS + p) * lanes + lane);
+        to[0] = make_float4(v[0], v[1], v[2], v[3]);
+        to[PARTS * lanes] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+    __device__ __forceinline__ void get(float (&v)[8], int vector, int p) const {
+        const float4 *from = room + ((vector * 2 * PARTS + p) * lanes + lane);
+        const float4 a = from[0], b = from[PARTS * lanes];
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+};
+
+template <class T, int KIND, int PARTS, bool EVEN, int THREADS>
+__global__ __launch_bounds__(THREADS, 4) void gated_kernel(GatedForward a, uint32_t lanes, uint32_t run_blocks, bool rms,
+                                                           bool even) {
+    using G = typename GateType<T, KIND>::type;
+    extern __shared__ float4 room[];
+    __shared__ float shared[2][THREADS / 64];
+    RowSum<THREADS / 64> row_sum{shared, lanes};
+    const uint32_t lane = threadIdx.x & (lanes - 1u), in_block = threadIdx.x / lanes, per_block = THREADS / lanes;
+    const float width = (float)a.width;
+    const Vectors<PARTS> vectors{room, lanes, lane};
+    Columns at[PARTS];
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) at[p] = Columns(((uint32_t)p * lanes + lane) * kGroup, a.width);
+    // Rows of one run; with gates of their own all rows are one.
+    const uint32_t run = blockIdx.x / run_blocks;
+    const uint64_t count = KIND == kFolded ? a.gate.run : a.rows, before = run * count;
+    const uint64_t stride = (uint64_t)run_blocks * per_block;
+    uint64_t r = (uint64_t)(blockIdx.x % run_blocks) * per_block + in_block;
+    Raw8<T> x[PARTS], residual[PARTS];
+    Raw8<G> gate[PARTS];
+    const auto fetch = [&](uint64_t which) {
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            if (which >= count || at[p].column >= a.width) continue;
+            const uint64_t base = (before + which) * a.width;
+            load8<T, false>(x[p], a.x, base + at[p].column);
+            load8<T, false>(residual[p], a.residual, base + at[p].column);
+            if constexpr (KIND != kFolded)
+                load8<G, false>(gate[p], a.gate.at, a.gate.row(which) * a.width + at[p].column);
+        }
+    };
+    fetch(r);
+    // Vector v of part p: the first norm's weight and bias, times a shared gate, the second's.
+    const auto vector = [&](float (&v)[8], int which, int p) {
+        uint32_t column = at[p].column;
+        __asm__ volatile("" : "+v"(column));            // no addresses kept from one vector for the next
+        const void *from[4] = {a.inner_weight, a.inner_bias, a.weight, a.bias};
+        load_params(v, from[which], a.weight_dtype, column, a.width, which % 2 == 0 ? 1.0f : 0.0f);
+        if (KIND == kFolded && which < 2 && a.gate.at != nullptr) {
+            float g[8];
+            const char *line = static_cast<const char *>(a.gate.at) +
+                               (uint64_t)run * a.width * (a.gate.dtype == NT_F32 ? 4u : 2u);
+            load_params(g, line, a.gate.dtype, column, a.width, 1.0f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] *= g[k];
+        }
+    };
+    for (uint32_t which = in_block; which < 4u; which += per_block)
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            float v[8];
+            vector(v, (int)which, p);
+            vectors.keep((int)which, p, v);
+        }
+    __syncthreads();
+    const auto norm = [&](float (&t)[PARTS][8], float &mean, float &rstd) {
+        mean = 0.0f;
+        if (!rms) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) sum = at[p].template has<EVEN>(k, a.width) ? sum + t[p][k] : sum;
+            mean = row_sum(sum) / width;
+        }
+        float squares = 0.0f;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float d = t[p][k] - mean;
+                squares = at[p].template has<EVEN>(k, a.width) ? __builtin_fmaf(d, d, squares) : squares;
+            }
+        rstd = 1.0f / __builtin_sqrtf(row_sum(squares) / width + a.eps);
+    };
+    for (uint64_t round = (uint64_t)(blockIdx.x % run_blocks) * per_block; round < count; round += stride) {
+        const uint64_t base = (before + r) * a.width;
+        const bool active = r < count;
+        float t[PARTS][8];
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) widen8<T>(t[p], x[p]);
+        float inner_mean, inner_rstd, mean, rstd;
+        norm(t, inner_mean, inner_rstd);
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            float u[8], b[8], add[8];
+            __builtin_amdgcn_sched_barrier(0);          // one part's vectors in registers at a time
+            vectors.get(u, 0, p);
+            vectors.get(b, 1, p);
+            widen8<T>(add, residual[p]);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t[p][k] = __builtin_fmaf((t[p][k] - inner_mean) * inner_rstd, u[k], b[k]);
+            if constexpr (KIND != kFolded) {
+                float g[8];
+                widen8<G>(g, gate[p]);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) t[p][k] *= g[k];
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t[p][k] = __builtin_fmaf(a.scale, add[k], t[p][k]);
+        }
+        fetch(r + stride);
+        norm(t, mean, rstd);
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            if (!active || at[p].column >= a.width) continue;
+            __builtin_amdgcn_sched_barrier(0);
+            store_row<T>(a.total, base + at[p].column, even, t[p]);
+            float w[8], b[8];
+            vectors.get(w, 2, p);
+            vectors.get(b, 3, p);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t[p][k] = __builtin_fmaf((t[p][k] - mean) * rstd, w[k], b[k]);
+            store_row<T>(a.y, base + at[p].column, even, t[p]);
+        }
+        if (active && lane == 0u && a.rstd != nullptr) {
+            a.inner_rstd[before + r] = inner_rstd;
+            a.rstd[before + r] = rstd;
+            if (!rms) {
+                a.inner_mean[before + r] = inner_mean;
+                a.mean[before + r] = mean;
+            }
+        }
+        r += stride;
+    }
+}
+
+// The backward pass, a group of eight a lane.  The four sums over rows of a
+// lane's columns stay in registers over all rows of the workgroup, which are
+// of one run; rows that share a workgroup are joined at the end, in order, and
+// each workgroup writes one row of partial sums for each.
+template <class T, int KIND, bool EVEN, int THREADS>
+__global__ __launch_bounds__(THREADS, 4) void gated_backward_kernel(GatedBackward a, uint32_t lanes, bool rms, bool even) {
+    using G = typename GateType<T, KIND>::type;
+    extern __shared__ float4 room[];
+    __shared__ float shared[2][2][THREADS / 64];
+    RowSum2<THREADS / 64> row_sum{shared, lanes};
+    const uint32_t lane = threadIdx.x & (lanes - 1u), in_block = threadIdx.x / lanes, per_block = THREADS / lanes;
+    const float width = (float)a.width;
+    const Vectors<1> vectors{room, lanes, lane};
+    const Columns at(lane * kGroup, a.width);
+    const uint32_t c = at.column, run = blockIdx.x / a.run_blocks;
+    const uint64_t count = KIND == kFolded ? a.gate.run : a.rows, before = run * count;
+    const uint64_t stride = (uint64_t)a.run_blocks * per_block;
+    uint64_t r = (uint64_t)(blockIdx.x % a.run_blocks) * per_block + in_block;
+    const bool mine = c < a.width;
+    Raw8<T> dy, t, dtotal, x;
+    Raw8<G> gate;
+    const auto fetch_outer = [&](uint64_t which) {
+        if (which >= count || !mine) return;
+        const uint64_t base = (before + which) * a.width;
+        load8<T, false>(dy, a.dy, base + c);
+        load8<T, false>(t, a.t, base + c);
+        if (a.dtotal != nullptr) load8<T, false>(dtotal, a.dtotal, base + c);
+    };
+    const auto fetch_inner = [&](uint64_t which) {
+        if (which >= count || !mine) return;
+        const uint64_t base = (before + which) * a.width;
+        load8<T, false>(x, a.x, base + c);
+        if constexpr (KIND != kFolded) load8<G, false>(gate, a.gate.at, base + c);
+    };
+    float next[4] = {0.0f, 0.0f, 0.0f, 0.0f};           // mean, rstd, inner mean, inner rstd
+    const auto fetch_stats = [&](uint64_t which) {
+        if (which >= count) return;
+        if (!rms) {
+            next[0] = a.mean[before + which];
+            next[2] = a.inner_mean[before + which];
+        }
+        next[1] = a.rstd[before + which];
+        next[3] = a.inner_rstd[before + which];
+    };
+    fetch_outer(r);
+    fetch_inner(r);
+    fetch_stats(r);
+    // 0: the second norm's weight; 1: the first's, times a shared gate; 2: the first's bias, where rows have gates.
+    for (uint32_t which = in_block; which < (KIND == kFolded ? 2u : 3u); which += per_block) {
+        float v[8];
+        uint32_t column = c;
+        __asm__ volatile("" : "+v"(column));            // no addresses kept from one vector for the next
+        load_params(v, which == 0u ? a.weight : which == 1u ? a.inner_weight : a.inner_bias, a.weight_dtype, column,
+                    a.width, which == 2u ? 0.0f : 1.0f);
+        if (KIND == kFolded && which == 1u && a.gate.at != nullptr) {
+            float g[8];
+            const char *line = static_cast<const char *>(a.gate.at) +
+                               (uint64_t)run * a.width * (a.gate.dtype == NT_F32 ? 4u : 2u);
+            load_params(g, line, a.gate.dtype, column, a.width, 1.0f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] *= g[k];
+        }
+        vectors.keep((int)which, 0, v);
+    }
+    __syncthreads();
+    float sums[4][8];
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sums[v][k] = 0.0f;
+    const auto has = [&](int k) { return EVEN || at.template has<false>((uint32_t)k, a.width); };
+    for (uint64_t round = (uint64_t)(blockIdx.x % a.run_blocks) * per_block; round < count; round += stride) {
+        const uint64_t base = (before + r) * a.width;
+        const bool active = r < count && mine;
+        const float mean = next[0], rstd = next[1], inner_mean = next[2], inner_rstd = next[3];
+        float g[8], h[8], w[8];
+        float level = 0.0f, along = 0.0f;
+        vectors.get(w, 0, 0);
+        widen8<T>(g, dy);
+        widen8<T>(h, t);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const bool in_row = active && has(k);
+            h[k] = (h[k] - mean) * rstd;
+            sums[2][k] = in_row ? __builtin_fmaf(g[k], h[k], sums[2][k]) : sums[2][k];
+            sums[3][k] = in_row ? sums[3][k] + g[k] : sums[3][k];
+            g[k] *= w[k];
+            level = in_row ? level + g[k] : level;
+            along = in_row ? __builtin_fmaf(g[k], h[k], along) : along;
+        }
+        row_sum(level, along);
+        level = rms ? 0.0f : level / width;
+        along /= width;
+        float add[8];
+        widen8<T>(add, dtotal);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            g[k] = rstd * (g[k] - level - h[k] * along);
+            g[k] = a.dtotal != nullptr ? g[k] + add[k] : g[k];
+            w[k] = a.scale * g[k];
+        }
+        fetch_outer(r + stride);                        // into the registers that were just read
+        if (active) store_row<T>(a.dresidual, base + c, even, w);
+        level = along = 0.0f;
+        widen8<T>(h, x);
+        vectors.get(w, 1, 0);
+        if constexpr (KIND != kFolded) {
+            float own[8], bias[8], by_gate[8];
+            widen8<G>(own, gate);
+            vectors.get(bias, 2, 0);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                h[k] = (h[k] - inner_mean) * inner_rstd;
+                by_gate[k] = g[k] * __builtin_fmaf(h[k], w[k], bias[k]);
+                g[k] *= own[k];
+            }
+            if (active && a.dgate != nullptr) store_row<G>(a.dgate, base + c, even, by_gate);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) h[k] = (h[k] - inner_mean) * inner_rstd;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const bool in_row = active && has(k);
+            sums[0][k] = in_row ? __builtin_fmaf(g[k], h[k], sums[0][k]) : sums[0][k];
+            sums[1][k] = in_row ? sums[1][k] + g[k] : sums[1][k];
+            g[k] *= w[k];
+            level = in_row ? level + g[k] : level;
+            along = in_row ? __builtin_fmaf(g[k], h[k], along) : along;
+        }
+        fetch_inner(r + stride);
+        fetch_stats(r + stride);
+        row_sum(level, along);
+        level = rms ? 0.0f : level / width;
+        along /= width;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) g[k] = inner_rstd * (g[k] - level - h[k] * along);
+        if (active) store_row<T>(a.dx, base + c, even, g);
+        r += stride;
+    }
+
+    // Rows of one wave, then the workgroup's waves or wider rows in order.
+    for (uint32_t off = lanes; off < 64u; off <<= 1)
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sums[v][k] += __shfl_xor(sums[v][k], (int)off, 64);
+    const uint32_t span = lanes < 64u ? 64u : lanes, members = THREADS / span, member = threadIdx.x / span;
+    const uint32_t place = threadIdx.x & (span - 1u);
+    for (uint32_t half = members / 2u; half > 0u; half >>= 1) {
+        __syncthreads();                                // the vectors, or the last half, are read
+        if (member >= half && member < 2u * half && place < lanes)
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                room[((member - half) * 8 + q) * lanes + place] =
+                    make_float4(sums[q >> 1][4 * (q & 1)], sums[q >> 1][4 * (q & 1) + 1], sums[q >> 1][4 * (q & 1) + 2],
+                                sums[q >> 1][4 * (q & 1) + 3]);
+        __syncthreads();
+        if (member < half && place < lanes)
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const float4 other = room[(member * 8 + q) * lanes + place];
+                sums[q >> 1][4 * (q & 1)] += other.x;
+                sums[q >> 1][4 * (q & 1) + 1] += other.y;
+                sums[q >> 1][4 * (q & 1) + 2] += other.z;
+                sums[q >> 1][4 * (q & 1) + 3] += other.w;
+            }
+    }
+    if (member != 0u || place >= lanes || !mine) return;
+    float *out = a.partials + blockIdx.x * 4ull * a.width;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+        if (at.first == 0u && c + kGroup <= a.width) {
+            Raw8<TF32> raw;
+            narrow8<TF32>(raw, sums[v]);
+            store8<TF32, false>(out, (uint64_t)v * a.width + c, raw);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (has(k)) out[(uint64_t)v * a.width + c + k] = sums[v][k];
+        }
+    }
 }
 
 // ---- rows of any width: a workgroup a row ----------------------------------------------------------
@@ -226,8 +577,8 @@ __global__ __launch_bounds__(kBlock) void gated_columns_kernel(GatedBackward a, 
 }
 
 // The vectors' gradients from the partial sums: 32 columns and 32 slices a
-// workgroup.  A slice takes whole runs where there are several, else a share
-// of the one run's blocks; slices are joined in order.
+// workgroup.  Slices share out the runs, and where those are fewer, the blocks
+// of each; a run's sums are joined before its gate, slices in order.
 struct GatedVectors {
     void *inner_weight, *inner_bias, *gate, *weight, *bias;     // each may be null
 };
@@ -241,58 +592,158 @@ __global__ __launch_bounds__(kVectorColumns * kVectorSlices) void gated_vectors_
     const uint64_t line = a.width, block = 4u * line;
     const bool there = c < a.width;
     const float u = there ? load_param(a.inner_weight, a.weight_dtype, c, 1.0f) : 0.0f;
-    const float k = there ? load_param(a.inner_bias, a.weight_dtype, c, 0.0f) : 0.0f;
-    const auto gate_of = [&](uint32_t run) {
-        return each ? 1.0f : load_param(a.gate.at, a.gate.dtype, run * line + c, 1.0f);
-    };
+    const float bias = there ? load_param(a.inner_bias, a.weight_dtype, c, 0.0f) : 0.0f;
+    uint32_t subs = kVectorSlices;
+    while (subs > 1u && kVectorSlices / subs < runs) subs >>= 1;
+    const uint32_t at_once = kVectorSlices / subs, sub = slice % subs;
     float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (there && runs == 1u) {
-        for (uint32_t b = slice; b < a.run_blocks; b += kVectorSlices)
-            for (int v = 0; v < 4; ++v) sums[v] += a.partials[b * block + v * line + c];
-    } else if (there) {
-        for (uint32_t run = slice; run < runs; run += kVectorSlices) {
-            float own[2] = {0.0f, 0.0f};
-            for (uint32_t b = run * a.run_blocks; b < (run + 1u) * a.run_blocks; ++b) {
-                own[0] += a.partials[b * block + c];
-                own[1] += a.partials[b * block + line + c];
-                sums[2] += a.partials[b * block + 2u * line + c];
-                sums[3] += a.partials[b * block + 3u * line + c];
+    for (uint32_t first = 0; first < runs; first += at_once) {
+        const uint32_t run = first + slice / subs;
+        float own[2] = {0.0f, 0.0f};
+        if (there && run < runs) {
+            const float *from = a.partials + run * (uint64_t)a.run_blocks * block + c;
+#pragma unroll 4
+            for (uint32_t b = sub; b < a.run_blocks; b += subs) {
+                own[0] += from[b * block];
+                own[1] += from[b * block + line];
+                sums[2] += from[b * block + 2u * line];
+                sums[3] += from[b * block + 3u * line];
             }
-            if (to.gate != nullptr)
-                store_param(to.gate, a.gate.dtype, run * line + c, __builtin_fmaf(u, own[0], k * own[1]));
-            const float gate = gate_of(run);
-            sums[0] = __builtin_fmaf(gate, own[0], sums[0]);
-            sums[1] = __builtin_fmaf(gate, own[1], sums[1]);
         }
+        if (subs > 1u) {
+            __syncthreads();
+            shared[0][slice][column] = own[0];
+            shared[1][slice][column] = own[1];
+            __syncthreads();
+            if (sub == 0u)
+                for (uint32_t k = 1; k < subs; ++k) {
+                    own[0] += shared[0][slice + k][column];
+                    own[1] += shared[1][slice + k][column];
+                }
+        }
+        if (!there || run >= runs || sub != 0u) continue;
+        if (to.gate != nullptr)
+            store_param(to.gate, a.gate.dtype, run * line + c, __builtin_fmaf(u, own[0], bias * own[1]));
+        const float gate = each ? 1.0f : load_param(a.gate.at, a.gate.dtype, run * line + c, 1.0f);
+        sums[0] = __builtin_fmaf(gate, own[0], sums[0]);
+        sums[1] = __builtin_fmaf(gate, own[1], sums[1]);
     }
+    __syncthreads();
     for (int v = 0; v < 4; ++v) shared[v][slice][column] = sums[v];
     __syncthreads();
     if (slice >= 4u || !there) return;
     float sum = 0.0f;
     for (uint32_t s = 0; s < kVectorSlices; ++s) sum += shared[slice][s][column];
-    const float gate = runs == 1u ? gate_of(0) : 1.0f;
     void *out = slice == 0u ? to.inner_weight : slice == 1u ? to.inner_bias : slice == 2u ? to.weight : to.bias;
-    if (out != nullptr) store_param(out, a.weight_dtype, c, slice < 2u ? sum * gate : sum);
-    if (runs != 1u || each || to.gate == nullptr || slice != 0u) return;
-    float other = 0.0f;
-    for (uint32_t s = 0; s < kVectorSlices; ++s) other += shared[1][s][column];
-    store_param(to.gate, a.gate.dtype, c, __builtin_fmaf(u, sum, k * other));
+    if (out != nullptr) store_param(out, a.weight_dtype, c, sum);
 }
 
 // ---- launches ----------------------------------------------------------------------------------------
 constexpr uint32_t kMostBlocks = 8192;
-constexpr uint32_t kRunGroups = 256;                    // groups of rows of the column sums, over all runs
+constexpr uint32_t kRunGroups = 256;                    // groups of rows of the column sums of long rows, over all runs
 constexpr uint64_t kMostWidth = 1ull << 24;
+constexpr uint32_t kGatedWaves = 4;                     // per SIMD, which the registers leave room for
+constexpr uint32_t kLdsColumns = 8192;                  // whose vectors fit in LDS
+// A shared gate's runs of fewer rows than this many workgroups hold at a time
+// are taken as gates of the rows' own: each run's workgroups load the vectors.
+constexpr uint32_t kShortRun = 4;
 
-template <class T>
-static void launch_gated(const GatedForward &a, bool rms, hipStream_t s) {
-    const dim3 grid((unsigned)std::min<uint64_t>(a.rows, kMostBlocks));
-    if (rms) gated_rows_kernel<T, true><<<grid, dim3(kBlock), 0, s>>>(a);
-    else gated_rows_kernel<T, false><<<grid, dim3(kBlock), 0, s>>>(a);
+// Workgroups of each run: as many as are resident, where there are rows for them.
+static uint32_t run_blocks_of(uint64_t run, uint64_t runs, uint32_t per_block, uint32_t threads) {
+    const uint64_t most = std::max<uint64_t>(1u, kSimds * kGatedWaves * 64u / threads / runs);
+    return (uint32_t)std::min<uint64_t>((run + per_block - 1) / per_block, most);
+}
+
+// How the forward pass takes the gate, and how many runs keep their rows apart.
+static int gate_kind(const GatedForward &a, int32_t dtype, uint32_t per_block, uint64_t &runs) {
+    runs = a.gate.runs;
+    if (runs == 1u || a.gate.run >= (uint64_t)kShortRun * per_block) return kFolded;
+    runs = 1u;
+    return a.gate.dtype == dtype ? kOwn : kOwnFloat;
+}
+
+// A group a lane: the tiling of the backward pass, and of rows that are not
+// whole groups (whose predicates of two or three groups do not fit in the
+// scalar registers).
+static RowTiling single_tiling(uint32_t width) {
+    const uint32_t groups = (width + kGroup - 1) / kGroup;
+    uint32_t lanes = 1;
+    while (lanes < groups) lanes <<= 1;
+    if (width < kGroup || lanes > (uint32_t)kWideThreads) return RowTiling{0, 0, 0};
+    return RowTiling{lanes, 1, uint32_t(lanes <= (uint32_t)kRowThreads ? kRowThreads : kWideThreads)};
+}
+
+template <class T, int KIND, int PARTS, bool EVEN, int THREADS>
+static void launch_gated_tiled(const GatedForward &a, const RowTiling &g, uint64_t runs, bool rms, bool aligned,
+                               hipStream_t s) {
+    const uint32_t blocks = run_blocks_of(a.rows / runs, runs, g.threads / g.lanes, g.threads);
+    const dim3 grid((unsigned)(runs * blocks));
+    gated_kernel<T, KIND, PARTS, EVEN, THREADS>
+        <<<grid, dim3(THREADS), g.lanes * g.parts * kGroup * 16u, s>>>(a, g.lanes, blocks, rms, aligned);
+}
+
+template <class T, int KIND, bool EVEN>
+static void launch_gated_kind(const GatedForward &a, const RowTiling &g, uint64_t runs, bool rms, bool aligned,
+                              hipStream_t s) {
+    if (g.threads == (uint32_t)kWideThreads) {
+        launch_gated_tiled<T, KIND, 1, EVEN, kWideThreads>(a, g, runs, rms, aligned, s);
+    } else if (g.parts == 1) {
+        launch_gated_tiled<T, KIND, 1, EVEN, kRowThreads>(a, g, runs, rms, aligned, s);
+    } else if constexpr (EVEN && T::code != NT_F32) {
+        if (g.parts == 2) launch_gated_tiled<T, KIND, 2, EVEN, kRowThreads>(a, g, runs, rms, aligned, s);
+        else launch_gated_tiled<T, KIND, 3, EVEN, kRowThreads>(a, g, runs, rms, aligned, s);
+    }
 }
 
 template <class T>
-static void launch_gated_backward(const GatedBackward &a, bool rms, uint32_t groups, hipStream_t s) {
+static void launch_gated(const GatedForward &a, bool rms, hipStream_t s) {
+    const bool even = a.width % kGroup == 0, aligned = aligned16({a.total, a.y});
+    RowTiling g = even ? forward_tiling(a.rows, a.width, T::code) : single_tiling(a.width);
+    if (g.lanes * g.parts * kGroup > kLdsColumns) g = single_tiling(a.width);
+    if (g.parts == 0) {
+        const dim3 grid((unsigned)std::min<uint64_t>(a.rows, kMostBlocks));
+        if (rms) gated_rows_kernel<T, true><<<grid, dim3(kBlock), 0, s>>>(a);
+        else gated_rows_kernel<T, false><<<grid, dim3(kBlock), 0, s>>>(a);
+        return;
+    }
+    uint64_t runs = 1;
+    const int kind = gate_kind(a, T::code, g.threads / g.lanes, runs);
+    const auto launch = [&](auto k) {
+        if (even) launch_gated_kind<T, decltype(k)::value, true>(a, g, runs, rms, aligned, s);
+        else launch_gated_kind<T, decltype(k)::value, false>(a, g, runs, rms, aligned, s);
+    };
+    if (kind == kFolded) launch(std::integral_constant<int, kFolded>{});
+    else if (kind == kOwn) launch(std::integral_constant<int, kOwn>{});
+    else if constexpr (T::code != NT_F32) launch(std::integral_constant<int, kOwnFloat>{});
+}
+
+template <class T, int KIND, int THREADS>
+static void launch_gated_backward_tiled(const GatedBackward &a, const RowTiling &g, bool rms, uint32_t groups,
+                                        hipStream_t s) {
+    const bool aligned = aligned16({a.dx, a.dresidual, a.dgate});
+    // The vectors, or half of the rows that are joined.
+    const uint32_t span = g.lanes < 64u ? 64u : g.lanes;
+    const uint32_t room = std::max(g.lanes * kGroup * (KIND == kFolded ? 8u : 12u), THREADS / span / 2u * g.lanes * 128u);
+    if (a.width % kGroup == 0)
+        gated_backward_kernel<T, KIND, true, THREADS><<<dim3(groups), dim3(THREADS), room, s>>>(a, g.lanes, rms, aligned);
+    else
+        gated_backward_kernel<T, KIND, false, THREADS><<<dim3(groups), dim3(THREADS), room, s>>>(a, g.lanes, rms, aligned);
+}
+
+template <class T>
+static void launch_gated_backward(const GatedBackward &a, bool rms, bool each, uint32_t groups, hipStream_t s) {
+    const RowTiling g = single_tiling(a.width);
+    if (g.parts != 0) {
+        const auto launch = [&](auto kind) {
+            constexpr int KIND = decltype(kind)::value;
+            if (g.threads == (uint32_t)kWideThreads) launch_gated_backward_tiled<T, KIND, kWideThreads>(a, g, rms, groups, s);
+            else launch_gated_backward_tiled<T, KIND, kRowThreads>(a, g, rms, groups, s);
+        };
+        if (!each) launch(std::integral_constant<int, kFolded>{});
+        else if (a.gate.dtype == T::code) launch(std::integral_constant<int, kOwn>{});
+        else if constexpr (T::code != NT_F32) launch(std::integral_constant<int, kOwnFloat>{});
+        return;
+    }
     const dim3 grid((unsigned)std::min<uint64_t>(a.rows, kMostBlocks));
     const dim3 columns((a.width + kBlock - 1) / kBlock, std::min(groups, 65535u));
     if (rms) gated_rows_backward_kernel<T, true><<<grid, dim3(kBlock), 0, s>>>(a);
@@ -412,17 +863,19 @@ int32_t nt_norm_gate_add_norm_backward(int32_t device, const void *dy, const voi
                     {gate, gate_dtype, (uint32_t)gate_runs, rows / gate_runs}, inner_mean, inner_rstd, mean, rstd,
                     dx, dresidual, each ? dgate : nullptr, nullptr, nullptr, rows, (uint32_t)width, weight_dtype,
                     residual_scale, 1};
-    a.run_blocks = (uint32_t)std::min<uint64_t>(rows / runs, std::max(1u, kRunGroups / runs));
+    const RowTiling tiling = single_tiling((uint32_t)width);
+    a.run_blocks = tiling.parts != 0 ? run_blocks_of(rows / runs, runs, tiling.threads / tiling.lanes, tiling.threads)
+                                     : (uint32_t)std::min<uint64_t>(rows / runs, std::max(1u, kRunGroups / runs));
     Workspace room;
-    room.want(&a.row_sums, 2u * rows);
+    if (tiling.parts == 0) room.want(&a.row_sums, 2u * rows);
     room.want(&a.partials, 4ull * width * runs * a.run_blocks);
     rc = room.allocate(device, stream);
     if (rc != NT_OK) return rc;
     const uint32_t groups = runs * a.run_blocks;
     switch (dtype) {
-        case NT_F32: launch_gated_backward<TF32>(a, rms, groups, s); break;
-        case NT_F16: launch_gated_backward<TF16>(a, rms, groups, s); break;
-        default: launch_gated_backward<TBF16>(a, rms, groups, s); break;
+        case NT_F32: launch_gated_backward<TF32>(a, rms, each, groups, s); break;
+        case NT_F16: launch_gated_backward<TF16>(a, rms, each, groups, s); break;
+        default: launch_gated_backward<TBF16>(a, rms, each, groups, s); break;
     }
     const GatedVectors vectors{dinner_weight, dinner_bias, each ? nullptr : dgate, dweight, dbias};
     gated_vectors_kernel<<<dim3((unsigned)((width + kVectorColumns - 1) / kVectorColumns)),
