@@ -87,6 +87,8 @@ __device__ __forceinline__ float block_total(double v, double *shared) {
 // LDS as float32; a gate that a workgroup's rows share is multiplied into the
 // first norm's weight and bias there.  Rows of less than eight, or of more than
 // 8192 (whose vectors LDS does not hold), take the kernels for any width.
+constexpr uint32_t kGatedWaves = 4;     // per SIMD
+
 enum GateKind { kFolded = 0, kOwn = 1, kOwnFloat = 2 };   // none or shared; a row's own, of the data's type or float32
 
 template <class T, int KIND> struct GateType { using type = T; };
@@ -100,59 +102,103 @@ __device__ __forceinline__ void store_row(void *base, uint64_t i, bool even, con
     else store8<T, false>(base, i, out);
 }
 
-// The vectors of a lane's columns in LDS: [vector][half of a group][part][lane].
-template <int PARTS>
+// Sums of one value, or of two, over the lanes of a row, the same on each: as
+// RowSum, for rows of any number of waves.
+template <int MAX_WAVES>
+struct GatedSum {
+    float (*shared)[MAX_WAVES];
+    uint32_t lanes, in_block;
+    uint32_t half = 0;
+    __device__ __forceinline__ float operator()(float v) {
+        v = lanes_sum(v, lanes);
+        if (lanes <= 64u) return v;
+        float *slot = shared[half];
+        half ^= 1u;
+        if ((threadIdx.x & 63u) == 0u) slot[threadIdx.x >> 6] = v;
+        __syncthreads();
+        float total = 0.0f;
+        const uint32_t waves = lanes / 64u, first = in_block * waves;
+        for (uint32_t k = first; k < first + waves; ++k) total += slot[k];
+        return total;
+    }
+};
+template <int MAX_WAVES>
+struct GatedSum2 {
+    float (*shared)[2][MAX_WAVES];
+    uint32_t lanes, in_block;
+    uint32_t half = 0;
+    __device__ __forceinline__ void operator()(float &u, float &v) {
+        u = lanes_sum(u, lanes);
+        v = lanes_sum(v, lanes);
+        if (lanes <= 64u) return;
+        float (*slot)[MAX_WAVES] = shared[half];
+        half ^= 1u;
+        if ((threadIdx.x & 63u) == 0u) {
+            slot[0][threadIdx.x >> 6] = u;
+            slot[1][threadIdx.x >> 6] = v;
+        }
+        __syncthreads();
+        u = v = 0.0f;
+        const uint32_t waves = lanes / 64u, first = in_block * waves;
+        for (uint32_t k = first; k < first + waves; ++k) {
+            u += slot[0][k];
+            v += slot[1][k];
+        }
+    }
+};
+
+// The vectors of a lane's columns in LDS: [vector][half of a group][lane].
 struct Vectors {
     float4 *room;
     uint32_t lanes, lane;
-    __device__ __forceinline__ void keep(int vector, int p, const float (&v)[8]) const {
-        float4 *to = room + ((vector * 2 * PARTS + p) * lanes + lane);
+    __device__ __forceinline__ void keep(int vector, const float (&v)[8]) const {
+        float4 *to = room + vector * 2 * lanes + lane;
         to[0] = make_float4(v[0], v[1], v[2], v[3]);
-        to[PARTS * lanes] = make_float4(v[4], v[5], v[6], v[7]);
+        to[lanes] = make_float4(v[4], v[5], v[6], v[7]);
     }
-    __device__ __forceinline__ void get(float (&v)[8], int vector, int p) const {
-        const float4 *from = room + ((vector * 2 * PARTS + p) * lanes + lane);
-        const float4 a = from[0], b = from[PARTS * lanes];
+    __device__ __forceinline__ void get(float (&v)[8], int vector) const {
+        const float4 *from = room + vector * 2 * lanes + lane;
+        const float4 a = from[0], b = from[lanes];
         v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
         v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
     }
 };
 
-template <class T, int KIND, int PARTS, bool EVEN, int THREADS>
-__global__ __launch_bounds__(THREADS, 4) void gated_kernel(GatedForward a, uint32_t lanes, uint32_t run_blocks, bool rms,
+//
+// Four waves per SIMD; at six (80 registers) 16384 x 4096 bfloat16 takes 121 us
+// instead of 102, 8192 x 768 as long as at four (17.5 us a call).
+template <class T, int KIND, bool EVEN, int THREADS>
+__global__ __launch_bounds__(THREADS, kGatedWaves) void gated_kernel(GatedForward a, uint32_t lanes, uint32_t run_blocks, bool rms,
                                                            bool even) {
     using G = typename GateType<T, KIND>::type;
     extern __shared__ float4 room[];
     __shared__ float shared[2][THREADS / 64];
-    RowSum<THREADS / 64> row_sum{shared, lanes};
-    const uint32_t lane = threadIdx.x & (lanes - 1u), in_block = threadIdx.x / lanes, per_block = THREADS / lanes;
+    const uint32_t in_block = threadIdx.x / lanes, lane = threadIdx.x - in_block * lanes, per_block = blockDim.x / lanes;
     const float width = (float)a.width;
-    const Vectors<PARTS> vectors{room, lanes, lane};
-    Columns at[PARTS];
-#pragma unroll
-    for (int p = 0; p < PARTS; ++p) at[p] = Columns(((uint32_t)p * lanes + lane) * kGroup, a.width);
+    GatedSum<THREADS / 64> row_sum{shared, lanes, in_block};
+    const Vectors vectors{room, lanes, lane};
+    const Columns at(lane * kGroup, a.width);
+    const uint32_t c = at.column;
     // Rows of one run; with gates of their own all rows are one.
     const uint32_t run = blockIdx.x / run_blocks;
     const uint64_t count = KIND == kFolded ? a.gate.run : a.rows, before = run * count;
     const uint64_t stride = (uint64_t)run_blocks * per_block;
     uint64_t r = (uint64_t)(blockIdx.x % run_blocks) * per_block + in_block;
-    Raw8<T> x[PARTS], residual[PARTS];
-    Raw8<G> gate[PARTS];
+    const bool mine = c < a.width;
+    Raw8<T> x, residual;
+    Raw8<G> gate;
     const auto fetch = [&](uint64_t which) {
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
-            if (which >= count || at[p].column >= a.width) continue;
-            const uint64_t base = (before + which) * a.width;
-            load8<T, false>(x[p], a.x, base + at[p].column);
-            load8<T, false>(residual[p], a.residual, base + at[p].column);
-            if constexpr (KIND != kFolded)
-                load8<G, false>(gate[p], a.gate.at, a.gate.row(which) * a.width + at[p].column);
-        }
+        if (which >= count || !mine) return;
+        const uint64_t base = (before + which) * a.width;
+        load8<T, false>(x, a.x, base + c);
+        load8<T, false>(residual, a.residual, base + c);
+        if constexpr (KIND != kFolded) load8<G, false>(gate, a.gate.at, a.gate.row(which) * a.width + c);
     };
     fetch(r);
-    // Vector v of part p: the first norm's weight and bias, times a shared gate, the second's.
-    const auto vector = [&](float (&v)[8], int which, int p) {
-        uint32_t column = at[p].column;
+    // The vectors: the first norm's weight and bias, times a shared gate, the second's.
+    for (uint32_t which = in_block; which < 4u; which += per_block) {
+        float v[8];
+        uint32_t column = c;
         __asm__ volatile("" : "+v"(column));            // no addresses kept from one vector for the next
         const void *from[4] = {a.inner_weight, a.inner_bias, a.weight, a.bias};
         load_params(v, from[which], a.weight_dtype, column, a.width, which % 2 == 0 ? 1.0f : 0.0f);
@@ -164,74 +210,58 @@ __global__ __launch_bounds__(THREADS, 4) void gated_kernel(GatedForward a, uint3
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] *= g[k];
         }
-    };
-    for (uint32_t which = in_block; which < 4u; which += per_block)
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
-            float v[8];
-            vector(v, (int)which, p);
-            vectors.keep((int)which, p, v);
-        }
+        vectors.keep((int)which, v);
+    }
     __syncthreads();
-    const auto norm = [&](float (&t)[PARTS][8], float &mean, float &rstd) {
+    const auto norm = [&](const float (&t)[8], float &mean, float &rstd) {
         mean = 0.0f;
         if (!rms) {
             float sum = 0.0f;
 #pragma unroll
-            for (int p = 0; p < PARTS; ++p)
-#pragma unroll
-                for (int k = 0; k < 8; ++k) sum = at[p].template has<EVEN>(k, a.width) ? sum + t[p][k] : sum;
+                for (int k = 0; k < 8; ++k) sum = at.template has<EVEN>(k, a.width) ? sum + t[k] : sum;
             mean = row_sum(sum) / width;
         }
         float squares = 0.0f;
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p)
-#pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const float d = t[p][k] - mean;
-                squares = at[p].template has<EVEN>(k, a.width) ? __builtin_fmaf(d, d, squares) : squares;
+                const float d = t[k] - mean;
+                squares = at.template has<EVEN>(k, a.width) ? __builtin_fmaf(d, d, squares) : squares;
             }
         rstd = 1.0f / __builtin_sqrtf(row_sum(squares) / width + a.eps);
     };
     for (uint64_t round = (uint64_t)(blockIdx.x % run_blocks) * per_block; round < count; round += stride) {
         const uint64_t base = (before + r) * a.width;
         const bool active = r < count;
-        float t[PARTS][8];
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) widen8<T>(t[p], x[p]);
+        float t[8];
+        widen8<T>(t, x);
         float inner_mean, inner_rstd, mean, rstd;
         norm(t, inner_mean, inner_rstd);
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
+        {
             float u[8], b[8], add[8];
-            __builtin_amdgcn_sched_barrier(0);          // one part's vectors in registers at a time
-            vectors.get(u, 0, p);
-            vectors.get(b, 1, p);
-            widen8<T>(add, residual[p]);
+            vectors.get(u, 0);
+            vectors.get(b, 1);
+            widen8<T>(add, residual);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) t[p][k] = __builtin_fmaf((t[p][k] - inner_mean) * inner_rstd, u[k], b[k]);
+            for (int k = 0; k < 8; ++k) t[k] = __builtin_fmaf((t[k] - inner_mean) * inner_rstd, u[k], b[k]);
             if constexpr (KIND != kFolded) {
                 float g[8];
-                widen8<G>(g, gate[p]);
+                widen8<G>(g, gate);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) t[p][k] *= g[k];
+                for (int k = 0; k < 8; ++k) t[k] *= g[k];
             }
 #pragma unroll
-            for (int k = 0; k < 8; ++k) t[p][k] = __builtin_fmaf(a.scale, add[k], t[p][k]);
+            for (int k = 0; k < 8; ++k) t[k] = __builtin_fmaf(a.scale, add[k], t[k]);
         }
         fetch(r + stride);
         norm(t, mean, rstd);
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
-            if (!active || at[p].column >= a.width) continue;
-            __builtin_amdgcn_sched_barrier(0);
-            store_row<T>(a.total, base + at[p].column, even, t[p]);
+        if (active && mine) {
+            store_row<T>(a.total, base + c, even, t);
             float w[8], b[8];
-            vectors.get(w, 2, p);
-            vectors.get(b, 3, p);
+            vectors.get(w, 2);
+            vectors.get(b, 3);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) t[p][k] = __builtin_fmaf((t[p][k] - mean) * rstd, w[k], b[k]);
-            store_row<T>(a.y, base + at[p].column, even, t[p]);
+            for (int k = 0; k < 8; ++k) t[k] = __builtin_fmaf((t[k] - mean) * rstd, w[k], b[k]);
+            store_row<T>(a.y, base + c, even, t);
         }
         if (active && lane == 0u && a.rstd != nullptr) {
             a.inner_rstd[before + r] = inner_rstd;
@@ -249,15 +279,22 @@ __global__ __launch_bounds__(THREADS, 4) void gated_kernel(GatedForward a, uint3
 // lane's columns stay in registers over all rows of the workgroup, which are
 // of one run; rows that share a workgroup are joined at the end, in order, and
 // each workgroup writes one row of partial sums for each.
+//
+// Waves per SIMD: float32, and a gate of the rows' own, take more than the 128
+// registers of four (with four, 5003 x 1001 float32 with such gates 70 us, with
+// two 46; 8192 x 2048 bfloat16 84 and 65, float32 with a shared one 119 and 91).
+static constexpr uint32_t gated_backward_waves(int32_t dtype, int kind, uint32_t threads) {
+    return threads > (uint32_t)kRowThreads || (dtype != NT_F32 && kind == kFolded) ? 4u : 2u;
+}
 template <class T, int KIND, bool EVEN, int THREADS>
-__global__ __launch_bounds__(THREADS, 4) void gated_backward_kernel(GatedBackward a, uint32_t lanes, bool rms, bool even) {
+__global__ __launch_bounds__(THREADS, gated_backward_waves(T::code, KIND, THREADS)) void gated_backward_kernel(GatedBackward a, uint32_t lanes, bool rms, bool even) {
     using G = typename GateType<T, KIND>::type;
     extern __shared__ float4 room[];
     __shared__ float shared[2][2][THREADS / 64];
-    RowSum2<THREADS / 64> row_sum{shared, lanes};
-    const uint32_t lane = threadIdx.x & (lanes - 1u), in_block = threadIdx.x / lanes, per_block = THREADS / lanes;
+    const uint32_t in_block = threadIdx.x / lanes, lane = threadIdx.x - in_block * lanes, per_block = blockDim.x / lanes;
     const float width = (float)a.width;
-    const Vectors<1> vectors{room, lanes, lane};
+    GatedSum2<THREADS / 64> row_sum{shared, lanes, in_block};
+    const Vectors vectors{room, lanes, lane};
     const Columns at(lane * kGroup, a.width);
     const uint32_t c = at.column, run = blockIdx.x / a.run_blocks;
     const uint64_t count = KIND == kFolded ? a.gate.run : a.rows, before = run * count;
@@ -307,7 +344,7 @@ __global__ __launch_bounds__(THREADS, 4) void gated_backward_kernel(GatedBackwar
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] *= g[k];
         }
-        vectors.keep((int)which, 0, v);
+        vectors.keep((int)which, v);
     }
     __syncthreads();
     float sums[4][8];
@@ -322,7 +359,7 @@ __global__ __launch_bounds__(THREADS, 4) void gated_backward_kernel(GatedBackwar
         const float mean = next[0], rstd = next[1], inner_mean = next[2], inner_rstd = next[3];
         float g[8], h[8], w[8];
         float level = 0.0f, along = 0.0f;
-        vectors.get(w, 0, 0);
+        vectors.get(w, 0);
         widen8<T>(g, dy);
         widen8<T>(h, t);
 #pragma unroll
@@ -350,11 +387,11 @@ __global__ __launch_bounds__(THREADS, 4) void gated_backward_kernel(GatedBackwar
         if (active) store_row<T>(a.dresidual, base + c, even, w);
         level = along = 0.0f;
         widen8<T>(h, x);
-        vectors.get(w, 1, 0);
+        vectors.get(w, 1);
         if constexpr (KIND != kFolded) {
             float own[8], bias[8], by_gate[8];
             widen8<G>(own, gate);
-            vectors.get(bias, 2, 0);
+            vectors.get(bias, 2);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 h[k] = (h[k] - inner_mean) * inner_rstd;
@@ -392,8 +429,8 @@ __global__ __launch_bounds__(THREADS, 4) void gated_backward_kernel(GatedBackwar
         for (int v = 0; v < 4; ++v)
 #pragma unroll
             for (int k = 0; k < 8; ++k) sums[v][k] += __shfl_xor(sums[v][k], (int)off, 64);
-    const uint32_t span = lanes < 64u ? 64u : lanes, members = THREADS / span, member = threadIdx.x / span;
-    const uint32_t place = threadIdx.x & (span - 1u);
+    const uint32_t span = lanes < 64u ? 64u : lanes, members = blockDim.x / span, member = threadIdx.x / span;
+    const uint32_t place = threadIdx.x - member * span;
     for (uint32_t half = members / 2u; half > 0u; half >>= 1) {
         __syncthreads();                                // the vectors, or the last half, are read
         if (member >= half && member < 2u * half && place < lanes)
@@ -576,19 +613,20 @@ __global__ __launch_bounds__(kBlock) void gated_columns_kernel(GatedBackward a, 
     }
 }
 
-// The vectors' gradients from the partial sums: 32 columns and 32 slices a
-// workgroup.  Slices share out the runs, and where those are fewer, the blocks
+// The vectors' gradients from the partial sums: 16 columns and 64 slices a
+// workgroup, of one norm's two.  Slices share out the runs, and where those are fewer, the blocks
 // of each; a run's sums are joined before its gate, slices in order.
 struct GatedVectors {
     void *inner_weight, *inner_bias, *gate, *weight, *bias;     // each may be null
 };
-constexpr uint32_t kVectorColumns = 32, kVectorSlices = 32;
+constexpr uint32_t kVectorColumns = 16, kVectorSlices = 64;
 
 __global__ __launch_bounds__(kVectorColumns * kVectorSlices) void gated_vectors_kernel(GatedBackward a, GatedVectors to,
                                                                                         uint32_t runs, bool each) {
-    __shared__ float shared[4][kVectorSlices][kVectorColumns + 1];
+    __shared__ float shared[2][kVectorSlices][kVectorColumns + 1];
     const uint32_t column = threadIdx.x % kVectorColumns, slice = threadIdx.x / kVectorColumns;
     const uint32_t c = blockIdx.x * kVectorColumns + column;
+    const bool inner = blockIdx.y == 0u;                    // the first norm's two sums, or the second's
     const uint64_t line = a.width, block = 4u * line;
     const bool there = c < a.width;
     const float u = there ? load_param(a.inner_weight, a.weight_dtype, c, 1.0f) : 0.0f;
@@ -596,19 +634,22 @@ __global__ __launch_bounds__(kVectorColumns * kVectorSlices) void gated_vectors_
     uint32_t subs = kVectorSlices;
     while (subs > 1u && kVectorSlices / subs < runs) subs >>= 1;
     const uint32_t at_once = kVectorSlices / subs, sub = slice % subs;
-    float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float sums[2] = {0.0f, 0.0f};
     for (uint32_t first = 0; first < runs; first += at_once) {
         const uint32_t run = first + slice / subs;
         float own[2] = {0.0f, 0.0f};
         if (there && run < runs) {
-            const float *from = a.partials + run * (uint64_t)a.run_blocks * block + c;
-#pragma unroll 4
+            const float *from = a.partials + run * (uint64_t)a.run_blocks * block + c + (inner ? 0u : 2u * line);
+#pragma unroll 8
             for (uint32_t b = sub; b < a.run_blocks; b += subs) {
                 own[0] += from[b * block];
                 own[1] += from[b * block + line];
-                sums[2] += from[b * block + 2u * line];
-                sums[3] += from[b * block + 3u * line];
             }
+        }
+        if (!inner) {
+            sums[0] += own[0];
+            sums[1] += own[1];
+            continue;
         }
         if (subs > 1u) {
             __syncthreads();
@@ -629,12 +670,14 @@ __global__ __launch_bounds__(kVectorColumns * kVectorSlices) void gated_vectors_
         sums[1] = __builtin_fmaf(gate, own[1], sums[1]);
     }
     __syncthreads();
-    for (int v = 0; v < 4; ++v) shared[v][slice][column] = sums[v];
+    shared[0][slice][column] = sums[0];
+    shared[1][slice][column] = sums[1];
     __syncthreads();
-    if (slice >= 4u || !there) return;
+    if (slice >= 2u || !there) return;
     float sum = 0.0f;
+#pragma unroll 8
     for (uint32_t s = 0; s < kVectorSlices; ++s) sum += shared[slice][s][column];
-    void *out = slice == 0u ? to.inner_weight : slice == 1u ? to.inner_bias : slice == 2u ? to.weight : to.bias;
+    void *out = inner ? (slice == 0u ? to.inner_weight : to.inner_bias) : slice == 0u ? to.weight : to.bias;
     if (out != nullptr) store_param(out, a.weight_dtype, c, sum);
 }
 
@@ -642,15 +685,14 @@ __global__ __launch_bounds__(kVectorColumns * kVectorSlices) void gated_vectors_
 constexpr uint32_t kMostBlocks = 8192;
 constexpr uint32_t kRunGroups = 256;                    // groups of rows of the column sums of long rows, over all runs
 constexpr uint64_t kMostWidth = 1ull << 24;
-constexpr uint32_t kGatedWaves = 4;                     // per SIMD, which the registers leave room for
-constexpr uint32_t kLdsColumns = 8192;                  // whose vectors fit in LDS
 // A shared gate's runs of fewer rows than this many workgroups hold at a time
 // are taken as gates of the rows' own: each run's workgroups load the vectors.
 constexpr uint32_t kShortRun = 4;
 
 // Workgroups of each run: as many as are resident, where there are rows for them.
-static uint32_t run_blocks_of(uint64_t run, uint64_t runs, uint32_t per_block, uint32_t threads) {
-    const uint64_t most = std::max<uint64_t>(1u, kSimds * kGatedWaves * 64u / threads / runs);
+static uint32_t run_blocks_of(uint64_t run, uint64_t runs, const RowTiling &g, uint32_t waves) {
+    const uint64_t most = std::max<uint64_t>(1u, kSimds * waves * 64u / g.threads / runs);
+    const uint32_t per_block = g.threads / g.lanes;
     return (uint32_t)std::min<uint64_t>((run + per_block - 1) / per_block, most);
 }
 
@@ -662,44 +704,33 @@ static int gate_kind(const GatedForward &a, int32_t dtype, uint32_t per_block, u
     return a.gate.dtype == dtype ? kOwn : kOwnFloat;
 }
 
-// A group a lane: the tiling of the backward pass, and of rows that are not
-// whole groups (whose predicates of two or three groups do not fit in the
-// scalar registers).
-static RowTiling single_tiling(uint32_t width) {
+// A group a lane: a power of two of lanes up to 32, then whole waves, and as
+// many rows (a power of two of them) as fit in 512 lanes, or one.  No parts:
+// rows that the tilings do not take.
+static RowTiling gated_tiling(uint32_t width) {
     const uint32_t groups = (width + kGroup - 1) / kGroup;
-    uint32_t lanes = 1;
-    while (lanes < groups) lanes <<= 1;
-    if (width < kGroup || lanes > (uint32_t)kWideThreads) return RowTiling{0, 0, 0};
-    return RowTiling{lanes, 1, uint32_t(lanes <= (uint32_t)kRowThreads ? kRowThreads : kWideThreads)};
+    if (width < kGroup || groups > (uint32_t)kWideThreads) return RowTiling{0, 0, 0};
+    uint32_t lanes = 1, rows = 1;
+    while (lanes < groups && lanes < 64u) lanes <<= 1;
+    if (groups > 64u) lanes = (groups + 63u) / 64u * 64u;
+    while (lanes * rows * 2u <= (uint32_t)kRowThreads) rows <<= 1;
+    return RowTiling{lanes, 1, lanes * rows};
 }
 
-template <class T, int KIND, int PARTS, bool EVEN, int THREADS>
-static void launch_gated_tiled(const GatedForward &a, const RowTiling &g, uint64_t runs, bool rms, bool aligned,
-                               hipStream_t s) {
-    const uint32_t blocks = run_blocks_of(a.rows / runs, runs, g.threads / g.lanes, g.threads);
+template <class T, int KIND, int THREADS>
+static void launch_gated_tiled(const GatedForward &a, const RowTiling &g, uint64_t runs, bool rms, hipStream_t s) {
+    const bool aligned = aligned16({a.total, a.y});
+    const uint32_t blocks = run_blocks_of(a.rows / runs, runs, g, kGatedWaves);
     const dim3 grid((unsigned)(runs * blocks));
-    gated_kernel<T, KIND, PARTS, EVEN, THREADS>
-        <<<grid, dim3(THREADS), g.lanes * g.parts * kGroup * 16u, s>>>(a, g.lanes, blocks, rms, aligned);
-}
-
-template <class T, int KIND, bool EVEN>
-static void launch_gated_kind(const GatedForward &a, const RowTiling &g, uint64_t runs, bool rms, bool aligned,
-                              hipStream_t s) {
-    if (g.threads == (uint32_t)kWideThreads) {
-        launch_gated_tiled<T, KIND, 1, EVEN, kWideThreads>(a, g, runs, rms, aligned, s);
-    } else if (g.parts == 1) {
-        launch_gated_tiled<T, KIND, 1, EVEN, kRowThreads>(a, g, runs, rms, aligned, s);
-    } else if constexpr (EVEN && T::code != NT_F32) {
-        if (g.parts == 2) launch_gated_tiled<T, KIND, 2, EVEN, kRowThreads>(a, g, runs, rms, aligned, s);
-        else launch_gated_tiled<T, KIND, 3, EVEN, kRowThreads>(a, g, runs, rms, aligned, s);
-    }
+    const uint32_t room = g.lanes * kGroup * 16u;
+    if (a.width % kGroup == 0)
+        gated_kernel<T, KIND, true, THREADS><<<grid, dim3(g.threads), room, s>>>(a, g.lanes, blocks, rms, aligned);
+    else gated_kernel<T, KIND, false, THREADS><<<grid, dim3(g.threads), room, s>>>(a, g.lanes, blocks, rms, aligned);
 }
 
 template <class T>
 static void launch_gated(const GatedForward &a, bool rms, hipStream_t s) {
-    const bool even = a.width % kGroup == 0, aligned = aligned16({a.total, a.y});
-    RowTiling g = even ? forward_tiling(a.rows, a.width, T::code) : single_tiling(a.width);
-    if (g.lanes * g.parts * kGroup > kLdsColumns) g = single_tiling(a.width);
+    const RowTiling g = gated_tiling(a.width);
     if (g.parts == 0) {
         const dim3 grid((unsigned)std::min<uint64_t>(a.rows, kMostBlocks));
         if (rms) gated_rows_kernel<T, true><<<grid, dim3(kBlock), 0, s>>>(a);
@@ -709,8 +740,9 @@ static void launch_gated(const GatedForward &a, bool rms, hipStream_t s) {
     uint64_t runs = 1;
     const int kind = gate_kind(a, T::code, g.threads / g.lanes, runs);
     const auto launch = [&](auto k) {
-        if (even) launch_gated_kind<T, decltype(k)::value, true>(a, g, runs, rms, aligned, s);
-        else launch_gated_kind<T, decltype(k)::value, false>(a, g, runs, rms, aligned, s);
+        constexpr int KIND = decltype(k)::value;
+        if (g.threads > (uint32_t)kRowThreads) launch_gated_tiled<T, KIND, kWideThreads>(a, g, runs, rms, s);
+        else launch_gated_tiled<T, KIND, kRowThreads>(a, g, runs, rms, s);
     };
     if (kind == kFolded) launch(std::integral_constant<int, kFolded>{});
     else if (kind == kOwn) launch(std::integral_constant<int, kOwn>{});
@@ -723,20 +755,20 @@ static void launch_gated_backward_tiled(const GatedBackward &a, const RowTiling 
     const bool aligned = aligned16({a.dx, a.dresidual, a.dgate});
     // The vectors, or half of the rows that are joined.
     const uint32_t span = g.lanes < 64u ? 64u : g.lanes;
-    const uint32_t room = std::max(g.lanes * kGroup * (KIND == kFolded ? 8u : 12u), THREADS / span / 2u * g.lanes * 128u);
+    const uint32_t room = std::max(g.lanes * kGroup * (KIND == kFolded ? 8u : 12u), g.threads / span / 2u * g.lanes * 128u);
     if (a.width % kGroup == 0)
-        gated_backward_kernel<T, KIND, true, THREADS><<<dim3(groups), dim3(THREADS), room, s>>>(a, g.lanes, rms, aligned);
+        gated_backward_kernel<T, KIND, true, THREADS><<<dim3(groups), dim3(g.threads), room, s>>>(a, g.lanes, rms, aligned);
     else
-        gated_backward_kernel<T, KIND, false, THREADS><<<dim3(groups), dim3(THREADS), room, s>>>(a, g.lanes, rms, aligned);
+        gated_backward_kernel<T, KIND, false, THREADS><<<dim3(groups), dim3(g.threads), room, s>>>(a, g.lanes, rms, aligned);
 }
 
 template <class T>
 static void launch_gated_backward(const GatedBackward &a, bool rms, bool each, uint32_t groups, hipStream_t s) {
-    const RowTiling g = single_tiling(a.width);
+    const RowTiling g = gated_tiling(a.width);
     if (g.parts != 0) {
         const auto launch = [&](auto kind) {
             constexpr int KIND = decltype(kind)::value;
-            if (g.threads == (uint32_t)kWideThreads) launch_gated_backward_tiled<T, KIND, kWideThreads>(a, g, rms, groups, s);
+            if (g.threads > (uint32_t)kRowThreads) launch_gated_backward_tiled<T, KIND, kWideThreads>(a, g, rms, groups, s);
             else launch_gated_backward_tiled<T, KIND, kRowThreads>(a, g, rms, groups, s);
         };
         if (!each) launch(std::integral_constant<int, kFolded>{});
@@ -863,8 +895,8 @@ int32_t nt_norm_gate_add_norm_backward(int32_t device, const void *dy, const voi
                     {gate, gate_dtype, (uint32_t)gate_runs, rows / gate_runs}, inner_mean, inner_rstd, mean, rstd,
                     dx, dresidual, each ? dgate : nullptr, nullptr, nullptr, rows, (uint32_t)width, weight_dtype,
                     residual_scale, 1};
-    const RowTiling tiling = single_tiling((uint32_t)width);
-    a.run_blocks = tiling.parts != 0 ? run_blocks_of(rows / runs, runs, tiling.threads / tiling.lanes, tiling.threads)
+    const RowTiling tiling = gated_tiling((uint32_t)width);
+    a.run_blocks = tiling.parts != 0 ? run_blocks_of(rows / runs, runs, tiling, gated_backward_waves(dtype, each ? kOwn : kFolded, tiling.threads))
                                      : (uint32_t)std::min<uint64_t>(rows / runs, std::max(1u, kRunGroups / runs));
     Workspace room;
     if (tiling.parts == 0) room.want(&a.row_sums, 2u * rows);
@@ -878,7 +910,7 @@ int32_t nt_norm_gate_add_norm_backward(int32_t device, const void *dy, const voi
         default: launch_gated_backward<TBF16>(a, rms, each, groups, s); break;
     }
     const GatedVectors vectors{dinner_weight, dinner_bias, each ? nullptr : dgate, dweight, dbias};
-    gated_vectors_kernel<<<dim3((unsigned)((width + kVectorColumns - 1) / kVectorColumns)),
+    gated_vectors_kernel<<<dim3((unsigned)((width + kVectorColumns - 1) / kVectorColumns), 2),
                            dim3(kVectorColumns * kVectorSlices), 0, s>>>(a, vectors, runs, each);
     return hip_check(hipGetLastError(), "gated norm backward launch");
 }
