@@ -467,48 +467,101 @@ __global__ __launch_bounds__(THREADS, gated_backward_waves(T::code, KIND, THREAD
 }
 
 // ---- rows of any width: a workgroup a row ----------------------------------------------------------
+// Rows of less than eight elements or more than 8192: a workgroup goes over the
+// row once for each statistic, eight elements a lane, from the caches; a lane's
+// share is added in 64 bits, since its chain grows with the row.
+constexpr int kLongThreads = 512;
+
+// Elements [c, c + 8) of an array from element `row` on; what lies past the width reads as zero.
 template <class T>
-__device__ __forceinline__ float total_of(const GatedForward &a, uint64_t base, uint64_t gate_row, uint32_t c, float mean,
-                                          float rstd) {
-    const float x = load1<T>(reinterpret_cast<const typename T::raw *>(a.x), base + c);
-    const float n = __builtin_fmaf((x - mean) * rstd, load_param(a.inner_weight, a.weight_dtype, c, 1.0f),
-                                   load_param(a.inner_bias, a.weight_dtype, c, 0.0f));
-    const float gate = load_param(a.gate.at, a.gate.dtype, gate_row * a.width + c, 1.0f);
-    const float r = load1<T>(reinterpret_cast<const typename T::raw *>(a.residual), base + c);
-    return __builtin_fmaf(gate, n, a.scale * r);
+__device__ __forceinline__ void long_load(float (&out)[8], const void *base, uint64_t row, uint32_t c, uint32_t width) {
+    Raw8<T> raw;
+    if (c + kGroup <= width) load8<T, false>(raw, base, row + c);
+    else load_end<T>(raw, base, row + c, width - c);
+    widen8<T>(out, raw);
+}
+template <class T>
+__device__ __forceinline__ void long_store(void *base, uint64_t row, uint32_t c, uint32_t width, const float (&v)[8]) {
+    Raw8<T> raw;
+    narrow8<T>(raw, v);
+    if (c + kGroup <= width) store8<T, false>(base, row + c, raw);
+    else store_end<T>(base, row + c, raw, width - c);
+}
+__device__ __forceinline__ void long_gate(float (&out)[8], const Gate &gate, uint64_t row, uint32_t c, uint32_t width) {
+    if (gate.at == nullptr) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) out[k] = 1.0f;
+    } else if (gate.dtype == NT_F32) {
+        long_load<TF32>(out, gate.at, row, c, width);
+    } else if (gate.dtype == NT_F16) {
+        long_load<TF16>(out, gate.at, row, c, width);
+    } else {
+        long_load<TBF16>(out, gate.at, row, c, width);
+    }
+}
+template <class F>
+__device__ __forceinline__ void long_groups(uint32_t width, F &&use) {
+    for (uint32_t c = threadIdx.x * kGroup; c < width; c += kLongThreads * kGroup) use(c);
+}
+
+template <class T>
+__device__ __forceinline__ void total_of(float (&t)[8], const GatedForward &a, uint64_t base, uint64_t gate_row, uint32_t c,
+                                         float mean, float rstd) {
+    float u[8], k[8], gate[8], r[8];
+    long_load<T>(t, a.x, base, c, a.width);
+    load_params(u, a.inner_weight, a.weight_dtype, c, a.width, 1.0f);
+    load_params(k, a.inner_bias, a.weight_dtype, c, a.width, 0.0f);
+    long_gate(gate, a.gate, gate_row, c, a.width);
+    long_load<T>(r, a.residual, base, c, a.width);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        t[e] = __builtin_fmaf(gate[e], __builtin_fmaf((t[e] - mean) * rstd, u[e], k[e]), a.scale * r[e]);
 }
 
 template <class T, bool RMS>
-__global__ __launch_bounds__(kBlock) void gated_rows_kernel(GatedForward a) {
-    __shared__ double shared[kBlock / 64];
+__global__ __launch_bounds__(kLongThreads) void gated_rows_kernel(GatedForward a) {
+    __shared__ double shared[kLongThreads / 64];
     const float width = (float)a.width;
-    const auto *x = reinterpret_cast<const typename T::raw *>(a.x);
     for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const uint64_t base = row * a.width, gate_row = a.gate.row(row);
+        const uint64_t base = row * a.width, gate_row = a.gate.row(row) * a.width;
         float means[2] = {0.0f, 0.0f}, rstds[2];
-        const auto value = [&](int which, uint32_t c) {
-            return which == 0 ? load1<T>(x, base + c) : total_of<T>(a, base, gate_row, c, means[0], rstds[0]);
+        const auto value = [&](float (&t)[8], int which, uint32_t c) {
+            if (which == 0) long_load<T>(t, a.x, base, c, a.width);
+            else total_of<T>(t, a, base, gate_row, c, means[0], rstds[0]);
         };
         for (int which = 0; which < 2; ++which) {
             if constexpr (!RMS) {
                 double sum = 0.0;
-                for (uint32_t c = threadIdx.x; c < a.width; c += kBlock) sum += value(which, c);
+                long_groups(a.width, [&](uint32_t c) {
+                    float t[8];
+                    value(t, which, c);
+#pragma unroll
+                    for (uint32_t k = 0; k < 8; ++k) sum += c + k < a.width ? t[k] : 0.0f;
+                });
                 means[which] = block_total(sum, shared) / width;
             }
             double squares = 0.0;
-            for (uint32_t c = threadIdx.x; c < a.width; c += kBlock) {
-                const float d = value(which, c) - means[which];
-                squares = __builtin_fma((double)d, (double)d, squares);
-            }
+            long_groups(a.width, [&](uint32_t c) {
+                float t[8];
+                value(t, which, c);
+#pragma unroll
+                for (uint32_t k = 0; k < 8; ++k) {
+                    const float d = c + k < a.width ? t[k] - means[which] : 0.0f;
+                    squares = __builtin_fma((double)d, (double)d, squares);
+                }
+            });
             rstds[which] = 1.0f / __builtin_sqrtf(block_total(squares, shared) / width + a.eps);
         }
-        for (uint32_t c = threadIdx.x; c < a.width; c += kBlock) {
-            const float t = value(1, c);
-            store1<T>(reinterpret_cast<typename T::raw *>(a.total), base + c, t);
-            store1<T>(reinterpret_cast<typename T::raw *>(a.y), base + c,
-                      __builtin_fmaf((t - means[1]) * rstds[1], load_param(a.weight, a.weight_dtype, c, 1.0f),
-                                     load_param(a.bias, a.weight_dtype, c, 0.0f)));
-        }
+        long_groups(a.width, [&](uint32_t c) {
+            float t[8], w[8], b[8];
+            value(t, 1, c);
+            long_store<T>(a.total, base, c, a.width, t);
+            load_params(w, a.weight, a.weight_dtype, c, a.width, 1.0f);
+            load_params(b, a.bias, a.weight_dtype, c, a.width, 0.0f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t[k] = __builtin_fmaf((t[k] - means[1]) * rstds[1], w[k], b[k]);
+            long_store<T>(a.y, base, c, a.width, t);
+        });
         if (threadIdx.x == 0 && a.rstd != nullptr) {
             a.inner_rstd[row] = rstds[0];
             a.rstd[row] = rstds[1];
@@ -520,109 +573,150 @@ __global__ __launch_bounds__(kBlock) void gated_rows_kernel(GatedForward a) {
     }
 }
 
-// dt of an element, from its row's sums of g and g h over W.
+// dt of a group, and of the second norm dy and its normalized input, from the row's sums of g and g h over W.
 template <class T>
-__device__ __forceinline__ float total_grad(const GatedBackward &a, uint64_t base, uint32_t c, float mean, float rstd,
-                                            float level, float along) {
-    const float g = load1<T>(reinterpret_cast<const typename T::raw *>(a.dy), base + c) *
-                    load_param(a.weight, a.weight_dtype, c, 1.0f);
-    const float h = (load1<T>(reinterpret_cast<const typename T::raw *>(a.t), base + c) - mean) * rstd;
-    const float dt = rstd * (g - level - h * along);
-    return a.dtotal == nullptr ? dt : dt + load1<T>(reinterpret_cast<const typename T::raw *>(a.dtotal), base + c);
+__device__ __forceinline__ void total_grad(float (&dt)[8], float (&dy)[8], float (&h)[8], const GatedBackward &a,
+                                           uint64_t base, uint32_t c, float mean, float rstd, float level, float along) {
+    float w[8];
+    long_load<T>(dy, a.dy, base, c, a.width);
+    long_load<T>(h, a.t, base, c, a.width);
+    load_params(w, a.weight, a.weight_dtype, c, a.width, 1.0f);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        h[k] = (h[k] - mean) * rstd;
+        dt[k] = rstd * (dy[k] * w[k] - level - h[k] * along);
+    }
+    if (a.dtotal == nullptr) return;
+    float add[8];
+    long_load<T>(add, a.dtotal, base, c, a.width);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) dt[k] += add[k];
 }
 
 template <class T, bool RMS>
-__global__ __launch_bounds__(kBlock) void gated_rows_backward_kernel(GatedBackward a) {
-    __shared__ double shared[kBlock / 64];
+__global__ __launch_bounds__(kLongThreads) void gated_rows_backward_kernel(GatedBackward a) {
+    __shared__ double shared[kLongThreads / 64];
     const float width = (float)a.width;
-    const auto *dy = reinterpret_cast<const typename T::raw *>(a.dy);
-    const auto *t = reinterpret_cast<const typename T::raw *>(a.t);
-    const auto *x = reinterpret_cast<const typename T::raw *>(a.x);
-    const bool each = a.dgate != nullptr && a.gate.runs == a.rows;
+    const bool each = a.dgate != nullptr;
     for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const uint64_t base = row * a.width, gate_row = a.gate.row(row) * a.width;
         const float mean = RMS ? 0.0f : a.mean[row], rstd = a.rstd[row];
         const float inner_mean = RMS ? 0.0f : a.inner_mean[row], inner_rstd = a.inner_rstd[row];
         double levels = 0.0, alongs = 0.0;
-        for (uint32_t c = threadIdx.x; c < a.width; c += kBlock) {
-            const float g = load1<T>(dy, base + c) * load_param(a.weight, a.weight_dtype, c, 1.0f);
-            levels += g;
-            alongs = __builtin_fma((double)g, (double)((load1<T>(t, base + c) - mean) * rstd), alongs);
-        }
+        long_groups(a.width, [&](uint32_t c) {
+            float g[8], h[8], w[8];
+            long_load<T>(g, a.dy, base, c, a.width);
+            long_load<T>(h, a.t, base, c, a.width);
+            load_params(w, a.weight, a.weight_dtype, c, a.width, 1.0f);
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) {
+                g[k] = c + k < a.width ? g[k] * w[k] : 0.0f;
+                levels += g[k];
+                alongs = __builtin_fma((double)g[k], (double)((h[k] - mean) * rstd), alongs);
+            }
+        });
         const float along = block_total(alongs, shared) / width;
         const float level = RMS ? 0.0f : block_total(levels, shared) / width;
         if (threadIdx.x == 0) {
             a.row_sums[2 * row] = level;
             a.row_sums[2 * row + 1] = along;
         }
-        levels = alongs = 0.0;
-        const auto inner_grad = [&](uint32_t c, float dt) {
-            return dt * load_param(a.gate.at, a.gate.dtype, gate_row + c, 1.0f) *
-                   load_param(a.inner_weight, a.weight_dtype, c, 1.0f);
+        // dt and, of the first norm, its normalized input, its gradient by gate and weight.
+        const auto inner = [&](float (&dt)[8], float (&i)[8], float (&q)[8], float (&u)[8], uint32_t c) {
+            float dy[8], h[8], gate[8];
+            total_grad<T>(dt, dy, h, a, base, c, mean, rstd, level, along);
+            long_load<T>(i, a.x, base, c, a.width);
+            load_params(u, a.inner_weight, a.weight_dtype, c, a.width, 1.0f);
+            long_gate(gate, a.gate, gate_row, c, a.width);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                i[k] = (i[k] - inner_mean) * inner_rstd;
+                q[k] = dt[k] * gate[k] * u[k];
+            }
         };
-        for (uint32_t c = threadIdx.x; c < a.width; c += kBlock) {
-            const float q = inner_grad(c, total_grad<T>(a, base, c, mean, rstd, level, along));
-            levels += q;
-            alongs = __builtin_fma((double)q, (double)((load1<T>(x, base + c) - inner_mean) * inner_rstd), alongs);
-        }
+        levels = alongs = 0.0;
+        long_groups(a.width, [&](uint32_t c) {
+            float dt[8], i[8], q[8], u[8];
+            inner(dt, i, q, u, c);
+#pragma unroll
+            for (uint32_t k = 0; k < 8; ++k) {
+                q[k] = c + k < a.width ? q[k] : 0.0f;
+                levels += q[k];
+                alongs = __builtin_fma((double)q[k], (double)i[k], alongs);
+            }
+        });
         const float inner_along = block_total(alongs, shared) / width;
         const float inner_level = RMS ? 0.0f : block_total(levels, shared) / width;
-        for (uint32_t c = threadIdx.x; c < a.width; c += kBlock) {
-            const float dt = total_grad<T>(a, base, c, mean, rstd, level, along);
-            const float i = (load1<T>(x, base + c) - inner_mean) * inner_rstd;
-            store1<T>(reinterpret_cast<typename T::raw *>(a.dresidual), base + c, a.scale * dt);
-            store1<T>(reinterpret_cast<typename T::raw *>(a.dx), base + c,
-                      inner_rstd * (inner_grad(c, dt) - inner_level - i * inner_along));
+        long_groups(a.width, [&](uint32_t c) {
+            float dt[8], i[8], q[8], u[8];
+            inner(dt, i, q, u, c);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) q[k] = inner_rstd * (q[k] - inner_level - i[k] * inner_along);
+            long_store<T>(a.dx, base, c, a.width, q);
             if (each) {
-                const float n = __builtin_fmaf(i, load_param(a.inner_weight, a.weight_dtype, c, 1.0f),
-                                               load_param(a.inner_bias, a.weight_dtype, c, 0.0f));
-                store_param(a.dgate, a.gate.dtype, base + c, dt * n);
+                float bias[8];
+                load_params(bias, a.inner_bias, a.weight_dtype, c, a.width, 0.0f);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) q[k] = dt[k] * __builtin_fmaf(i[k], u[k], bias[k]);
+                if (a.gate.dtype == NT_F32) long_store<TF32>(a.dgate, base, c, a.width, q);
+                else if (a.gate.dtype == NT_F16) long_store<TF16>(a.dgate, base, c, a.width, q);
+                else long_store<TBF16>(a.dgate, base, c, a.width, q);
             }
-        }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) dt[k] *= a.scale;
+            long_store<T>(a.dresidual, base, c, a.width, dt);
+        });
     }
 }
 
-// The four column sums over a group of a run's rows, one column a lane.
+// The four column sums over a group of a run's rows, eight columns a lane.
 // Where each row has a gate of its own, dt is taken with it.
 template <class T, bool RMS>
-__global__ __launch_bounds__(kBlock) void gated_columns_kernel(GatedBackward a, uint32_t groups) {
-    const uint32_t c = blockIdx.x * kBlock + threadIdx.x;
+__global__ __launch_bounds__(kBlock) void gated_columns_kernel(GatedBackward a, uint32_t groups, bool each) {
+    const uint32_t c = (blockIdx.x * kBlock + threadIdx.x) * kGroup;
     if (c >= a.width) return;
-    const auto *dy = reinterpret_cast<const typename T::raw *>(a.dy);
-    const auto *t = reinterpret_cast<const typename T::raw *>(a.t);
-    const auto *x = reinterpret_cast<const typename T::raw *>(a.x);
-    const bool each = a.gate.at != nullptr && a.gate.runs == a.rows && a.rows > 1;
     const uint64_t run = each ? a.rows : a.gate.run;
     for (uint32_t group = blockIdx.y; group < groups; group += gridDim.y) {
         const uint64_t first = group / a.run_blocks * run;
-        float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        float sums[4][8] = {};
         for (uint64_t r = group % a.run_blocks; r < run; r += a.run_blocks) {
             const uint64_t row = first + r, base = row * a.width;
-            const float mean = RMS ? 0.0f : a.mean[row], rstd = a.rstd[row];
-            float dt = total_grad<T>(a, base, c, mean, rstd, a.row_sums[2 * row], a.row_sums[2 * row + 1]);
-            if (each) dt *= load_param(a.gate.at, a.gate.dtype, base + c, 1.0f);
-            const float i = (load1<T>(x, base + c) - (RMS ? 0.0f : a.inner_mean[row])) * a.inner_rstd[row];
-            const float g = load1<T>(dy, base + c);
-            sums[0] = __builtin_fmaf(dt, i, sums[0]);
-            sums[1] += dt;
-            sums[2] = __builtin_fmaf(g, (load1<T>(t, base + c) - mean) * rstd, sums[2]);
-            sums[3] += g;
+            float dt[8], dy[8], h[8], i[8];
+            total_grad<T>(dt, dy, h, a, base, c, RMS ? 0.0f : a.mean[row], a.rstd[row], a.row_sums[2 * row],
+                          a.row_sums[2 * row + 1]);
+            long_load<T>(i, a.x, base, c, a.width);
+            const float inner_mean = RMS ? 0.0f : a.inner_mean[row], inner_rstd = a.inner_rstd[row];
+            if (each) {
+                float gate[8];
+                long_gate(gate, a.gate, base, c, a.width);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) dt[k] *= gate[k];
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                sums[0][k] = __builtin_fmaf(dt[k], (i[k] - inner_mean) * inner_rstd, sums[0][k]);
+                sums[1][k] += dt[k];
+                sums[2][k] = __builtin_fmaf(dy[k], h[k], sums[2][k]);
+                sums[3][k] += dy[k];
+            }
         }
-        float *out = a.partials + group * 4ull * a.width + c;
-        for (int k = 0; k < 4; ++k) out[k * (uint64_t)a.width] = sums[k];
+        float *out = a.partials + group * 4ull * a.width;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) long_store<TF32>(out, (uint64_t)v * a.width, c, a.width, sums[v]);
     }
 }
 
 // The vectors' gradients from the partial sums: 16 columns and 64 slices a
-// workgroup, of one norm's two.  Slices share out the runs, and where those are fewer, the blocks
+// workgroup, of one norm's two; of 2048 columns and more 32 and 32 (512
+// workgroups' sums: 768 columns 8.7 and 12.5 us, 4096 17.1 and 13.7).  Slices share out the runs, and where those are fewer, the blocks
 // of each; a run's sums are joined before its gate, slices in order.
 struct GatedVectors {
     void *inner_weight, *inner_bias, *gate, *weight, *bias;     // each may be null
 };
-constexpr uint32_t kVectorColumns = 16, kVectorSlices = 64;
-
-__global__ __launch_bounds__(kVectorColumns * kVectorSlices) void gated_vectors_kernel(GatedBackward a, GatedVectors to,
+template <uint32_t kVectorColumns>
+__global__ __launch_bounds__(1024) void gated_vectors_kernel(GatedBackward a, GatedVectors to,
                                                                                         uint32_t runs, bool each) {
+    constexpr uint32_t kVectorSlices = 1024u / kVectorColumns;
     __shared__ float shared[2][kVectorSlices][kVectorColumns + 1];
     const uint32_t column = threadIdx.x % kVectorColumns, slice = threadIdx.x / kVectorColumns;
     const uint32_t c = blockIdx.x * kVectorColumns + column;
@@ -733,8 +827,8 @@ static void launch_gated(const GatedForward &a, bool rms, hipStream_t s) {
     const RowTiling g = gated_tiling(a.width);
     if (g.parts == 0) {
         const dim3 grid((unsigned)std::min<uint64_t>(a.rows, kMostBlocks));
-        if (rms) gated_rows_kernel<T, true><<<grid, dim3(kBlock), 0, s>>>(a);
-        else gated_rows_kernel<T, false><<<grid, dim3(kBlock), 0, s>>>(a);
+        if (rms) gated_rows_kernel<T, true><<<grid, dim3(kLongThreads), 0, s>>>(a);
+        else gated_rows_kernel<T, false><<<grid, dim3(kLongThreads), 0, s>>>(a);
         return;
     }
     uint64_t runs = 1;
@@ -777,11 +871,11 @@ static void launch_gated_backward(const GatedBackward &a, bool rms, bool each, u
         return;
     }
     const dim3 grid((unsigned)std::min<uint64_t>(a.rows, kMostBlocks));
-    const dim3 columns((a.width + kBlock - 1) / kBlock, std::min(groups, 65535u));
-    if (rms) gated_rows_backward_kernel<T, true><<<grid, dim3(kBlock), 0, s>>>(a);
-    else gated_rows_backward_kernel<T, false><<<grid, dim3(kBlock), 0, s>>>(a);
-    if (rms) gated_columns_kernel<T, true><<<columns, dim3(kBlock), 0, s>>>(a, groups);
-    else gated_columns_kernel<T, false><<<columns, dim3(kBlock), 0, s>>>(a, groups);
+    const dim3 columns((a.width + kBlock * kGroup - 1) / (kBlock * kGroup), std::min(groups, 65535u));
+    if (rms) gated_rows_backward_kernel<T, true><<<grid, dim3(kLongThreads), 0, s>>>(a);
+    else gated_rows_backward_kernel<T, false><<<grid, dim3(kLongThreads), 0, s>>>(a);
+    if (rms) gated_columns_kernel<T, true><<<columns, dim3(kBlock), 0, s>>>(a, groups, each);
+    else gated_columns_kernel<T, false><<<columns, dim3(kBlock), 0, s>>>(a, groups, each);
 }
 
 static int32_t check_gated(const char *entry, int32_t dtype, int32_t weight_dtype, bool has_params, const void *gate,
@@ -910,8 +1004,8 @@ int32_t nt_norm_gate_add_norm_backward(int32_t device, const void *dy, const voi
         default: launch_gated_backward<TBF16>(a, rms, each, groups, s); break;
     }
     const GatedVectors vectors{dinner_weight, dinner_bias, each ? nullptr : dgate, dweight, dbias};
-    gated_vectors_kernel<<<dim3((unsigned)((width + kVectorColumns - 1) / kVectorColumns), 2),
-                           dim3(kVectorColumns * kVectorSlices), 0, s>>>(a, vectors, runs, each);
+    if (width < 2048u) gated_vectors_kernel<16><<<dim3((a.width + 15u) / 16u, 2), dim3(1024), 0, s>>>(a, vectors, runs, each);
+    else gated_vectors_kernel<32><<<dim3((a.width + 31u) / 32u, 2), dim3(1024), 0, s>>>(a, vectors, runs, each);
     return hip_check(hipGetLastError(), "gated norm backward launch");
 }
 

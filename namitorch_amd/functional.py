@@ -454,16 +454,15 @@ def _gated(x, residual, normalized_shape, inner_weight, inner_bias, gate, weight
         reject_during_capture("Layer norm without out")
     y = _result(given[0], "output", x._shape, x._dtype, x)
     total = _result(given[1], "total", x._shape, x._dtype, x)
-    kept = [None] * 4
+    kept, at = (None,) * 4, (None,) * 4
     if stats:
-        for place, name in enumerate(("inner_mean", "inner_rstd", "mean", "rstd")):
-            if not rms or place % 2:
-                kept[place] = _result(given[2 + place], name, lead, float32, x)
+        kept = tuple(None if rms and place % 2 == 0 else _result(given[2 + place], name, lead, float32, x)
+                     for place, name in enumerate(("inner_mean", "inner_rstd", "mean", "rstd")))
+        at = tuple(None if k is None else k._ptr for k in kept)
     device = x._device.index
     _launch(_native.load().nt_norm_gate_add_norm(
         device, source, stream_in, x._dtype._code, vectors[0], vectors[1], gate_at, gate_code, gate_rows, vectors[2],
-        vectors[3], code, scale, eps, rms, total._ptr, y._ptr, *(None if k is None else k._ptr for k in kept), rows,
-        width, current_stream(device)), given)
+        vectors[3], code, scale, eps, rms, total._ptr, y._ptr, *at, rows, width, current_stream(device)), given)
     return (y, total, *kept)
 
 
@@ -520,12 +519,17 @@ def norm_gate_add_norm_backward(grad_output, grad_total, input, total, inner_mea
 
 def _vectors(values, shape: tuple, like: Tensor) -> tuple:
     """(addresses of the weights and biases, their dtype code)."""
-    names = ("inner_weight", "inner_bias", "weight", "bias")
-    at = [_affine(value, name, shape, like) for value, name in zip(values, names)]
-    kinds = {value._dtype for value in values if value is not None}
-    if len(kinds) > 1:
-        raise TypeError(f"weights and biases must have one dtype, got {' and '.join(sorted(k.name for k in kinds))}.")
-    return at, (kinds.pop() if kinds else like._dtype)._code
+    at, kind = [], None
+    for value, name in zip(values, ("inner_weight", "inner_bias", "weight", "bias")):
+        if value is None:
+            at.append(None)
+            continue
+        at.append(_affine(value, name, shape, like))
+        if kind is None:
+            kind = value._dtype
+        elif kind is not value._dtype:
+            raise TypeError(f"weights and biases must have one dtype, got {kind.name} and {value._dtype.name}.")
+    return at, (like._dtype if kind is None else kind)._code
 
 
 def _gate(value, lead: tuple, shape: tuple, like: Tensor) -> tuple:
@@ -551,9 +555,10 @@ def _gate(value, lead: tuple, shape: tuple, like: Tensor) -> tuple:
 
 
 def _scale(value) -> float:
-    if isinstance(value, bool) or not isinstance(value, Real):
-        raise TypeError("residual_scale must be a real number.")
-    value = float(value)
+    if type(value) is not float:
+        if isinstance(value, bool) or not isinstance(value, Real):
+            raise TypeError("residual_scale must be a real number.")
+        value = float(value)
     if not abs(value) <= _MOST_EPS:
         raise ValueError(f"residual_scale must be finite as a float32, got {value}.")
     return value
