@@ -381,18 +381,20 @@ struct FinishGrad {
     }
 };
 
-// A piece's part of dx, in float32: stored, or added to the pieces before.
+// Sums in float32 of a product that is split along k, or goes on with the next
+// piece of the vocabulary: stored, or added to those before.
 struct FinishSum {
     float *sums;                // [split][rows][width]
     uint64_t split_stride;
     uint32_t width;             // a multiple of 8
-    const uint32_t *live;
+    uint32_t rows;
+    const uint32_t *live;       // how many of the rows there are; or null, all
     bool add;
 
     template <class T>
     __device__ __forceinline__ void operator()(const f32x4 (&acc)[T::TP][T::TQ], uint32_t p_first, uint32_t q_first,
                                                uint32_t split, uint32_t lane) const {
-        const uint32_t count = *live, up = p_first + 4u * (lane >> 4);
+        const uint32_t count = live != nullptr ? *live : rows, up = p_first + 4u * (lane >> 4);
 #pragma unroll
         for (int j = 0; j < T::TQ; ++j) {
             const uint32_t q = q_first + 16u * j + (lane & 15u);
@@ -624,16 +626,17 @@ __global__ __launch_bounds__(kRowsBlock) void few_loss_kernel(const Partial2 *pa
 }
 
 // ---- dx -------------------------------------------------------------------------------------------------
-// dx from its sums, eight columns a lane; rows that are not counted are zero.
+// dx (or split rows of dW, with no `place`) from its sums, eight columns a
+// lane; rows that are not counted are zero.
 template <class T>
-__global__ __launch_bounds__(kBlock) void grad_input_kernel(const float *sums, uint64_t split_stride, uint32_t splits,
-                                                            uint32_t pitch, Rows rows, uint32_t all, uint32_t width,
-                                                            bool even, typename T::raw *dx) {
-    const float by = *rows.unscale;
+__global__ __launch_bounds__(kBlock) void grad_kernel(const float *sums, uint64_t split_stride, uint32_t splits,
+                                                      uint32_t pitch, const uint32_t *place, const float *unscale,
+                                                      uint32_t all, uint32_t width, bool even, typename T::raw *dx) {
+    const float by = *unscale;
     const uint32_t groups = (width + 7u) / 8u;
     const uint64_t items = all * (uint64_t)groups;
     for (uint64_t g = blockIdx.x * (uint64_t)kBlock + threadIdx.x; g < items; g += (uint64_t)gridDim.x * kBlock) {
-        const uint32_t i = (uint32_t)(g / groups), c = (uint32_t)(g % groups) * 8u, j = rows.place[i];
+        const uint32_t i = (uint32_t)(g / groups), c = (uint32_t)(g % groups) * 8u, j = place != nullptr ? place[i] : i;
         f32x4 v[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
         if (j != ~0u) {
             const float *from = sums + j * (uint64_t)pitch + c;
@@ -691,12 +694,20 @@ static void with_grads_tile(uint64_t rows, F &&launch) {
     else launch(Large{});
 }
 
-// Splits of dx's product along k, of which each tile has `steps`, beside
-// `other` steps of tiles: such that no workgroup has more than half of what
-// each compute unit gets, and at least four steps.
-static uint32_t splits_of(uint64_t tiles, uint32_t steps, uint64_t other) {
-    const uint64_t share = std::max<uint64_t>((tiles * steps + other) / (2u * kUnits), 4u);
-    return (uint32_t)std::max<uint64_t>(1u, (steps + share - 1) / share);
+// How the two products of dz are split along k.  dx: such that no workgroup has
+// more than half of what each compute unit gets, nor less than four steps.  dW,
+// whose tiles are many as a rule, likewise, but only where one would be longer
+// than twice that (11127 rows of 720 x 64 bfloat16 have three tiles of dW: a
+// call 251 us in one piece, 72 split; but 777 x 10007 x 1001 float32, 13 steps
+// beside 18 on each unit: 423 split, 362 not).
+struct Splits {
+    uint32_t input, weight;
+};
+static Splits splits_of(uint64_t input_tiles, uint32_t input_steps, uint64_t weight_tiles, uint32_t weight_steps) {
+    const uint64_t share =
+        std::max<uint64_t>((input_tiles * input_steps + weight_tiles * weight_steps) / (2u * kUnits), 4u);
+    const auto of = [&](uint32_t steps) { return (uint32_t)std::max<uint64_t>(1u, (steps + share - 1) / share); };
+    return Splits{of(input_steps), weight_steps > 4u * share ? of(weight_steps) : 1u};
 }
 
 struct Problem {
@@ -832,17 +843,17 @@ static int32_t backward_of(const Problem &a, int32_t device, const float *grad, 
     const uint32_t piece = piece_of(a, pitch, planes, pack_w, true);
     const uint32_t pieces = (a.classes + piece - 1) / piece;
     const uint32_t dz_pitch = whole_steps(piece);
-    uint32_t splits = 1;
+    Splits splits{1, 1};
     with_grads_tile(a.rows, [&](auto shape) {
         using Shape = decltype(shape);
         const uint32_t tiles_h = tiles_of(pitch, Shape::BP);
         splits = splits_of((uint64_t)tiles_h * tiles_of(a.rows, Shape::BQ), tiles_of(piece, kDepth),
-                           (uint64_t)tiles_h * tiles_of(piece, Shape::BQ) * tiles_of(a.rows, kDepth));
+                           (uint64_t)tiles_h * tiles_of(piece, Shape::BQ), tiles_of(a.rows, kDepth));
     });
 
     Rows rows{};
     uint16_t *px = nullptr, *pw = nullptr, *dz = nullptr;
-    float *sums = nullptr;
+    float *sums = nullptr, *weight_sums = nullptr;
     Workspace room;
     room.want(&rows.count, 1);
     room.want(&rows.unscale, 1);
@@ -856,7 +867,8 @@ static int32_t backward_of(const Problem &a, int32_t device, const float *grad, 
     if (pack_w) room.want(&pw, (uint64_t)planes * whole_steps(piece) * pitch);
     else if (ragged) room.want(&pw, (uint64_t)kDepth * pitch);
     room.want(&dz, (uint64_t)planes * padded * dz_pitch);
-    room.want(&sums, (uint64_t)splits * a.rows * pitch);
+    room.want(&sums, (uint64_t)splits.input * a.rows * pitch);
+    if (splits.weight > 1u) room.want(&weight_sums, (uint64_t)splits.weight * piece * pitch);
     int32_t rc = room.allocate(device, stream);
     if (rc != NT_OK) return rc;
 
@@ -899,32 +911,42 @@ static int32_t backward_of(const Problem &a, int32_t device, const float *grad, 
         Product input{};                    // dx[i][h] = sum over v of dz[i][v] W[v][h]
         input.p = Operand{w, ragged && k + 1u == pieces ? pw : nullptr, pitch, plane_w, pitch};
         input.q = Operand{dz, nullptr, line, plane_dz, a.rows};
-        input.splits = splits;
+        input.splits = splits.input;
         input.depth = line;
         input.live = rows.count;
-        const FinishSum sum{sums, (uint64_t)a.rows * pitch, pitch, rows.count, k > 0};
+        const FinishSum sum{sums, (uint64_t)a.rows * pitch, pitch, a.rows, rows.count, k > 0};
 
         Product weight{};                   // dW[v][h] = sum over i of dz[i][v] x[i][h]
         weight.p = Operand{px, nullptr, pitch, plane_x, pitch};
         weight.q = Operand{dz, nullptr, line, plane_dz, line};
-        weight.splits = 1;
+        weight.splits = splits.weight;
         weight.depth = a.rows;
         weight.live = rows.count;
         weight.live_depth = true;
         Raw *to = static_cast<Raw *>(dw) + (uint64_t)first * a.width;
-        const FinishWeight<T> last{to, rows.unscale, a.width, classes,
-                                   a.width % 8u == 0 && (uintptr_t)dw % 16u == 0};
+        const bool even_weight = a.width % 8u == 0 && (uintptr_t)dw % 16u == 0;
         with_grads_tile(a.rows, [&](auto shape) {
             using Shape = decltype(shape);
             input.tiles_p = weight.tiles_p = tiles_of(pitch, Shape::BP);
             input.tiles_q = tiles_of(a.rows, Shape::BQ);
             weight.tiles_q = tiles_of(classes, Shape::BQ);
-            launch_two_products<half, Shape, planes>(input, sum, weight, last, s);
+            if (weight_sums == nullptr) {
+                const FinishWeight<T> last{to, rows.unscale, a.width, classes, even_weight};
+                launch_two_products<half, Shape, planes>(input, sum, weight, last, s);
+            } else {
+                const FinishSum last{weight_sums, (uint64_t)piece * pitch, pitch, classes, nullptr, false};
+                launch_two_products<half, Shape, planes>(input, sum, weight, last, s);
+            }
         });
+        if (weight_sums != nullptr)
+            grad_kernel<T><<<blocks_of(classes * (uint64_t)((a.width + 7u) / 8u), kBlock), kBlock, 0, s>>>(
+                weight_sums, (uint64_t)piece * pitch, splits.weight, pitch, nullptr, rows.unscale, classes, a.width,
+                even_weight, to);
     }
     const bool even = a.width % 8u == 0 && (uintptr_t)dx % 16u == 0;
-    grad_input_kernel<T><<<blocks_of(a.rows * (uint64_t)((a.width + 7u) / 8u), kBlock), kBlock, 0, s>>>(
-        sums, (uint64_t)a.rows * pitch, splits, pitch, rows, a.rows, a.width, even, static_cast<Raw *>(dx));
+    grad_kernel<T><<<blocks_of(a.rows * (uint64_t)((a.width + 7u) / 8u), kBlock), kBlock, 0, s>>>(
+        sums, (uint64_t)a.rows * pitch, splits.input, pitch, rows.place, rows.unscale, a.rows, a.width, even,
+        static_cast<Raw *>(dx));
     return hip_check(hipGetLastError(), "linear cross entropy backward launch");
 }
 

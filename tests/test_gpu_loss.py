@@ -360,6 +360,20 @@ def test_pieces_of_the_vocabulary(dtype, rows, classes, width):
         assert (got - exact).norm() <= 1.2 * share * (terms + exact.norm())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows, classes, width", [(2500, 90, 24), (1500, 700, 72), (4000, 5, 8), (3000, 300, 100)])
+def test_many_rows_of_few_classes(rows, classes, width, dtype):
+    """The weight's gradient is a few tiles of a long sum, which is split."""
+    x, weight, target = _problem(_rng(16, rows, classes), rows, classes, width, dtype)
+    at = _targets(target)
+    loss, lse = F.linear_cross_entropy_forward(x, weight, at)
+    _check_forward(loss, lse, _values(x), _values(weight), target, dtype)
+    dx, dw = F.linear_cross_entropy_backward(1.0, x, weight, at, lse)
+    _check_backward(dx, dw, 1.0, _values(x), _values(weight), target, _values(lse), dtype)
+    again = F.linear_cross_entropy_backward(1.0, x, weight, at, lse)
+    assert np.array_equal(dx.bits(), again[0].bits()) and np.array_equal(dw.bits(), again[1].bits())
+
+
 def test_streams():
     """Calls of two streams at once: each is what it is alone."""
     problems = [_problem(_rng(13, k), 300 + 50 * k, 2000, 256, "bfloat16") for k in range(2)]
