@@ -52,6 +52,7 @@ struct GatedForward {
     uint32_t width;
     int32_t weight_dtype;
     float scale, eps;
+    uint32_t first_block;       // of this launch
 };
 
 struct GatedBackward {
@@ -66,6 +67,7 @@ struct GatedBackward {
     int32_t weight_dtype;
     float scale;
     uint32_t run_blocks;        // workgroups, or groups of rows, of each run
+    uint32_t first_block;       // of this launch
 };
 
 // Sum of a value of 64 bits over the workgroup, as float32 on every lane.
@@ -180,10 +182,10 @@ __global__ __launch_bounds__(THREADS, kGatedWaves) void gated_kernel(GatedForwar
     const Columns at(lane * kGroup, a.width);
     const uint32_t c = at.column;
     // Rows of one run; with gates of their own all rows are one.
-    const uint32_t run = blockIdx.x / run_blocks;
+    const uint32_t block = a.first_block + blockIdx.x, run = block / run_blocks;
     const uint64_t count = KIND == kFolded ? a.gate.run : a.rows, before = run * count;
     const uint64_t stride = (uint64_t)run_blocks * per_block;
-    uint64_t r = (uint64_t)(blockIdx.x % run_blocks) * per_block + in_block;
+    uint64_t r = (uint64_t)(block % run_blocks) * per_block + in_block;
     const bool mine = c < a.width;
     Raw8<T> x, residual;
     Raw8<G> gate;
@@ -229,7 +231,7 @@ __global__ __launch_bounds__(THREADS, kGatedWaves) void gated_kernel(GatedForwar
             }
         rstd = 1.0f / __builtin_sqrtf(row_sum(squares) / width + a.eps);
     };
-    for (uint64_t round = (uint64_t)(blockIdx.x % run_blocks) * per_block; round < count; round += stride) {
+    for (uint64_t round = (uint64_t)(block % run_blocks) * per_block; round < count; round += stride) {
         const uint64_t base = (before + r) * a.width;
         const bool active = r < count;
         float t[8];
@@ -296,10 +298,10 @@ __global__ __launch_bounds__(THREADS, gated_backward_waves(T::code, KIND, THREAD
     GatedSum2<THREADS / 64> row_sum{shared, lanes, in_block};
     const Vectors vectors{room, lanes, lane};
     const Columns at(lane * kGroup, a.width);
-    const uint32_t c = at.column, run = blockIdx.x / a.run_blocks;
+    const uint32_t block = a.first_block + blockIdx.x, c = at.column, run = block / a.run_blocks;
     const uint64_t count = KIND == kFolded ? a.gate.run : a.rows, before = run * count;
     const uint64_t stride = (uint64_t)a.run_blocks * per_block;
-    uint64_t r = (uint64_t)(blockIdx.x % a.run_blocks) * per_block + in_block;
+    uint64_t r = (uint64_t)(block % a.run_blocks) * per_block + in_block;
     const bool mine = c < a.width;
     Raw8<T> dy, t, dtotal, x;
     Raw8<G> gate;
@@ -353,7 +355,7 @@ __global__ __launch_bounds__(THREADS, gated_backward_waves(T::code, KIND, THREAD
 #pragma unroll
         for (int k = 0; k < 8; ++k) sums[v][k] = 0.0f;
     const auto has = [&](int k) { return EVEN || at.template has<false>((uint32_t)k, a.width); };
-    for (uint64_t round = (uint64_t)(blockIdx.x % a.run_blocks) * per_block; round < count; round += stride) {
+    for (uint64_t round = (uint64_t)(block % a.run_blocks) * per_block; round < count; round += stride) {
         const uint64_t base = (before + r) * a.width;
         const bool active = r < count && mine;
         const float mean = next[0], rstd = next[1], inner_mean = next[2], inner_rstd = next[3];
@@ -451,7 +453,7 @@ __global__ __launch_bounds__(THREADS, gated_backward_waves(T::code, KIND, THREAD
             }
     }
     if (member != 0u || place >= lanes || !mine) return;
-    float *out = a.partials + blockIdx.x * 4ull * a.width;
+    float *out = a.partials + block * 4ull * a.width;
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
         if (at.first == 0u && c + kGroup <= a.width) {
@@ -811,15 +813,25 @@ static RowTiling gated_tiling(uint32_t width) {
     return RowTiling{lanes, 1, lanes * rows};
 }
 
+// Calls launch(grid, args) for all blocks, below 2**32 work-items at a time.
+template <class Args, class F>
+static void in_launches(Args a, uint64_t blocks, F &&launch) {
+    constexpr uint64_t most = 1ull << 21;               // of at most 1024 lanes
+    for (uint64_t first = 0; first < blocks; first += most) {
+        a.first_block = (uint32_t)first;
+        launch(dim3((unsigned)std::min(most, blocks - first)), a);
+    }
+}
+
 template <class T, int KIND, int THREADS>
-static void launch_gated_tiled(const GatedForward &a, const RowTiling &g, uint64_t runs, bool rms, hipStream_t s) {
-    const bool aligned = aligned16({a.total, a.y});
-    const uint32_t blocks = run_blocks_of(a.rows / runs, runs, g, kGatedWaves);
-    const dim3 grid((unsigned)(runs * blocks));
-    const uint32_t room = g.lanes * kGroup * 16u;
-    if (a.width % kGroup == 0)
-        gated_kernel<T, KIND, true, THREADS><<<grid, dim3(g.threads), room, s>>>(a, g.lanes, blocks, rms, aligned);
-    else gated_kernel<T, KIND, false, THREADS><<<grid, dim3(g.threads), room, s>>>(a, g.lanes, blocks, rms, aligned);
+static void launch_gated_tiled(const GatedForward &args, const RowTiling &g, uint64_t runs, bool rms, hipStream_t s) {
+    const bool aligned = aligned16({args.total, args.y});
+    const uint32_t blocks = run_blocks_of(args.rows / runs, runs, g, kGatedWaves), room = g.lanes * kGroup * 16u;
+    in_launches(args, runs * blocks, [&](dim3 grid, const GatedForward &a) {
+        if (a.width % kGroup == 0)
+            gated_kernel<T, KIND, true, THREADS><<<grid, dim3(g.threads), room, s>>>(a, g.lanes, blocks, rms, aligned);
+        else gated_kernel<T, KIND, false, THREADS><<<grid, dim3(g.threads), room, s>>>(a, g.lanes, blocks, rms, aligned);
+    });
 }
 
 template <class T>
@@ -844,16 +856,17 @@ static void launch_gated(const GatedForward &a, bool rms, hipStream_t s) {
 }
 
 template <class T, int KIND, int THREADS>
-static void launch_gated_backward_tiled(const GatedBackward &a, const RowTiling &g, bool rms, uint32_t groups,
+static void launch_gated_backward_tiled(const GatedBackward &args, const RowTiling &g, bool rms, uint32_t groups,
                                         hipStream_t s) {
-    const bool aligned = aligned16({a.dx, a.dresidual, a.dgate});
+    const bool aligned = aligned16({args.dx, args.dresidual, args.dgate});
     // The vectors, or half of the rows that are joined.
     const uint32_t span = g.lanes < 64u ? 64u : g.lanes;
     const uint32_t room = std::max(g.lanes * kGroup * (KIND == kFolded ? 8u : 12u), g.threads / span / 2u * g.lanes * 128u);
-    if (a.width % kGroup == 0)
-        gated_backward_kernel<T, KIND, true, THREADS><<<dim3(groups), dim3(g.threads), room, s>>>(a, g.lanes, rms, aligned);
-    else
-        gated_backward_kernel<T, KIND, false, THREADS><<<dim3(groups), dim3(g.threads), room, s>>>(a, g.lanes, rms, aligned);
+    in_launches(args, groups, [&](dim3 grid, const GatedBackward &a) {
+        if (a.width % kGroup == 0)
+            gated_backward_kernel<T, KIND, true, THREADS><<<grid, dim3(g.threads), room, s>>>(a, g.lanes, rms, aligned);
+        else gated_backward_kernel<T, KIND, false, THREADS><<<grid, dim3(g.threads), room, s>>>(a, g.lanes, rms, aligned);
+    });
 }
 
 template <class T>
@@ -931,7 +944,7 @@ int32_t nt_norm_gate_add_norm(int32_t device, const void *x, const void *residua
     const uint64_t runs = gate == nullptr ? 1u : gate_rows;
     const GatedForward a{x, residual, inner_weight, inner_bias, weight, bias,
                          {gate, gate_dtype, (uint32_t)runs, rows / runs}, total, y, inner_mean, inner_rstd, mean, rstd,
-                         rows, (uint32_t)width, weight_dtype, residual_scale, eps};
+                         rows, (uint32_t)width, weight_dtype, residual_scale, eps, 0};
     hipStream_t s = (hipStream_t)stream;
     switch (dtype) {
         case NT_F32: launch_gated<TF32>(a, rms != 0, s); break;
@@ -988,7 +1001,7 @@ int32_t nt_norm_gate_add_norm_backward(int32_t device, const void *dy, const voi
     GatedBackward a{dy, dtotal, x, total, inner_weight, inner_bias, weight,
                     {gate, gate_dtype, (uint32_t)gate_runs, rows / gate_runs}, inner_mean, inner_rstd, mean, rstd,
                     dx, dresidual, each ? dgate : nullptr, nullptr, nullptr, rows, (uint32_t)width, weight_dtype,
-                    residual_scale, 1};
+                    residual_scale, 1, 0};
     const RowTiling tiling = gated_tiling((uint32_t)width);
     a.run_blocks = tiling.parts != 0 ? run_blocks_of(rows / runs, runs, tiling, gated_backward_waves(dtype, each ? kOwn : kFolded, tiling.threads))
                                      : (uint32_t)std::min<uint64_t>(rows / runs, std::max(1u, kRunGroups / runs));
