@@ -6,8 +6,18 @@
 // Either operand lies in memory as [row][k] ("deep": k runs along a line) or
 // as [k][row].  A workgroup makes one tile of BP x BQ elements, in steps of 64
 // along k: a step's slices of both operands go straight from memory to LDS
-// while the slices before are multiplied, so there are two such rooms.  Sums
-// are float32 in the matrix cores' accumulators.
+// while the slices before are multiplied, so there are two rooms for them, or
+// three.  Sums are float32 in the matrix cores' accumulators.
+//
+// What bounds it: large products run at 1.15 to 1.25 PFLOP/s (8192 x 32000 x
+// 4096 bfloat16: 1.6 ms in each of the three layouts, where a library's plain
+// product of that size takes 1.61), the matrix cores busy 58 % of the cycles at
+// clocks that fall to 1.5 to 1.8 GHz under the load.  Tried and not kept: 32 x 32
+// instead of 16 x 16 instructions (1.70 to 1.83 ms), the two waves of a SIMD
+// taking turns at LDS and the matrix cores (1.77 to 1.95), four waves of 128 x 64
+// (2.2 to 2.4), workgroups that stride over tiles with the next one's first slice
+// on its way (spills), and steps in another order for each XCD (no difference).
+// Few rows are bound by the one read of the weights, at 4 to 5 TB/s.
 //
 // A 16-byte group of a slice does not lie where its place in memory says, but
 // with its index in the line changed by an exclusive or, so that the lanes
@@ -18,8 +28,8 @@
 // Float32 operands come as three bfloat16 planes whose sum they are (8 + 8 + 8
 // significand bits): of the nine products of planes the six largest are made,
 // one after the other at each step, and what is left out is below 2^-24 of the
-// product.  The matrix cores' own float32 instructions reach 157 TFLOP/s, a
-// sixth of the bfloat16 rate more.
+// product.  That gives 100 to 175 TFLOP/s; the matrix cores' own float32
+// instructions have 157 at their peak, and a library reaches 154 with them.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -40,6 +50,8 @@ typedef short s16x8_t __attribute__((ext_vector_type(8)));
 constexpr uint32_t kDepth = 64;             // elements along k in a step
 constexpr uint32_t kMostPitch = 1u << 22;   // elements of a line: a tile's offsets stay below 2**32 bytes
 
+__host__ __device__ __forceinline__ uint32_t whole_steps(uint32_t n) { return (n + kDepth - 1u) / kDepth * kDepth; }
+
 // There is no end of k inside a step: deep lines are padded with zeros to
 // whole steps, and so is one operand's number of lines otherwise, where the
 // other has `tail`, a copy of its last lines that fills a step.
@@ -54,8 +66,6 @@ struct Operand {
 // How many rows there are may be known on the device alone (`live`, at most
 // what the grid is made for): then they are operand q's rows, or, with
 // `live_depth`, the length of k of both.
-__host__ __device__ __forceinline__ uint32_t whole_steps(uint32_t n) { return (n + kDepth - 1u) / kDepth * kDepth; }
-
 struct Product {
     Operand p, q;
     uint32_t tiles_p, tiles_q, splits, depth;   // depth: along k, in steps of 64 that are shared out among the splits
@@ -283,12 +293,13 @@ __device__ __forceinline__ void product(Product a, const Finish &finish, uint32_
         }
     };
     // One step: its slice is there, in every wave's part, once the loads before the last ROOMS - 2 slices are
-    // done and all waves say so; that also ends every read of the room that is loaded next.
+    // done and all waves say so.  Each has then also ended its reads of the room that is loaded next: the wait
+    // before the barrier is for those too.
     const auto step = [&](const uint16_t *room, uint16_t *free, uint32_t s) {
         constexpr int ahead = (T::ROOMS - 2) * (decltype(load_p)::kLoads + decltype(load_q)::kLoads);
         static_assert(ahead < 64, "the counter of loads on their way has six bits");
         __asm__ volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt((ahead & 15) | (ahead >> 4) << 14 | 0x0f70);     // vmcnt(ahead)
+        __builtin_amdgcn_s_waitcnt((ahead & 15) | (ahead >> 4) << 14 | 0x0070);     // vmcnt(ahead) lgkmcnt(0)
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
         __asm__ volatile("" ::: "memory");
