@@ -74,88 +74,94 @@ struct Rows {
 // ---- counted rows ----------------------------------------------------------------------------------
 constexpr int kRowsBlock = 1024;
 
-// One workgroup: each lane takes a run of consecutive rows, eight of whose
-// targets are read at a time (8192 rows: 11 us one after the other).  Forward,
-// the lse and loss of rows that are not counted are set to zero here.
-template <class F>
-__device__ __forceinline__ void each_class(const Targets &t, uint32_t begin, uint32_t end, F &&use) {
-    for (uint32_t i = begin; i < end; i += 8u) {
-        int32_t c[8];
-#pragma unroll
-        for (uint32_t k = 0; k < 8; ++k) c[k] = class_of(t, i + k < end ? i + k : end - 1u);
-#pragma unroll
-        for (uint32_t k = 0; k < 8; ++k)
-            if (i + k < end) use(i + k, c[k]);
-    }
-}
+// One workgroup, 8192 rows at a time: eight rows of a lane lie 1024 apart, so
+// that reads and writes are whole lines, and the counts of all waves are summed
+// at once.  Forward, the lse and loss of rows that are not counted are set to
+// zero here.
+constexpr int kRowsAtOnce = 8;
 
 template <bool BACKWARD>
 __global__ __launch_bounds__(kRowsBlock) void rows_kernel(Targets t, uint32_t rows, Rows out, const float *grad,
                                                           float grad_value, int32_t reduction, bool scaled, float *lse,
                                                           float *loss) {
-    __shared__ uint32_t counts[kRowsBlock / 64];
-    __shared__ float most[kRowsBlock / 64];
+    constexpr uint32_t waves = kRowsBlock / 64, slots = waves * kRowsAtOnce;
+    __shared__ uint32_t counts[slots];
+    __shared__ float most[waves];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const uint32_t each = (rows + kRowsBlock - 1) / kRowsBlock;
-    const uint32_t begin = threadIdx.x * each < rows ? threadIdx.x * each : rows;
-    const uint32_t end = rows - begin < each ? rows : begin + each;
-    uint32_t mine = 0;
-    float largest = 0.0f;
-    each_class(t, begin, end, [&](uint32_t i, int32_t c) {
-        if (c == kIgnored) return;
-        ++mine;
-        if (BACKWARD && reduction == kEach) largest = fmaxf(largest, fabsf(grad[i]));
-    });
-    uint32_t before = mine;                                // inclusive sums over the wave
+    float scale = 1.0f;
+    if (BACKWARD && scaled) {
+        float largest = reduction == kEach ? 0.0f : 1.0f;
+        if (reduction == kEach) {
+            for (uint32_t i = threadIdx.x; i < rows; i += kRowsBlock)
+                if (class_of(t, i) != kIgnored) largest = fmaxf(largest, fabsf(grad[i]));
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const uint32_t other = __shfl_up(before, off, 64);
-        if (lane >= (uint32_t)off) before += other;
-        if (BACKWARD) largest = fmaxf(largest, __shfl_xor(largest, off, 64));
-    }
-    if (lane == 63u) {
-        counts[wave] = before;
-        most[wave] = largest;
-    }
-    __syncthreads();
-    uint32_t count = 0;
-    for (uint32_t k = 0; k < kRowsBlock / 64; ++k) {
-        if (k < wave) before += counts[k];
-        count += counts[k];
-        if (BACKWARD) largest = fmaxf(largest, most[k]);
-    }
-    float common = 0.0f, scale = 1.0f;
-    if constexpr (BACKWARD) {
-        if (reduction != kEach) {
-            common = grad != nullptr ? *grad : grad_value;
-            if (reduction == kMean) common = common / (float)(count > 0 ? count : 1u);
-            largest = 1.0f;
+            for (int off = 32; off > 0; off >>= 1) largest = fmaxf(largest, __shfl_xor(largest, off, 64));
+            if (lane == 0u) most[wave] = largest;
+            __syncthreads();
+            for (uint32_t k = 0; k < waves; ++k) largest = fmaxf(largest, most[k]);
         }
-        if (scaled && largest > 0.0f && largest < kInfinity) {
+        if (largest > 0.0f && largest < kInfinity) {
             int exponent;
             frexpf(largest, &exponent);
             exponent = 15 - exponent;
             scale = ldexpf(1.0f, exponent > 126 ? 126 : exponent < -126 ? -126 : exponent);
         }
     }
-    if (threadIdx.x == 0) {
-        *out.count = count;
-        if (BACKWARD) *out.unscale = (reduction == kEach ? 1.0f : common) / scale;
-    }
-    uint32_t j = before - mine;
-    each_class(t, begin, end, [&](uint32_t i, int32_t c) {
-        if (BACKWARD) out.place[i] = c == kIgnored ? ~0u : j;
-        if (c == kIgnored) {
-            if (lse != nullptr) lse[i] = 0.0f;
-            if (loss != nullptr) loss[i] = 0.0f;
-            return;
+    uint32_t done = 0;                                      // counted rows of the rounds before
+    for (uint64_t first = 0; first < rows; first += kRowsBlock * kRowsAtOnce) {
+        int32_t c[kRowsAtOnce];
+        uint64_t votes[kRowsAtOnce];
+#pragma unroll
+        for (int k = 0; k < kRowsAtOnce; ++k) {
+            const uint64_t i = first + (uint32_t)k * kRowsBlock + threadIdx.x;
+            c[k] = i < rows ? class_of(t, i) : kIgnored;
         }
-        out.row[j] = i;
-        out.target[j] = c;
-        if constexpr (BACKWARD)
-            out.weight[j] = c == kOutside ? __builtin_nanf("") : (reduction == kEach ? grad[i] : 1.0f) * scale;
-        ++j;
-    });
+        __syncthreads();                                    // the last round's counts are read
+#pragma unroll
+        for (int k = 0; k < kRowsAtOnce; ++k) {
+            votes[k] = __builtin_amdgcn_ballot_w64(c[k] != kIgnored);
+            if (lane == 0u) counts[(uint32_t)k * waves + wave] = (uint32_t)__builtin_popcountll(votes[k]);
+        }
+        __syncthreads();
+        // Every wave sums them alike: before each slot, and all.
+        static_assert(slots == 128, "two slots a lane");
+        const uint32_t mine = counts[2u * lane], pair = mine + counts[2u * lane + 1u];
+        uint32_t upto = pair;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const uint32_t other = __shfl_up(upto, off, 64);
+            if (lane >= (uint32_t)off) upto += other;
+        }
+#pragma unroll
+        for (int k = 0; k < kRowsAtOnce; ++k) {
+            const uint64_t i = first + (uint32_t)k * kRowsBlock + threadIdx.x;
+            const uint32_t slot = (uint32_t)k * waves + wave;
+            const uint32_t before = __shfl(upto - pair, (int)(slot / 2u), 64);
+            const uint32_t half = __shfl(mine, (int)(slot / 2u), 64);
+            if (i >= rows) continue;
+            const uint32_t j = done + before + (slot % 2u ? half : 0u) +
+                               (uint32_t)__builtin_popcountll(votes[k] & ((1ull << lane) - 1ull));
+            if (BACKWARD) out.place[i] = c[k] == kIgnored ? ~0u : j;
+            if (c[k] == kIgnored) {
+                if (lse != nullptr) lse[i] = 0.0f;
+                if (loss != nullptr) loss[i] = 0.0f;
+                continue;
+            }
+            out.row[j] = (uint32_t)i;
+            out.target[j] = c[k];
+            if constexpr (BACKWARD)
+                out.weight[j] = c[k] == kOutside ? __builtin_nanf("") : (reduction == kEach ? grad[i] : 1.0f) * scale;
+        }
+        done += __shfl(upto, 63, 64);
+    }
+    if (threadIdx.x != 0u) return;
+    *out.count = done;
+    if constexpr (BACKWARD) {
+        float common = 1.0f;
+        if (reduction != kEach) common = grad != nullptr ? *grad : grad_value;
+        if (reduction == kMean) common = common / (float)(done > 0u ? done : 1u);
+        *out.unscale = common / scale;
+    }
 }
 
 // ---- operands as the products take them --------------------------------------------------------------
@@ -185,14 +191,18 @@ __global__ __launch_bounds__(kBlock) void pack_kernel(const void *from, uint32_t
         const uint32_t r = (uint32_t)(g / groups), c = (uint32_t)(g % groups) * 8u;
         const uint64_t source = (row == nullptr || r >= rows ? r : row[r]) * (uint64_t)width + c;
         const uint32_t end = r < rows ? width : 0u;
-        const auto *in = reinterpret_cast<const typename T::raw *>(from) + source;
+        Raw8<T> in;
+        if (c + 8u <= end) load8<T, false>(in, from, source);
+        else load_end<T>(in, from, source, c < end ? end - c : 0u);
         uint16_t *out = to + r * (uint64_t)pitch + c;
         if constexpr (T::code == NT_F32) {
+            float v[8];
+            widen8<T>(v, in);
             uint16_t planes[3][8];
 #pragma unroll
             for (uint32_t k = 0; k < 8; ++k) {
                 uint16_t one[3];
-                three_planes(c + k < end ? in[k] : 0.0f, one);
+                three_planes(v[k], one);
                 planes[0][k] = one[0];
                 planes[1][k] = one[1];
                 planes[2][k] = one[2];
@@ -200,10 +210,7 @@ __global__ __launch_bounds__(kBlock) void pack_kernel(const void *from, uint32_t
             for (int k = 0; k < 3; ++k)
                 *reinterpret_cast<u32x4_t *>(out + k * plane) = __builtin_bit_cast(u32x4_t, planes[k]);
         } else {
-            uint16_t group[8];
-#pragma unroll
-            for (uint32_t k = 0; k < 8; ++k) group[k] = c + k < end ? in[k] : (uint16_t)0;
-            *reinterpret_cast<u32x4_t *>(out) = __builtin_bit_cast(u32x4_t, group);
+            *reinterpret_cast<u32x4_t *>(out) = in.w[0];
         }
     }
 }
