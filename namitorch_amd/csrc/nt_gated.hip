@@ -82,13 +82,19 @@ __device__ __forceinline__ float block_total(double v, double *shared) {
 }
 
 // ---- rows that fit in registers ---------------------------------------------------------------------
-// As in the residual path's norms (nt_rows.hpp): a row lies over `lanes` lanes
-// in `parts` groups of eight, is read once, and variances are of centred
-// values; rows share workgroups, which make as many rounds as they need, and
-// the next row is on its way while this one is summed.  The vectors wait in
-// LDS as float32; a gate that a workgroup's rows share is multiplied into the
-// first norm's weight and bias there.  Rows of less than eight, or of more than
-// 8192 (whose vectors LDS does not hold), take the kernels for any width.
+// A row lies over lanes, eight consecutive elements (nt_rows.hpp) a lane, is
+// read once, and variances are of centred values; rows share workgroups, which
+// make as many turns as they need, and the next row is on its way while this
+// one is summed.  (Three groups a lane, which the residual path's norms take
+// for 768 columns: 8192 x 768 bfloat16 25 us, with one 17.5.)  The vectors wait
+// in LDS as float32; a gate that a workgroup's rows share is multiplied into
+// the first norm's weight and bias there.  Rows of less than eight, or of more
+// than 8192 (whose vectors LDS does not hold), take the kernels for any width.
+//
+// Bound by memory where rows are long: 16384 x 4096 bfloat16 with root mean
+// squares 96 us (5.6 TB/s), layer norms 114 (two sums more in turn); 8192 x 2048
+// float32 55 (4.9).  Narrow rows are bound by latency, four sums over lanes in
+// turn with few turns to share them: 8192 x 768 bfloat16 17.2 us (2.9 TB/s).
 constexpr uint32_t kGatedWaves = 4;     // per SIMD
 
 enum GateKind { kFolded = 0, kOwn = 1, kOwnFloat = 2 };   // none or shared; a row's own, of the data's type or float32
@@ -166,7 +172,6 @@ struct Vectors {
     }
 };
 
-//
 // Four waves per SIMD; at six (80 registers) 16384 x 4096 bfloat16 takes 121 us
 // instead of 102, 8192 x 768 as long as at four (17.5 us a call).
 template <class T, int KIND, bool EVEN, int THREADS>
@@ -285,6 +290,10 @@ __global__ __launch_bounds__(THREADS, kGatedWaves) void gated_kernel(GatedForwar
 // Waves per SIMD: float32, and a gate of the rows' own, take more than the 128
 // registers of four (with four, 5003 x 1001 float32 with such gates 70 us, with
 // two 46; 8192 x 2048 bfloat16 84 and 65, float32 with a shared one 119 and 91).
+//
+// 16384 x 4096 bfloat16 with root mean squares 176 us: four reads and two
+// writes at 4.7 TB/s, each row two exchanges over eight waves; 8192 x 768 23.6
+// us (3.2 TB/s), four turns, whose latency and joined sums show.
 static constexpr uint32_t gated_backward_waves(int32_t dtype, int kind, uint32_t threads) {
     return threads > (uint32_t)kRowThreads || (dtype != NT_F32 && kind == kFolded) ? 4u : 2u;
 }
@@ -710,8 +719,9 @@ __global__ __launch_bounds__(kBlock) void gated_columns_kernel(GatedBackward a, 
 
 // The vectors' gradients from the partial sums: 16 columns and 64 slices a
 // workgroup, of one norm's two; of 2048 columns and more 32 and 32 (512
-// workgroups' sums: 768 columns 8.7 and 12.5 us, 4096 17.1 and 13.7).  Slices share out the runs, and where those are fewer, the blocks
-// of each; a run's sums are joined before its gate, slices in order.
+// workgroups' sums: 768 columns 8.7 and 12.5 us, 4096 17.1 and 13.7).  Slices
+// share out the runs, and where those are fewer, the blocks of each; a run's
+// sums are joined before its gate, slices in order.
 struct GatedVectors {
     void *inner_weight, *inner_bias, *gate, *weight, *bias;     // each may be null
 };
@@ -783,6 +793,9 @@ constexpr uint32_t kRunGroups = 256;                    // groups of rows of the
 constexpr uint64_t kMostWidth = 1ull << 24;
 // A shared gate's runs of fewer rows than this many workgroups hold at a time
 // are taken as gates of the rows' own: each run's workgroups load the vectors.
+// Runs of 2, 4, 8, 16 and 32 rows of 8192 x 768 bfloat16, four to a workgroup:
+// 39.1, 22.9, 19.6, 17.9 and 18.7 us apart, 18 to 19 as the rows' own; of 8192 x
+// 4096, one to a workgroup: 83.5, 68.5, 62.1, 59.0 and 58.8, and 61 to 66.
 constexpr uint32_t kShortRun = 4;
 
 // Workgroups of each run: as many as are resident, where there are rows for them.
