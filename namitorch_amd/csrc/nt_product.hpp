@@ -27,9 +27,13 @@
 //
 // Float32 operands come as three bfloat16 planes whose sum they are (8 + 8 + 8
 // significand bits): of the nine products of planes the six largest are made,
-// one after the other at each step, and what is left out is below 2^-24 of the
-// product.  That gives 100 to 175 TFLOP/s; the matrix cores' own float32
-// instructions have 157 at their peak, and a library reaches 154 with them.
+// and what is left out is below 2^-24 of the product.  The five small ones of
+// all steps come first, so that only a sixth of the additions round at the
+// result's size: the gradients of 777 x 10007 x 1001 are 7.9e-7 off instead of
+// 1.6e-6 with all six at each step, for 2 to 5 % of the time, since the first
+// planes are then read twice.  They run at 100 to 175 TFLOP/s; the matrix
+// cores' own float32 instructions have 157 at their peak, and a library reaches
+// 154 with them.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -249,8 +253,9 @@ __device__ __forceinline__ void product(Product a, const Finish &finish, uint32_
         s = s < total ? s : total - 1u;
         uint32_t k = begin + s, plane_p = 0, plane_q = 0;
         if constexpr (PLANES == 3) {
-            const uint32_t which = s % 6u;          // (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
-            k = begin + s / 6u;
+            // (0,2) (2,0) (1,1) (0,1) (1,0) of all steps, then (0,0) of all.
+            const uint32_t small = (end - begin) * 5u, which = s < small ? s % 5u : 5u;
+            k = begin + (s < small ? s / 5u : s - small);
             plane_p = (0x010120u >> (4u * which)) & 15u;
             plane_q = (0x001102u >> (4u * which)) & 15u;
         }

@@ -9,6 +9,8 @@ factor, 3 e, and rounded once, off by TINY where they are subnormal."""
 
 from __future__ import annotations
 
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -87,3 +89,42 @@ def test_tiles(rows, classes, width, dtype):
         bound = bound + (u + 3 * E) * (exact.abs() + bound) + TINY[dtype]
         wrong = (_get(got) - exact).abs() > bound
         assert not wrong.any(), (int(wrong.sum()), wrong.nonzero()[:4].tolist())
+
+
+def test_two_threads():
+    """Calls of two threads, on streams of their own and on one, give what each gives alone."""
+    generator = torch.Generator(device="cuda").manual_seed(3)
+    wrap = nt.Tensor._from_storage
+
+    def made(rows, classes, width):
+        weight = torch.randn(classes, width, generator=generator, device="cuda") * 0.1
+        x = torch.randn(rows, width, generator=generator, device="cuda")
+        target = torch.randint(0, classes, (rows,), generator=generator, device="cuda")
+        return wrap(x), wrap(weight), wrap(target)
+
+    def call(problem):
+        loss, lse = F.linear_cross_entropy_forward(*problem)
+        return (loss, lse, *F.linear_cross_entropy_backward(1.0, *problem, lse))
+
+    problems = [made(300, 1500, 72), made(70, 4000, 128)]
+    alone = [[np.array(t.numpy()) for t in call(problem)] for problem in problems]
+    torch.cuda.synchronize()
+    for shared in (True, False):
+        found = [None, None]
+
+        def work(k, stream):
+            with torch.cuda.stream(stream):
+                results = [call(problems[k]) for _ in range(20)]
+                stream.synchronize()
+                found[k] = [[np.array(t.numpy()) for t in result] for result in results]
+
+        one = torch.cuda.Stream()
+        threads = [threading.Thread(target=work, args=(k, one if shared else torch.cuda.Stream())) for k in range(2)]
+        for thread in threads:
+            thread.start()
+        for thread in threads:
+            thread.join()
+        for k in range(2):
+            assert found[k] is not None
+            for result in found[k]:
+                assert all(np.array_equal(a, b, equal_nan=True) for a, b in zip(result, alone[k]))
