@@ -656,11 +656,16 @@ int32_t nt_norm_gate_add_norm_backward(int32_t device, const void *dy, const voi
  *
  *   dz = g (exp(z - lse) - [class = target]), dx = dz weight, dweight = dz^T x
  *
- * with dz rounded once to `dtype`.  Both take workspace of the library's pool
- * in the order of `stream` (about the size of x for the forward pass, and for
- * the backward pass up to 512 MiB for a piece of dz and two to six times x)
- * and refuse a stream in capture.  Rows: fewer than 2**24; classes: fewer than
- * 2**30; width: at most 2**21.  No counterpart in the reference's kernels.
+ * with dz rounded once to `dtype` (and float32 operands multiplied as three
+ * bfloat16 parts each).  Both take workspace of the library's pool in the order
+ * of `stream` and refuse a stream in capture.  Forward: the size of x and 8 bytes
+ * for each row and 32 (few rows) to 128 classes.  Backward: up to 1 GiB, or 256
+ * classes, for a piece of dz, the size of x and float32 sums of it, in up to 512
+ * MiB more where the work is split.  Float32 takes 6 bytes for an element of x;
+ * packed weights (float32, a width that is no multiple of 64, an address that is
+ * none of 16) join them, at most 1 GiB at a time.  Rows: fewer than 2**24;
+ * classes: fewer than 2**30; width: at most 2**21.  No counterpart in the
+ * reference's kernels.
  */
 int32_t nt_linear_cross_entropy(int32_t device, const void *x, const void *weight, int32_t dtype,
                                 const void *target, int32_t target_size, int64_t ignore_index,

@@ -6,7 +6,8 @@ behind NamiTorch's Python API, computed by hand-written gfx950 HIP kernels
 through ctypes.  Optimizer and scaler state read and write NamiTorch's
 ``.nt`` archive and checkpoint layout (``serialization``, ``checkpoint``).
 ``functional`` has the operators of a transformer's residual path (layer
-norm, dropout, and the two joined) with their backward passes.
+norm, dropout, the edges that join them) and the loss over a large vocabulary,
+with their backward passes.
 
 The package needs NumPy and the library, not PyTorch: device memory comes
 from the library's caching allocator (``array.DeviceArray``) and streams and

@@ -1,9 +1,9 @@
-"""Operators between a transformer's matrix products: layer norm, dropout,
-and the residual edge that joins them.
+"""Operators between a transformer's matrix products, layer norm, dropout
+and the edges of the residual path that join them, and the loss at its end.
 
-The reference has them in ``namitorch/nn`` (layer norm over the kernels of
-``backends/cuda/normalization.py:56-157``, dropout as a layer).  This package
-has no autograd, so each operator comes as a forward call that returns what
+The reference has layer norm, root mean square norm, dropout and cross entropy
+in ``namitorch/nn`` (the norms over the kernels of
+``backends/cuda/normalization.py:56-157``).  This package has no autograd, so each operator comes as a forward call that returns what
 its backward call reads, and a backward call that returns gradients to hand
 to ``accumulate_grads`` or to the layer below:
 
@@ -11,12 +11,18 @@ to ``accumulate_grads`` or to the layer below:
 * ``dropout`` / ``dropout_backward``;
 * ``dropout_add_layer_norm`` / ``..._forward`` / ``..._backward``:
   ``total = dropout(input) + residual`` and the layer norm of it, the edge
-  between two sublayers, in one pass over the data.
+  between two sublayers, in one pass over the data;
+* ``norm_gate_add_norm`` / ``..._forward`` / ``..._backward``: ``total =
+  residual_scale * residual + gate * N(input)`` and the norm of it, the edge
+  after a block that is normalized on both sides;
+* ``linear_cross_entropy`` / ``..._forward`` / ``..._backward``: softmax cross
+  entropy of ``input @ weight.T``, whose logits are never in memory.
 
 Tensors are float16, bfloat16 or float32 on a HIP device; weight and bias
 (and their gradients) have the activations' dtype or float32.  Statistics and
-sums are float32, values are rounded once.  A row that holds an infinity or
-NaN gives NaN outputs.
+sums are float32, values are rounded once (the loss's backward call rounds
+the logits' gradient to the operands' dtype too).  A row that holds an
+infinity or NaN gives NaN outputs.
 
 No mask is stored.  Whether element ``i`` of the flattened tensor is dropped
 depends on ``(seed, offset, i)`` alone (Philox4x32-10, 16 bits per element),
@@ -30,8 +36,9 @@ zero, whatever it held.
 the order of the results (``None`` entries are allocated).  They overlap
 neither inputs nor one another; ``dropout`` may write its own input.  Launches
 go to the calling thread's current stream.  In a stream capture the forward
-calls run when ``out`` names every result and nothing is dropped (a replay
-would repeat the mask); the others raise, and so does a call that is given a
+calls of the norms and edges run when ``out`` names every result and nothing
+is dropped (a replay would repeat the mask); the others raise, those of the
+loss among them (they take workspace), and so does a call that is given a
 gradient whose accumulation or unscaling is still deferred.
 """
 
