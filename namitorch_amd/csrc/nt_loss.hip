@@ -691,8 +691,8 @@ constexpr uint32_t kUnits = 256;                     // compute units
 
 using Large = Tile<256, 256, 2, 4>;
 using Middle = Tile<128, 128, 2, 2>;
-using Tall = Tile<256, 128, 4, 2, 3>;                // 65 to 256 rows
-using Few = Tile<128, 64, 4, 1, 3>;                  // up to 64, or too few tiles of the others
+using Tall = Tile<256, 128, 4, 2, 3>;                // logits of 65 to 256 rows
+using Few = Tile<128, 64, 4, 1, 3>;                  // up to 64 rows, or too few tiles of the others
 
 static uint32_t tiles_of(uint64_t n, uint32_t each) { return (uint32_t)((n + each - 1) / each); }
 
@@ -702,8 +702,8 @@ static uint32_t tiles_of(uint64_t n, uint32_t each) { return (uint32_t)((n + eac
 // 63 with the last; 777 x 10007 x 1001 float32, 160 or 553: 129 us and 90.
 // Up to 256 rows tall ones, where half of the units get one (they wait for the
 // weights, which larger tiles ask for sooner): 129 rows of 50304 x 2048 float16
-// forward 48.4 us, with small ones 58.7; but 200 rows of 10007 x 1001 float32,
-// 80 tiles, 104 and 71.
+// forward 48.4 us, with small ones 58.7, and 256 rows 79 and with 128 x 128 85;
+// but 200 rows of 10007 x 1001 float32, 80 tiles, 104 and 71.
 template <class F>
 static void with_logits_tile(uint64_t classes, uint64_t rows, F &&launch) {
     if (rows <= 64u) launch(Few{});
@@ -713,23 +713,19 @@ static void with_logits_tile(uint64_t classes, uint64_t rows, F &&launch) {
     else launch(Few{});
 }
 
-// The same for the two products of dz.  Of few rows dW has the most tiles: tall
-// ones if there are four for each unit.  A call of 129 rows of 50304 x 2048
-// float16 179 us, with small ones 204; of 200 rows of 10007 x 1001 float32, 316
-// tall tiles, 203 and 151.  Of more rows large ones, where each unit gets 64
+// The same for the two products of dz.  Large tiles, where each unit gets 64
 // steps of them (whose ends are then a small part): 8192 x 50257 x 768 bfloat16,
-// 590 steps, 1.74 ms and with 128 x 128 1.88; 512 x 32000 x 4096, 125 steps, 475
-// us and 507; but 1500 x 10007 x 1001, 30 steps, 161 and 146, and 300 x 50257 x
-// 768 155 and 130.
+// 590 steps, a call 1.74 ms and with 128 x 128 1.88; 512 x 32000 x 4096, 125
+// steps, 475 us and 507; 200 x 128000 x 4096 947 and 1042; but 1500 x 10007 x
+// 1001, 30 steps, 161 and 146, and 300 x 50257 x 768 155 and 130.  They leave
+// half of themselves idle up to 128 rows: 70 x 128000 x 4096 739 and 723.
 template <class F>
 static void with_grads_tile(uint64_t classes, uint64_t rows, uint64_t pitch, F &&launch) {
     const uint64_t steps = tiles_of(pitch, 256) * ((uint64_t)tiles_of(rows, 256) * tiles_of(classes, kDepth) +
                                                    (uint64_t)tiles_of(classes, 256) * tiles_of(rows, kDepth));
-    if (rows > 256u) {
-        if (steps >= 64u * kUnits) launch(Large{});
-        else launch(Middle{});
-    } else if (rows > 64u && (uint64_t)tiles_of(pitch, 256) * tiles_of(classes, 128) >= 4u * kUnits) launch(Tall{});
-    else launch(Few{});
+    if (rows <= 64u) launch(Few{});
+    else if (rows > 128u && steps >= 64u * kUnits) launch(Large{});
+    else launch(Middle{});
 }
 
 // How the two products of dz are split along k.  dx: such that no workgroup has
@@ -767,10 +763,10 @@ template <class T> struct Kind {            // how the products take a type
 };
 
 // The pieces of the vocabulary: as few as keep dz and the packed weights
-// within their bytes, and a launch of large tiles below 2**32 work-items; of
-// whole tiles.
+// within their bytes, and a launch below 2**32 work-items (512 for each large
+// tile, twice as many for as much in tall ones); of whole tiles.
 static uint32_t piece_of(const Problem &a, uint32_t pitch, int planes, bool packed, bool backward) {
-    uint64_t most = (1ull << 22) / tiles_of(a.rows, 256) * 256u;
+    uint64_t most = (1ull << 21) / tiles_of(a.rows, 256) * 256u;
     if (backward) most = std::min<uint64_t>(most, kPieceBytes / (2ull * planes * whole_steps(a.rows)));
     if (packed) most = std::min<uint64_t>(most, kPieceBytes / (2ull * planes * pitch));
     if (most >= a.classes) return a.classes;

@@ -40,10 +40,10 @@ def _product(a, b):
 
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
 @pytest.mark.parametrize("rows, classes, width", [
-    (129, 50304, 520),      # tall tiles, of both passes
-    (256, 33001, 1024),     # the same, weights read in place whose last lines do not fill a step
-    (200, 17000, 72),       # tall logits, small gradients
-    (200, 10007, 1001),     # small ones for want of tiles
+    (129, 50304, 520),      # tall logits, gradients of 128 x 128
+    (256, 33001, 1024),     # the same, with weights read in place whose last lines do not fill a step
+    (200, 17000, 72),       # the same, little of it
+    (200, 10007, 1001),     # small logits for want of tiles
     (300, 3000, 520),       # 128 x 128
     (777, 10007, 1001),     # large logits, gradients of 128 x 128
     (1040, 32100, 1000),    # large ones
