@@ -175,8 +175,8 @@ struct Vectors {
 // Four waves per SIMD; at six (80 registers) 16384 x 4096 bfloat16 takes 121 us
 // instead of 102, 8192 x 768 as long as at four (17.5 us a call).
 template <class T, int KIND, bool EVEN, int THREADS>
-__global__ __launch_bounds__(THREADS, kGatedWaves) void gated_kernel(GatedForward a, uint32_t lanes, uint32_t run_blocks, bool rms,
-                                                           bool even) {
+__global__ __launch_bounds__(THREADS, kGatedWaves)
+void gated_kernel(GatedForward a, uint32_t lanes, uint32_t run_blocks, bool rms, bool even) {
     using G = typename GateType<T, KIND>::type;
     extern __shared__ float4 room[];
     __shared__ float shared[2][THREADS / 64];
@@ -298,7 +298,8 @@ static constexpr uint32_t gated_backward_waves(int32_t dtype, int kind, uint32_t
     return threads > (uint32_t)kRowThreads || (dtype != NT_F32 && kind == kFolded) ? 4u : 2u;
 }
 template <class T, int KIND, bool EVEN, int THREADS>
-__global__ __launch_bounds__(THREADS, gated_backward_waves(T::code, KIND, THREADS)) void gated_backward_kernel(GatedBackward a, uint32_t lanes, bool rms, bool even) {
+__global__ __launch_bounds__(THREADS, gated_backward_waves(T::code, KIND, THREADS))
+void gated_backward_kernel(GatedBackward a, uint32_t lanes, bool rms, bool even) {
     using G = typename GateType<T, KIND>::type;
     extern __shared__ float4 room[];
     __shared__ float shared[2][2][THREADS / 64];
@@ -718,16 +719,16 @@ __global__ __launch_bounds__(kBlock) void gated_columns_kernel(GatedBackward a, 
 }
 
 // The vectors' gradients from the partial sums: 16 columns and 64 slices a
-// workgroup, of one norm's two; of 2048 columns and more 32 and 32 (512
-// workgroups' sums: 768 columns 8.7 and 12.5 us, 4096 17.1 and 13.7).  Slices
+// workgroup, of one norm's two; of 4096 columns and more 32 and 32 (512
+// workgroups' sums: 768 columns 8.7 and 12.5 us, with 8 columns 8.8; 4096 17.1
+// and 13.7; a backward call of 8192 x 2048 56.8 and 59.7).  Slices
 // share out the runs, and where those are fewer, the blocks of each; a run's
 // sums are joined before its gate, slices in order.
 struct GatedVectors {
     void *inner_weight, *inner_bias, *gate, *weight, *bias;     // each may be null
 };
 template <uint32_t kVectorColumns>
-__global__ __launch_bounds__(1024) void gated_vectors_kernel(GatedBackward a, GatedVectors to,
-                                                                                        uint32_t runs, bool each) {
+__global__ __launch_bounds__(1024) void gated_vectors_kernel(GatedBackward a, GatedVectors to, uint32_t runs, bool each) {
     constexpr uint32_t kVectorSlices = 1024u / kVectorColumns;
     __shared__ float shared[2][kVectorSlices][kVectorColumns + 1];
     const uint32_t column = threadIdx.x % kVectorColumns, slice = threadIdx.x / kVectorColumns;
@@ -789,6 +790,7 @@ __global__ __launch_bounds__(1024) void gated_vectors_kernel(GatedBackward a, Ga
 
 // ---- launches ----------------------------------------------------------------------------------------
 constexpr uint32_t kMostBlocks = 8192;
+constexpr uint32_t kUnits = 256;                        // compute units
 constexpr uint32_t kRunGroups = 256;                    // groups of rows of the column sums of long rows, over all runs
 constexpr uint64_t kMostWidth = 1ull << 24;
 // A shared gate's runs of fewer rows than this many workgroups hold at a time
@@ -798,9 +800,19 @@ constexpr uint64_t kMostWidth = 1ull << 24;
 // 4096, one to a workgroup: 83.5, 68.5, 62.1, 59.0 and 58.8, and 61 to 66.
 constexpr uint32_t kShortRun = 4;
 
-// Workgroups of each run: as many as are resident, where there are rows for them.
-static uint32_t run_blocks_of(uint64_t run, uint64_t runs, const RowTiling &g, uint32_t waves) {
-    const uint64_t most = std::max<uint64_t>(1u, kSimds * waves * 64u / g.threads / runs);
+// Workgroups of each run: as many as are resident at a time, where there are
+// rows for them; those past them would have a turn of their own.  `waves` of a
+// SIMD's are counted by whole workgroups, over a unit where the kernel leaves
+// registers for a wave more (16-bit forward), otherwise over each SIMD: of five
+// waves a unit of 16 then holds two workgroups, not three.  16384 x 2560
+// bfloat16 forward 78 to 85 us (two: 101; counted by waves alone, 819 workgroups
+// in 768 places: 115), backward 140 (three: 177; by waves: 220); 8192 x 2560
+// float32 forward 85 (three: 94); 4096 x 7168 bfloat16 67 and 100 instead of 113
+// and 153.
+static uint32_t run_blocks_of(uint64_t run, uint64_t runs, const RowTiling &g, uint32_t waves, bool each_simd) {
+    const uint32_t of_block = (g.threads + 63u) / 64u, simds = kSimds / kUnits;
+    const uint32_t per_unit = each_simd ? waves / ((of_block + simds - 1u) / simds) : waves * simds / of_block;
+    const uint64_t most = std::max<uint64_t>(1u, kUnits * (uint64_t)std::max(1u, per_unit) / runs);
     const uint32_t per_block = g.threads / g.lanes;
     return (uint32_t)std::min<uint64_t>((run + per_block - 1) / per_block, most);
 }
@@ -814,15 +826,19 @@ static int gate_kind(const GatedForward &a, int32_t dtype, uint32_t per_block, u
 }
 
 // A group a lane: a power of two of lanes up to 32, then whole waves, and as
-// many rows (a power of two of them) as fit in 512 lanes, or one.  No parts:
-// rows that the tilings do not take.
-static RowTiling gated_tiling(uint32_t width) {
+// many rows (a power of two of them) as fit in 512 lanes, or one.  Rows of three
+// waves share no workgroup in the forward pass: a unit holds five alone and four
+// in pairs (8192 x 1536 bfloat16 25.3 us and 29.9; backward, with partial sums
+// for each workgroup, 55.6 and 51.7).  No parts: rows that the tilings do not
+// take.
+static RowTiling gated_tiling(uint32_t width, bool backward) {
     const uint32_t groups = (width + kGroup - 1) / kGroup;
     if (width < kGroup || groups > (uint32_t)kWideThreads) return RowTiling{0, 0, 0};
     uint32_t lanes = 1, rows = 1;
     while (lanes < groups && lanes < 64u) lanes <<= 1;
     if (groups > 64u) lanes = (groups + 63u) / 64u * 64u;
-    while (lanes * rows * 2u <= (uint32_t)kRowThreads) rows <<= 1;
+    if (lanes != 192u || backward)
+        while (lanes * rows * 2u <= (uint32_t)kRowThreads) rows <<= 1;
     return RowTiling{lanes, 1, lanes * rows};
 }
 
@@ -839,7 +855,8 @@ static void in_launches(Args a, uint64_t blocks, F &&launch) {
 template <class T, int KIND, int THREADS>
 static void launch_gated_tiled(const GatedForward &args, const RowTiling &g, uint64_t runs, bool rms, hipStream_t s) {
     const bool aligned = aligned16({args.total, args.y});
-    const uint32_t blocks = run_blocks_of(args.rows / runs, runs, g, kGatedWaves), room = g.lanes * kGroup * 16u;
+    const uint32_t blocks = run_blocks_of(args.rows / runs, runs, g, kGatedWaves, T::code == NT_F32);
+    const uint32_t room = g.lanes * kGroup * 16u;
     in_launches(args, runs * blocks, [&](dim3 grid, const GatedForward &a) {
         if (a.width % kGroup == 0)
             gated_kernel<T, KIND, true, THREADS><<<grid, dim3(g.threads), room, s>>>(a, g.lanes, blocks, rms, aligned);
@@ -849,7 +866,7 @@ static void launch_gated_tiled(const GatedForward &args, const RowTiling &g, uin
 
 template <class T>
 static void launch_gated(const GatedForward &a, bool rms, hipStream_t s) {
-    const RowTiling g = gated_tiling(a.width);
+    const RowTiling g = gated_tiling(a.width, false);
     if (g.parts == 0) {
         const dim3 grid((unsigned)std::min<uint64_t>(a.rows, kMostBlocks));
         if (rms) gated_rows_kernel<T, true><<<grid, dim3(kLongThreads), 0, s>>>(a);
@@ -884,7 +901,7 @@ static void launch_gated_backward_tiled(const GatedBackward &args, const RowTili
 
 template <class T>
 static void launch_gated_backward(const GatedBackward &a, bool rms, bool each, uint32_t groups, hipStream_t s) {
-    const RowTiling g = gated_tiling(a.width);
+    const RowTiling g = gated_tiling(a.width, true);
     if (g.parts != 0) {
         const auto launch = [&](auto kind) {
             constexpr int KIND = decltype(kind)::value;
@@ -1015,8 +1032,9 @@ int32_t nt_norm_gate_add_norm_backward(int32_t device, const void *dy, const voi
                     {gate, gate_dtype, (uint32_t)gate_runs, rows / gate_runs}, inner_mean, inner_rstd, mean, rstd,
                     dx, dresidual, each ? dgate : nullptr, nullptr, nullptr, rows, (uint32_t)width, weight_dtype,
                     residual_scale, 1, 0};
-    const RowTiling tiling = gated_tiling((uint32_t)width);
-    a.run_blocks = tiling.parts != 0 ? run_blocks_of(rows / runs, runs, tiling, gated_backward_waves(dtype, each ? kOwn : kFolded, tiling.threads))
+    const RowTiling tiling = gated_tiling((uint32_t)width, true);
+    const uint32_t waves = gated_backward_waves(dtype, each ? kOwn : kFolded, tiling.threads);
+    a.run_blocks = tiling.parts != 0 ? run_blocks_of(rows / runs, runs, tiling, waves, true)
                                      : (uint32_t)std::min<uint64_t>(rows / runs, std::max(1u, kRunGroups / runs));
     Workspace room;
     if (tiling.parts == 0) room.want(&a.row_sums, 2u * rows);
@@ -1030,7 +1048,7 @@ int32_t nt_norm_gate_add_norm_backward(int32_t device, const void *dy, const voi
         default: launch_gated_backward<TBF16>(a, rms, each, groups, s); break;
     }
     const GatedVectors vectors{dinner_weight, dinner_bias, each ? nullptr : dgate, dweight, dbias};
-    if (width < 2048u) gated_vectors_kernel<16><<<dim3((a.width + 15u) / 16u, 2), dim3(1024), 0, s>>>(a, vectors, runs, each);
+    if (width < 4096u) gated_vectors_kernel<16><<<dim3((a.width + 15u) / 16u, 2), dim3(1024), 0, s>>>(a, vectors, runs, each);
     else gated_vectors_kernel<32><<<dim3((a.width + 31u) / 32u, 2), dim3(1024), 0, s>>>(a, vectors, runs, each);
     return hip_check(hipGetLastError(), "gated norm backward launch");
 }

@@ -390,3 +390,13 @@ def test_streams():
         torch.cuda.synchronize()
         for want, have in zip(expected, got):
             assert all(np.array_equal(a.bits(), b.bits()) for a, b in zip(want, have))
+
+
+@pytest.mark.parametrize("dtype, gate", [("bfloat16", "run"), ("float32", "row"), ("float16", "shared")])
+@pytest.mark.parametrize("runs, run, width", [(2, 1400, 1536), (2, 900, 2560), (2, 300, 5120)])
+def test_rows_of_odd_numbers_of_waves(runs, run, width, gate, dtype):
+    """More rows than workgroups hold at a time, of three, five and ten waves each."""
+    edge = _Edge(_rng(19, runs, run, width), runs, run, width, dtype, "float32", gate)
+    made = _run_forward(edge)
+    _check_forward(edge, made)
+    _check_backward(edge, _run_backward(edge, made, edge.dtotal), made[1], made[2:], edge.dtotal)
