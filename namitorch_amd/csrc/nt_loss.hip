@@ -22,8 +22,8 @@
 // and most targets' -1 is exact: rounded together with that factor, which is
 // as far off for each of them, the gradient of 8192 rows by 50257 classes was
 // 1.7 times as far from the 64-bit one as a single rounding.  In float16 dz is
-// multiplied by a power of two first, such that the largest |g_i| comes to
-// 2**14 to 2**15: exp(z - lse) is some 1 / V, which float16 alone would hold
+// multiplied by a power of two first, such that the largest finite |g_i| comes
+// to 2**14 to 2**15: exp(z - lse) is some 1 / V, which float16 alone would hold
 // with few digits or none.  Float32 is three bfloat16 planes (nt_product.hpp).
 #include <hip/hip_runtime.h>
 
@@ -92,15 +92,18 @@ __global__ __launch_bounds__(kRowsBlock) void rows_kernel(Targets t, uint32_t ro
     if (BACKWARD && scaled) {
         float largest = reduction == kEach ? 0.0f : 1.0f;
         if (reduction == kEach) {
-            for (uint32_t i = threadIdx.x; i < rows; i += kRowsBlock)
-                if (class_of(t, i) != kIgnored) largest = fmaxf(largest, fabsf(grad[i]));
+            // Of rows whose gradients are finite: the others are NaN or infinite at any scale.
+            for (uint32_t i = threadIdx.x; i < rows; i += kRowsBlock) {
+                const float size = fabsf(grad[i]);
+                if (class_of(t, i) >= 0 && size < kInfinity) largest = fmaxf(largest, size);
+            }
 #pragma unroll
             for (int off = 32; off > 0; off >>= 1) largest = fmaxf(largest, __shfl_xor(largest, off, 64));
             if (lane == 0u) most[wave] = largest;
             __syncthreads();
             for (uint32_t k = 0; k < waves; ++k) largest = fmaxf(largest, most[k]);
         }
-        if (largest > 0.0f && largest < kInfinity) {
+        if (largest > 0.0f) {
             int exponent;
             frexpf(largest, &exponent);
             exponent = 15 - exponent;

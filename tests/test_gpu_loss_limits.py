@@ -5,10 +5,14 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
+import namitorch_amd as nt
 import test_gpu_loss as base
 from namitorch_amd import functional as F
 
 pytestmark = pytest.mark.gpu
+
+DEV, DTYPES = base.DEV, base.DTYPES
+
 
 # Powers of two by which the operands' logits come to 1.5 * 2**(a + b), and at most 1.25 of it for other classes:
 # float32 holds these logits, and lse, without rounding, as the others' exponentials are zero beside the largest's.
@@ -45,3 +49,48 @@ def test_far_logits_are_exact(rows, dtype, a, b, sign):
     for got, exact in ((dx, dz @ weight / rows), (dw, dz.T @ x / rows)):
         # The sums are whole multiples of a power of two; 1 / rows and its product round once each, then the result.
         assert np.all(np.abs(base._values(got) - exact) <= (base.HALF_ULP[dtype] + 3 * base.E) * np.abs(exact))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [2.0 ** -20, 1.0, 2.0 ** 17])
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
+def test_a_row_gradient_that_is_not_finite(value, size, dtype):
+    """It reaches its own row and the weight's gradient; the other rows' are what they are without it."""
+    rows = 50
+    x, weight, target = base._problem(base._rng(22), rows, 300, 64, dtype)
+    # Float16 then holds the results of all three sizes, with digits to see.
+    by_weight, by_x = (256.0, 1 / 256.0) if size < 1.0 else (1 / 64.0, 1 / 64.0)
+    x, weight = base._tensor(base._values(x) * by_x, dtype), base._tensor(base._values(weight) * by_weight, dtype)
+    target = np.where(target < 0, 3, target)
+    grad = (size * (0.5 + base._rng(23).random(rows))).astype(np.float32)
+    at = base._targets(target)
+    _, lse = F.linear_cross_entropy_forward(x, weight, at)
+    held = grad.copy()
+    held[1] = value
+    dx, dw = F.linear_cross_entropy_backward(nt.Tensor(held, device=DEV), x, weight, at, lse, reduction="none")
+    assert not np.any(np.isfinite(dx.numpy()[1])) and not np.any(np.isfinite(dw.numpy()))
+    rest = np.arange(rows) != 1
+    without = base._targets(np.where(rest, target, -100))
+    _, dw = F.linear_cross_entropy_backward(nt.Tensor(held, device=DEV), x, weight, without, lse, reduction="none")
+    base._check_backward(nt.Tensor(dx.numpy()[rest]), dw, grad[rest].astype(np.float64), base._values(x)[rest],
+                         base._values(weight), target[rest], base._values(lse)[rest], dtype, reduction="none")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_row_of_no_class_takes_no_digits_from_others(dtype):
+    """Its gradient is NaN whatever it is multiplied by, and the other rows' what they are without it."""
+    rows = 50
+    x, weight, target = base._problem(base._rng(26), rows, 300, 64, dtype)
+    target = np.where(target < 0, 3, target)
+    grad = (0.5 + base._rng(27).random(rows)).astype(np.float32)
+    _, lse = F.linear_cross_entropy_forward(x, weight, base._targets(target))
+    rest = np.arange(rows) != 1
+    held, outside = grad.copy(), np.where(rest, target, 300)
+    held[1] = 2.0 ** 60
+    given = nt.Tensor(held, device=DEV)
+    dx, dw = F.linear_cross_entropy_backward(given, x, weight, base._targets(outside), lse, reduction="none")
+    assert np.isnan(dx.numpy()[1]).all() and np.isnan(dw.numpy()).all()
+    without = base._targets(np.where(rest, target, -100))
+    _, dw = F.linear_cross_entropy_backward(given, x, weight, without, lse, reduction="none")
+    base._check_backward(nt.Tensor(dx.numpy()[rest]), dw, grad[rest].astype(np.float64), base._values(x)[rest],
+                         base._values(weight), target[rest], base._values(lse)[rest], dtype, reduction="none")
