@@ -24,7 +24,8 @@
 // 1.7 times as far from the 64-bit one as a single rounding.  In float16 dz is
 // multiplied by a power of two first, such that the largest finite |g_i| comes
 // to 2**14 to 2**15: exp(z - lse) is some 1 / V, which float16 alone would hold
-// with few digits or none.  Float32 is three bfloat16 planes (nt_product.hpp).
+// with few digits or none; row gradients of the other types are brought below
+// one likewise.  Float32 is three bfloat16 planes (nt_product.hpp).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -82,14 +83,16 @@ constexpr int kRowsAtOnce = 8;
 
 template <bool BACKWARD>
 __global__ __launch_bounds__(kRowsBlock) void rows_kernel(Targets t, uint32_t rows, Rows out, const float *grad,
-                                                          float grad_value, int32_t reduction, bool scaled, float *lse,
+                                                          float grad_value, int32_t reduction, bool half, float *lse,
                                                           float *loss) {
     constexpr uint32_t waves = kRowsBlock / 64, slots = waves * kRowsAtOnce;
     __shared__ uint32_t counts[slots];
     __shared__ float most[waves];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    // A power of two: float16's as said above; with row gradients of the other types, such that the largest
+    // comes to 0.5 to 1, since a product of 2^-122 and a probability would have few digits, or none.
     float scale = 1.0f;
-    if (BACKWARD && scaled) {
+    if (BACKWARD && (half || reduction == kEach)) {
         float largest = reduction == kEach ? 0.0f : 1.0f;
         if (reduction == kEach) {
             // Of rows whose gradients are finite: the others are NaN or infinite at any scale.
@@ -106,7 +109,7 @@ __global__ __launch_bounds__(kRowsBlock) void rows_kernel(Targets t, uint32_t ro
         if (largest > 0.0f) {
             int exponent;
             frexpf(largest, &exponent);
-            exponent = 15 - exponent;
+            exponent = (half ? 15 : 0) - exponent;
             scale = ldexpf(1.0f, exponent > 126 ? 126 : exponent < -126 ? -126 : exponent);
         }
     }

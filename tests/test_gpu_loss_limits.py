@@ -94,3 +94,21 @@ def test_a_row_of_no_class_takes_no_digits_from_others(dtype):
     _, dw = F.linear_cross_entropy_backward(given, x, weight, without, lse, reduction="none")
     base._check_backward(nt.Tensor(dx.numpy()[rest]), dw, grad[rest].astype(np.float64), base._values(x)[rest],
                          base._values(weight), target[rest], base._values(lse)[rest], dtype, reduction="none")
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("exponent", [-122, -60, 60, 100])
+def test_row_gradients_at_the_ends_of_the_range(exponent, dtype):
+    """A product of a row's gradient and a probability may lie where the dtype has few digits, or none; the weight's
+    gradient does not, as x is large, and is as precise as others.  Large gradients meet a small x."""
+    rows, classes, width = 60, 300, 64
+    rng = base._rng(24, exponent + 200)
+    x, weight, target = base._problem(rng, rows, classes, width, dtype)
+    by = 2.0 ** (20 if exponent < 0 else -20)
+    x, weight = base._tensor(base._values(x) * by, dtype), base._tensor(base._values(weight) / by, dtype)
+    grad = (2.0 ** exponent * (0.5 + rng.random(rows))).astype(np.float32)
+    at = base._targets(target)
+    _, lse = F.linear_cross_entropy_forward(x, weight, at)
+    dx, dw = F.linear_cross_entropy_backward(nt.Tensor(grad, device=DEV), x, weight, at, lse, reduction="none")
+    base._check_backward(dx, dw, grad.astype(np.float64), base._values(x), base._values(weight), target,
+                         base._values(lse), dtype, reduction="none")
