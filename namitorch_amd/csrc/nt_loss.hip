@@ -166,7 +166,7 @@ __global__ __launch_bounds__(kRowsBlock) void rows_kernel(Targets t, uint32_t ro
         float common = 1.0f;
         if (reduction != kEach) common = grad != nullptr ? *grad : grad_value;
         if (reduction == kMean) common = common / (float)(done > 0u ? done : 1u);
-        *out.unscale = common / scale;
+        *out.unscale = done > 0u ? common / scale : 0.0f;   // rows that do not count give none of an infinity either
     }
 }
 

@@ -112,3 +112,20 @@ def test_row_gradients_at_the_ends_of_the_range(exponent, dtype):
     dx, dw = F.linear_cross_entropy_backward(nt.Tensor(grad, device=DEV), x, weight, at, lse, reduction="none")
     base._check_backward(dx, dw, grad.astype(np.float64), base._values(x), base._values(weight), target,
                          base._values(lse), dtype, reduction="none")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("grad", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("rows", [1, 70])
+def test_no_row_counts_under_a_gradient_that_is_not_finite(rows, grad, dtype):
+    """Rows that do not count give no gradient, whatever the loss's own is."""
+    x, weight, _ = base._problem(base._rng(25, rows), rows, 50, 24, dtype)
+    at = base._targets(np.full(rows, -100))
+    lse = nt.Tensor(np.zeros(rows, np.float32), device=DEV)
+    for reduction in ("mean", "sum"):
+        for given in (float(grad), nt.Tensor(np.float32(grad), device=DEV)):
+            dx, dw = F.linear_cross_entropy_backward(given, x, weight, at, lse, reduction=reduction)
+            assert not np.any(dx.numpy()) and not np.any(dw.numpy())
+    each = nt.Tensor(np.full(rows, grad, np.float32), device=DEV)
+    dx, dw = F.linear_cross_entropy_backward(each, x, weight, at, lse, reduction="none")
+    assert not np.any(dx.numpy()) and not np.any(dw.numpy())
