@@ -623,7 +623,8 @@ def linear_cross_entropy_backward(grad_loss, input, weight, target, lse, *, igno
     """``(grad_input, grad_weight)`` of :func:`linear_cross_entropy_forward`
     with its ``lse`` and the same ``ignore_index`` and ``reduction``.
     ``grad_loss``, the gradient of the loss: a float32 Tensor of the loss's
-    shape or, for a mean or sum, a number (a loss scale; 1 without one)."""
+    shape or, for a mean or sum, a number within float32's range (a loss scale;
+    1 without one)."""
     given = _given(out, 2)
     x = _activation(input, "input", None, "Linear cross entropy")
     head, classes, width = _head(weight, input)
@@ -638,6 +639,8 @@ def linear_cross_entropy_backward(grad_loss, input, weight, target, lse, *, igno
                         (", as each row has a loss." if code == 0 else " or a real number."))
     else:
         value = float(grad_loss)
+        if _MOST_EPS < abs(value) < math.inf:
+            raise ValueError(f"grad_loss must be within float32's range, got {value}.")
     reject_during_capture("Linear cross entropy backward")
     dx = _result(given[0], "grad_input", input._shape, input._dtype, input)
     dw = _result(given[1], "grad_weight", weight._shape, weight._dtype, input)
