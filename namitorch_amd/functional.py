@@ -448,7 +448,7 @@ def norm_gate_add_norm_forward(input, residual, normalized_shape, inner_weight=N
 
 def _gated(x, residual, normalized_shape, inner_weight, inner_bias, gate, weight, bias, residual_scale, eps, norm, given,
            stats: bool) -> tuple:
-    source = _activation(x, "input")
+    source = _activation(x, "input", None, "The gated edge")
     stream_in = _activation(residual, "residual", x)
     lead, shape, rows, width = _normalized(x, normalized_shape)
     vectors, code = _vectors((inner_weight, inner_bias, weight, bias), shape, x)
@@ -458,7 +458,7 @@ def _gated(x, residual, normalized_shape, inner_weight, inner_bias, gate, weight
         raise ValueError("out: a mean was given, but root mean square norms have none.")
     needed = given if not (stats and rms) else (given[0], given[1], given[3], given[5])
     if None in needed:
-        reject_during_capture("Layer norm without out")
+        reject_during_capture("The gated edge without out")
     y = _result(given[0], "output", x._shape, x._dtype, x)
     total = _result(given[1], "total", x._shape, x._dtype, x)
     kept, at = (None,) * 4, (None,) * 4
@@ -483,7 +483,7 @@ def norm_gate_add_norm_backward(grad_output, grad_total, input, total, inner_mea
     nothing else reads ``total``).  A parameter's gradient has its shape and
     dtype, and is None where the parameter is None."""
     given = _given(out, 7)
-    t = _activation(total, "total")
+    t = _activation(total, "total", None, "The gated edge")
     source = _activation(input, "input", total)
     dy = _activation(grad_output, "grad_output", total)
     dt = None if grad_total is None else _activation(grad_total, "grad_total", total)
@@ -503,7 +503,7 @@ def norm_gate_add_norm_backward(grad_output, grad_total, input, total, inner_mea
     gate_at, gate_code, gate_rows = _gate(gate, lead, shape, total)
     scale = _scale(residual_scale)
     if None in given:
-        reject_during_capture("Layer norm backward")
+        reject_during_capture("The gated edge's backward call")
     dx = _result(given[0], "grad_input", total._shape, total._dtype, total)
     dr = _result(given[1], "grad_residual", total._shape, total._dtype, total)
     made = []

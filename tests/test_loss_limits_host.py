@@ -26,3 +26,19 @@ def test_loss_gradients_that_it_holds(launches, value):  # noqa: F811
     F.linear_cross_entropy_backward(value, x, w, t, lse, out=(_tensor((3, 8)), _tensor((50, 8))))
     (name, arguments), = launches
     assert name == "nt_linear_cross_entropy_backward" and arguments[2] == float(value)
+
+
+def test_the_edge_is_refused_in_its_own_name(launches, monkeypatch):  # noqa: F811
+    from namitorch_amd.backends import _graph_capture
+
+    host, device, stat = nt.Tensor(np.ones((3, 8), np.float32)), _tensor((3, 8)), _tensor((3,))
+    for call in (lambda: F.norm_gate_add_norm(host, host, 8),
+                 lambda: F.norm_gate_add_norm_backward(host, None, host, host, stat, stat, stat, stat)):
+        with pytest.raises(RuntimeError, match="^The gated edge runs only on HIP devices"):
+            call()
+    monkeypatch.setattr(_graph_capture, "capturing", lambda: True)
+    for call in (lambda: F.norm_gate_add_norm(device, device, 8), lambda: F.norm_gate_add_norm_forward(device, device, 8),
+                 lambda: F.norm_gate_add_norm_backward(device, None, device, device, stat, stat, stat, stat)):
+        with pytest.raises(RuntimeError, match="^The gated edge.* capture"):
+            call()
+    assert not launches
