@@ -11,12 +11,6 @@
 
 namespace nt {
 
-inline bool aligned16(std::initializer_list<const void *> arrays) {
-    uintptr_t bits = 0;
-    for (const void *p : arrays) bits |= (uintptr_t)p;
-    return bits % 16 == 0;
-}
-
 inline bool half_or_float(int32_t dtype) { return dtype == NT_F32 || dtype == NT_F16 || dtype == NT_BF16; }
 
 // One array argument: `count` elements of `dtype` (or kInt32, kInt64), written or only read.

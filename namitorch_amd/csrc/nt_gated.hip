@@ -854,7 +854,7 @@ static void in_launches(Args a, uint64_t blocks, F &&launch) {
 
 template <class T, int KIND, int THREADS>
 static void launch_gated_tiled(const GatedForward &args, const RowTiling &g, uint64_t runs, bool rms, hipStream_t s) {
-    const bool aligned = aligned16({args.total, args.y});
+    const bool aligned = aligned_rows(args.width, {args.total, args.y});
     const uint32_t blocks = run_blocks_of(args.rows / runs, runs, g, kGatedWaves, T::code == NT_F32);
     const uint32_t room = g.lanes * kGroup * 16u;
     in_launches(args, runs * blocks, [&](dim3 grid, const GatedForward &a) {
@@ -888,7 +888,7 @@ static void launch_gated(const GatedForward &a, bool rms, hipStream_t s) {
 template <class T, int KIND, int THREADS>
 static void launch_gated_backward_tiled(const GatedBackward &args, const RowTiling &g, bool rms, uint32_t groups,
                                         hipStream_t s) {
-    const bool aligned = aligned16({args.dx, args.dresidual, args.dgate});
+    const bool aligned = aligned_rows(args.width, {args.dx, args.dresidual, args.dgate});
     // The vectors, or half of the rows that are joined.
     const uint32_t span = g.lanes < 64u ? 64u : g.lanes;
     const uint32_t room = std::max(g.lanes * kGroup * (KIND == kFolded ? 8u : 12u), g.threads / span / 2u * g.lanes * 128u);

@@ -720,7 +720,7 @@ static void launch_forward_edge(const NormForward &a, hipStream_t s) {
         norm_rows_kernel<T, EDGE><<<dim3(strided_grid(a.rows, kBlock)), dim3(kBlock), 0, s>>>(a);
         return;
     }
-    const bool even = a.width % kGroup == 0 && aligned16({a.x, a.residual, a.total, a.y});
+    const bool even = aligned_rows(a.width, {a.x, a.residual, a.total, a.y});
     with_tiling<T::code == NT_F32 ? 2 : 3>(
         g, even, [&](auto parts, auto e) { launch_norm<T, EDGE, parts.value, e.value>(a, g, s); });
 }
@@ -734,7 +734,7 @@ static void launch_backward_edge(const NormBackward &a, hipStream_t s) {
             norm_columns_kernel<T><<<dim3((a.width + kBlock - 1) / kBlock, a.row_blocks), dim3(kBlock), 0, s>>>(a);
         return;
     }
-    const bool even = a.width % kGroup == 0 && aligned16({a.dy, a.dtotal, a.t, a.dx, a.dresidual});
+    const bool even = aligned_rows(a.width, {a.dy, a.dtotal, a.t, a.dx, a.dresidual});
     with_tiling<2>(g, even,
                    [&](auto parts, auto e) { launch_norm_backward<T, EDGE, parts.value, e.value>(a, g, s); });
 }

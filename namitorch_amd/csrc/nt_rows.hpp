@@ -5,6 +5,8 @@
 
 #include <stdint.h>
 
+#include <initializer_list>
+
 #include "../../include/namitorch_amd.h"
 
 #if defined(__HIPCC__)
@@ -45,6 +47,18 @@ struct Columns {
         return EVEN ? column < width : k >= first && column + k < width;
     }
 };
+
+inline bool aligned16(std::initializer_list<const void *> arrays) {
+    uintptr_t bits = 0;
+    for (const void *p : arrays) bits |= (uintptr_t)p;
+    return bits % 16 == 0;
+}
+
+// Whether every group of every row lies on 16 bytes, in any dtype: arrays that
+// start there are not enough where rows do not end on a whole group.
+inline bool aligned_rows(uint32_t width, std::initializer_list<const void *> arrays) {
+    return width % kGroup == 0 && aligned16(arrays);
+}
 
 // How a row is laid over lanes; parts == 0: it does not fit.
 struct RowTiling {
