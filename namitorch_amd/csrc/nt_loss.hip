@@ -37,6 +37,7 @@
 #include "nt_pool.hpp"
 #include "nt_product.hpp"
 #include "nt_row_ops.hpp"
+#include "nt_tiles.hpp"
 
 namespace nt {
 
@@ -683,63 +684,29 @@ __global__ __launch_bounds__(kBlock) void grad_kernel(const float *sums, uint64_
 }
 
 // ---- launches ----------------------------------------------------------------------------------------
-constexpr uint64_t kPieceBytes = 1ull << 30;       // of dz, and of packed weights, at a time
-
-constexpr uint32_t kUnits = 256;                     // compute units
+template <TileShape SHAPE, class T>
+constexpr bool is_shape() { return T::BP == size_p(SHAPE) && T::BQ == size_q(SHAPE); }
 
 using Large = Tile<256, 256, 2, 4>;
 using Middle = Tile<128, 128, 2, 2>;
-using Tall = Tile<256, 128, 4, 2, 3>;                // logits of 65 to 256 rows
-using Few = Tile<128, 64, 4, 1, 3>;                  // up to 64 rows, or too few tiles of the others
+using Tall = Tile<256, 128, 4, 2, 3>;
+using Few = Tile<128, 64, 4, 1, 3>;
+static_assert(is_shape<kLarge, Large>() && is_shape<kMiddle, Middle>() && is_shape<kTall, Tall>() &&
+              is_shape<kFew, Few>(), "nt_tiles.hpp counts tiles of these");
 
-static uint32_t tiles_of(uint64_t n, uint32_t each) { return (uint32_t)((n + each - 1) / each); }
-
-// Calls launch(shape) with the tile shape of the logits of `rows` and `classes`:
-// the largest of which each unit gets one.  1920 x 718 x 6208 bfloat16, 23 large
-// tiles or 90 of 128 x 128 or 180 small ones: forward 96 us with the second,
-// 63 with the last; 777 x 10007 x 1001 float32, 160 or 553: 129 us and 90.
-// Up to 256 rows tall ones, where half of the units get one (they wait for the
-// weights, which larger tiles ask for sooner): 129 rows of 50304 x 2048 float16
-// forward 48.4 us, with small ones 58.7, and 256 rows 79 and with 128 x 128 85;
-// but 200 rows of 10007 x 1001 float32, 80 tiles, 104 and 71.
+// Calls launch(shape) with the tile of the logits, or of the two products of dz.
 template <class F>
-static void with_logits_tile(uint64_t classes, uint64_t rows, F &&launch) {
-    if (rows <= 64u) launch(Few{});
-    else if (rows <= 256u && (uint64_t)tiles_of(classes, 256) * tiles_of(rows, 128) >= kUnits / 2u) launch(Tall{});
-    else if ((uint64_t)tiles_of(classes, 256) * tiles_of(rows, 256) >= kUnits) launch(Large{});
-    else if ((uint64_t)tiles_of(classes, 128) * tiles_of(rows, 128) >= kUnits) launch(Middle{});
+static void with_logits_tile(TileShape shape, F &&launch) {
+    if (shape == kLarge) launch(Large{});
+    else if (shape == kMiddle) launch(Middle{});
+    else if (shape == kTall) launch(Tall{});
     else launch(Few{});
 }
-
-// The same for the two products of dz.  Large tiles, where each unit gets 64
-// steps of them (whose ends are then a small part): 8192 x 50257 x 768 bfloat16,
-// 590 steps, a call 1.74 ms and with 128 x 128 1.88; 512 x 32000 x 4096, 125
-// steps, 475 us and 507; 200 x 128000 x 4096 947 and 1042; but 1500 x 10007 x
-// 1001, 30 steps, 161 and 146, and 300 x 50257 x 768 155 and 130.  They leave
-// half of themselves idle up to 128 rows: 70 x 128000 x 4096 739 and 723.
 template <class F>
-static void with_grads_tile(uint64_t classes, uint64_t rows, uint64_t pitch, F &&launch) {
-    const uint64_t steps = tiles_of(pitch, 256) * ((uint64_t)tiles_of(rows, 256) * tiles_of(classes, kDepth) +
-                                                   (uint64_t)tiles_of(classes, 256) * tiles_of(rows, kDepth));
-    if (rows <= 64u) launch(Few{});
-    else if (rows > 128u && steps >= 64u * kUnits) launch(Large{});
-    else launch(Middle{});
-}
-
-// How the two products of dz are split along k.  dx: such that no workgroup has
-// more than half of what each compute unit gets, nor less than four steps.  dW,
-// whose tiles are many as a rule, likewise, but only where one would be longer
-// than twice that (11127 rows of 720 x 64 bfloat16 have three tiles of dW: a
-// call 251 us in one piece, 72 split; but 777 x 10007 x 1001 float32, 13 steps
-// beside 18 on each unit: 423 split, 362 not; both in large tiles).
-struct Splits {
-    uint32_t input, weight;
-};
-static Splits splits_of(uint64_t input_tiles, uint32_t input_steps, uint64_t weight_tiles, uint32_t weight_steps) {
-    const uint64_t share =
-        std::max<uint64_t>((input_tiles * input_steps + weight_tiles * weight_steps) / (2u * kUnits), 4u);
-    const auto of = [&](uint32_t steps) { return (uint32_t)std::max<uint64_t>(1u, (steps + share - 1) / share); };
-    return Splits{of(input_steps), weight_steps > 4u * share ? of(weight_steps) : 1u};
+static void with_grads_tile(TileShape shape, F &&launch) {
+    if (shape == kLarge) launch(Large{});
+    else if (shape == kMiddle) launch(Middle{});
+    else launch(Few{});
 }
 
 struct Problem {
@@ -759,19 +726,6 @@ template <class T> struct Kind {            // how the products take a type
     static constexpr bool kHalf = T::code == NT_F16;
     static constexpr int kPlanes = T::code == NT_F32 ? 3 : 1;
 };
-
-// The pieces of the vocabulary: as few as keep dz and the packed weights
-// within their bytes, and a launch below 2**32 work-items (512 for each large
-// tile, twice as many for as much in tall ones); of whole tiles.
-static uint32_t piece_of(const Problem &a, uint32_t pitch, int planes, bool packed, bool backward) {
-    uint64_t most = (1ull << 21) / tiles_of(a.rows, 256) * 256u;
-    if (backward) most = std::min<uint64_t>(most, kPieceBytes / (2ull * planes * whole_steps(a.rows)));
-    if (packed) most = std::min<uint64_t>(most, kPieceBytes / (2ull * planes * pitch));
-    if (most >= a.classes) return a.classes;
-    most = std::max<uint64_t>(most, 256u);
-    const uint64_t pieces = (a.classes + most - 1) / most, each = (a.classes + pieces - 1) / pieces;
-    return (uint32_t)((each + 255u) / 256u * 256u);
-}
 
 template <class T>
 static int32_t few_rows_of(const Problem &a, int32_t device, float *loss, float *lse, void *stream) {
@@ -801,13 +755,12 @@ static int32_t forward_of(const Problem &a, int32_t device, float *loss, float *
     constexpr int planes = Kind<T>::kPlanes;
     constexpr bool half = Kind<T>::kHalf;
     hipStream_t s = (hipStream_t)stream;
-    const uint32_t pitch = whole_steps(a.width), padded = whole_steps(a.rows);
-    const bool pack_w = planes > 1 || pitch != a.width || (uintptr_t)a.w % 16u != 0;
+    const LossPlan plan = loss_plan(a.rows, a.classes, a.width, planes, (uintptr_t)a.w % 16u == 0, false);
+    const uint32_t pitch = plan.pitch, padded = whole_steps(a.rows), piece = plan.piece, pieces = plan.pieces;
+    const bool pack_w = plan.packed;
     if (a.rows <= (planes > 1 || pitch != a.width ? kFewRows : 1u)) return few_rows_of<T>(a, device, loss, lse, stream);
-    const uint32_t piece = piece_of(a, pitch, planes, pack_w, false);
-    const uint32_t pieces = (a.classes + piece - 1) / piece;
     uint32_t slots_piece = 0, slots = 0;                  // of a whole piece, of all
-    with_logits_tile(piece, a.rows, [&](auto shape) {
+    with_logits_tile(plan.logits, [&](auto shape) {
         using Shape = decltype(shape);
         slots_piece = tiles_of(piece, Shape::BP) * Shape::WP;
         slots = (pieces - 1) * slots_piece + tiles_of(a.classes - (pieces - 1) * piece, Shape::BP) * Shape::WP;
@@ -847,7 +800,7 @@ static int32_t forward_of(const Problem &a, int32_t device, float *loss, float *
         product.depth = pitch;
         product.live = rows.count;
         const FinishLoss finish{partials, target_logit, rows.target, rows.count, first, classes, k * slots_piece, a.rows};
-        with_logits_tile(piece, a.rows, [&](auto shape) {
+        with_logits_tile(plan.logits, [&](auto shape) {
             using Shape = decltype(shape);
             product.tiles_p = tiles_of(classes, Shape::BP);
             product.tiles_q = tiles_of(a.rows, Shape::BQ);
@@ -871,18 +824,11 @@ static int32_t backward_of(const Problem &a, int32_t device, const float *grad, 
     constexpr bool half = Kind<T>::kHalf;
     using Raw = typename T::raw;
     hipStream_t s = (hipStream_t)stream;
-    const uint32_t pitch = whole_steps(a.width), padded = whole_steps(a.rows);
-    const bool pack_w = planes > 1 || pitch != a.width || (uintptr_t)a.w % 16u != 0;
-    const uint32_t piece = piece_of(a, pitch, planes, pack_w, true);
-    const uint32_t pieces = (a.classes + piece - 1) / piece;
+    const LossPlan plan = loss_plan(a.rows, a.classes, a.width, planes, (uintptr_t)a.w % 16u == 0, true);
+    const uint32_t pitch = plan.pitch, padded = whole_steps(a.rows), piece = plan.piece, pieces = plan.pieces;
+    const bool pack_w = plan.packed;
     const uint32_t dz_pitch = whole_steps(piece);
-    Splits splits{1, 1};
-    with_grads_tile(piece, a.rows, pitch, [&](auto shape) {
-        using Shape = decltype(shape);
-        const uint32_t tiles_h = tiles_of(pitch, Shape::BP);
-        splits = splits_of((uint64_t)tiles_h * tiles_of(a.rows, Shape::BQ), tiles_of(piece, kDepth),
-                           (uint64_t)tiles_h * tiles_of(piece, Shape::BQ), tiles_of(a.rows, kDepth));
-    });
+    const Splits splits = plan.splits;
 
     Rows rows{};
     uint16_t *px = nullptr, *pw = nullptr, *dz = nullptr;
@@ -934,7 +880,7 @@ static int32_t backward_of(const Problem &a, int32_t device, const float *grad, 
         logits.live = rows.count;
         const FinishGrad<half, planes> grads{dz,         plane_dz,    line,     lse, rows.weight, rows.target,
                                              rows.row, rows.count, first, classes};
-        with_logits_tile(piece, padded, [&](auto shape) {
+        with_logits_tile(plan.logits, [&](auto shape) {
             using Shape = decltype(shape);
             logits.tiles_p = tiles_of(line, Shape::BP);
             logits.tiles_q = tiles_of(padded, Shape::BQ);
@@ -958,7 +904,7 @@ static int32_t backward_of(const Problem &a, int32_t device, const float *grad, 
         weight.live_depth = true;
         Raw *to = static_cast<Raw *>(dw) + (uint64_t)first * a.width;
         const bool even_weight = a.width % 8u == 0 && (uintptr_t)dw % 16u == 0;
-        with_grads_tile(piece, a.rows, pitch, [&](auto shape) {
+        with_grads_tile(plan.grads, [&](auto shape) {
             using Shape = decltype(shape);
             input.tiles_p = weight.tiles_p = tiles_of(pitch, Shape::BP);
             input.tiles_q = tiles_of(a.rows, Shape::BQ);

@@ -40,6 +40,7 @@
 #include <stdint.h>
 
 #include "nt_common.hpp"
+#include "nt_tiles.hpp"
 
 namespace nt {
 
@@ -51,10 +52,7 @@ typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef short s16x8_t __attribute__((ext_vector_type(8)));
 
-constexpr uint32_t kDepth = 64;             // elements along k in a step
 constexpr uint32_t kMostPitch = 1u << 22;   // elements of a line: a tile's offsets stay below 2**32 bytes
-
-__host__ __device__ __forceinline__ uint32_t whole_steps(uint32_t n) { return (n + kDepth - 1u) / kDepth * kDepth; }
 
 // There is no end of k inside a step: deep lines are padded with zeros to
 // whole steps, and so is one operand's number of lines otherwise, where the
