@@ -84,8 +84,8 @@ inline uint32_t piece_of(uint32_t rows, uint32_t classes, uint32_t pitch, int pl
     uint64_t most = (1ull << 21) / tiles_of(rows, 256) * 256u;
     if (backward) most = std::min<uint64_t>(most, kPieceBytes / (2ull * planes * whole_steps(rows)));
     if (packed) most = std::min<uint64_t>(most, kPieceBytes / (2ull * planes * pitch));
+    most = std::max<uint64_t>(most / 256u * 256u, 256u);
     if (most >= classes) return classes;
-    most = std::max<uint64_t>(most, 256u);
     const uint64_t pieces = (classes + most - 1) / most, each = (classes + pieces - 1) / pieces;
     return (uint32_t)((each + 255u) / 256u * 256u);
 }

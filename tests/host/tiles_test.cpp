@@ -3,7 +3,8 @@
 // With arguments rows, classes, width, planes and whether the pass is the
 // backward one: prints the plan's pieces, the logits' and the gradients' tiles
 // and the splits of both products.  Without: over sizes of every magnitude the
-// pieces cover the classes and no launch reaches 2**32 work-items.
+// pieces cover the classes, keep their bytes unless they are the smallest, and
+// no launch reaches 2**32 work-items.
 #include <cstdio>
 #include <cstdlib>
 
@@ -38,6 +39,11 @@ int main(int argc, char **argv) {
                         const uint64_t last = classes - (p.pieces - 1ull) * p.piece;
                         check(p.pieces >= 1 && last >= 1 && last <= p.piece, "pieces cover the classes", rows, classes, width);
                         check(p.pieces == 1 || p.piece % 256 == 0, "pieces of whole tiles", rows, classes, width);
+                        const bool least = p.piece <= 256;
+                        const uint64_t packed = 2ull * planes * p.pitch * whole_steps(p.piece);
+                        const uint64_t dz = 2ull * planes * whole_steps((uint32_t)rows) * whole_steps(p.piece);
+                        check(least || !p.packed || packed <= kPieceBytes, "bytes of packed weights", rows, classes, width);
+                        check(least || !pass || dz <= kPieceBytes, "bytes of dz", rows, classes, width);
                         const uint64_t logits = (uint64_t)tiles_of(whole_steps(p.piece), size_p(p.logits)) *
                                                 tiles_of(whole_steps((uint32_t)rows), size_q(p.logits)) * threads_of(p.logits);
                         check(logits < 1ull << 32, "work-items of the logits", rows, classes, width);
