@@ -611,7 +611,10 @@ int32_t nt_dropout_add_layer_norm_backward(int32_t device, const void *dy, const
  * consecutive rows.  The four statistics (float32, one per row) are given
  * together or not at all, without the means for `rms`; the backward entry
  * takes NULL means as rms.  It writes dx, dresidual and, where not NULL, the
- * gradients of the vectors and the gate (sums over rows in a fixed order).
+ * gradients of the vectors and the gate (sums over rows in a fixed order), and
+ * takes workspace of the library's pool: 16 bytes x width for each of up to 512
+ * workgroups, or for each row of the gate where it has more (and does not have
+ * one for each row), and 8 bytes a row above 8192 columns or below 8.
  * dtotal, the gradient total receives elsewhere, may be NULL.  Types, widths,
  * overlaps, captures and empty batches as in nt_layer_norm.
  */
@@ -657,7 +660,9 @@ int32_t nt_norm_gate_add_norm_backward(int32_t device, const void *dy, const voi
  *   dz = g (exp(z - lse) - [class = target]), dx = dz weight, dweight = dz^T x
  *
  * with dz rounded once to `dtype` (and float32 operands multiplied as three
- * bfloat16 parts each).  Both take workspace of the library's pool in the order
+ * bfloat16 parts each).  Float16's dz is scaled by one power of two, by the
+ * largest finite g of a row whose target is a class: rows of 2^-20 of it or less
+ * keep few digits of their probabilities.  Both take workspace of the library's pool in the order
  * of `stream` and refuse a stream in capture.  Forward: the size of x and 8 bytes
  * for each row and 32 (few rows) to 128 classes.  Backward: up to 1 GiB, or 256
  * classes, for a piece of dz, the size of x and float32 sums of it, in up to 512

@@ -93,8 +93,10 @@ __device__ __forceinline__ float block_total(double v, double *shared) {
 //
 // Bound by memory where rows are long: 16384 x 4096 bfloat16 with root mean
 // squares 96 us (5.6 TB/s), layer norms 114 (two sums more in turn); 8192 x 2048
-// float32 55 (4.9).  Narrow rows are bound by latency, four sums over lanes in
-// turn with few turns to share them: 8192 x 768 bfloat16 17.2 us (2.9 TB/s).
+// float32 55 (4.9).  Narrow rows are bound by the vector units: 8192 x 768
+// bfloat16 17.3 us (2.9 TB/s), 387 instructions of each of a row's two waves, of
+// four cycles each, which keep a SIMD busy 79 % of the time that its four waves
+// live; they wait half of it, in turn, at the four sums over lanes.
 constexpr uint32_t kGatedWaves = 4;     // per SIMD
 
 enum GateKind { kFolded = 0, kOwn = 1, kOwnFloat = 2 };   // none or shared; a row's own, of the data's type or float32
@@ -292,8 +294,8 @@ void gated_kernel(GatedForward a, uint32_t lanes, uint32_t run_blocks, bool rms,
 // two 46; 8192 x 2048 bfloat16 84 and 65, float32 with a shared one 119 and 91).
 //
 // 16384 x 4096 bfloat16 with root mean squares 176 us: four reads and two
-// writes at 4.7 TB/s, each row two exchanges over eight waves; 8192 x 768 23.6
-// us (3.2 TB/s), four turns, whose latency and joined sums show.
+// writes at 4.7 TB/s, each row two exchanges over eight waves, the vector units
+// busy 74 % of the time; 8192 x 768 23.8 us (3.2 TB/s), 83 %.
 static constexpr uint32_t gated_backward_waves(int32_t dtype, int kind, uint32_t threads) {
     return threads > (uint32_t)kRowThreads || (dtype != NT_F32 && kind == kFolded) ? 4u : 2u;
 }

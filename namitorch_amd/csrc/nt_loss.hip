@@ -227,7 +227,7 @@ __global__ __launch_bounds__(kBlock) void pack_kernel(const void *from, uint32_t
 // ---- what becomes of the products' tiles ------------------------------------------------------------------
 // Of a difference that is made first.  With log2(e) multiplied into both sides
 // of it, for one operation less (a forward call of 8192 x 50257 x 768 bfloat16
-// 566 us, so 575, a backward call the same), the rounding of a product stayed
+// 512 us, so 518, a backward call the same), the rounding of a product stayed
 // in the exponent, 2^-24 of a logit: exp(z - lse) - 1 of a target at 1536 was
 // off by 9e-5 where it is zero, and of logits past 2^32 sums were zero or
 // infinite.
@@ -246,7 +246,7 @@ __device__ __forceinline__ Partial2 join(Partial2 a, Partial2 b) {
 // Logits to a maximum and sum of each row's part of a wave's tile, and the
 // target's logit: a lane has four classes of a row in each of its tiles, and 8
 // bytes a row and 128 classes (of large tiles) are stored for what would be 256.
-// 8192 x 50257 x 768 bfloat16, a tenth ignored: 575 us with the product, 0.99
+// 8192 x 50257 x 768 bfloat16, a tenth ignored: 531 us with the product, 1.07
 // PFLOP/s; the product's 12 steps are short for these ends.
 struct FinishLoss {
     Partial2 *partials;         // [slot][rows]
@@ -322,7 +322,7 @@ struct Pair {
 };
 
 // Logits to dz, stored 16 bytes a lane.  8192 x 32000 x 4096 bfloat16, a tenth
-// ignored: 1.65 ms with the product, 1.17 PFLOP/s; 50257 x 768 0.71 ms, 0.80
+// ignored: 1.64 ms with the product, 1.18 PFLOP/s; 50257 x 768 0.69 ms, 0.82
 // with 0.74 GB stored.  The columns from the piece's last class to the line's
 // end and the rows from the last counted one to a whole step are zero.
 template <bool HALF, int PLANES>
@@ -427,7 +427,7 @@ struct FinishSum {
 };
 
 // A piece's rows of dW.  Both products of 8192 x 32000 x 4096 bfloat16, a tenth
-// of the rows ignored: 3.17 ms, 1.22 PFLOP/s; of 50257 x 768 1.01 ms, 1.12.
+// of the rows ignored: 3.10 ms, 1.25 PFLOP/s; of 50257 x 768 0.98 ms, 1.16.
 template <class S>
 struct FinishWeight {
     typename S::raw *to;

@@ -9,14 +9,16 @@
 // while the slices before are multiplied, so there are two rooms for them, or
 // three.  Sums are float32 in the matrix cores' accumulators.
 //
-// What bounds it: large products run at 1.15 to 1.25 PFLOP/s (8192 x 32000 x
-// 4096 bfloat16: 1.6 ms in each of the three layouts, where a library's plain
-// product of that size takes 1.61), the matrix cores busy 58 % of the cycles at
-// clocks that fall to 1.5 to 1.8 GHz under the load.  Tried and not kept: 32 x 32
-// instead of 16 x 16 instructions (1.70 to 1.83 ms), the two waves of a SIMD
-// taking turns at LDS and the matrix cores (1.77 to 1.95), four waves of 128 x 64
-// (2.2 to 2.4), workgroups that stride over tiles with the next one's first slice
-// on its way (spills), and steps in another order for each XCD (no difference).
+// What bounds it: 8192 counted rows of 32000 x 4096 bfloat16 take 1.57 ms with
+// the loss's end, 1.69 with dz's, and the two products of dz 3.28 together, 1.27
+// to 1.37 PFLOP/s, where a library's plain product of that size takes 1.61 ms
+// (1.33); 7373 rows, whose last round of tiles is nearly empty, run at 1.18 to
+// 1.25.  The matrix cores are busy 60 % of the cycles, at clocks that fall to 1.5
+// to 1.8 GHz under the load.  Tried and not kept: 32 x 32 instead of 16 x 16
+// instructions (6 to 14 % longer), the two waves of a SIMD taking turns at LDS
+// and the matrix cores (11 to 22 %), four waves of 128 x 64 (38 to 50 %),
+// workgroups that stride over tiles with the next one's first slice on its way
+// (spills), and steps in another order for each XCD (no difference).
 // Few rows are bound by the one read of the weights, at 4 to 5 TB/s.
 //
 // A 16-byte group of a slice does not lie where its place in memory says, but

@@ -3,9 +3,11 @@ and the edges of the residual path that join them, and the loss at its end.
 
 The reference has layer norm, root mean square norm, dropout and cross entropy
 in ``namitorch/nn`` (the norms over the kernels of
-``backends/cuda/normalization.py:56-157``).  This package has no autograd, so each operator comes as a forward call that returns what
-its backward call reads, and a backward call that returns gradients to hand
-to ``accumulate_grads`` or to the layer below:
+``backends/cuda/normalization.py:56-157``); root mean square norms are here
+within the gated edge alone.  This package has no autograd, so each operator
+comes as a forward call that returns what its backward call reads, and a
+backward call that returns gradients to hand to ``accumulate_grads`` or to the
+layer below:
 
 * ``layer_norm`` / ``layer_norm_forward`` / ``layer_norm_backward``;
 * ``dropout`` / ``dropout_backward``;
@@ -22,7 +24,8 @@ Tensors are float16, bfloat16 or float32 on a HIP device; weight and bias
 (and their gradients) have the activations' dtype or float32.  Statistics and
 sums are float32, values are rounded once (the loss's backward call rounds
 the logits' gradient to the operands' dtype too).  A row that holds an
-infinity or NaN gives NaN outputs.
+infinity or NaN gives NaN outputs (but the gated edge's ``total`` of a root
+mean square norm over an infinity NaN there alone: the norm is zero beside it).
 
 No mask is stored.  Whether element ``i`` of the flattened tensor is dropped
 depends on ``(seed, offset, i)`` alone (Philox4x32-10, 16 bits per element),
@@ -621,7 +624,10 @@ def _linear_cross_entropy(x, weight, target, ignore_index, reduction, given, kee
 def linear_cross_entropy_backward(grad_loss, input, weight, target, lse, *, ignore_index=-100, reduction="mean",
                                   out=None) -> tuple:
     """``(grad_input, grad_weight)`` of :func:`linear_cross_entropy_forward`
-    with its ``lse`` and the same ``ignore_index`` and ``reduction``.
+    with its ``lse`` and the same ``ignore_index`` and ``reduction``.  The
+    logits' gradient is rounded to the operands' dtype on the way; float16's is
+    scaled by one power of two for all rows, so that a row whose own gradient is
+    2**-20 of the largest or less keeps few digits of its probabilities.
     ``grad_loss``, the gradient of the loss: a float32 Tensor of the loss's
     shape or, for a mean or sum, a number within float32's range (a loss scale;
     1 without one)."""
